@@ -57,13 +57,56 @@ def load_library() -> None:
                          scale, coefficients):
         return None
 
+    def fake_distill_topk(student, values, indices, lse, temperature):
+        rows = student.shape[0]
+        return (student.new_empty((rows,), dtype=torch.float32),
+                student.new_empty((rows, 2), dtype=torch.float32))
+
+    def fake_distill_topk_backward(grad_loss, student, values, indices, lse, stats, temperature):
+        return torch.empty_like(student)
+
+    def fake_distill_topk_grad(student, values, indices, row_scale, lse, temperature):
+        return student.new_empty((student.shape[0],), dtype=torch.float32), torch.empty_like(student)
+
+    def fake_residual_norm(block_out, residual, post, pre, gate, scale, eps):
+        rows, width = block_out.shape
+        f32 = torch.float32
+        return (block_out.new_empty((rows, width)),
+                block_out.new_empty((rows if pre is not None else 0, width)),
+                block_out.new_empty((rows if post is not None else 0,), dtype=f32),
+                block_out.new_empty((rows if pre is not None else 0,), dtype=f32))
+
+    def fake_residual_norm_backward(grad_hidden, grad_normed, block_out, residual, post, pre, gate,
+                                    scale, rstd_post, rstd_pre, eps, wanted):
+        inputs = (block_out, residual, post, pre, gate, scale)
+        return tuple(torch.empty_like(t, memory_format=torch.contiguous_format)
+                     if want and t is not None else block_out.new_empty((0,))
+                     for t, want in zip(inputs, wanted))
+
+    def fake_route_experts(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale):
+        tokens, experts = logits.shape
+        return (logits.new_empty((tokens, k), dtype=torch.float32),
+                logits.new_empty((tokens, k), dtype=torch.int64),
+                logits.new_empty((experts,), dtype=torch.int64))
+
+    def fake_route_experts_backward(grad_weights, logits, indices, score, renormalize, scale):
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
     # Extensions of this build: polar_step_t (the step of x^T in x's layout)
     # has polar_step's output contract; polar_express returns bf16 of x's
-    # shape; muon_update_ mutates its arguments and returns nothing.
+    # shape; muon_update_ mutates its arguments and returns nothing.  The
+    # training-step operators (training.py) return fresh tensors.
     fakes = (("muon_ascend950::polar_step", fake_polar_step),
              ("muon_ascend950::polar_step_t", fake_polar_step),
              ("muon_ascend950::polar_express", fake_polar_express),
-             ("muon_ascend950::muon_update_", fake_muon_update))
+             ("muon_ascend950::muon_update_", fake_muon_update),
+             ("muon_ascend950::distill_topk", fake_distill_topk),
+             ("muon_ascend950::distill_topk_backward", fake_distill_topk_backward),
+             ("muon_ascend950::distill_topk_grad", fake_distill_topk_grad),
+             ("muon_ascend950::residual_norm", fake_residual_norm),
+             ("muon_ascend950::residual_norm_backward", fake_residual_norm_backward),
+             ("muon_ascend950::route_experts", fake_route_experts),
+             ("muon_ascend950::route_experts_backward", fake_route_experts_backward))
     for name, fn in fakes:
         try:
             torch.library.register_fake(name)(fn)

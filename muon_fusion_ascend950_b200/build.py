@@ -2,13 +2,17 @@
 
 * ``libmuon_polar_sm100.so`` -- the sm_100a kernels and the C ABI declared in
   ``include/muon_polar_sm100.h`` (nvcc, static CUDA runtime, no torch): the
-  Polar Express step (``muon_polar_sm100.cu``) and the Muon update around it
-  (``muon_update_sm100.cu``).
-* ``_C.so`` -- the PyTorch operator ``muon_ascend950::polar_step`` on the CUDA
-  dispatch key, linked against the library above (rpath ``$ORIGIN``).
+  Polar Express step (``muon_polar_sm100.cu``), the Muon update around it
+  (``muon_update_sm100.cu``) and the training-step operators declared in
+  ``include/muon_train_sm100.h`` (``distill_topk_sm100.cu``,
+  ``residual_norm_sm100.cu``, ``route_experts_sm100.cu``).
+* ``_C.so`` -- the PyTorch operators ``muon_ascend950::*`` on the CUDA
+  dispatch key (``polar_step_op.cpp``, ``train_ops.cpp``), linked against the
+  library above (rpath ``$ORIGIN``).
 
-Both land next to this file so that they travel with the source tree.  The
-build is skipped when the outputs are newer than every input.  Run with
+Both land next to this file so that they travel with the source tree.  Each
+source compiles to an object under ``_build/`` (all in parallel); what is newer
+than every input is not built again.  Run with
 ``python -m muon_fusion_ascend950_b200.build`` (``--force`` to rebuild).
 """
 from __future__ import annotations
@@ -17,12 +21,14 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = REPO / "include"
+BUILD = PKG / "_build"
 LIB_NAME = "libmuon_polar_sm100.so"
 OP_NAME = "_C.so"
 
@@ -51,35 +57,63 @@ def _run(cmd) -> None:
     subprocess.run([str(c) for c in cmd], check=True, cwd=REPO)
 
 
+CU_SOURCES = {  # source -> the headers it includes
+    "muon_polar_sm100.cu": ["sm100_ptx.cuh", "muon_polar_sm100.h"],
+    "muon_update_sm100.cu": ["sm100_ptx.cuh", "muon_polar_sm100.h"],
+    "distill_topk_sm100.cu": ["train_common.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "residual_norm_sm100.cu": ["train_common.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "route_experts_sm100.cu": ["train_common.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+}
+OP_SOURCES = {
+    "polar_step_op.cpp": ["muon_polar_sm100.h"],
+    "train_ops.cpp": ["muon_train_sm100.h", "muon_polar_sm100.h"],
+}
+
+
+def _compile(sources: dict, command, force: bool) -> list:
+    """Objects of `sources` by `command`, those that are out of date in parallel."""
+    BUILD.mkdir(exist_ok=True)
+    objects, todo = [], []
+    for name, headers in sources.items():
+        obj = BUILD / (name + ".o")
+        inputs = [CSRC / name, Path(__file__)]
+        inputs += [CSRC / h if h.endswith(".cuh") else INCLUDE / h for h in headers]
+        objects.append(obj)
+        if force or not _newer(obj, inputs):
+            todo.append([*command, "-c", CSRC / name, "-o", obj])
+    with ThreadPoolExecutor(max_workers=len(sources)) as pool:
+        list(pool.map(_run, todo))
+    return objects
+
+
 def build_library(force: bool = False, verbose_ptxas: bool = False) -> Path:
     """nvcc -> libmuon_polar_sm100.so (kernels + C ABI)."""
     out = PKG / LIB_NAME
-    cu = [CSRC / "muon_polar_sm100.cu", CSRC / "muon_update_sm100.cu"]
-    sources = [*cu, CSRC / "sm100_ptx.cuh", INCLUDE / "muon_polar_sm100.h"]
-    if not force and _newer(out, sources):
-        return out
     nvcc = _cuda_home() / "bin" / "nvcc"
-    cmd = [nvcc, *NVCC_ARCH, "-O3", "-std=c++17", "-lineinfo",
-           "-Xcompiler", "-fPIC", "-shared", "-I", INCLUDE, *cu, "-o", out]
+    cmd = [nvcc, *NVCC_ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", INCLUDE]
     if verbose_ptxas:
-        cmd.insert(1, "-Xptxas=-v")
-    _run(cmd)
+        cmd.append("-Xptxas=-v")
+    objects = _compile(CU_SOURCES, cmd, force)
+    if force or not _newer(out, objects):
+        _run([nvcc, *NVCC_ARCH, "-shared", "-Xcompiler", "-fPIC", *objects, "-o", out])
     return out
 
 
 def build_op(force: bool = False) -> Path:
-    """g++ -> _C.so (torch operator), linked to the C ABI library."""
+    """g++ -> _C.so (torch operators), linked to the C ABI library."""
     import torch
     from torch.utils import cpp_extension
 
     lib = build_library(force=force)
     out = PKG / OP_NAME
-    sources = [CSRC / "polar_step_op.cpp", INCLUDE / "muon_polar_sm100.h", lib]
-    if not force and _newer(out, sources):
-        return out
     cuda_home = _cuda_home()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     includes = cpp_extension.include_paths() + [str(cuda_home / "include"), str(INCLUDE)]
+    objects = _compile(OP_SOURCES, ["g++", "-O2", "-std=c++17", "-fPIC",
+                                    f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
+                                    *[f"-I{p}" for p in includes]], force)
+    if not force and _newer(out, [*objects, lib]):
+        return out
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
     # The operator's inline ATen/c10 helpers call the CUDA runtime: bind them
     # to the same libcudart torch itself loads.
@@ -88,15 +122,11 @@ def build_op(force: bool = False) -> Path:
         cudart = [f"-L{cudart_dir}", "-l:libcudart.so.12", f"-Wl,-rpath,{cudart_dir}"]
     else:
         cudart = [f"-L{cuda_home / 'lib64'}", "-lcudart"]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
-           *[f"-I{p}" for p in includes],
-           CSRC / "polar_step_op.cpp", "-o", out,
-           f"-L{torch_lib}", f"-L{PKG}",
-           "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-ltorch_cuda",
-           "-lmuon_polar_sm100", *cudart,
-           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
-    _run(cmd)
+    _run(["g++", "-shared", *objects, "-o", out,
+          f"-L{torch_lib}", f"-L{PKG}",
+          "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-ltorch_cuda",
+          "-lmuon_polar_sm100", *cudart,
+          "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
     return out
 
 

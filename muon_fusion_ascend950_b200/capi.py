@@ -94,6 +94,59 @@ SIGNATURES = {
     "muon_polar_unpack_sym_sm100": (ctypes.c_int, [_VP, _VP, _I64, _I64, _VP]),
 }
 
+
+# The training-step operators of include/muon_train_sm100.h.
+class DistillArgs(ctypes.Structure):
+    """muon_train_distill_args"""
+    _fields_ = [("logits", _VP), ("rows", _I64), ("vocab", _I64), ("ld", _I64),
+                ("teacher_logits", _VP), ("teacher_indices", _VP), ("teacher_lse", _VP),
+                ("row_scale", _VP), ("loss", _VP), ("stats", _VP), ("grad", _VP),
+                ("ld_grad", _I64), ("top", _I64), ("temperature", ctypes.c_float),
+                ("dtype", ctypes.c_int), ("teacher_dtype", ctypes.c_int),
+                ("index_bytes", ctypes.c_int)]
+
+
+class NormArgs(ctypes.Structure):
+    """muon_train_norm_args"""
+    _fields_ = [("block_out", _VP), ("residual", _VP), ("post_weight", _VP), ("pre_weight", _VP),
+                ("gate", _VP), ("residual_scale", _VP), ("hidden", _VP), ("normed", _VP),
+                ("rstd_post", _VP), ("rstd_pre", _VP), ("rows", _I64), ("width", _I64),
+                ("gate_rows", _I64), ("scale_count", _I64), ("eps", ctypes.c_float),
+                ("dtype", ctypes.c_int), ("post_dtype", ctypes.c_int), ("pre_dtype", ctypes.c_int),
+                ("gate_dtype", ctypes.c_int), ("scale_dtype", ctypes.c_int)]
+
+
+class NormGrads(ctypes.Structure):
+    """muon_train_norm_grads"""
+    _fields_ = [("grad_hidden", _VP), ("grad_normed", _VP), ("grad_block_out", _VP),
+                ("grad_residual", _VP), ("grad_post_weight", _VP), ("grad_pre_weight", _VP),
+                ("grad_gate", _VP), ("grad_residual_scale", _VP), ("workspace", _VP),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+class RouteArgs(ctypes.Structure):
+    """muon_train_route_args"""
+    _fields_ = [("logits", _VP), ("bias", _VP), ("weights", _VP), ("indices", _VP),
+                ("counts", _VP), ("tokens", _I64), ("experts", _I64), ("ld", _I64),
+                ("dtype", ctypes.c_int), ("score", ctypes.c_int), ("k", ctypes.c_int),
+                ("groups", ctypes.c_int), ("top_groups", ctypes.c_int),
+                ("group_top", ctypes.c_int), ("renormalize", ctypes.c_int),
+                ("scale", ctypes.c_float)]
+
+
+_DISTILL, _NORM, _GRADS, _ROUTE = (ctypes.POINTER(t) for t in (DistillArgs, NormArgs, NormGrads,
+                                                               RouteArgs))
+TRAIN_SIGNATURES = {
+    "muon_train_launch_count": (ctypes.c_uint64, []),
+    "muon_train_distill_sm100": (ctypes.c_int, [_DISTILL, _VP]),
+    "muon_train_distill_backward_sm100": (ctypes.c_int, [_DISTILL, _VP]),
+    "muon_train_residual_norm_sm100": (ctypes.c_int, [_NORM, _VP]),
+    "muon_train_residual_norm_workspace_bytes": (ctypes.c_size_t, [_NORM]),
+    "muon_train_residual_norm_backward_sm100": (ctypes.c_int, [_NORM, _GRADS, _VP]),
+    "muon_train_route_sm100": (ctypes.c_int, [_ROUTE, _VP]),
+    "muon_train_route_backward_sm100": (ctypes.c_int, [_ROUTE, _VP, _VP, _VP]),
+}
+
 WATCHDOG_PRODUCER = 0x1
 WATCHDOG_MMA = 0x2
 WATCHDOG_EPILOGUE = 0x4
@@ -136,7 +189,7 @@ class CAPI:
                 f"{path} is missing; build it with `python -m muon_fusion_ascend950_b200.build`")
         self.path = path
         self.lib = ctypes.CDLL(str(path))
-        for name, (restype, argtypes) in SIGNATURES.items():
+        for name, (restype, argtypes) in {**SIGNATURES, **TRAIN_SIGNATURES}.items():
             fn = getattr(self.lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -156,6 +209,10 @@ class CAPI:
         if stream is None:
             stream = torch.cuda.current_stream()
         return int(getattr(stream, "cuda_stream", stream))
+
+    def train_launch_count(self) -> int:
+        """Kernels launched by the training-step operators so far."""
+        return int(self.lib.muon_train_launch_count())
 
     def abi_version(self) -> int:
         return int(self.lib.muon_polar_abi_version())

@@ -1,0 +1,597 @@
+// train_ops.cpp -- PyTorch operators of the training step around the Muon
+// update: distillation from a teacher's top logits, the norms around a
+// residual block, routing to experts.  CUDA kernels through the C ABI
+// (include/muon_train_sm100.h); gradients on the Autograd key.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <array>
+#include <cmath>
+#include <optional>
+#include <tuple>
+
+#include "muon_train_sm100.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+void CheckStatus(int rc, const char* who) {
+  TORCH_CHECK(rc == MUON_POLAR_OK, who, " failed, status=", rc,
+              ", detail=", muon_polar_status_string(rc));
+}
+
+int Dtype(const Tensor& t, const char* who, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return MUON_TRAIN_F32;
+    case at::kBFloat16: return MUON_TRAIN_BF16;
+    case at::kHalf: return MUON_TRAIN_F16;
+    default: TORCH_CHECK_TYPE(false, who, ": ", name, " must be float32, bfloat16 or float16, got ",
+                              t.scalar_type());
+  }
+}
+
+void CheckCuda(const Tensor& t, const char* who, const char* name) {
+  TORCH_CHECK_VALUE(t.device().is_cuda(), who, ": ", name, " must be a CUDA tensor, got ", t.device());
+}
+void CheckDevice(const Tensor& t, const Tensor& like, const char* who, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == like.device(), who, ": ", name, " must be on ", like.device(),
+                    ", got ", t.device());
+}
+
+void* Ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const Tensor& Given(const OptTensor& t) {
+  static const Tensor none;
+  return t.has_value() && t->defined() ? *t : none;
+}
+void* Stream(const Tensor& t) {
+  return static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
+}
+
+// A gradient of a gradient is not computed: say so instead of returning a
+// result that autograd would take for a constant.
+void NoSecondOrder(const char* who) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), who,
+                              ": the gradient cannot be differentiated again (create_graph=True)");
+}
+
+// ------------------------------------------------------------ distillation
+// Rows of logits as they are when their elements are contiguous and the rows
+// do not overlap (a slice of padded logits is read in place).
+Tensor Rows2d(const Tensor& t) {
+  const bool in_place = (t.size(1) <= 1 || t.stride(1) == 1) &&
+                        (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  return in_place ? t : t.contiguous();
+}
+int64_t RowStride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// The gradient in the logits' own layout, their padding and their offset from
+// a 16-byte boundary included, so that its rows are written in the vectors
+// that the logits' are read in.
+Tensor GradLike(const Tensor& z) {
+  const int64_t ld = RowStride(z), rows = z.size(0), cols = z.size(1);
+  if (rows == 0 || ld > 2 * cols) return at::empty({rows, cols}, z.options());
+  const int64_t item = z.element_size();
+  const int64_t shift = static_cast<int64_t>(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / item;
+  const int64_t used = (rows - 1) * ld + cols;
+  return at::empty({used + shift}, z.options()).as_strided({rows, cols}, {ld, 1}, shift);
+}
+
+struct DistillInputs {
+  Tensor student, values, indices, lse;
+  muon_train_distill_args args{};
+};
+
+DistillInputs CheckDistill(const Tensor& student, const Tensor& values, const Tensor& indices,
+                           const OptTensor& teacher_lse, double temperature, const char* who) {
+  CheckCuda(student, who, "student_logits");
+  TORCH_CHECK_VALUE(student.dim() == 2 && values.dim() == 2 && student.size(1) > 0,
+                    who, ": student_logits must have shape [rows, vocab] and teacher_logits [rows, top]");
+  TORCH_CHECK_VALUE(values.size(0) == student.size(0) && indices.sizes() == values.sizes(), who,
+                    ": teacher_logits and teacher_indices must have one list for each row");
+  TORCH_CHECK_VALUE(values.size(1) >= 1 && values.size(1) <= MUON_TRAIN_MAX_TOP, who,
+                    ": a list must have 1 to ", MUON_TRAIN_MAX_TOP, " entries, got ", values.size(1));
+  CheckDevice(values, student, who, "teacher_logits");
+  CheckDevice(indices, student, who, "teacher_indices");
+  TORCH_CHECK_TYPE(indices.scalar_type() == at::kLong || indices.scalar_type() == at::kInt, who,
+                   ": teacher_indices must be int64 or int32, got ", indices.scalar_type());
+  TORCH_CHECK_VALUE(static_cast<float>(temperature) > 0.f && std::isfinite(static_cast<float>(temperature)), who,
+                    ": temperature must be positive and finite, got ", temperature);
+  DistillInputs in;
+  const Tensor& lse = Given(teacher_lse);
+  if (lse.defined()) {
+    CheckDevice(lse, student, who, "teacher_lse");
+    TORCH_CHECK_VALUE(lse.dim() == 1 && lse.size(0) == student.size(0), who,
+                      ": teacher_lse must have one value for each row");
+    TORCH_CHECK_TYPE(lse.is_floating_point(), who, ": teacher_lse must be a floating tensor");
+    in.lse = lse.to(at::kFloat).contiguous();
+  }
+  in.args.dtype = Dtype(student, who, "student_logits");
+  in.args.teacher_dtype = Dtype(values, who, "teacher_logits");
+  in.student = Rows2d(student);
+  in.values = values.contiguous();
+  in.indices = indices.contiguous();
+  in.args.logits = Ptr(in.student);
+  in.args.rows = student.size(0);
+  in.args.vocab = student.size(1);
+  in.args.ld = RowStride(in.student);
+  in.args.teacher_logits = Ptr(in.values);
+  in.args.teacher_indices = Ptr(in.indices);
+  in.args.teacher_lse = static_cast<const float*>(Ptr(in.lse));
+  in.args.top = values.size(1);
+  in.args.temperature = static_cast<float>(temperature);
+  in.args.index_bytes = indices.scalar_type() == at::kLong ? 8 : 4;
+  return in;
+}
+
+std::tuple<Tensor, Tensor> DistillCuda(const Tensor& student, const Tensor& values,
+                                       const Tensor& indices, const OptTensor& teacher_lse,
+                                       double temperature) {
+  const char* who = "distill_topk";
+  DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
+  const c10::cuda::CUDAGuard guard(student.device());
+  const auto f32 = student.options().dtype(at::kFloat);
+  Tensor loss = at::empty({student.size(0)}, f32), stats = at::empty({student.size(0), 2}, f32);
+  in.args.loss = static_cast<float*>(Ptr(loss));
+  in.args.stats = static_cast<float*>(Ptr(stats));
+  CheckStatus(muon_train_distill_sm100(&in.args, Stream(student)), who);
+  return {loss, stats};
+}
+
+Tensor DistillBackwardCuda(const Tensor& grad_loss, const Tensor& student, const Tensor& values,
+                           const Tensor& indices, const OptTensor& teacher_lse, const Tensor& stats,
+                           double temperature) {
+  const char* who = "distill_topk_backward";
+  DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
+  TORCH_CHECK_VALUE(grad_loss.dim() == 1 && grad_loss.size(0) == student.size(0) &&
+                        stats.dim() == 2 && stats.size(0) == student.size(0) && stats.size(1) == 2,
+                    who, ": grad_loss and stats must have a row for each row of student_logits");
+  CheckDevice(grad_loss, student, who, "grad_loss");
+  CheckDevice(stats, student, who, "stats");
+  TORCH_CHECK_TYPE(stats.scalar_type() == at::kFloat, who, ": stats must be float32");
+  const c10::cuda::CUDAGuard guard(student.device());
+  const Tensor scale = grad_loss.to(at::kFloat).contiguous(), kept = stats.contiguous();
+  Tensor grad = GradLike(in.student);
+  in.args.row_scale = static_cast<const float*>(Ptr(scale));
+  in.args.stats = static_cast<float*>(Ptr(kept));
+  in.args.grad = Ptr(grad);
+  in.args.ld_grad = RowStride(grad);
+  CheckStatus(muon_train_distill_backward_sm100(&in.args, Stream(student)), who);
+  return grad;
+}
+
+std::tuple<Tensor, Tensor> DistillGradCuda(const Tensor& student, const Tensor& values,
+                                           const Tensor& indices, const OptTensor& row_scale,
+                                           const OptTensor& teacher_lse, double temperature) {
+  const char* who = "distill_topk_grad";
+  DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
+  const c10::cuda::CUDAGuard guard(student.device());
+  Tensor scale;
+  if (Given(row_scale).defined()) {
+    CheckDevice(*row_scale, student, who, "row_scale");
+    TORCH_CHECK_VALUE(row_scale->dim() == 1 && row_scale->size(0) == student.size(0), who,
+                      ": row_scale must have one value for each row");
+    TORCH_CHECK_TYPE(row_scale->is_floating_point(), who, ": row_scale must be a floating tensor");
+    scale = row_scale->to(at::kFloat).contiguous();
+  }
+  Tensor loss = at::empty({student.size(0)}, student.options().dtype(at::kFloat));
+  Tensor grad = GradLike(in.student);
+  in.args.row_scale = static_cast<const float*>(Ptr(scale));
+  in.args.loss = static_cast<float*>(Ptr(loss));
+  in.args.grad = Ptr(grad);
+  in.args.ld_grad = RowStride(grad);
+  CheckStatus(muon_train_distill_sm100(&in.args, Stream(student)), who);
+  return {loss, grad};
+}
+
+// ------------------------------------------------------------ residual norm
+struct NormInputs {
+  Tensor block_out, residual, post, pre, gate, scale;
+  muon_train_norm_args args{};
+};
+
+NormInputs CheckNorm(const Tensor& block_out, const Tensor& residual, const OptTensor& post,
+                     const OptTensor& pre, const OptTensor& gate, const OptTensor& scale,
+                     double eps, const char* who) {
+  CheckCuda(block_out, who, "block_out");
+  CheckDevice(residual, block_out, who, "residual");
+  TORCH_CHECK_VALUE(block_out.dim() == 2 && block_out.size(1) > 0, who,
+                    ": block_out must have shape [rows, width]");
+  TORCH_CHECK_VALUE(residual.sizes() == block_out.sizes(), who,
+                    ": residual must have block_out's shape");
+  TORCH_CHECK_TYPE(residual.scalar_type() == block_out.scalar_type(), who,
+                   ": residual must have block_out's dtype");
+  TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), who, ": eps must be finite and not negative, got ", eps);
+  const int64_t rows = block_out.size(0), width = block_out.size(1);
+  NormInputs in;
+  auto& a = in.args;
+  const auto weight = [&](const OptTensor& w, const char* name, Tensor* to, int* dtype) {
+    const Tensor& t = Given(w);
+    if (!t.defined()) return;
+    CheckDevice(t, block_out, who, name);
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == width, who, ": ", name, " must have shape [width]");
+    *dtype = Dtype(t, who, name);
+    *to = t.contiguous();
+  };
+  a.dtype = Dtype(block_out, who, "block_out");
+  weight(post, "post_weight", &in.post, &a.post_dtype);
+  weight(pre, "pre_weight", &in.pre, &a.pre_dtype);
+  if (Given(gate).defined()) {
+    CheckDevice(*gate, block_out, who, "gate");
+    TORCH_CHECK_VALUE(gate->dim() == 2 && gate->size(1) == width && (rows == 0 || (gate->size(0) > 0 && rows % gate->size(0) == 0)),
+                      who, ": gate must have shape [gate_rows, width], gate_rows dividing the rows");
+    a.gate_dtype = Dtype(*gate, who, "gate");
+    in.gate = gate->contiguous();
+    a.gate_rows = gate->size(0);
+  }
+  if (Given(scale).defined()) {
+    CheckDevice(*scale, block_out, who, "residual_scale");
+    TORCH_CHECK_VALUE(scale->dim() == 1 && (scale->size(0) == 1 || scale->size(0) == width), who,
+                      ": residual_scale must have one element or shape [width]");
+    a.scale_dtype = Dtype(*scale, who, "residual_scale");
+    in.scale = scale->contiguous();
+    a.scale_count = scale->size(0);
+  }
+  in.block_out = block_out.contiguous();
+  in.residual = residual.contiguous();
+  a.block_out = Ptr(in.block_out);
+  a.residual = Ptr(in.residual);
+  a.post_weight = Ptr(in.post);
+  a.pre_weight = Ptr(in.pre);
+  a.gate = Ptr(in.gate);
+  a.residual_scale = Ptr(in.scale);
+  a.rows = rows;
+  a.width = width;
+  a.eps = static_cast<float>(eps);
+  return in;
+}
+
+// (hidden, normed, rstd_post, rstd_pre); what is not computed is empty.
+std::tuple<Tensor, Tensor, Tensor, Tensor> ResidualNormCuda(
+    const Tensor& block_out, const Tensor& residual, const OptTensor& post, const OptTensor& pre,
+    const OptTensor& gate, const OptTensor& scale, double eps) {
+  const char* who = "residual_norm";
+  NormInputs in = CheckNorm(block_out, residual, post, pre, gate, scale, eps, who);
+  const c10::cuda::CUDAGuard guard(block_out.device());
+  const auto options = in.block_out.options();
+  const auto f32 = options.dtype(at::kFloat);
+  const int64_t rows = in.args.rows;
+  Tensor hidden = at::empty({rows, in.args.width}, options);
+  Tensor normed = at::empty({in.pre.defined() ? rows : 0, in.args.width}, options);
+  Tensor rstd_post = at::empty({in.post.defined() ? rows : 0}, f32);
+  Tensor rstd_pre = at::empty({in.pre.defined() ? rows : 0}, f32);
+  in.args.hidden = Ptr(hidden);
+  in.args.normed = Ptr(normed);
+  in.args.rstd_post = static_cast<float*>(Ptr(rstd_post));
+  in.args.rstd_pre = static_cast<float*>(Ptr(rstd_pre));
+  CheckStatus(muon_train_residual_norm_sm100(&in.args, Stream(block_out)), who);
+  return {hidden, normed, rstd_post, rstd_pre};
+}
+
+// Gradients of (block_out, residual, post_weight, pre_weight, gate,
+// residual_scale); those not asked for by `wanted` are empty.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> ResidualNormBackwardCuda(
+    const OptTensor& grad_hidden, const OptTensor& grad_normed, const Tensor& block_out,
+    const Tensor& residual, const OptTensor& post, const OptTensor& pre, const OptTensor& gate,
+    const OptTensor& scale, const Tensor& rstd_post, const Tensor& rstd_pre, double eps,
+    std::array<bool, 6> wanted) {
+  const char* who = "residual_norm_backward";
+  NormInputs in = CheckNorm(block_out, residual, post, pre, gate, scale, eps, who);
+  const c10::cuda::CUDAGuard guard(block_out.device());
+  const int64_t rows = in.args.rows;
+  const auto upstream = [&](const OptTensor& g, const char* name) -> Tensor {
+    if (!Given(g).defined()) return Tensor();
+    CheckDevice(*g, block_out, who, name);
+    TORCH_CHECK_VALUE(g->sizes() == block_out.sizes(), who, ": ", name, " must have block_out's shape");
+    TORCH_CHECK_TYPE(g->scalar_type() == block_out.scalar_type(), who, ": ", name,
+                     " must have block_out's dtype");
+    return g->contiguous();
+  };
+  const Tensor dh = upstream(grad_hidden, "grad_hidden"), dn = upstream(grad_normed, "grad_normed");
+  const auto rstd = [&](const Tensor& t, bool needed, const char* name) -> Tensor {
+    if (!needed) return Tensor();
+    CheckDevice(t, block_out, who, name);
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, who, ": ", name, " must be float32");
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == rows, who, ": ", name, " must have one value for each row");
+    return t.contiguous();
+  };
+  const Tensor rp = rstd(rstd_post, in.post.defined(), "rstd_post");
+  const Tensor rn = rstd(rstd_pre, in.pre.defined(), "rstd_pre");
+  in.args.rstd_post = static_cast<float*>(Ptr(rp));
+  in.args.rstd_pre = static_cast<float*>(Ptr(rn));
+  const Tensor* like[6] = {&in.block_out, &in.residual, &in.post, &in.pre, &in.gate, &in.scale};
+  std::array<Tensor, 6> out;
+  const bool none = rows == 0 || (!dh.defined() && !dn.defined());
+  for (int i = 0; i < 6; ++i) {
+    if (!wanted[i] || !like[i]->defined())
+      out[i] = at::empty({0}, in.block_out.options());
+    else
+      out[i] = none ? at::zeros_like(*like[i]) : at::empty_like(*like[i]);
+  }
+  const auto result = [&] { return std::make_tuple(out[0], out[1], out[2], out[3], out[4], out[5]); };
+  if (none) return result();
+  muon_train_norm_grads g{};
+  g.grad_hidden = Ptr(dh);
+  g.grad_normed = Ptr(dn);
+  void** to[6] = {&g.grad_block_out, &g.grad_residual, &g.grad_post_weight,
+                  &g.grad_pre_weight, &g.grad_gate, &g.grad_residual_scale};
+  for (int i = 0; i < 6; ++i) *to[i] = wanted[i] && like[i]->defined() ? Ptr(out[i]) : nullptr;
+  g.workspace_bytes = muon_train_residual_norm_workspace_bytes(&in.args);
+  const Tensor workspace = at::empty({static_cast<int64_t>(g.workspace_bytes)},
+                                     in.block_out.options().dtype(at::kByte));
+  g.workspace = Ptr(workspace);
+  CheckStatus(muon_train_residual_norm_backward_sm100(&in.args, &g, Stream(block_out)), who);
+  return result();
+}
+
+// ------------------------------------------------------------ routing
+muon_train_route_args CheckRoute(const Tensor& logits, int64_t k, int64_t score, int64_t groups,
+                                 int64_t top_groups, int64_t group_top, bool renormalize,
+                                 double scale, Tensor* rows, const char* who) {
+  CheckCuda(logits, who, "logits");
+  TORCH_CHECK_VALUE(logits.dim() == 2, who, ": logits must have shape [tokens, experts]");
+  const int64_t experts = logits.size(1);
+  TORCH_CHECK_VALUE(experts >= 1 && experts <= MUON_TRAIN_MAX_EXPERTS, who, ": 1 to ",
+                    MUON_TRAIN_MAX_EXPERTS, " experts are supported, got ", experts);
+  TORCH_CHECK_VALUE(score == 0 || score == 1, who, ": score must be 0 (softmax) or 1 (sigmoid)");
+  TORCH_CHECK_VALUE(groups >= 1 && experts % groups == 0, who,
+                    ": groups must divide the experts, got ", groups, " and ", experts);
+  TORCH_CHECK_VALUE(top_groups >= 1 && top_groups <= groups, who,
+                    ": top_groups must be 1 to groups, got ", top_groups);
+  TORCH_CHECK_VALUE(group_top == 1 || (group_top == 2 && (groups == 1 || experts / groups >= 2)), who,
+                    ": group_top must be 1, or 2 with groups of two experts or more");
+  TORCH_CHECK_VALUE(k >= 1 && k <= MUON_TRAIN_MAX_ROUTES && k <= top_groups * (experts / groups),
+                    who, ": k must be 1 to ", MUON_TRAIN_MAX_ROUTES,
+                    " and at most the experts of the chosen groups, got ", k);
+  TORCH_CHECK_VALUE(std::isfinite(scale), who, ": scale must be finite, got ", scale);
+  *rows = Rows2d(logits);
+  muon_train_route_args a{};
+  a.logits = Ptr(*rows);
+  a.tokens = logits.size(0);
+  a.experts = experts;
+  a.ld = RowStride(*rows);
+  a.dtype = Dtype(logits, who, "logits");
+  a.score = static_cast<int>(score);
+  a.k = static_cast<int>(k);
+  a.groups = static_cast<int>(groups);
+  a.top_groups = static_cast<int>(top_groups);
+  a.group_top = static_cast<int>(group_top);
+  a.renormalize = renormalize ? 1 : 0;
+  a.scale = static_cast<float>(scale);
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> RouteCuda(const Tensor& logits, const OptTensor& bias, int64_t k,
+                                             int64_t score, int64_t groups, int64_t top_groups,
+                                             int64_t group_top, bool renormalize, double scale) {
+  const char* who = "route_experts";
+  Tensor rows, b;
+  muon_train_route_args a =
+      CheckRoute(logits, k, score, groups, top_groups, group_top, renormalize, scale, &rows, who);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  if (Given(bias).defined()) {
+    CheckDevice(*bias, logits, who, "bias");
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == a.experts, who,
+                      ": bias must have shape [experts]");
+    TORCH_CHECK_TYPE(bias->is_floating_point(), who, ": bias must be a floating tensor");
+    b = bias->to(at::kFloat).contiguous();
+    a.bias = static_cast<const float*>(Ptr(b));
+  }
+  const auto i64 = logits.options().dtype(at::kLong);
+  Tensor weights = at::empty({a.tokens, k}, logits.options().dtype(at::kFloat));
+  Tensor indices = at::empty({a.tokens, k}, i64), counts = at::empty({a.experts}, i64);
+  a.weights = static_cast<float*>(Ptr(weights));
+  a.indices = static_cast<int64_t*>(Ptr(indices));
+  a.counts = static_cast<int64_t*>(Ptr(counts));
+  CheckStatus(muon_train_route_sm100(&a, Stream(logits)), who);
+  return {weights, indices, counts};
+}
+
+Tensor RouteBackwardCuda(const Tensor& grad_weights, const Tensor& logits, const Tensor& indices,
+                         int64_t score, bool renormalize, double scale) {
+  const char* who = "route_experts_backward";
+  TORCH_CHECK_VALUE(indices.dim() == 2 && logits.dim() == 2 && indices.size(0) == logits.size(0) &&
+                        grad_weights.sizes() == indices.sizes(),
+                    who, ": indices and grad_weights must have shape [tokens, k]");
+  TORCH_CHECK_TYPE(indices.scalar_type() == at::kLong, who, ": indices must be int64");
+  Tensor rows;
+  muon_train_route_args a = CheckRoute(logits, indices.size(1), score, 1, 1, 1, renormalize, scale, &rows, who);
+  CheckDevice(grad_weights, logits, who, "grad_weights");
+  CheckDevice(indices, logits, who, "indices");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Tensor g = grad_weights.to(at::kFloat).contiguous(), chosen = indices.contiguous();
+  a.indices = static_cast<int64_t*>(Ptr(chosen));
+  Tensor grad = at::empty({a.tokens, a.experts}, logits.options());
+  CheckStatus(muon_train_route_backward_sm100(&a, static_cast<const float*>(Ptr(g)), Ptr(grad),
+                                              Stream(logits)), who);
+  return grad;
+}
+
+// ------------------------------------------------------------ autograd
+template <typename Fn>
+auto Op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
+}
+
+// Whether autograd records a call: otherwise it goes to the kernels directly.
+bool Recorded(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+class DistillFunction : public torch::autograd::Function<DistillFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& student, const Tensor& values,
+                               const Tensor& indices, const OptTensor& lse, double temperature) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = Op<decltype(DistillCuda)>("muon_ascend950::distill_topk");
+    auto [loss, stats] = op.call(student, values, indices, lse, temperature);
+    ctx->save_for_backward({student, values, indices, Given(lse), stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->mark_non_differentiable({stats});
+    return {loss, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    NoSecondOrder("distill_topk");
+    const auto saved = ctx->get_saved_variables();
+    Tensor grad;
+    if (grads[0].defined()) {
+      static auto op = Op<decltype(DistillBackwardCuda)>("muon_ascend950::distill_topk_backward");
+      const OptTensor lse = saved[3].defined() ? OptTensor(saved[3]) : OptTensor();
+      grad = op.call(grads[0], saved[0], saved[1], saved[2], lse, saved[4],
+                     ctx->saved_data["temperature"].toDouble());
+    }
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> DistillAutograd(const Tensor& student, const Tensor& values,
+                                           const Tensor& indices, const OptTensor& lse,
+                                           double temperature) {
+  if (!Recorded({&student})) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = Op<decltype(DistillCuda)>("muon_ascend950::distill_topk");
+    return op.call(student, values, indices, lse, temperature);
+  }
+  auto out = DistillFunction::apply(student, values, indices, lse, temperature);
+  return {out[0], out[1]};
+}
+
+class ResidualNormFunction : public torch::autograd::Function<ResidualNormFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& block_out, const Tensor& residual,
+                               const OptTensor& post, const OptTensor& pre, const OptTensor& gate,
+                               const OptTensor& scale, double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = Op<decltype(ResidualNormCuda)>("muon_ascend950::residual_norm");
+    auto [hidden, normed, rstd_post, rstd_pre] = op.call(block_out, residual, post, pre, gate, scale, eps);
+    ctx->save_for_backward({block_out, residual, Given(post), Given(pre), Given(gate), Given(scale),
+                            rstd_post, rstd_pre});
+    ctx->saved_data["eps"] = eps;
+    const Tensor* inputs[6] = {&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)};
+    int64_t wanted = 0;  // a bit for each input that takes a gradient
+    for (int i = 0; i < 6; ++i)
+      if (inputs[i]->defined() && inputs[i]->requires_grad()) wanted |= int64_t{1} << i;
+    ctx->saved_data["wanted"] = wanted;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({rstd_post, rstd_pre});
+    return {hidden, normed, rstd_post, rstd_pre};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    NoSecondOrder("residual_norm");
+    const auto s = ctx->get_saved_variables();
+    const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const int64_t bits = ctx->saved_data["wanted"].toInt();
+    std::array<bool, 6> wanted;
+    for (size_t i = 0; i < 6; ++i) wanted[i] = (bits >> i) & 1;
+    static auto op = Op<decltype(ResidualNormBackwardCuda)>("muon_ascend950::residual_norm_backward");
+    const OptTensor dn = s[3].defined() ? opt(grads[1]) : OptTensor();
+    auto [d0, d1, d2, d3, d4, d5] = op.call(opt(grads[0]), dn, s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]),
+                                            opt(s[5]), s[6], s[7], ctx->saved_data["eps"].toDouble(), wanted);
+    const Tensor all[6] = {d0, d1, d2, d3, d4, d5};
+    variable_list out(7);
+    for (size_t i = 0; i < 6; ++i)
+      if (wanted[i]) out[i] = all[i];
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> ResidualNormAutograd(
+    const Tensor& block_out, const Tensor& residual, const OptTensor& post, const OptTensor& pre,
+    const OptTensor& gate, const OptTensor& scale, double eps) {
+  if (!Recorded({&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)})) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = Op<decltype(ResidualNormCuda)>("muon_ascend950::residual_norm");
+    return op.call(block_out, residual, post, pre, gate, scale, eps);
+  }
+  auto out = ResidualNormFunction::apply(block_out, residual, post, pre, gate, scale, eps);
+  return {out[0], out[1], out[2], out[3]};
+}
+
+class RouteFunction : public torch::autograd::Function<RouteFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& bias,
+                               int64_t k, int64_t score, int64_t groups, int64_t top_groups,
+                               int64_t group_top, bool renormalize, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = Op<decltype(RouteCuda)>("muon_ascend950::route_experts");
+    auto [weights, indices, counts] =
+        op.call(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
+    ctx->save_for_backward({logits, indices});
+    ctx->saved_data["score"] = score;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({indices, counts});
+    return {weights, indices, counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    NoSecondOrder("route_experts");
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(9);
+    if (grads[0].defined()) {
+      static auto op = Op<decltype(RouteBackwardCuda)>("muon_ascend950::route_experts_backward");
+      out[0] = op.call(grads[0], saved[0], saved[1], ctx->saved_data["score"].toInt(),
+                       ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
+    }
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> RouteAutograd(const Tensor& logits, const OptTensor& bias, int64_t k,
+                                                 int64_t score, int64_t groups, int64_t top_groups,
+                                                 int64_t group_top, bool renormalize, double scale) {
+  if (!Recorded({&logits})) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = Op<decltype(RouteCuda)>("muon_ascend950::route_experts");
+    return op.call(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
+  }
+  auto out = RouteFunction::apply(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
+  return {out[0], out[1], out[2]};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
+  m.def("distill_topk(Tensor student_logits, Tensor teacher_logits, Tensor teacher_indices, "
+        "Tensor? teacher_lse, float temperature) -> (Tensor loss, Tensor stats)");
+  m.def("distill_topk_backward(Tensor grad_loss, Tensor student_logits, Tensor teacher_logits, "
+        "Tensor teacher_indices, Tensor? teacher_lse, Tensor stats, float temperature) -> Tensor");
+  m.def("distill_topk_grad(Tensor student_logits, Tensor teacher_logits, Tensor teacher_indices, "
+        "Tensor? row_scale, Tensor? teacher_lse, float temperature) -> (Tensor loss, Tensor grad)");
+  m.def("residual_norm(Tensor block_out, Tensor residual, Tensor? post_weight, Tensor? pre_weight, "
+        "Tensor? gate, Tensor? residual_scale, float eps) -> (Tensor hidden, Tensor normed, "
+        "Tensor rstd_post, Tensor rstd_pre)");
+  m.def("residual_norm_backward(Tensor? grad_hidden, Tensor? grad_normed, Tensor block_out, "
+        "Tensor residual, Tensor? post_weight, Tensor? pre_weight, Tensor? gate, "
+        "Tensor? residual_scale, Tensor rstd_post, Tensor rstd_pre, float eps, bool[6] wanted) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("route_experts(Tensor logits, Tensor? bias, int k, int score, int groups, int top_groups, "
+        "int group_top, bool renormalize, float scale) -> (Tensor weights, Tensor indices, Tensor counts)");
+  m.def("route_experts_backward(Tensor grad_weights, Tensor logits, Tensor indices, int score, "
+        "bool renormalize, float scale) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(muon_ascend950, CUDA, m) {
+  m.impl("distill_topk", &DistillCuda);
+  m.impl("distill_topk_backward", &DistillBackwardCuda);
+  m.impl("distill_topk_grad", &DistillGradCuda);
+  m.impl("residual_norm", &ResidualNormCuda);
+  m.impl("residual_norm_backward", &ResidualNormBackwardCuda);
+  m.impl("route_experts", &RouteCuda);
+  m.impl("route_experts_backward", &RouteBackwardCuda);
+}
+
+TORCH_LIBRARY_IMPL(muon_ascend950, Autograd, m) {
+  m.impl("distill_topk", &DistillAutograd);
+  m.impl("residual_norm", &ResidualNormAutograd);
+  m.impl("route_experts", &RouteAutograd);
+}

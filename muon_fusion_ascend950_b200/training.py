@@ -1,0 +1,227 @@
+"""Operators of the training step around the Muon update, on the B200 kernels.
+
+``Muon`` updates the matrices of a language model; these are the parts of the
+step beside them that are bound by memory, each with its gradient:
+
+* ``distill_topk`` / ``distill_topk_grad`` -- the distillation loss over a
+  teacher's top logits, and the loss with its gradient in one call;
+* ``residual_norm`` -- the norms before and after a residual block, fused with
+  its gate and residual scale;
+* ``route_experts`` -- the routing of tokens to the experts whose batched
+  matrices ``Muon`` updates.
+
+They are the operators ``torch.ops.muon_ascend950.*`` of the same names with
+the arguments' shapes and types checked here, run on the current stream, and
+take part in autograd (gradients of gradients are refused).
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _check(name: str, t, floats: bool = True) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
+    if floats and t.dtype not in _FLOATS:
+        raise TypeError(f"{name} must use torch.float32, bfloat16 or float16, got {t.dtype}")
+
+
+def _distill_args(student_logits, teacher_logits, teacher_indices, rows, rows_name):
+    _check("student_logits", student_logits)
+    _check("teacher_logits", teacher_logits)
+    _check("teacher_indices", teacher_indices, floats=False)
+    if teacher_indices.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"teacher_indices must use torch.int64 or int32, got {teacher_indices.dtype}")
+    if student_logits.ndim < 1 or student_logits.shape[-1] < 1:
+        raise ValueError(f"student_logits must have shape [..., vocab], got {tuple(student_logits.shape)}")
+    lead = student_logits.shape[:-1]
+    if teacher_logits.shape != teacher_indices.shape or teacher_logits.ndim < 1 or (
+            teacher_logits.shape[:-1] != lead):
+        raise ValueError("teacher_logits and teacher_indices must both have shape "
+                         f"{tuple(lead) + ('top',)}, got {tuple(teacher_logits.shape)} and "
+                         f"{tuple(teacher_indices.shape)}")
+    for name, t in zip(rows_name, rows):
+        if t is not None:
+            _check(name, t)
+            if t.shape != lead:
+                raise ValueError(f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+    if student_logits.ndim == 2:
+        return (student_logits, teacher_logits, teacher_indices, *rows)
+    top = teacher_logits.shape[-1]
+    count = lead.numel()
+    return (student_logits.reshape(count, student_logits.shape[-1]),
+            teacher_logits.reshape(count, top), teacher_indices.reshape(count, top),
+            *(t if t is None else t.reshape(count) for t in rows))
+
+
+def distill_topk(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
+                 teacher_indices: torch.Tensor, *, temperature: float = 1.0,
+                 teacher_lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Kullback-Leibler divergence of the student from the teacher's top
+    logits, one fp32 value for each row.
+
+    ``student_logits``: ``[..., vocab]``; ``teacher_logits`` and
+    ``teacher_indices`` (int64 or int32): ``[..., top]``, up to 1024 entries of
+    the same rows.  With ``tau = temperature`` the teacher's probabilities are
+    the softmax of ``teacher_logits / tau`` over the row's entries, or, with
+    ``teacher_lse`` (``[...]``: the log-sum-exp of the teacher's whole
+    vocabulary at ``tau``), ``exp(teacher_logits / tau - teacher_lse)``, whose
+    sum stays below one.  The loss is ``sum q (log q - log p)`` with ``p`` the
+    softmax of ``student_logits / tau`` over the vocabulary.
+
+    An entry whose index is outside the vocabulary (-1 pads a short list) or
+    whose logit is -inf is left out; a row without entries has loss 0 and
+    gradient 0.  Differentiable in ``student_logits``; the teacher's tensors
+    are constants.
+    """
+    s, t, i, lse = _distill_args(student_logits, teacher_logits, teacher_indices, (teacher_lse,),
+                                 ("teacher_lse",))
+    loss = torch.ops.muon_ascend950.distill_topk(s, t, i, lse, float(temperature))[0]
+    return loss if student_logits.ndim == 2 else loss.reshape(student_logits.shape[:-1])
+
+
+def distill_topk_grad(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
+                      teacher_indices: torch.Tensor, row_scale: Optional[torch.Tensor] = None, *,
+                      temperature: float = 1.0, teacher_lse: Optional[torch.Tensor] = None
+                      ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``distill_topk`` and the gradient of ``sum(row_scale * loss)`` in
+    ``student_logits``, from one reading of the logits.
+
+    ``row_scale`` (``[...]``, default 1) is what the rows weigh in the total,
+    e.g. one over the number of tokens, or 0 for tokens that do not count.
+    Returns ``(loss, grad)``, the gradient with the logits' shape and type; use
+    it as ``student_logits.backward(grad)``.  Not recorded by autograd.
+    """
+    with torch.no_grad():
+        s, t, i, scale, lse = _distill_args(student_logits, teacher_logits, teacher_indices,
+                                            (row_scale, teacher_lse), ("row_scale", "teacher_lse"))
+        loss, grad = torch.ops.muon_ascend950.distill_topk_grad(s, t, i, scale, lse, float(temperature))
+        if student_logits.ndim == 2:
+            return loss, grad
+        return loss.reshape(student_logits.shape[:-1]), grad.reshape(student_logits.shape)
+
+
+def _gate_rows(gate: torch.Tensor, shape: torch.Size) -> torch.Tensor:
+    """``gate`` as [gate_rows, width]: its leading sizes are ``shape``'s up to
+    some axis and 1 from there on, or it is one row."""
+    width = shape[-1]
+    if gate.ndim >= 1 and gate.shape[-1] == width:
+        lead = tuple(gate.shape[:-1])
+        if all(n == 1 for n in lead):
+            return gate.reshape(1, width)
+        if len(lead) == len(shape) - 1:
+            same = 0
+            while same < len(lead) and lead[same] == shape[same]:
+                same += 1
+            if all(n == 1 for n in lead[same:]):
+                return gate.reshape(lead and gate.shape[:-1].numel(), width)
+    raise ValueError(f"gate must have shape [{width}] or {tuple(shape)} with trailing leading sizes of 1, "
+                     f"got {tuple(gate.shape)}")
+
+
+def residual_norm(block_out: torch.Tensor, residual: torch.Tensor,
+                  post_weight: Optional[torch.Tensor] = None,
+                  pre_weight: Optional[torch.Tensor] = None, *,
+                  gate: Optional[torch.Tensor] = None,
+                  residual_scale: Optional[torch.Tensor] = None, eps: float = 1e-6
+                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The end of a residual block and the beginning of the next, in one pass:
+
+        hidden = residual_scale * residual + gate * rms_norm(block_out, post_weight)
+        normed = rms_norm(hidden, pre_weight)
+
+    ``block_out``, ``residual``: ``[..., width]`` of one type (fp32, bf16 or
+    fp16).  ``post_weight``, ``pre_weight``: ``[width]``; without
+    ``post_weight`` the block's output is not normed, without ``pre_weight``
+    ``normed`` is None.  ``gate``: ``[width]``, or the inputs' shape with 1 in
+    place of trailing leading sizes (``[batch, 1, width]``: one row for each
+    sequence).  ``residual_scale``: one element or ``[width]``.  Parameters may
+    be of any of the three types.
+
+    Statistics and sums are fp32, ``normed`` is computed from ``hidden`` before
+    it is rounded, and each output is rounded once.  Differentiable in all
+    tensor arguments; parameter gradients are summed in a fixed order.
+    """
+    _check("block_out", block_out)
+    _check("residual", residual)
+    if residual.dtype != block_out.dtype:
+        raise TypeError(f"residual must use block_out's {block_out.dtype}, got {residual.dtype}")
+    shape = block_out.shape
+    if block_out.ndim < 1 or shape[-1] < 1:
+        raise ValueError(f"block_out must have shape [..., width], got {tuple(shape)}")
+    if residual.shape != shape:
+        raise ValueError(f"residual must have block_out's shape {tuple(shape)}, got {tuple(residual.shape)}")
+    width = shape[-1]
+    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if w is not None:
+            _check(name, w)
+            if w.shape != (width,):
+                raise ValueError(f"{name} must have shape ({width},), got {tuple(w.shape)}")
+    if gate is not None:
+        _check("gate", gate)
+        gate = _gate_rows(gate, shape)
+    if residual_scale is not None:
+        _check("residual_scale", residual_scale)
+        if residual_scale.numel() == 1:
+            residual_scale = residual_scale.reshape(1)
+        elif residual_scale.shape != (width,):
+            raise ValueError(f"residual_scale must have one element or shape ({width},), "
+                             f"got {tuple(residual_scale.shape)}")
+    if block_out.ndim != 2:
+        rows = shape[:-1].numel()
+        block_out, residual = block_out.reshape(rows, width), residual.reshape(rows, width)
+    hidden, normed, _, _ = torch.ops.muon_ascend950.residual_norm(
+        block_out, residual, post_weight, pre_weight, gate, residual_scale, float(eps))
+    if len(shape) != 2:
+        hidden = hidden.reshape(shape)
+        normed = normed.reshape(shape) if pre_weight is not None else None
+    return hidden, normed if pre_weight is not None else None
+
+
+def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax",
+                  bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: int = 1,
+                  group_top: Optional[int] = None, renormalize: bool = True, scale: float = 1.0
+                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Choose ``k`` experts for each token.
+
+    ``logits``: ``[..., experts]``, up to 1024 experts.  The scores are the
+    softmax or the sigmoid of the logits.  ``bias`` (``[experts]``) is added to
+    the scores for the choice only; balancing the experts is moving it.  With
+    ``groups`` equal runs of experts, only the ``top_groups`` groups with the
+    largest sum of their ``group_top`` best biased scores take part
+    (``group_top``: 1 or 2, by default 1 for softmax and 2 for sigmoid).  The
+    ``k`` best are returned in descending order; equal ones go to the lowest
+    index.  Their weights are ``scale`` times their scores (without the bias),
+    divided by the sum of the chosen scores when ``renormalize``.
+
+    Returns ``(weights, indices, counts)``: fp32 and int64 ``[..., k]``, and
+    int64 ``[experts]``, how many tokens each expert got.  Differentiable in
+    ``logits`` through the weights.
+    """
+    _check("logits", logits)
+    if score not in _SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape [..., experts], got {tuple(logits.shape)}")
+    if bias is not None:
+        _check("bias", bias)
+        if bias.shape != (logits.shape[-1],):
+            raise ValueError(f"bias must have shape ({logits.shape[-1]},), got {tuple(bias.shape)}")
+    if group_top is None:
+        group_top = 2 if score == "sigmoid" and groups > 1 and logits.shape[-1] // groups > 1 else 1
+    shape = logits.shape
+    if len(shape) != 2:
+        logits = logits.reshape(shape[:-1].numel(), shape[-1])
+    weights, indices, counts = torch.ops.muon_ascend950.route_experts(
+        logits, bias, int(k), _SCORES[score], int(groups), int(top_groups), int(group_top),
+        bool(renormalize), float(scale))
+    if len(shape) != 2:
+        weights, indices = (t.reshape(shape[:-1] + (k,)) for t in (weights, indices))
+    return weights, indices, counts
