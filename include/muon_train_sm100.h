@@ -11,7 +11,6 @@
  *   - launches asynchronously on `stream` of the current device and returns
  *     0, a negative MUON_POLAR_ERR_* code (nothing was launched) or the
  *     cudaError_t of the launch.
- * Rows are independent: no entry point waits for another block or rank.
  * Sums, maxima and statistics are held in 32 bits or more, and each stored
  * value is rounded once.  All results are deterministic.
  */
@@ -40,6 +39,12 @@ extern "C" {
 
 /* Kernels launched by the entry points of this header. */
 uint64_t muon_train_launch_count(void);
+
+/* Device status word (zero: no trouble).  Every wait inside a kernel is
+ * bounded; a kernel that gives up a wait sets a bit here, runs on without
+ * waiting and returns, its results void.  Synchronises the device. */
+#define MUON_TRAIN_STATUS_WAIT 0x1u
+int muon_train_read_device_status(int device, uint32_t* flags, int clear);
 
 /* ---- distillation from a teacher's top logits ------------------------------
  * One row has student logits z[vocab] and a list of `top` teacher logits t
@@ -71,8 +76,9 @@ typedef struct {
   int index_bytes;             /* 4 or 8 */
 } muon_train_distill_args;
 
-/* loss, with stats (may be NULL) for a later backward call, and grad (may be
- * NULL): the loss and its gradient from one reading of the logits. */
+/* loss, with stats (may be NULL without grad) for a later backward call, and
+ * grad (may be NULL): the loss and its gradient from one reading of the
+ * logits (two for rows of more than about a million bytes). */
 int muon_train_distill_sm100(const muon_train_distill_args* args, void* stream);
 
 /* grad from the stats of an earlier call on the same inputs (loss unused). */

@@ -57,40 +57,51 @@ def load_library() -> None:
                          scale, coefficients):
         return None
 
+    # The fake kernels of the training-step operators check their arguments as
+    # the native ones do, so that a traced call is refused where a real one is.
     def fake_distill_topk(student, values, indices, lse, temperature):
-        rows = student.shape[0]
-        return (student.new_empty((rows,), dtype=torch.float32),
-                student.new_empty((rows, 2), dtype=torch.float32))
+        from .training import check_distill
+
+        check_distill(student, values, indices, temperature, teacher_lse=lse)
+        lead = student.shape[:-1]
+        return (student.new_empty(lead, dtype=torch.float32),
+                student.new_empty((lead.numel(), 2), dtype=torch.float32))
 
     def fake_distill_topk_backward(grad_loss, student, values, indices, lse, stats, temperature):
         return torch.empty_like(student)
 
     def fake_distill_topk_grad(student, values, indices, row_scale, lse, temperature):
-        return student.new_empty((student.shape[0],), dtype=torch.float32), torch.empty_like(student)
+        from .training import check_distill
+
+        check_distill(student, values, indices, temperature, row_scale=row_scale, teacher_lse=lse)
+        return student.new_empty(student.shape[:-1], dtype=torch.float32), torch.empty_like(student)
 
     def fake_residual_norm(block_out, residual, post, pre, gate, scale, eps):
-        rows, width = block_out.shape
-        f32 = torch.float32
-        return (block_out.new_empty((rows, width)),
-                block_out.new_empty((rows if pre is not None else 0, width)),
-                block_out.new_empty((rows if post is not None else 0,), dtype=f32),
-                block_out.new_empty((rows if pre is not None else 0,), dtype=f32))
+        from .training import check_norm
+
+        check_norm(block_out, residual, post, pre, gate, scale, eps)
+        rows = block_out.shape[:-1].numel()
+        return (block_out.new_empty(block_out.shape),
+                block_out.new_empty(block_out.shape if pre is not None else (0,)),
+                block_out.new_empty((2, rows), dtype=torch.float32))
 
     def fake_residual_norm_backward(grad_hidden, grad_normed, block_out, residual, post, pre, gate,
-                                    scale, rstd_post, rstd_pre, eps, wanted):
+                                    scale, rstd, eps, wanted):
         inputs = (block_out, residual, post, pre, gate, scale)
-        return tuple(torch.empty_like(t, memory_format=torch.contiguous_format)
-                     if want and t is not None else block_out.new_empty((0,))
+        return tuple(t.new_empty(t.shape) if want and t is not None else block_out.new_empty((0,))
                      for t, want in zip(inputs, wanted))
 
     def fake_route_experts(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale):
-        tokens, experts = logits.shape
-        return (logits.new_empty((tokens, k), dtype=torch.float32),
-                logits.new_empty((tokens, k), dtype=torch.int64),
-                logits.new_empty((experts,), dtype=torch.int64))
+        from .training import check_route
+
+        check_route(logits, bias, k, groups, top_groups)
+        shape = (*logits.shape[:-1], k)
+        return (logits.new_empty(shape, dtype=torch.float32),
+                logits.new_empty(shape, dtype=torch.int64),
+                logits.new_empty((logits.shape[-1],), dtype=torch.int64))
 
     def fake_route_experts_backward(grad_weights, logits, indices, score, renormalize, scale):
-        return torch.empty_like(logits, memory_format=torch.contiguous_format)
+        return logits.new_empty(logits.shape)
 
     # Extensions of this build: polar_step_t (the step of x^T in x's layout)
     # has polar_step's output contract; polar_express returns bf16 of x's

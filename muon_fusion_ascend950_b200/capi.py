@@ -138,6 +138,8 @@ _DISTILL, _NORM, _GRADS, _ROUTE = (ctypes.POINTER(t) for t in (DistillArgs, Norm
                                                                RouteArgs))
 TRAIN_SIGNATURES = {
     "muon_train_launch_count": (ctypes.c_uint64, []),
+    "muon_train_read_device_status": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_uint32),
+                                                     ctypes.c_int]),
     "muon_train_distill_sm100": (ctypes.c_int, [_DISTILL, _VP]),
     "muon_train_distill_backward_sm100": (ctypes.c_int, [_DISTILL, _VP]),
     "muon_train_residual_norm_sm100": (ctypes.c_int, [_NORM, _VP]),
@@ -213,6 +215,13 @@ class CAPI:
     def train_launch_count(self) -> int:
         """Kernels launched by the training-step operators so far."""
         return int(self.lib.muon_train_launch_count())
+
+    def train_device_status(self, device: int = 0, clear: bool = True) -> int:
+        """Status word of the training-step kernels (0: every wait ended)."""
+        flags = ctypes.c_uint32(0)
+        self._check("muon_train_read_device_status",
+                    self.lib.muon_train_read_device_status(int(device), ctypes.byref(flags), int(clear)))
+        return int(flags.value)
 
     def abi_version(self) -> int:
         return int(self.lib.muon_polar_abi_version())

@@ -8,6 +8,9 @@
 //
 // Bound by memory: the vocabulary is read once (and the gradient written
 // once); the lists are a thousandth of it.
+#include <algorithm>
+
+#include "sm100_ptx.cuh"
 #include "train_common.cuh"
 
 namespace muon_train {
@@ -19,27 +22,25 @@ std::atomic<uint64_t>& launch_counter() {
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-
 // A row's list in shared memory: index (-1: not counted), q, log q and the
 // student's logit.
 struct List {
-  int index[MUON_TRAIN_MAX_TOP];
-  float q[MUON_TRAIN_MAX_TOP];
-  float log_q[MUON_TRAIN_MAX_TOP];
-  float z[MUON_TRAIN_MAX_TOP];
+  int* index;
+  float *q, *log_q, *z;
+  static __host__ __device__ size_t bytes(int64_t top) { return static_cast<size_t>(top) * 16; }
+  __device__ List(void* at, int top)
+      : index(static_cast<int*>(at)), q(reinterpret_cast<float*>(index + top)), log_q(q + top), z(log_q + top) {}
 };
 
 template <typename T>
 __device__ __forceinline__ float logit(const T* row, int64_t i) { return to_float(row[i]); }
 
-// Fills the list (z only for the loss) and returns Q; one whole warp, each
+// Fills the list and returns Q; one whole warp, each
 // lane its own entries.  The differences to the largest entry are taken
 // before the division by tau, so that entries of the type's lowest value stay
 // finite.
 template <typename T>
-__device__ float load_list(const muon_train_distill_args& a, int64_t row, const T* z, List* list) {
+__device__ float load_list(const muon_train_distill_args& a, int64_t row, const T* z, const List& list) {
   const int lane = threadIdx.x & 31;
   const int top = static_cast<int>(a.top);
   const float inv_tau = 1.0f / a.temperature;
@@ -51,11 +52,11 @@ __device__ float load_list(const muon_train_distill_args& a, int64_t row, const 
                           : static_cast<const int32_t*>(a.teacher_indices)[base + j];
     const float t = load_any(a.teacher_logits, a.teacher_dtype, base + j);
     const bool counted = i >= 0 && i < a.vocab && t > -INFINITY;
-    list->index[j] = counted ? static_cast<int>(i) : -1;
-    list->log_q[j] = t;
+    list.index[j] = counted ? static_cast<int>(i) : -1;
+    list.log_q[j] = t;
     if (counted) {
       best = fmaxf(best, t);
-      if (a.loss != nullptr) list->z[j] = logit(z, i);
+      list.z[j] = logit(z, i);
     }
   }
   best = warp_max(best);
@@ -67,15 +68,15 @@ __device__ float load_list(const muon_train_distill_args& a, int64_t row, const 
     shift = best;
     float s = 0.f;
     for (int j = lane; j < top; j += 32)
-      if (list->index[j] >= 0) s += expf((list->log_q[j] - shift) * inv_tau);
+      if (list.index[j] >= 0) s += expf((list.log_q[j] - shift) * inv_tau);
     log_norm = logf(warp_sum(s));
   }
   float total = 0.f;
   for (int j = lane; j < top; j += 32) {
-    const float log_q = (list->log_q[j] - shift) * inv_tau - log_norm;
-    const float q = list->index[j] >= 0 ? expf(log_q) : 0.f;
-    list->log_q[j] = log_q;
-    list->q[j] = q;
+    const float log_q = (list.log_q[j] - shift) * inv_tau - log_norm;
+    const float q = list.index[j] >= 0 ? expf(log_q) : 0.f;
+    list.log_q[j] = log_q;
+    list.q[j] = q;
     total += q;
   }
   return warp_sum(total);
@@ -97,6 +98,7 @@ __device__ float row_loss(const List& list, int top, float inv_tau, float max, f
 // entries of one index all find the same value.
 __device__ __forceinline__ float q_of_index(const List& list, int top, int index) {
   float q = 0.f;
+#pragma unroll 8
   for (int l = 0; l < top; ++l)
     if (list.index[l] == index) q += list.q[l];
   return q;
@@ -117,67 +119,566 @@ __device__ __forceinline__ float2 warp_join(float2 v, float c) {
   return v;
 }
 
-// One block a row, any vocabulary: reads the row for its statistics (unless
-// `from_stats`), then, for the gradient, once more.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    distill_row_kernel(const __grid_constant__ muon_train_distill_args a, bool from_stats) {
-  __shared__ List list;
+// ------------------------------------------------------------ rows in registers
+// A row is held in registers by the threads of one block, or of a cluster of
+// up to 8, so that the loss and its gradient read it once.  It is cut into
+// granules of 16 bytes on 16-byte boundaries, whatever the row's own
+// alignment; a thread has kVectors of them, and the elements of the first and
+// last granule outside the row count as -inf.  A further warp loads the list
+// meanwhile and makes the loss.
+constexpr int kBlockThreads = 256;  // that hold granules, at most
+constexpr int kMaxCluster = 8;
+
+enum Mode { kLoss, kLossGrad, kGradFromStats };
+
+struct Cut {
+  int parts;       // blocks of a row
+  bool same_phase; // the gradient's rows begin as far off a 16-byte boundary as the logits'
+};
+
+// exp2((e - base) c) of two elements.
+__device__ __forceinline__ float2 exp2_of(float x, float y, float2 minus_base, float2 c) {
+  const float2 t = mul2(add2(make_float2(x, y), minus_base), c);
+  return make_float2(fast_exp2(t.x), fast_exp2(t.y));
+}
+
+template <typename T, int kVectors, Mode kMode>
+__global__ void __launch_bounds__(kBlockThreads + 32, 4)
+    distill_kernel(const __grid_constant__ muon_train_distill_args a, Cut cut) {
+  constexpr int kN = kVec<T>;
+  extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ float total_shared;
-  __shared__ float2 part[kWarps];
-  const int64_t row = blockIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + row * a.ld;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float2 warp_part[kBlockThreads / 32];
+  __shared__ float2 block_part[kMaxCluster];
+  const List list(dynamic, static_cast<int>(a.top));
+  const int64_t row = blockIdx.x / cut.parts;
+  const int part = static_cast<int>(blockIdx.x - row * cut.parts);
+  const int threads = blockDim.x - 32;  // that hold granules
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = threads >> 5;
+  const bool list_warp = warp == warps;
+  const int vocab = static_cast<int>(a.vocab);
   const float c = kLog2e / a.temperature;
-  if (warp == 0) {
-    const float total = load_list(a, row, z, &list);
+  const float2 cc = make_float2(c, c);
+  const T* z = static_cast<const T*>(a.logits) + row * a.ld;
+  if constexpr (kMode != kGradFromStats)
+    if (cut.parts > 1) muon_sm100::cluster_sync();  // every block has begun
+
+  // this block's granules of the row: [first, last)
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(z) & 15u) / static_cast<int>(sizeof(T));
+  const int granules = (vocab + shift + kN - 1) / kN;
+  const int each = (granules + cut.parts - 1) / cut.parts;
+  const int first = part * each, last = min(granules, first + each);
+  const int mine = first + static_cast<int>(threadIdx.x);
+  const auto inside = [&](int element) { return element >= 0 && element + kN <= vocab; };
+  uint4 raw[kVectors];
+  float max, sum;
+  if (list_warp) {
+    const float total = load_list(a, row, z, list);
     if (lane == 0) total_shared = total;
-  }
-  float2 v = make_float2(-INFINITY, 0.f);
-  if (!from_stats) {
-    for (int64_t i = threadIdx.x; i < a.vocab; i += kThreads) v = join(v, make_float2(logit(z, i), 1.f), c);
-    v = warp_join(v, c);
-    if (lane == 0) part[warp] = v;
-  }
-  __syncthreads();
-  if (from_stats) {
-    v = make_float2(a.stats[2 * row], a.stats[2 * row + 1]);
   } else {
-    v = part[0];
-    for (int w = 1; w < kWarps; ++w) v = join(v, part[w], c);
-  }
-  const float total = total_shared;
-  if (warp == 0 && a.loss != nullptr) {
-    const float loss = row_loss(list, static_cast<int>(a.top), 1.0f / a.temperature, v.x, v.y);
-    if (lane == 0) a.loss[row] = loss;
-  }
-  if (threadIdx.x == 0) {
-    if (a.stats != nullptr && !from_stats) {
-      a.stats[2 * row] = v.x;
-      a.stats[2 * row + 1] = v.y;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+      const int granule = mine + v * threads, element = granule * kN - shift;
+      if (granule < last && inside(element)) {
+        raw[v] = *reinterpret_cast<const uint4*>(z + element);
+      } else {
+        float e[kN];
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          e[j] = granule < last && element + j >= 0 && element + j < vocab ? logit(z, element + j) : -INFINITY;
+        raw[v] = pack<T>(e);
+      }
+    }
+    if constexpr (kMode != kGradFromStats) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) m = vector_max(raw[v], m, T());
+      m = warp_max(m);
+      const float base = m == -INFINITY ? 0.f : m;  // nothing finite: a sum of 0
+      float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) {
+        float e[kN];
+        unpack<T>(raw[v], e);
+#pragma unroll
+        for (int j = 0; j < kN; j += 2)
+          s = add2(s, exp2_of(e[j], e[j + 1], make_float2(-base, -base), cc));
+      }
+      const float all = warp_sum(s.x + s.y);
+      if (lane == 0) warp_part[warp] = make_float2(m, all);
     }
   }
-  if (a.grad == nullptr) return;
-  T* dz = static_cast<T*>(a.grad) + row * a.ld_grad;
-  const float g = (a.row_scale != nullptr ? a.row_scale[row] : 1.f) / a.temperature;
-  const bool none = g == 0.f || total == 0.f;  // zero whatever the logits hold
-  const float p_scale = g * total / v.y;
-  for (int64_t i = threadIdx.x; i < a.vocab; i += kThreads)
-    dz[i] = from_float<T>(none ? 0.f : p_scale * fast_exp2((logit(z, i) - v.x) * c));
-  if (none) return;
-  __syncthreads();  // the listed elements are written again, with their q
-  for (int j = threadIdx.x; j < a.top; j += kThreads) {
-    const int i = list.index[j];
-    if (i < 0) continue;
-    const float q = q_of_index(list, static_cast<int>(a.top), i);
-    dz[i] = from_float<T>(p_scale * fast_exp2((logit(z, i) - v.x) * c) - g * q);
+  __syncthreads();
+  if constexpr (kMode == kGradFromStats) {
+    max = a.stats[2 * row];
+    sum = a.stats[2 * row + 1];
+  } else {
+    float2 both = warp_join(lane < warps ? warp_part[lane] : make_float2(-INFINITY, 0.f), c);
+    if (cut.parts > 1) {
+      if (warp == 0 && lane < cut.parts) {
+        const uint32_t to = muon_sm100::map_to_cta(muon_sm100::smem_addr(&block_part[part]),
+                                                   static_cast<uint32_t>(lane));
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(both.x), "f"(both.y) : "memory");
+      }
+      muon_sm100::cluster_sync();
+      both = block_part[0];
+      for (int i = 1; i < cut.parts; ++i) both = join(both, block_part[i], c);
+    }
+    max = both.x;
+    sum = both.y;
+    if (part == 0 && list_warp) {
+      const float loss = row_loss(list, static_cast<int>(a.top), 1.0f / a.temperature, max, sum);
+      if (lane == 0) {
+        a.loss[row] = loss;
+        if (a.stats != nullptr) {
+          a.stats[2 * row] = max;
+          a.stats[2 * row + 1] = sum;
+        }
+      }
+    }
+  }
+  if constexpr (kMode != kLoss) {
+    const float total = total_shared;
+    const float g = (a.row_scale != nullptr ? a.row_scale[row] : 1.f) / a.temperature;
+    const bool none = g == 0.f || total == 0.f;  // zero whatever the logits hold
+    const float p_scale = none ? 0.f : g * total / sum;
+    const float2 scale2 = make_float2(p_scale, p_scale), minus_max = make_float2(-max, -max);
+    T* dz = static_cast<T*>(a.grad) + row * a.ld_grad;
+    if (!list_warp) {
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) {
+        const int granule = mine + v * threads, element = granule * kN - shift;
+        if (granule >= last) continue;
+        float e[kN];
+        if (none) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) e[j] = 0.f;
+        } else {
+          unpack<T>(raw[v], e);
+#pragma unroll
+          for (int j = 0; j < kN; j += 2) {
+            const float2 p = mul2(scale2, exp2_of(e[j], e[j + 1], minus_max, cc));
+            e[j] = p.x;
+            e[j + 1] = p.y;
+          }
+        }
+        if (cut.same_phase && inside(element)) {
+          *reinterpret_cast<uint4*>(dz + element) = pack<T>(e);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+            if (element + j >= 0 && element + j < vocab) dz[element + j] = from_float<T>(e[j]);
+        }
+      }
+    }
+    if (none) return;
+    __syncthreads();  // the listed elements are written again, with their q
+    for (int j = threadIdx.x; j < static_cast<int>(a.top); j += blockDim.x) {
+      const int i = list.index[j];
+      const int granule = (i + shift) / kN;
+      if (i < 0 || granule < first || granule >= last) continue;
+      const float q = q_of_index(list, static_cast<int>(a.top), i);
+      dz[i] = from_float<T>(p_scale * fast_exp2((list.z[j] - max) * c) - g * q);
+    }
   }
 }
 
+// ------------------------------------------------------------ rows through a ring
+// Long rows: one persistent block an SM, or a cluster of them a row.  A
+// producer warp streams the blocks' slices of row after row into a ring of
+// 16 KiB stages with bulk copies, a list warp makes the lists one row ahead,
+// and 512 consumer threads take the statistics from the stages as they land
+// and the gradient from the same stages, which only then are free again.  So
+// the next row is on its way while this one is worked on, and neither the
+// list nor the sums of the row hold up the memory.
+constexpr int kConsumers = 512;
+constexpr int kConsumerWarps = kConsumers / 32;
+constexpr int kStageGranules = 2 * kConsumers;
+constexpr int kStageBytes = kStageGranules * 16;
+constexpr int kMaxStages = 13;
+constexpr size_t kRingBytes = 224 * 1024;  // of dynamic shared memory
+constexpr double kRowNs = 700.0, kClusterNs = 500.0;
+
+struct Ring {
+  Cut cut;
+  int stages;
+};
+
+__device__ uint32_t g_status = 0;
+
+// Waits for the phase of `bar`; gives up after the wait limit, or once another
+// thread of the block has: the block then runs on without waiting, and the
+// device status tells.
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(muon_sm100::smem_addr(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+template <bool kCluster>
+__device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  const auto done = [&] {
+    return kCluster ? try_wait_cluster(bar, parity) : muon_sm100::mbar_try_wait(bar, parity);
+  };
+  if (done()) return;
+  const uint64_t t0 = muon_sm100::global_timer_ns();
+  for (uint32_t spins = 1;; ++spins) {
+    if (done()) return;
+    if ((spins & 63u) != 0) continue;
+    if (*failed) return;
+    if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
+      *failed = 1;
+      atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
+      return;
+    }
+  }
+}
+
+// A block's slice of one row.
 template <typename T>
-int run(const muon_train_distill_args& a, bool from_stats, void* stream) {
-  return launch(distill_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), kThreads, 0, 1, stream,
-                a, from_stats);
+struct Slice {
+  const T* z;
+  int shift, first, last;  // granules [first, last), the row beginning `shift` elements into granule 0
+  __device__ Slice(const muon_train_distill_args& a, const Cut& cut, int64_t row, int part) {
+    constexpr int kN = kVec<T>;
+    z = static_cast<const T*>(a.logits) + row * a.ld;
+    shift = static_cast<int>(reinterpret_cast<uintptr_t>(z) & 15u) / static_cast<int>(sizeof(T));
+    const int granules = static_cast<int>((a.vocab + shift + kN - 1) / kN);
+    const int each = (granules + cut.parts - 1) / cut.parts;
+    first = min(granules, part * each);
+    last = min(granules, first + each);
+  }
+};
+
+template <typename T, Mode kMode>
+__global__ void __launch_bounds__(kConsumers + 64, 1)
+    distill_ring_kernel(const __grid_constant__ muon_train_distill_args a, Ring ring) {
+  using namespace muon_sm100;
+  constexpr int kN = kVec<T>;
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], heard[2];
+  __shared__ float2 warp_part[2][kConsumerWarps];
+  __shared__ float2 block_part[2][kMaxCluster];
+  __shared__ float4 row_info[2];  // Q, g, and the statistics of an earlier call
+  __shared__ volatile int failed;
+  const int parts = ring.cut.parts, stages = ring.stages;
+  const int part = static_cast<int>(blockIdx.x % parts);
+  const int64_t workers = gridDim.x / parts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int vocab = static_cast<int>(a.vocab), top = static_cast<int>(a.top);
+  const float c = kLog2e / a.temperature;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kConsumerWarps);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&heard[i], static_cast<uint32_t>(parts));
+    failed = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (parts > 1) cluster_sync();  // every block has begun, its barriers are there
+
+  int stage = 0;
+  uint32_t phase = 0;
+  const auto advance = [&] {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  };
+  // The row's statistics from the parts of this block's warps, and of the
+  // cluster's blocks; `turn` counts the worker's rows.  Each block's list warp
+  // tells every block its part, and goes on to the next row only after it has
+  // heard all of them: so no block is ever more than one row ahead of another,
+  // and two slots are enough.
+  const auto statistics = [&](uint32_t turn) {
+    float2 v = lane < kConsumerWarps ? warp_part[turn & 1][lane] : make_float2(-INFINITY, 0.f);
+    v = warp_join(v, c);
+    if (parts > 1) {
+      if (warp == kConsumerWarps + 1 && lane < parts) {
+        const uint32_t peer = static_cast<uint32_t>(lane);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+                         map_to_cta(smem_addr(&block_part[turn & 1][part]), peer)),
+                     "f"(v.x), "f"(v.y) : "memory");
+        mbar_arrive_cluster(map_to_cta(smem_addr(&heard[turn & 1]), peer));
+      }
+      ring_wait<true>(&heard[turn & 1], (turn >> 1) & 1, &failed);
+      v = block_part[turn & 1][0];
+      for (int i = 1; i < parts; ++i) v = join(v, block_part[turn & 1][i], c);
+    }
+    return v;
+  };
+
+  if (warp == kConsumerWarps) {  // producer
+    for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers) {
+      const Slice<T> slice(a, ring.cut, row, part);
+      for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
+        const int g1 = min(slice.last, g0 + kStageGranules);
+        // whole granules [lo, hi); at most one more at either end of the row
+        const int lo = g0 * kN < slice.shift ? g0 + 1 : g0;
+        const int hi = g1 * kN - slice.shift > vocab ? g1 - 1 : g1;
+        uint8_t* to = dynamic + stage * kStageBytes;
+        if (lane == 0) ring_wait<false>(&empty[stage], phase ^ 1, &failed);
+        __syncwarp();
+        if (lane < 2 * kN) {
+          const bool left = lane < kN;
+          const int granule = left ? g0 : g1 - 1, j = lane % kN;
+          if (left ? lo > g0 : (hi < g1 && g1 - 1 >= lo)) {
+            const int element = granule * kN - slice.shift + j;
+            reinterpret_cast<T*>(to)[(granule - g0) * kN + j] =
+                element >= 0 && element < vocab ? slice.z[element] : from_float<T>(-INFINITY);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t bytes = hi > lo ? static_cast<uint32_t>(hi - lo) * 16u : 0u;
+          mbar_arrive_expect_tx(&full[stage], bytes);
+          if (bytes > 0)
+            bulk_load(to + (lo - g0) * 16, slice.z + (static_cast<int64_t>(lo) * kN - slice.shift), bytes, &full[stage]);
+        }
+        advance();
+      }
+    }
+  } else if (warp == kConsumerWarps + 1) {  // lists
+    uint32_t turn = 0;
+    for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers, ++turn) {
+      const List list(dynamic + stages * kStageBytes + (turn & 1) * List::bytes(top), top);
+      const float total = load_list(a, row, static_cast<const T*>(a.logits) + row * a.ld, list);
+      if (lane == 0) {
+        float4 info = make_float4(total, 1.f, 0.f, 0.f);
+        if (a.row_scale != nullptr) info.y = a.row_scale[row];
+        info.y /= a.temperature;
+        if constexpr (kMode == kGradFromStats) {
+          info.z = a.stats[2 * row];
+          info.w = a.stats[2 * row + 1];
+        }
+        row_info[turn & 1] = info;
+      }
+      named_barrier(1, kConsumers + 32);
+      if constexpr (kMode != kGradFromStats) {
+        const float2 v = statistics(turn);
+        if (part == 0) {
+          const float loss = row_loss(list, top, 1.0f / a.temperature, v.x, v.y);
+          if (lane == 0) {
+            a.loss[row] = loss;
+            if (a.stats != nullptr) {
+              a.stats[2 * row] = v.x;
+              a.stats[2 * row + 1] = v.y;
+            }
+          }
+        }
+      }
+    }
+  } else {  // consumers
+    const float2 cc = make_float2(c, c);
+    uint32_t turn = 0;
+    for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers, ++turn) {
+      const Slice<T> slice(a, ring.cut, row, part);
+      const int row_stage = stage;
+      const uint32_t row_phase = phase;
+      const auto read = [&](int at) {
+        return *reinterpret_cast<const uint4*>(dynamic + stage * kStageBytes + at * 16);
+      };
+      const auto release = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      };
+      if constexpr (kMode != kGradFromStats) {
+        float m = -INFINITY;
+        float2 s = make_float2(0.f, 0.f);
+        for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
+          ring_wait<false>(&full[stage], phase, &failed);
+          uint4 u[2];
+          bool there[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = static_cast<int>(threadIdx.x) + i * kConsumers;
+            there[i] = g0 + at < slice.last;
+            u[i] = there[i] ? read(at) : make_uint4(0, 0, 0, 0);
+          }
+          if constexpr (kMode == kLoss) release();
+          float largest = m;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (there[i]) largest = vector_max(u[i], largest, T());
+          const float base = largest == -INFINITY ? 0.f : largest;  // nothing finite yet: a sum of 0
+          if (largest > m) {
+            const float down = fast_exp2((m - base) * c);
+            s = mul2(s, make_float2(down, down));
+            m = largest;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!there[i]) continue;
+            float e[kN];
+            unpack<T>(u[i], e);
+#pragma unroll
+            for (int j = 0; j < kN; j += 2)
+              s = add2(s, exp2_of(e[j], e[j + 1], make_float2(-base, -base), cc));
+          }
+          advance();
+        }
+        const float2 v = warp_join(make_float2(m, s.x + s.y), c);
+        if (lane == 0) warp_part[turn & 1][warp] = v;
+      }
+      named_barrier(1, kConsumers + 32);
+      if constexpr (kMode != kLoss) {
+        const float4 info = row_info[turn & 1];
+        float2 v = make_float2(info.z, info.w);
+        if constexpr (kMode != kGradFromStats) v = statistics(turn);
+        stage = row_stage;
+        phase = row_phase;
+        const float g = info.y;
+        const bool none = g == 0.f || info.x == 0.f;  // zero whatever the logits hold
+        const float p_scale = none ? 0.f : g * info.x / v.y;
+        const float2 scale2 = make_float2(p_scale, p_scale), minus_max = make_float2(-v.x, -v.x);
+        T* dz = static_cast<T*>(a.grad) + row * a.ld_grad;
+        for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
+          if constexpr (kMode == kGradFromStats) ring_wait<false>(&full[stage], phase, &failed);
+          uint4 u[2];
+          bool there[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = static_cast<int>(threadIdx.x) + i * kConsumers;
+            there[i] = g0 + at < slice.last;
+            u[i] = there[i] ? read(at) : make_uint4(0, 0, 0, 0);
+          }
+          release();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!there[i]) continue;
+            const int granule = g0 + static_cast<int>(threadIdx.x) + i * kConsumers;
+            const int element = granule * kN - slice.shift;
+            float e[kN];
+            if (none) {
+#pragma unroll
+              for (int j = 0; j < kN; ++j) e[j] = 0.f;
+            } else {
+              unpack<T>(u[i], e);
+#pragma unroll
+              for (int j = 0; j < kN; j += 2) {
+                const float2 p = mul2(scale2, exp2_of(e[j], e[j + 1], minus_max, cc));
+                e[j] = p.x;
+                e[j + 1] = p.y;
+              }
+            }
+            if (ring.cut.same_phase && element >= 0 && element + kN <= vocab) {
+              *reinterpret_cast<uint4*>(dz + element) = pack<T>(e);
+            } else {
+#pragma unroll
+              for (int j = 0; j < kN; ++j)
+                if (element + j >= 0 && element + j < vocab) dz[element + j] = from_float<T>(e[j]);
+            }
+          }
+          advance();
+        }
+        named_barrier(2, kConsumers);  // the listed elements are written again, with their q
+        const List list(dynamic + stages * kStageBytes + (turn & 1) * List::bytes(top), top);
+        for (int j = threadIdx.x; j < top && !none; j += kConsumers) {
+          const int i = list.index[j], granule = (i + slice.shift) / kN;
+          if (i < 0 || granule < slice.first || granule >= slice.last) continue;
+          const float q = q_of_index(list, top, i);
+          dz[i] = from_float<T>(p_scale * fast_exp2((list.z[j] - v.x) * c) - g * q);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (parts > 1) cluster_sync();  // no block leaves while another may still write to it
+}
+
+// ------------------------------------------------------------ host side
+bool same_phase(const muon_train_distill_args& a, size_t item) {
+  return a.grad != nullptr &&
+         ((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.logits)) & 15u) == 0 &&
+         (a.rows == 1 || ((a.ld_grad - a.ld) * static_cast<int64_t>(item)) % 16 == 0);
+}
+
+template <typename T, int kVectors>
+int run_vectors(const muon_train_distill_args& a, Mode mode, int threads, int parts, void* stream) {
+  const Cut cut{parts, same_phase(a, sizeof(T))};
+  const dim3 grid(static_cast<unsigned>(a.rows * parts));
+  const size_t smem = List::bytes(a.top);
+  threads += 32;
+  if (mode == kGradFromStats)
+    return launch(distill_kernel<T, kVectors, kGradFromStats>, grid, threads, smem, 1, stream, a, cut);
+  if (mode == kLossGrad)
+    return launch(distill_kernel<T, kVectors, kLossGrad>, grid, threads, smem, parts, stream, a, cut);
+  return launch(distill_kernel<T, kVectors, kLoss>, grid, threads, smem, parts, stream, a, cut);
+}
+
+template <typename T, Mode kMode>
+int run_ring(const muon_train_distill_args& a, int parts, int stages, int64_t workers, void* stream) {
+  const size_t smem = static_cast<size_t>(stages) * kStageBytes + 2 * List::bytes(a.top);
+  static const cudaError_t allowed = cudaFuncSetAttribute(
+      distill_ring_kernel<T, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  if (allowed != cudaSuccess) return static_cast<int>(allowed);
+  const Ring ring{Cut{parts, same_phase(a, sizeof(T))}, stages};
+  return launch(distill_ring_kernel<T, kMode>, dim3(static_cast<unsigned>(workers * parts)),
+                kConsumers + 64, smem, kMode == kGradFromStats ? 1 : parts, stream, a, ring);
+}
+
+template <typename T>
+int run(const muon_train_distill_args& a, Mode mode, void* stream) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc != MUON_POLAR_OK) return rc;
+  // granules of a row: one more where a row can begin off a boundary
+  const bool aligned = aligned16(a.logits) && (a.rows == 1 || a.ld % kVec<T> == 0);
+  const int64_t granules = (a.vocab + kVec<T> - 1) / kVec<T> + (aligned ? 0 : 1);
+  const int64_t register_row = static_cast<int64_t>(kBlockThreads) * 8;  // of one block
+  if (granules <= register_row || (granules <= kMaxCluster * register_row && a.rows * 2 <= sms)) {
+    // Parts of a row: as many as keep a thread at 8 vectors; more, down to one
+    // vector a thread, while the device is not full.
+    int parts = 1;
+    while (parts < kMaxCluster &&
+           (granules > parts * register_row || (a.rows * parts < 2 * sms && granules > parts * kBlockThreads)))
+      parts *= 2;
+    const int64_t each = (granules + parts - 1) / parts;
+    // Threads: 8 vectors each when there are blocks enough, else one each.
+    const int64_t want = a.rows * parts >= 4 * sms ? (each + 7) / 8 : each;
+    const int threads = static_cast<int>(want >= kBlockThreads ? kBlockThreads : want <= 64 ? 64 : (want + 31) / 32 * 32);
+    const int64_t vectors = (each + threads - 1) / threads;
+    if (vectors <= 1) return run_vectors<T, 1>(a, mode, threads, parts, stream);
+    if (vectors <= 2) return run_vectors<T, 2>(a, mode, threads, parts, stream);
+    if (vectors <= 4) return run_vectors<T, 4>(a, mode, threads, parts, stream);
+    return run_vectors<T, 8>(a, mode, threads, parts, stream);
+  }
+  const int stages = static_cast<int>(
+      std::min<size_t>(kMaxStages, (kRingBytes - 2 * List::bytes(a.top)) / kStageBytes));
+  // With the gradient a slice stays in the ring, and two stages are left for
+  // the next row; a longer row's gradient is made by a second pass.
+  const auto slice_stages = [&](int parts) {
+    return ((granules + parts - 1) / parts + kStageGranules - 1) / kStageGranules;
+  };
+  const int most = mode == kLossGrad ? stages - 2 : 1 << 30;
+  if (slice_stages(kMaxCluster) > most) {
+    const int first = run<T>(a, kLoss, stream);
+    return first != MUON_POLAR_OK ? first : run<T>(a, kGradFromStats, stream);
+  }
+  // Parts of a row by the smallest estimate: rounds of rows, each of a slice
+  // at an SM's share of the measured copy rate and what a row costs besides.
+  int parts = 0;
+  double least = 0.0;
+  for (int p = 1; p <= kMaxCluster; p *= 2) {
+    if (slice_stages(p) > most) continue;
+    const int64_t workers = std::max<int64_t>(1, sms / p);
+    const double rounds = static_cast<double>((a.rows + workers - 1) / workers);
+    const double slice_ns = static_cast<double>(granules) * 16.0 / p / 43.0 * (mode == kLossGrad ? 2.0 : mode == kGradFromStats ? 2.0 : 1.0);
+    const double estimate = rounds * (slice_ns + kRowNs + (p > 1 && mode != kGradFromStats ? kClusterNs : 0.0));
+    if (parts == 0 || estimate < least) {
+      parts = p;
+      least = estimate;
+    }
+  }
+  const int64_t workers = std::min<int64_t>(a.rows, std::max<int64_t>(1, sms / parts));
+  if (mode == kLossGrad) return run_ring<T, kLossGrad>(a, parts, stages, workers, stream);
+  if (mode == kLoss) return run_ring<T, kLoss>(a, parts, stages, workers, stream);
+  return run_ring<T, kGradFromStats>(a, parts, stages, workers, stream);
 }
 
 int check(const muon_train_distill_args* a) {
@@ -193,12 +694,12 @@ int check(const muon_train_distill_args* a) {
   return MUON_POLAR_OK;
 }
 
-int dispatch(const muon_train_distill_args& a, bool from_stats, void* stream) {
+int dispatch(const muon_train_distill_args& a, Mode mode, void* stream) {
   if (a.rows == 0) return MUON_POLAR_OK;
   switch (a.dtype) {
-    case MUON_TRAIN_F32: return run<float>(a, from_stats, stream);
-    case MUON_TRAIN_BF16: return run<__nv_bfloat16>(a, from_stats, stream);
-    default: return run<__half>(a, from_stats, stream);
+    case MUON_TRAIN_F32: return run<float>(a, mode, stream);
+    case MUON_TRAIN_BF16: return run<__nv_bfloat16>(a, mode, stream);
+    default: return run<__half>(a, mode, stream);
   }
 }
 
@@ -211,21 +712,40 @@ uint64_t muon_train_launch_count(void) {
   return muon_train::launch_counter().load(std::memory_order_relaxed);
 }
 
+int muon_train_read_device_status(int device, uint32_t* flags, int clear) {
+  using muon_train::g_status;
+  if (flags == nullptr) return MUON_POLAR_ERR_INVALID_ARGUMENT;
+  int prev = 0;
+  cudaError_t e = cudaGetDevice(&prev);
+  if (e == cudaSuccess && device != prev) e = cudaSetDevice(device);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  uint32_t v = 0;
+  const uint32_t zero = 0;
+  e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+  if (device != prev) cudaSetDevice(prev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  *flags = v;
+  return MUON_POLAR_OK;
+}
+
 int muon_train_distill_sm100(const muon_train_distill_args* args, void* stream) {
-  const int rc = muon_train::check(args);
+  using namespace muon_train;
+  const int rc = check(args);
   if (rc != MUON_POLAR_OK) return rc;
-  if (args->rows > 0 && args->loss == nullptr) return MUON_POLAR_ERR_INVALID_ARGUMENT;
-  return muon_train::dispatch(*args, false, stream);
+  if (args->rows > 0 && (args->loss == nullptr || (args->grad != nullptr && args->stats == nullptr)))
+    return MUON_POLAR_ERR_INVALID_ARGUMENT;
+  return dispatch(*args, args->grad != nullptr ? kLossGrad : kLoss, stream);
 }
 
 int muon_train_distill_backward_sm100(const muon_train_distill_args* args, void* stream) {
-  const int rc = muon_train::check(args);
+  using namespace muon_train;
+  const int rc = check(args);
   if (rc != MUON_POLAR_OK) return rc;
   if (args->rows > 0 && (args->stats == nullptr || args->grad == nullptr))
     return MUON_POLAR_ERR_INVALID_ARGUMENT;
-  muon_train_distill_args a = *args;
-  a.loss = nullptr;
-  return muon_train::dispatch(a, true, stream);
+  return dispatch(*args, kGradFromStats, stream);
 }
 
 }  // extern "C"

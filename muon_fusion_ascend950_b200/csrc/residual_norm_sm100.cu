@@ -16,6 +16,9 @@
 // Bound by memory: forward reads x, y and writes h, n; backward reads x, y,
 // dh, dn and writes dx, dy.  Parameter gradients: each block adds up its rows
 // in order, a second kernel adds up the blocks in order.
+#include <initializer_list>
+
+#include "sm100_ptx.cuh"
 #include "train_common.cuh"
 
 namespace muon_train {
@@ -60,6 +63,251 @@ __device__ __forceinline__ void block_sums(float (&v)[N], float* red, int thread
 
 __device__ __forceinline__ float rms_rstd(float sum, float width, float eps) {
   return rsqrtf(sum / width + eps);
+}
+
+// ------------------------------------------------------------ rows in registers
+// A row of up to 16384 elements is held in registers: each thread has 8 of
+// its columns, the same ones in every row, as 8 / N loads of N elements, so
+// that the columns' parameters stay in registers too.  A row belongs to one
+// warp (up to 256 columns, no barrier), to a block of up to 512 threads, or to
+// a cluster of 2 or 4 such blocks, which add up their sums over distributed
+// shared memory.
+constexpr int kElements = 8;       // a thread's columns
+constexpr int kMaxThreads = 512;
+constexpr int kWarpRowWarps = 8;   // rows in flight of a block, one a warp
+constexpr int kMaxCluster = 4;
+
+enum RowOwner { kWarpRow, kBlockRow, kClusterRow };
+
+// Shared memory of the sums of one row's parts, twice: a buffer is written
+// again only after a barrier that follows its last reading.
+struct SumSlots {
+  float warp[2][4][16];
+  float block[2][kMaxCluster][4];
+};
+
+// Four sums over a warp with 6 shuffles: each step halves the values that a
+// lane carries on.  Lane l ends with the sum of value (l >> 3) & 3 .. in the
+// order 0, 1, 2, 3 of its upper two bits.
+__device__ __forceinline__ float warp_sum4(const float (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool high = lane & 16, odd = lane & 8;
+  const float a0 = high ? v[2] : v[0], a1 = high ? v[3] : v[1];
+  const float b0 = high ? v[0] : v[2], b1 = high ? v[1] : v[3];
+  const float c0 = a0 + __shfl_xor_sync(kFullMask, b0, 16);
+  const float c1 = a1 + __shfl_xor_sync(kFullMask, b1, 16);
+  float d = (odd ? c1 : c0) + __shfl_xor_sync(kFullMask, odd ? c0 : c1, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) d += __shfl_xor_sync(kFullMask, d, o);
+  return d;
+}
+
+// Sums of four values over a row's threads, in a fixed order; every thread
+// gets them.  `turn` begins at 0 and alternates from call to call.
+template <RowOwner kOwner>
+__device__ __forceinline__ void row_sums(float (&v)[4], SumSlots& slots, int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  float d = warp_sum4(v);
+  if constexpr (kOwner != kWarpRow) {
+    if ((lane & 7) == 0) slots.warp[turn][lane >> 3][warp] = d;
+    __syncthreads();
+    const float* from = slots.warp[turn][lane >> 3];
+    d = ((lane & 7) < warps ? from[lane & 7] : 0.f) + ((lane & 7) + 8 < warps ? from[(lane & 7) + 8] : 0.f);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) d += __shfl_xor_sync(kFullMask, d, o);
+  }
+  if constexpr (kOwner == kClusterRow) {
+    const int rank = static_cast<int>(muon_sm100::cluster_cta_rank());
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    // each block puts its sums into every block's slots, by rank
+    if (warp < static_cast<int>(n) && (lane & 7) == 0) {
+      const uint32_t to = muon_sm100::map_to_cta(
+          muon_sm100::smem_addr(&slots.block[turn][rank][lane >> 3]), static_cast<uint32_t>(warp));
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(d) : "memory");
+    }
+    muon_sm100::cluster_sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float sum = 0.f;
+      for (uint32_t k = 0; k < n; ++k) sum += slots.block[turn][k][i];
+      v[i] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __shfl_sync(kFullMask, d, i * 8);
+  }
+  turn ^= 1;
+}
+
+// Which rows and columns a thread has.
+template <int N, RowOwner kOwner>
+struct Place {
+  int64_t worker, workers;  // rows go to workers: a warp, a block or a cluster
+  int tid, threads;         // of the row's threads
+  __device__ Place() {
+    if constexpr (kOwner == kWarpRow) {
+      tid = threadIdx.x & 31;
+      threads = 32;
+      worker = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+      workers = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    } else if constexpr (kOwner == kBlockRow) {
+      tid = threadIdx.x;
+      threads = blockDim.x;
+      worker = blockIdx.x;
+      workers = gridDim.x;
+    } else {
+      uint32_t n;
+      asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+      tid = static_cast<int>(muon_sm100::cluster_cta_rank() * blockDim.x + threadIdx.x);
+      threads = static_cast<int>(n * blockDim.x);
+      worker = blockIdx.x / n;
+      workers = gridDim.x / n;
+    }
+  }
+  __device__ int column(int i) const { return (i * threads + tid) * N; }
+};
+
+// One parameter's values in a thread's columns; `none` outside the row, and
+// everywhere when there is no such parameter.
+template <int N, typename P>
+__device__ __forceinline__ void load_columns(float (&v)[kElements], const P& place, int width,
+                                             const void* p, int dtype, int64_t offset, float none) {
+#pragma unroll
+  for (int i = 0; i < kElements / N; ++i) {
+    float part[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) part[j] = none;
+    const int c = place.column(i);
+    if (p != nullptr && c < width) load_any<N>(p, dtype, offset + c, part);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[i * N + j] = part[j];
+  }
+}
+
+template <typename T, int N>
+struct RowVectors {
+  using E = Elements<T, N>;
+  typename E::Raw raw[kElements / N];
+  template <typename P>
+  __device__ __forceinline__ void load(const T* row, const P& place, int width) {
+#pragma unroll
+    for (int i = 0; i < kElements / N; ++i)
+      raw[i] = place.column(i) < width ? E::load(row + place.column(i)) : typename E::Raw();
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kElements / N; ++i) raw[i] = typename E::Raw();
+  }
+  __device__ __forceinline__ void values(float (&v)[kElements]) const {
+#pragma unroll
+    for (int i = 0; i < kElements / N; ++i) {
+      float part[N];
+      E::unpack(raw[i], part);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i * N + j] = part[j];
+    }
+  }
+  template <typename P>
+  static __device__ __forceinline__ void store(T* row, const P& place, int width,
+                                               const float (&v)[kElements]) {
+#pragma unroll
+    for (int i = 0; i < kElements / N; ++i) {
+      float part[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) part[j] = v[i * N + j];
+      if (place.column(i) < width) E::store(row + place.column(i), E::pack(part));
+    }
+  }
+};
+
+// The row's gate row.
+__device__ __forceinline__ int64_t gate_row_of(const muon_train_norm_args& a, int64_t row) {
+  return a.gate_rows > 1 ? row / (a.rows / a.gate_rows) : 0;
+}
+
+// Blocks that an SM holds in forward: whole vectors need 64 registers a
+// thread, smaller ones 128.
+constexpr int forward_per_sm(int threads, bool whole_vectors) {
+  return (whole_vectors ? 1024 : 512) / threads;
+}
+
+// Forward.  The next row is loaded before this row's sums are awaited.
+template <typename T, int N, RowOwner kOwner>
+__global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads,
+                                  forward_per_sm(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads,
+                                                 N * sizeof(T) == 16))
+    norm_forward_kernel(const __grid_constant__ muon_train_norm_args a) {
+  __shared__ SumSlots slots;
+  int turn = 0;
+  if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // every block has begun
+  const Place<N, kOwner> place;
+  const int width = static_cast<int>(a.width);
+  const float inv_width = 1.0f / static_cast<float>(width);
+  const T* y_all = static_cast<const T*>(a.block_out);
+  const T* x_all = static_cast<const T*>(a.residual);
+  int64_t row = place.worker;
+  RowVectors<T, N> ry, rx;
+  if (row < a.rows) {
+    ry.load(y_all + row * width, place, width);
+    rx.load(x_all + row * width, place, width);
+  }
+  float gain[kElements], scale[kElements], pre[kElements];
+  int64_t gate_row = 0;
+  const auto load_gain = [&] {
+    float post[kElements];
+    load_columns<N>(gain, place, width, a.gate, a.gate_dtype, gate_row * width, 1.f);
+    load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
+#pragma unroll
+    for (int i = 0; i < kElements; ++i) gain[i] *= post[i];
+  };
+  if (row < a.rows) gate_row = gate_row_of(a, row);
+  load_gain();
+  load_columns<N>(pre, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
+  if (a.scale_count == 1) {
+    const float one = load_any(a.residual_scale, a.scale_dtype, 0);
+#pragma unroll
+    for (int i = 0; i < kElements; ++i) scale[i] = one;
+  } else {
+    load_columns<N>(scale, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+  }
+  for (; row < a.rows; row += place.workers) {
+    if (const int64_t g = gate_row_of(a, row); g != gate_row) {
+      gate_row = g;
+      load_gain();
+    }
+    float y[kElements], h[kElements];
+    ry.values(y);
+    rx.values(h);
+    if (const int64_t next = row + place.workers; next < a.rows) {
+      ry.load(y_all + next * width, place, width);
+      rx.load(x_all + next * width, place, width);
+    }
+    float r = 1.f;
+    if (a.post_weight != nullptr) {
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kElements; ++i) sums[0] = fmaf(y[i], y[i], sums[0]);
+      row_sums<kOwner>(sums, slots, turn);
+      r = rsqrtf(sums[0] * inv_width + a.eps);
+      if (place.tid == 0 && a.rstd_post != nullptr) a.rstd_post[row] = r;
+    }
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kElements; ++i) {
+      h[i] = fmaf(scale[i], h[i], gain[i] * (y[i] * r));
+      sums[0] = fmaf(h[i], h[i], sums[0]);
+    }
+    RowVectors<T, N>::store(static_cast<T*>(a.hidden) + row * width, place, width, h);
+    if (a.pre_weight == nullptr) continue;
+    row_sums<kOwner>(sums, slots, turn);
+    const float rh = rsqrtf(sums[0] * inv_width + a.eps);
+    if (place.tid == 0 && a.rstd_pre != nullptr) a.rstd_pre[row] = rh;
+#pragma unroll
+    for (int i = 0; i < kElements; ++i) h[i] = h[i] * rh * pre[i];
+    RowVectors<T, N>::store(static_cast<T*>(a.normed) + row * width, place, width, h);
+  }
+  if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed
 }
 
 // ------------------------------------------------------------ any width
@@ -132,7 +380,8 @@ Plan make_plan(const muon_train_norm_args& a, int64_t target) {
   p.gain_off = 0;
   p.pre_off = align(static_cast<size_t>(p.chunks * a.width) * sizeof(float));
   p.scale_off = p.pre_off + align(static_cast<size_t>(p.blocks * a.width) * sizeof(float));
-  p.bytes = p.scale_off + align(static_cast<size_t>(p.blocks * a.width) * sizeof(float));
+  // (with one value, one of every block of a cluster: at most kMaxCluster a worker)
+  p.bytes = p.scale_off + align(static_cast<size_t>(p.blocks * (a.width < kMaxCluster ? kMaxCluster : a.width)) * sizeof(float));
   return p;
 }
 
@@ -140,6 +389,7 @@ struct Backward {
   muon_train_norm_args a;
   muon_train_norm_grads g;
   Plan plan;
+  int64_t scale_rows;         // partial rows of `scale`
   float *gain, *pre, *scale;  // partial sums; NULL: not wanted
 };
 
@@ -150,6 +400,173 @@ __device__ __forceinline__ void chunk_rows(const Backward& b, int64_t chunk, int
   const int64_t i = chunk - *group * n;
   *r0 = *group * per_group + i * per_group / n;
   *r1 = *group * per_group + (i + 1) * per_group / n;
+}
+
+// Sums over a block's warps of each warp's columns (kWarpRow), written to a
+// partial row.
+__device__ __forceinline__ void store_warp_columns(float* to, int width, const float (&v)[kElements],
+                                                   int n, float (*columns)[32 * kElements]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kElements; ++i) columns[warp][((i / n) * 32 + lane) * n + i % n] = v[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < width; c += blockDim.x) {
+    float sum = 0.f;
+    for (int w = 0; w < kWarpRowWarps; ++w) sum += columns[w][c];
+    to[c] = sum;
+  }
+}
+
+// Backward.  A worker (block or cluster) takes whole chunks; with one warp a
+// row, the block's warps take every 8th row of the chunk and are added up
+// where the chunk ends.  kScaleColumns: residual_scale has a value for each
+// column (else one value, or none).
+template <typename T, int N, RowOwner kOwner, bool kScaleColumns>
+__global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads, 1)
+    norm_backward_kernel(const __grid_constant__ Backward b) {
+  __shared__ SumSlots slots;
+  __shared__ float columns[kOwner == kWarpRow ? kWarpRowWarps : 1][32 * kElements];
+  // the next row is loaded while this one is worked on where registers allow
+  constexpr bool kAhead = sizeof(T) == 2 && N > 1;
+  const muon_train_norm_args& a = b.a;
+  const Place<N, kOwner> place;
+  const int width = static_cast<int>(a.width);
+  const float inv_width = 1.0f / static_cast<float>(width);
+  int turn = 0;
+  if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // every block has begun
+  const int64_t worker = kOwner == kWarpRow ? blockIdx.x : place.worker;
+  const int64_t workers = kOwner == kWarpRow ? gridDim.x : place.workers;
+  const int step = kOwner == kWarpRow ? kWarpRowWarps : 1;
+  const int first = kOwner == kWarpRow ? threadIdx.x >> 5 : 0;
+
+  const T* y_all = static_cast<const T*>(a.block_out);
+  const T* x_all = static_cast<const T*>(a.residual);
+  const T* dh_all = static_cast<const T*>(b.g.grad_hidden);
+  const T* dn_all = static_cast<const T*>(b.g.grad_normed);
+  const bool has_pre = a.pre_weight != nullptr && dn_all != nullptr;
+  RowVectors<T, N> ry, rx, rdh, rdn;
+  const auto load_row = [&](int64_t row) {
+    ry.load(y_all + row * width, place, width);
+    rx.load(x_all + row * width, place, width);
+    if (dh_all != nullptr) rdh.load(dh_all + row * width, place, width);
+    if (dn_all != nullptr) rdn.load(dn_all + row * width, place, width);
+  };
+  rdh.clear();
+  rdn.clear();
+
+  float post[kElements], gate[kElements], pre[kElements], scale[kScaleColumns ? kElements : 1];
+  load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
+  load_columns<N>(gate, place, width, nullptr, 0, 0, 1.f);
+  load_columns<N>(pre, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
+  if constexpr (kScaleColumns)
+    load_columns<N>(scale, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+  else
+    scale[0] = a.residual_scale != nullptr ? load_any(a.residual_scale, a.scale_dtype, 0) : 1.f;
+
+  float sum_gain[kElements], sum_pre[kElements], sum_scale[kScaleColumns ? kElements : 1];
+#pragma unroll
+  for (int i = 0; i < kElements; ++i) sum_gain[i] = sum_pre[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < (kScaleColumns ? kElements : 1); ++i) sum_scale[i] = 0.f;
+
+  const auto store_columns = [&](float* to, const float(&v)[kElements]) {
+    if constexpr (kOwner == kWarpRow) {
+      store_warp_columns(to, width, v, N, columns);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kElements / N; ++i) {
+        if (place.column(i) >= width) continue;
+#pragma unroll
+        for (int j = 0; j < N; ++j) to[place.column(i) + j] = v[i * N + j];
+      }
+    }
+  };
+
+  for (int64_t chunk = worker; chunk < b.plan.chunks; chunk += workers) {
+    int64_t r0, r1, group;
+    chunk_rows(b, chunk, &r0, &r1, &group);
+    if (a.gate != nullptr && !b.plan.gate_per_row)
+      load_columns<N>(gate, place, width, a.gate, a.gate_dtype, group * width, 1.f);
+    if (kAhead && r0 + first < r1) load_row(r0 + first);
+    for (int64_t row = r0 + first; row < r1; row += step) {
+      if (!kAhead) load_row(row);
+      if (b.plan.gate_per_row)
+        load_columns<N>(gate, place, width, a.gate, a.gate_dtype, row * width, 1.f);
+      const float r = a.post_weight != nullptr ? a.rstd_post[row] : 1.f;
+      const float rh = has_pre ? a.rstd_pre[row] : 0.f;
+      float y[kElements], x[kElements], dh[kElements], dn[kElements];
+      ry.values(y);
+      rx.values(x);
+      rdh.values(dh);
+      rdn.values(dn);
+      if (kAhead && row + step < r1) load_row(row + step);
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kElements; ++i) {
+        const float gw = gate[i] * post[i];
+        const float h = fmaf(scale[kScaleColumns ? i : 0], x[i], gw * (y[i] * r));
+        const float an = dn[i] * pre[i];
+        sums[0] = fmaf(an, h, sums[0]);
+        sums[1] = fmaf(gw * fmaf(rh, an, dh[i]), y[i], sums[1]);
+        sums[2] = fmaf(gw * y[i], h, sums[2]);
+      }
+      row_sums<kOwner>(sums, slots, turn);
+      const float k = rh * rh * rh * sums[0] * inv_width;
+      const float ky = a.post_weight != nullptr ? r * r * r * (sums[1] - k * sums[2]) * inv_width : 0.f;
+#pragma unroll
+      for (int i = 0; i < kElements; ++i) {
+        const float sc = scale[kScaleColumns ? i : 0];
+        const float gw = gate[i] * post[i], yr = y[i] * r;
+        const float h = fmaf(sc, x[i], gw * yr);
+        const float d = fmaf(-k, h, fmaf(rh, dn[i] * pre[i], dh[i]));
+        const float gained = d * yr;
+        sum_gain[i] += b.plan.gate_per_row ? gained * gate[i] : gained;
+        sum_pre[i] = fmaf(dn[i] * h, rh, sum_pre[i]);
+        sum_scale[kScaleColumns ? i : 0] = fmaf(d, x[i], sum_scale[kScaleColumns ? i : 0]);
+        dn[i] = gained * post[i];  // the gate's gradient
+        x[i] = d * sc;
+        y[i] = fmaf(-ky, y[i], r * gw * d);
+      }
+      if (b.g.grad_residual != nullptr)
+        RowVectors<T, N>::store(static_cast<T*>(b.g.grad_residual) + row * width, place, width, x);
+      if (b.g.grad_block_out != nullptr)
+        RowVectors<T, N>::store(static_cast<T*>(b.g.grad_block_out) + row * width, place, width, y);
+      if (b.plan.gate_per_row && b.g.grad_gate != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kElements / N; ++i) {
+          if (place.column(i) >= width) continue;
+          float part[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) part[j] = dn[i * N + j];
+          store_any<N>(b.g.grad_gate, a.gate_dtype, row * width + place.column(i), part);
+        }
+      }
+    }
+    if (b.gain != nullptr) {
+      store_columns(b.gain + chunk * width, sum_gain);
+#pragma unroll
+      for (int i = 0; i < kElements; ++i) sum_gain[i] = 0.f;
+    }
+  }
+  if (b.pre != nullptr) store_columns(b.pre + worker * width, sum_pre);
+  if (b.scale != nullptr) {
+    if constexpr (kScaleColumns) {
+      store_columns(b.scale + worker * width, sum_scale);
+    } else {  // one value of each block
+      float sum = warp_sum(sum_scale[0]);
+      const int warp = threadIdx.x >> 5;
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) slots.warp[0][0][warp] = sum;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        sum = 0.f;
+        for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) sum += slots.warp[0][0][w];
+        b.scale[blockIdx.x] = sum;
+      }
+    }
+  }
+  if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed
 }
 
 template <typename T>
@@ -270,7 +687,7 @@ __global__ void __launch_bounds__(kSumWarps * 32)
     if (writes) store_any(b.g.grad_pre_weight, a.pre_dtype, column, v);
   } else if (what == 1) {
     if (b.scale == nullptr || static_cast<int64_t>(blockIdx.x) * 32 >= a.scale_count) return;
-    const float v = column_sum(b.scale, a.scale_count, 0, b.plan.blocks, nullptr, part);
+    const float v = column_sum(b.scale, a.scale_count, 0, b.scale_rows, nullptr, part);
     if (writes && column < a.scale_count)
       store_any(b.g.grad_residual_scale, a.scale_dtype, column, v);
   } else if (what == 2) {
@@ -314,22 +731,113 @@ muon_train_norm_args normalised(const muon_train_norm_args& args) {
   return a;
 }
 
-int target_blocks(int64_t* target) {
+// How a call's rows are laid out: the vectors they are read in, who has a row.
+struct Layout {
+  int elements;  // N: 16 bytes, two 16-bit elements, or one; 0: any width (one block a row)
+  RowOwner owner;
+  int threads, cluster;
+  int per_sm;    // blocks that an SM holds in backward
+};
+
+bool all_aligned16(std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+// Vectors of 16 bytes need rows, and so a width, of whole vectors, and every
+// pointer on a 16-byte boundary; pairs an even width.
+Layout make_layout(const muon_train_norm_args& a, const muon_train_norm_grads* g) {
+  Layout l{};
+  const int vec = static_cast<int>(16 / dtype_size(a.dtype));
+  bool aligned = all_aligned16({a.block_out, a.residual, a.hidden, a.normed, a.post_weight, a.pre_weight,
+                                a.gate, a.residual_scale});
+  if (g != nullptr)
+    aligned = aligned && all_aligned16({g->grad_hidden, g->grad_normed, g->grad_block_out,
+                                        g->grad_residual, g->grad_gate});
+  l.elements = !aligned ? 1 : a.width % vec == 0 ? vec : (vec == 8 && a.width % 2 == 0) ? 2 : 1;
+  l.cluster = 1;
+  if (a.width <= 32 * kElements) {
+    l.owner = kWarpRow;
+    l.threads = kWarpRowWarps * 32;
+  } else {
+    const int64_t most = kMaxThreads * kElements;
+    l.cluster = a.width <= most ? 1 : a.width <= 2 * most ? 2 : 4;
+    l.owner = l.cluster > 1 ? kClusterRow : kBlockRow;
+    const int64_t each = 32 * kElements * l.cluster;
+    l.threads = static_cast<int>((a.width + each - 1) / each * 32);
+    if (a.width > kMaxCluster * most) {
+      l.elements = 0;
+      l.owner = kBlockRow;
+      l.cluster = 1;
+      l.threads = kThreads;
+    }
+  }
+  l.per_sm = kMaxThreads / l.threads;
+  return l;
+}
+
+// Blocks (of all clusters) that the device works on at once in backward.
+int target_workers(const Layout& l, int64_t* target) {
   int sms = 0;
   const int rc = sm_count(&sms);
-  *target = static_cast<int64_t>(sms) * 2;
+  *target = static_cast<int64_t>(sms) * l.per_sm / l.cluster;
   return rc;
+}
+
+template <typename T, int N>
+int forward_rows(const muon_train_norm_args& a, const Layout& l, int sms, void* stream) {
+  const int64_t rows_a_block = l.owner == kWarpRow ? kWarpRowWarps : 1;
+  int64_t workers = (a.rows + rows_a_block - 1) / rows_a_block;
+  const int64_t most =
+      static_cast<int64_t>(sms) * forward_per_sm(l.threads, N * sizeof(T) == 16) / l.cluster;
+  if (workers > most) workers = most;
+  const dim3 grid(static_cast<unsigned>(workers * l.cluster));
+  if (l.owner == kWarpRow) return launch(norm_forward_kernel<T, N, kWarpRow>, grid, l.threads, 0, 1, stream, a);
+  if (l.owner == kBlockRow) return launch(norm_forward_kernel<T, N, kBlockRow>, grid, l.threads, 0, 1, stream, a);
+  return launch(norm_forward_kernel<T, N, kClusterRow>, grid, l.threads, 0, l.cluster, stream, a);
 }
 
 template <typename T>
 int forward(const muon_train_norm_args& a, void* stream) {
-  return launch(norm_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), kThreads, 0, 1, stream, a);
+  const Layout l = make_layout(a, nullptr);
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc != MUON_POLAR_OK) return rc;
+  if (l.elements == 0)
+    return launch(norm_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), kThreads, 0, 1, stream, a);
+  if (l.elements == kVec<T>) return forward_rows<T, kVec<T>>(a, l, sms, stream);
+  if constexpr (sizeof(T) == 2)
+    if (l.elements == 2) return forward_rows<T, 2>(a, l, sms, stream);
+  return forward_rows<T, 1>(a, l, sms, stream);
+}
+
+template <typename T, int N, bool kScaleColumns>
+int backward_rows(const Backward& b, const Layout& l, void* stream) {
+  const dim3 grid(static_cast<unsigned>(b.plan.blocks * l.cluster));
+  if (l.owner == kWarpRow)
+    return launch(norm_backward_kernel<T, N, kWarpRow, kScaleColumns>, grid, l.threads, 0, 1, stream, b);
+  if (l.owner == kBlockRow)
+    return launch(norm_backward_kernel<T, N, kBlockRow, kScaleColumns>, grid, l.threads, 0, 1, stream, b);
+  return launch(norm_backward_kernel<T, N, kClusterRow, kScaleColumns>, grid, l.threads, 0, l.cluster,
+                stream, b);
+}
+
+template <typename T, int N>
+int backward_rows(const Backward& b, const Layout& l, void* stream) {
+  return b.a.scale_count > 1 ? backward_rows<T, N, true>(b, l, stream)
+                             : backward_rows<T, N, false>(b, l, stream);
 }
 
 template <typename T>
-int backward(const Backward& b, void* stream) {
-  return launch(norm_backward_row_kernel<T>, dim3(static_cast<unsigned>(b.plan.blocks)), kThreads,
-                0, 1, stream, b);
+int backward(const Backward& b, const Layout& l, void* stream) {
+  if (l.elements == 0)
+    return launch(norm_backward_row_kernel<T>, dim3(static_cast<unsigned>(b.plan.blocks)), kThreads,
+                  0, 1, stream, b);
+  if (l.elements == kVec<T>) return backward_rows<T, kVec<T>>(b, l, stream);
+  if constexpr (sizeof(T) == 2)
+    if (l.elements == 2) return backward_rows<T, 2>(b, l, stream);
+  return backward_rows<T, 1>(b, l, stream);
 }
 
 }  // namespace
@@ -355,9 +863,10 @@ int muon_train_residual_norm_sm100(const muon_train_norm_args* args, void* strea
 size_t muon_train_residual_norm_workspace_bytes(const muon_train_norm_args* args) {
   using namespace muon_train;
   int64_t target = 0;
-  if (check(args) != MUON_POLAR_OK || args->rows == 0 || target_blocks(&target) != MUON_POLAR_OK)
-    return 0;
-  return make_plan(normalised(*args), target).bytes;
+  if (check(args) != MUON_POLAR_OK || args->rows == 0) return 0;
+  const muon_train_norm_args a = normalised(*args);
+  if (target_workers(make_layout(a, nullptr), &target) != MUON_POLAR_OK) return 0;
+  return make_plan(a, target).bytes;
 }
 
 int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
@@ -371,9 +880,6 @@ int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
       (args->pre_weight != nullptr && grads->grad_normed != nullptr && args->rstd_pre == nullptr) ||
       (args->pre_weight == nullptr && grads->grad_normed != nullptr))
     return MUON_POLAR_ERR_INVALID_ARGUMENT;
-  int64_t target = 0;
-  rc = target_blocks(&target);
-  if (rc != MUON_POLAR_OK) return rc;
   Backward b;
   b.a = normalised(*args);
   b.g = *grads;
@@ -381,7 +887,13 @@ int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
   if (b.a.pre_weight == nullptr) b.g.grad_pre_weight = nullptr;
   if (b.a.gate == nullptr) b.g.grad_gate = nullptr;
   if (b.a.residual_scale == nullptr) b.g.grad_residual_scale = nullptr;
+  b.a.hidden = b.a.normed = nullptr;
+  const Layout layout = make_layout(b.a, &b.g);
+  int64_t target = 0;
+  rc = target_workers(layout, &target);
+  if (rc != MUON_POLAR_OK) return rc;
   b.plan = make_plan(b.a, target);
+  b.scale_rows = b.plan.blocks * (b.a.scale_count == 1 ? layout.cluster : 1);
   if (grads->workspace == nullptr || !aligned16(grads->workspace) ||
       grads->workspace_bytes < b.plan.bytes)
     return MUON_POLAR_ERR_WORKSPACE;
@@ -393,9 +905,9 @@ int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
   b.scale = b.g.grad_residual_scale != nullptr ? reinterpret_cast<float*>(ws + b.plan.scale_off)
                                                : nullptr;
   switch (b.a.dtype) {
-    case MUON_TRAIN_F32: rc = backward<float>(b, stream); break;
-    case MUON_TRAIN_BF16: rc = backward<__nv_bfloat16>(b, stream); break;
-    default: rc = backward<__half>(b, stream); break;
+    case MUON_TRAIN_F32: rc = backward<float>(b, layout, stream); break;
+    case MUON_TRAIN_BF16: rc = backward<__nv_bfloat16>(b, layout, stream); break;
+    default: rc = backward<__half>(b, layout, stream); break;
   }
   if (rc != MUON_POLAR_OK || (b.gain == nullptr && b.pre == nullptr && b.scale == nullptr)) return rc;
   const unsigned columns = static_cast<unsigned>((b.a.width + 31) / 32);

@@ -105,6 +105,89 @@ __device__ __forceinline__ uint4 pack(const float (&v)[kVec<T>]) {
   return pack(v, T());
 }
 
+// N elements as one load or store of N * sizeof(T) bytes: 16 bytes where rows
+// keep that alignment, else pairs or single elements.
+template <int kBytes>
+struct RawOf;
+template <>
+struct RawOf<16> { using type = uint4; };
+template <>
+struct RawOf<8> { using type = uint2; };
+template <>
+struct RawOf<4> { using type = uint32_t; };
+template <>
+struct RawOf<2> { using type = uint16_t; };
+
+template <typename T, int N>
+struct Elements {
+  using Raw = typename RawOf<N * static_cast<int>(sizeof(T))>::type;
+  static __device__ __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  static __device__ __forceinline__ void store(T* p, const Raw& r) { *reinterpret_cast<Raw*>(p) = r; }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[N]) {
+    if constexpr (sizeof(Raw) == 16) {
+      muon_train::unpack<T>(r, v);
+    } else {
+      const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float (&v)[N]) {
+    if constexpr (sizeof(Raw) == 16) {
+      return muon_train::pack<T>(v);
+    } else {
+      Raw r;
+      T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = from_float<T>(v[i]);
+      return r;
+    }
+  }
+};
+
+// N elements from index i on of a parameter whose type is known at run time;
+// i is a multiple of N and the array aligned to 16 bytes (N > 1).
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, int64_t i, float (&v)[N]) {
+  constexpr int kPart = N * sizeof(T) > 16 ? 16 / static_cast<int>(sizeof(T)) : N;
+#pragma unroll
+  for (int j = 0; j < N; j += kPart) {
+    float part[kPart];
+    Elements<T, kPart>::unpack(Elements<T, kPart>::load(p + i + j), part);
+#pragma unroll
+    for (int l = 0; l < kPart; ++l) v[j + l] = part[l];
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_any(const void* p, int dtype, int64_t i, float (&v)[N]) {
+  if (dtype == MUON_TRAIN_F32)
+    load_run<float, N>(static_cast<const float*>(p), i, v);
+  else if (dtype == MUON_TRAIN_BF16)
+    load_run<__nv_bfloat16, N>(static_cast<const __nv_bfloat16*>(p), i, v);
+  else
+    load_run<__half, N>(static_cast<const __half*>(p), i, v);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T* p, int64_t i, const float (&v)[N]) {
+  constexpr int kPart = N * sizeof(T) > 16 ? 16 / static_cast<int>(sizeof(T)) : N;
+#pragma unroll
+  for (int j = 0; j < N; j += kPart) {
+    float part[kPart];
+#pragma unroll
+    for (int l = 0; l < kPart; ++l) part[l] = v[j + l];
+    Elements<T, kPart>::store(p + i + j, Elements<T, kPart>::pack(part));
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, const float (&v)[N]) {
+  if (dtype == MUON_TRAIN_F32)
+    store_run<float, N>(static_cast<float*>(p), i, v);
+  else if (dtype == MUON_TRAIN_BF16)
+    store_run<__nv_bfloat16, N>(static_cast<__nv_bfloat16*>(p), i, v);
+  else
+    store_run<__half, N>(static_cast<__half*>(p), i, v);
+}
+
 // ------------------------------------------------------------ arithmetic
 // 2^x in one instruction (ex2.approx: at most 2 ulp; 2^-inf = 0).
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -113,6 +196,43 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+
+// Two fp32 operations in one instruction, each rounded as alone.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// The largest element of a vector, joined to m; NaN elements are passed over.
+__device__ __forceinline__ float vector_max(const uint4& u, float m, float) {
+  return fmaxf(fmaxf(fmaxf(m, __uint_as_float(u.x)), fmaxf(__uint_as_float(u.y), __uint_as_float(u.z))),
+               __uint_as_float(u.w));
+}
+template <typename Pair>
+__device__ __forceinline__ Pair vector_max2(const uint4& u) {
+  const Pair* p = reinterpret_cast<const Pair*>(&u);
+  return __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+}
+__device__ __forceinline__ float vector_max(const uint4& u, float m, __nv_bfloat16) {
+  const float2 f = __bfloat1622float2(vector_max2<__nv_bfloat162>(u));
+  return fmaxf(m, fmaxf(f.x, f.y));
+}
+__device__ __forceinline__ float vector_max(const uint4& u, float m, __half) {
+  const float2 f = __half22float2(vector_max2<__half2>(u));
+  return fmaxf(m, fmaxf(f.x, f.y));
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -63,12 +63,14 @@ void NoSecondOrder(const char* who) {
 }
 
 // ------------------------------------------------------------ distillation
-// Rows of logits as they are when their elements are contiguous and the rows
-// do not overlap (a slice of padded logits is read in place).
+// [..., n] as [rows, n], read in place when the elements of a row are
+// contiguous and the rows are evenly spaced and apart (a slice of padded
+// logits), else copied.
 Tensor Rows2d(const Tensor& t) {
-  const bool in_place = (t.size(1) <= 1 || t.stride(1) == 1) &&
-                        (t.size(0) <= 1 || t.stride(0) >= t.size(1));
-  return in_place ? t : t.contiguous();
+  const int64_t n = t.size(-1);
+  const Tensor rows = t.dim() == 2 ? t : t.reshape({n > 0 ? t.numel() / n : 0, n});
+  const bool in_place = (n <= 1 || rows.stride(1) == 1) && (rows.size(0) <= 1 || rows.stride(0) >= n);
+  return in_place ? rows : rows.contiguous();
 }
 int64_t RowStride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
@@ -80,8 +82,21 @@ Tensor GradLike(const Tensor& z) {
   if (rows == 0 || ld > 2 * cols) return at::empty({rows, cols}, z.options());
   const int64_t item = z.element_size();
   const int64_t shift = static_cast<int64_t>(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / item;
+  if (ld == cols && shift == 0) return at::empty({rows, cols}, z.options());
   const int64_t used = (rows - 1) * ld + cols;
   return at::empty({used + shift}, z.options()).as_strided({rows, cols}, {ld, 1}, shift);
+}
+
+at::IntArrayRef Lead(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
+
+// One fp32 value for each row.
+Tensor RowValues(const OptTensor& t, const Tensor& like, const char* who, const char* name) {
+  if (!Given(t).defined()) return Tensor();
+  CheckDevice(*t, like, who, name);
+  TORCH_CHECK_VALUE(t->sizes() == Lead(like), who, ": ", name, " must have shape ", Lead(like),
+                    ", got ", t->sizes());
+  TORCH_CHECK_TYPE(t->is_floating_point(), who, ": ", name, " must be a floating tensor");
+  return t->to(at::kFloat).contiguous();
 }
 
 struct DistillInputs {
@@ -92,12 +107,15 @@ struct DistillInputs {
 DistillInputs CheckDistill(const Tensor& student, const Tensor& values, const Tensor& indices,
                            const OptTensor& teacher_lse, double temperature, const char* who) {
   CheckCuda(student, who, "student_logits");
-  TORCH_CHECK_VALUE(student.dim() == 2 && values.dim() == 2 && student.size(1) > 0,
-                    who, ": student_logits must have shape [rows, vocab] and teacher_logits [rows, top]");
-  TORCH_CHECK_VALUE(values.size(0) == student.size(0) && indices.sizes() == values.sizes(), who,
-                    ": teacher_logits and teacher_indices must have one list for each row");
-  TORCH_CHECK_VALUE(values.size(1) >= 1 && values.size(1) <= MUON_TRAIN_MAX_TOP, who,
-                    ": a list must have 1 to ", MUON_TRAIN_MAX_TOP, " entries, got ", values.size(1));
+  TORCH_CHECK_VALUE(student.dim() >= 1 && student.size(-1) > 0, who,
+                    ": student_logits must have shape [..., vocab], got ", student.sizes());
+  TORCH_CHECK_VALUE(values.dim() == student.dim() && indices.sizes() == values.sizes() &&
+                        Lead(values) == Lead(student),
+                    who, ": teacher_logits and teacher_indices must both have shape [..., top] with "
+                    "student_logits' leading sizes, got ", values.sizes(), " and ", indices.sizes());
+  const int64_t top = values.size(-1);
+  TORCH_CHECK_VALUE(top >= 1 && top <= MUON_TRAIN_MAX_TOP, who, ": a list must have 1 to ",
+                    MUON_TRAIN_MAX_TOP, " entries, got ", top);
   CheckDevice(values, student, who, "teacher_logits");
   CheckDevice(indices, student, who, "teacher_indices");
   TORCH_CHECK_TYPE(indices.scalar_type() == at::kLong || indices.scalar_type() == at::kInt, who,
@@ -105,27 +123,20 @@ DistillInputs CheckDistill(const Tensor& student, const Tensor& values, const Te
   TORCH_CHECK_VALUE(static_cast<float>(temperature) > 0.f && std::isfinite(static_cast<float>(temperature)), who,
                     ": temperature must be positive and finite, got ", temperature);
   DistillInputs in;
-  const Tensor& lse = Given(teacher_lse);
-  if (lse.defined()) {
-    CheckDevice(lse, student, who, "teacher_lse");
-    TORCH_CHECK_VALUE(lse.dim() == 1 && lse.size(0) == student.size(0), who,
-                      ": teacher_lse must have one value for each row");
-    TORCH_CHECK_TYPE(lse.is_floating_point(), who, ": teacher_lse must be a floating tensor");
-    in.lse = lse.to(at::kFloat).contiguous();
-  }
   in.args.dtype = Dtype(student, who, "student_logits");
   in.args.teacher_dtype = Dtype(values, who, "teacher_logits");
+  in.lse = RowValues(teacher_lse, student, who, "teacher_lse");
   in.student = Rows2d(student);
   in.values = values.contiguous();
   in.indices = indices.contiguous();
   in.args.logits = Ptr(in.student);
-  in.args.rows = student.size(0);
-  in.args.vocab = student.size(1);
+  in.args.rows = in.student.size(0);
+  in.args.vocab = in.student.size(1);
   in.args.ld = RowStride(in.student);
   in.args.teacher_logits = Ptr(in.values);
   in.args.teacher_indices = Ptr(in.indices);
   in.args.teacher_lse = static_cast<const float*>(Ptr(in.lse));
-  in.args.top = values.size(1);
+  in.args.top = top;
   in.args.temperature = static_cast<float>(temperature);
   in.args.index_bytes = indices.scalar_type() == at::kLong ? 8 : 4;
   return in;
@@ -138,7 +149,7 @@ std::tuple<Tensor, Tensor> DistillCuda(const Tensor& student, const Tensor& valu
   DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
   const c10::cuda::CUDAGuard guard(student.device());
   const auto f32 = student.options().dtype(at::kFloat);
-  Tensor loss = at::empty({student.size(0)}, f32), stats = at::empty({student.size(0), 2}, f32);
+  Tensor loss = at::empty(Lead(student), f32), stats = at::empty({in.args.rows, 2}, f32);
   in.args.loss = static_cast<float*>(Ptr(loss));
   in.args.stats = static_cast<float*>(Ptr(stats));
   CheckStatus(muon_train_distill_sm100(&in.args, Stream(student)), who);
@@ -150,21 +161,19 @@ Tensor DistillBackwardCuda(const Tensor& grad_loss, const Tensor& student, const
                            double temperature) {
   const char* who = "distill_topk_backward";
   DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
-  TORCH_CHECK_VALUE(grad_loss.dim() == 1 && grad_loss.size(0) == student.size(0) &&
-                        stats.dim() == 2 && stats.size(0) == student.size(0) && stats.size(1) == 2,
-                    who, ": grad_loss and stats must have a row for each row of student_logits");
-  CheckDevice(grad_loss, student, who, "grad_loss");
+  TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == in.args.rows && stats.size(1) == 2, who,
+                    ": stats must have shape [rows, 2]");
   CheckDevice(stats, student, who, "stats");
   TORCH_CHECK_TYPE(stats.scalar_type() == at::kFloat, who, ": stats must be float32");
   const c10::cuda::CUDAGuard guard(student.device());
-  const Tensor scale = grad_loss.to(at::kFloat).contiguous(), kept = stats.contiguous();
+  const Tensor scale = RowValues(grad_loss, student, who, "grad_loss"), kept = stats.contiguous();
   Tensor grad = GradLike(in.student);
   in.args.row_scale = static_cast<const float*>(Ptr(scale));
   in.args.stats = static_cast<float*>(Ptr(kept));
   in.args.grad = Ptr(grad);
   in.args.ld_grad = RowStride(grad);
   CheckStatus(muon_train_distill_backward_sm100(&in.args, Stream(student)), who);
-  return grad;
+  return student.dim() == 2 ? grad : grad.view(student.sizes());
 }
 
 std::tuple<Tensor, Tensor> DistillGradCuda(const Tensor& student, const Tensor& values,
@@ -173,22 +182,17 @@ std::tuple<Tensor, Tensor> DistillGradCuda(const Tensor& student, const Tensor& 
   const char* who = "distill_topk_grad";
   DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
   const c10::cuda::CUDAGuard guard(student.device());
-  Tensor scale;
-  if (Given(row_scale).defined()) {
-    CheckDevice(*row_scale, student, who, "row_scale");
-    TORCH_CHECK_VALUE(row_scale->dim() == 1 && row_scale->size(0) == student.size(0), who,
-                      ": row_scale must have one value for each row");
-    TORCH_CHECK_TYPE(row_scale->is_floating_point(), who, ": row_scale must be a floating tensor");
-    scale = row_scale->to(at::kFloat).contiguous();
-  }
-  Tensor loss = at::empty({student.size(0)}, student.options().dtype(at::kFloat));
+  const Tensor scale = RowValues(row_scale, student, who, "row_scale");
+  const auto f32 = student.options().dtype(at::kFloat);
+  Tensor loss = at::empty(Lead(student), f32), stats = at::empty({in.args.rows, 2}, f32);
   Tensor grad = GradLike(in.student);
   in.args.row_scale = static_cast<const float*>(Ptr(scale));
   in.args.loss = static_cast<float*>(Ptr(loss));
+  in.args.stats = static_cast<float*>(Ptr(stats));
   in.args.grad = Ptr(grad);
   in.args.ld_grad = RowStride(grad);
   CheckStatus(muon_train_distill_sm100(&in.args, Stream(student)), who);
-  return {loss, grad};
+  return {loss, student.dim() == 2 ? grad : grad.view(student.sizes())};
 }
 
 // ------------------------------------------------------------ residual norm
@@ -197,26 +201,45 @@ struct NormInputs {
   muon_train_norm_args args{};
 };
 
+// Rows of the gate: its leading sizes are block_out's up to some axis and 1
+// from there on, or it is one row; -1 for any other shape.
+int64_t GateRows(const Tensor& gate, const Tensor& block_out) {
+  const int64_t n = gate.dim() - 1;
+  if (n < 0 || gate.size(-1) != block_out.size(-1)) return -1;
+  int64_t rows = 1, same = 0;
+  for (int64_t i = 0; i < n; ++i) rows *= gate.size(i);
+  const auto ones_from = [&](int64_t i) {
+    while (i < n && gate.size(i) == 1) ++i;
+    return i == n;
+  };
+  if (ones_from(0)) return 1;
+  if (n != block_out.dim() - 1) return -1;
+  while (same < n && gate.size(same) == block_out.size(same)) ++same;
+  return ones_from(same) ? rows : -1;
+}
+
 NormInputs CheckNorm(const Tensor& block_out, const Tensor& residual, const OptTensor& post,
                      const OptTensor& pre, const OptTensor& gate, const OptTensor& scale,
                      double eps, const char* who) {
   CheckCuda(block_out, who, "block_out");
   CheckDevice(residual, block_out, who, "residual");
-  TORCH_CHECK_VALUE(block_out.dim() == 2 && block_out.size(1) > 0, who,
-                    ": block_out must have shape [rows, width]");
-  TORCH_CHECK_VALUE(residual.sizes() == block_out.sizes(), who,
-                    ": residual must have block_out's shape");
+  TORCH_CHECK_VALUE(block_out.dim() >= 1 && block_out.size(-1) > 0, who,
+                    ": block_out must have shape [..., width], got ", block_out.sizes());
+  TORCH_CHECK_VALUE(residual.sizes() == block_out.sizes(), who, ": residual must have block_out's shape ",
+                    block_out.sizes(), ", got ", residual.sizes());
   TORCH_CHECK_TYPE(residual.scalar_type() == block_out.scalar_type(), who,
-                   ": residual must have block_out's dtype");
+                   ": residual must have block_out's dtype ", block_out.scalar_type(), ", got ",
+                   residual.scalar_type());
   TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), who, ": eps must be finite and not negative, got ", eps);
-  const int64_t rows = block_out.size(0), width = block_out.size(1);
+  const int64_t width = block_out.size(-1);
   NormInputs in;
   auto& a = in.args;
   const auto weight = [&](const OptTensor& w, const char* name, Tensor* to, int* dtype) {
     const Tensor& t = Given(w);
     if (!t.defined()) return;
     CheckDevice(t, block_out, who, name);
-    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == width, who, ": ", name, " must have shape [width]");
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == width, who, ": ", name, " must have shape [", width,
+                      "], got ", t.sizes());
     *dtype = Dtype(t, who, name);
     *to = t.contiguous();
   };
@@ -225,19 +248,19 @@ NormInputs CheckNorm(const Tensor& block_out, const Tensor& residual, const OptT
   weight(pre, "pre_weight", &in.pre, &a.pre_dtype);
   if (Given(gate).defined()) {
     CheckDevice(*gate, block_out, who, "gate");
-    TORCH_CHECK_VALUE(gate->dim() == 2 && gate->size(1) == width && (rows == 0 || (gate->size(0) > 0 && rows % gate->size(0) == 0)),
-                      who, ": gate must have shape [gate_rows, width], gate_rows dividing the rows");
+    a.gate_rows = GateRows(*gate, block_out);
+    TORCH_CHECK_VALUE(a.gate_rows >= 0, who, ": gate must have shape [", width, "] or ", block_out.sizes(),
+                      " with trailing leading sizes of 1, got ", gate->sizes());
     a.gate_dtype = Dtype(*gate, who, "gate");
     in.gate = gate->contiguous();
-    a.gate_rows = gate->size(0);
   }
   if (Given(scale).defined()) {
     CheckDevice(*scale, block_out, who, "residual_scale");
-    TORCH_CHECK_VALUE(scale->dim() == 1 && (scale->size(0) == 1 || scale->size(0) == width), who,
-                      ": residual_scale must have one element or shape [width]");
+    TORCH_CHECK_VALUE(scale->numel() == 1 || (scale->dim() == 1 && scale->size(0) == width), who,
+                      ": residual_scale must have one element or shape [", width, "], got ", scale->sizes());
     a.scale_dtype = Dtype(*scale, who, "residual_scale");
     in.scale = scale->contiguous();
-    a.scale_count = scale->size(0);
+    a.scale_count = scale->numel();
   }
   in.block_out = block_out.contiguous();
   in.residual = residual.contiguous();
@@ -247,32 +270,31 @@ NormInputs CheckNorm(const Tensor& block_out, const Tensor& residual, const OptT
   a.pre_weight = Ptr(in.pre);
   a.gate = Ptr(in.gate);
   a.residual_scale = Ptr(in.scale);
-  a.rows = rows;
+  a.rows = block_out.numel() / width;
   a.width = width;
   a.eps = static_cast<float>(eps);
   return in;
 }
 
-// (hidden, normed, rstd_post, rstd_pre); what is not computed is empty.
-std::tuple<Tensor, Tensor, Tensor, Tensor> ResidualNormCuda(
+// (hidden, normed, rstd): rstd holds the two statistics of each row, [2,
+// rows].  Without pre_weight normed is empty.
+std::tuple<Tensor, Tensor, Tensor> ResidualNormCuda(
     const Tensor& block_out, const Tensor& residual, const OptTensor& post, const OptTensor& pre,
     const OptTensor& gate, const OptTensor& scale, double eps) {
   const char* who = "residual_norm";
   NormInputs in = CheckNorm(block_out, residual, post, pre, gate, scale, eps, who);
   const c10::cuda::CUDAGuard guard(block_out.device());
   const auto options = in.block_out.options();
-  const auto f32 = options.dtype(at::kFloat);
   const int64_t rows = in.args.rows;
-  Tensor hidden = at::empty({rows, in.args.width}, options);
-  Tensor normed = at::empty({in.pre.defined() ? rows : 0, in.args.width}, options);
-  Tensor rstd_post = at::empty({in.post.defined() ? rows : 0}, f32);
-  Tensor rstd_pre = at::empty({in.pre.defined() ? rows : 0}, f32);
+  Tensor hidden = at::empty(block_out.sizes(), options);
+  Tensor normed = in.pre.defined() ? at::empty(block_out.sizes(), options) : at::empty({0}, options);
+  Tensor rstd = at::empty({2, rows}, options.dtype(at::kFloat));
   in.args.hidden = Ptr(hidden);
-  in.args.normed = Ptr(normed);
-  in.args.rstd_post = static_cast<float*>(Ptr(rstd_post));
-  in.args.rstd_pre = static_cast<float*>(Ptr(rstd_pre));
+  in.args.normed = in.pre.defined() ? Ptr(normed) : nullptr;
+  in.args.rstd_post = static_cast<float*>(Ptr(rstd));
+  in.args.rstd_pre = in.args.rstd_post + rows;
   CheckStatus(muon_train_residual_norm_sm100(&in.args, Stream(block_out)), who);
-  return {hidden, normed, rstd_post, rstd_pre};
+  return {hidden, normed, rstd};
 }
 
 // Gradients of (block_out, residual, post_weight, pre_weight, gate,
@@ -280,8 +302,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> ResidualNormCuda(
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> ResidualNormBackwardCuda(
     const OptTensor& grad_hidden, const OptTensor& grad_normed, const Tensor& block_out,
     const Tensor& residual, const OptTensor& post, const OptTensor& pre, const OptTensor& gate,
-    const OptTensor& scale, const Tensor& rstd_post, const Tensor& rstd_pre, double eps,
-    std::array<bool, 6> wanted) {
+    const OptTensor& scale, const Tensor& rstd, double eps, std::array<bool, 6> wanted) {
   const char* who = "residual_norm_backward";
   NormInputs in = CheckNorm(block_out, residual, post, pre, gate, scale, eps, who);
   const c10::cuda::CUDAGuard guard(block_out.device());
@@ -295,17 +316,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> ResidualNormBackwardC
     return g->contiguous();
   };
   const Tensor dh = upstream(grad_hidden, "grad_hidden"), dn = upstream(grad_normed, "grad_normed");
-  const auto rstd = [&](const Tensor& t, bool needed, const char* name) -> Tensor {
-    if (!needed) return Tensor();
-    CheckDevice(t, block_out, who, name);
-    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, who, ": ", name, " must be float32");
-    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == rows, who, ": ", name, " must have one value for each row");
-    return t.contiguous();
-  };
-  const Tensor rp = rstd(rstd_post, in.post.defined(), "rstd_post");
-  const Tensor rn = rstd(rstd_pre, in.pre.defined(), "rstd_pre");
-  in.args.rstd_post = static_cast<float*>(Ptr(rp));
-  in.args.rstd_pre = static_cast<float*>(Ptr(rn));
+  CheckDevice(rstd, block_out, who, "rstd");
+  TORCH_CHECK_TYPE(rstd.scalar_type() == at::kFloat, who, ": rstd must be float32");
+  TORCH_CHECK_VALUE(rstd.dim() == 2 && rstd.size(0) == 2 && rstd.size(1) == rows, who,
+                    ": rstd must have shape [2, rows]");
+  const Tensor kept = rstd.contiguous();
+  in.args.rstd_post = static_cast<float*>(Ptr(kept));
+  in.args.rstd_pre = in.args.rstd_post + rows;
   const Tensor* like[6] = {&in.block_out, &in.residual, &in.post, &in.pre, &in.gate, &in.scale};
   std::array<Tensor, 6> out;
   const bool none = rows == 0 || (!dh.defined() && !dn.defined());
@@ -313,22 +330,23 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> ResidualNormBackwardC
     if (!wanted[i] || !like[i]->defined())
       out[i] = at::empty({0}, in.block_out.options());
     else
-      out[i] = none ? at::zeros_like(*like[i]) : at::empty_like(*like[i]);
+      out[i] = none ? at::zeros(like[i]->sizes(), like[i]->options())
+                    : at::empty(like[i]->sizes(), like[i]->options());
   }
-  const auto result = [&] { return std::make_tuple(out[0], out[1], out[2], out[3], out[4], out[5]); };
-  if (none) return result();
-  muon_train_norm_grads g{};
-  g.grad_hidden = Ptr(dh);
-  g.grad_normed = Ptr(dn);
-  void** to[6] = {&g.grad_block_out, &g.grad_residual, &g.grad_post_weight,
-                  &g.grad_pre_weight, &g.grad_gate, &g.grad_residual_scale};
-  for (int i = 0; i < 6; ++i) *to[i] = wanted[i] && like[i]->defined() ? Ptr(out[i]) : nullptr;
-  g.workspace_bytes = muon_train_residual_norm_workspace_bytes(&in.args);
-  const Tensor workspace = at::empty({static_cast<int64_t>(g.workspace_bytes)},
-                                     in.block_out.options().dtype(at::kByte));
-  g.workspace = Ptr(workspace);
-  CheckStatus(muon_train_residual_norm_backward_sm100(&in.args, &g, Stream(block_out)), who);
-  return result();
+  if (!none) {
+    muon_train_norm_grads g{};
+    g.grad_hidden = Ptr(dh);
+    g.grad_normed = Ptr(dn);
+    void** to[6] = {&g.grad_block_out, &g.grad_residual, &g.grad_post_weight,
+                    &g.grad_pre_weight, &g.grad_gate, &g.grad_residual_scale};
+    for (int i = 0; i < 6; ++i) *to[i] = wanted[i] && like[i]->defined() ? Ptr(out[i]) : nullptr;
+    g.workspace_bytes = muon_train_residual_norm_workspace_bytes(&in.args);
+    const Tensor workspace = at::empty({static_cast<int64_t>(g.workspace_bytes)},
+                                       in.block_out.options().dtype(at::kByte));
+    g.workspace = Ptr(workspace);
+    CheckStatus(muon_train_residual_norm_backward_sm100(&in.args, &g, Stream(block_out)), who);
+  }
+  return {out[0], out[1], out[2], out[3], out[4], out[5]};
 }
 
 // ------------------------------------------------------------ routing
@@ -336,8 +354,9 @@ muon_train_route_args CheckRoute(const Tensor& logits, int64_t k, int64_t score,
                                  int64_t top_groups, int64_t group_top, bool renormalize,
                                  double scale, Tensor* rows, const char* who) {
   CheckCuda(logits, who, "logits");
-  TORCH_CHECK_VALUE(logits.dim() == 2, who, ": logits must have shape [tokens, experts]");
-  const int64_t experts = logits.size(1);
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, who,
+                    ": logits must have shape [..., experts], got ", logits.sizes());
+  const int64_t experts = logits.size(-1);
   TORCH_CHECK_VALUE(experts >= 1 && experts <= MUON_TRAIN_MAX_EXPERTS, who, ": 1 to ",
                     MUON_TRAIN_MAX_EXPERTS, " experts are supported, got ", experts);
   TORCH_CHECK_VALUE(score == 0 || score == 1, who, ": score must be 0 (softmax) or 1 (sigmoid)");
@@ -354,7 +373,7 @@ muon_train_route_args CheckRoute(const Tensor& logits, int64_t k, int64_t score,
   *rows = Rows2d(logits);
   muon_train_route_args a{};
   a.logits = Ptr(*rows);
-  a.tokens = logits.size(0);
+  a.tokens = rows->size(0);
   a.experts = experts;
   a.ld = RowStride(*rows);
   a.dtype = Dtype(logits, who, "logits");
@@ -379,14 +398,16 @@ std::tuple<Tensor, Tensor, Tensor> RouteCuda(const Tensor& logits, const OptTens
   if (Given(bias).defined()) {
     CheckDevice(*bias, logits, who, "bias");
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == a.experts, who,
-                      ": bias must have shape [experts]");
+                      ": bias must have shape [", a.experts, "], got ", bias->sizes());
     TORCH_CHECK_TYPE(bias->is_floating_point(), who, ": bias must be a floating tensor");
     b = bias->to(at::kFloat).contiguous();
     a.bias = static_cast<const float*>(Ptr(b));
   }
   const auto i64 = logits.options().dtype(at::kLong);
-  Tensor weights = at::empty({a.tokens, k}, logits.options().dtype(at::kFloat));
-  Tensor indices = at::empty({a.tokens, k}, i64), counts = at::empty({a.experts}, i64);
+  at::DimVector shape(Lead(logits));
+  shape.push_back(k);
+  Tensor weights = at::empty(shape, logits.options().dtype(at::kFloat));
+  Tensor indices = at::empty(shape, i64), counts = at::empty({a.experts}, i64);
   a.weights = static_cast<float*>(Ptr(weights));
   a.indices = static_cast<int64_t*>(Ptr(indices));
   a.counts = static_cast<int64_t*>(Ptr(counts));
@@ -397,18 +418,18 @@ std::tuple<Tensor, Tensor, Tensor> RouteCuda(const Tensor& logits, const OptTens
 Tensor RouteBackwardCuda(const Tensor& grad_weights, const Tensor& logits, const Tensor& indices,
                          int64_t score, bool renormalize, double scale) {
   const char* who = "route_experts_backward";
-  TORCH_CHECK_VALUE(indices.dim() == 2 && logits.dim() == 2 && indices.size(0) == logits.size(0) &&
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && indices.dim() == logits.dim() && Lead(indices) == Lead(logits) &&
                         grad_weights.sizes() == indices.sizes(),
-                    who, ": indices and grad_weights must have shape [tokens, k]");
+                    who, ": indices and grad_weights must have shape [..., k]");
   TORCH_CHECK_TYPE(indices.scalar_type() == at::kLong, who, ": indices must be int64");
   Tensor rows;
-  muon_train_route_args a = CheckRoute(logits, indices.size(1), score, 1, 1, 1, renormalize, scale, &rows, who);
+  muon_train_route_args a = CheckRoute(logits, indices.size(-1), score, 1, 1, 1, renormalize, scale, &rows, who);
   CheckDevice(grad_weights, logits, who, "grad_weights");
   CheckDevice(indices, logits, who, "indices");
   const c10::cuda::CUDAGuard guard(logits.device());
   const Tensor g = grad_weights.to(at::kFloat).contiguous(), chosen = indices.contiguous();
   a.indices = static_cast<int64_t*>(Ptr(chosen));
-  Tensor grad = at::empty({a.tokens, a.experts}, logits.options());
+  Tensor grad = at::empty(logits.sizes(), logits.options());
   CheckStatus(muon_train_route_backward_sm100(&a, static_cast<const float*>(Ptr(g)), Ptr(grad),
                                               Stream(logits)), who);
   return grad;
@@ -437,6 +458,7 @@ class DistillFunction : public torch::autograd::Function<DistillFunction> {
     auto [loss, stats] = op.call(student, values, indices, lse, temperature);
     ctx->save_for_backward({student, values, indices, Given(lse), stats});
     ctx->saved_data["temperature"] = temperature;
+    ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({stats});
     return {loss, stats};
   }
@@ -466,6 +488,15 @@ std::tuple<Tensor, Tensor> DistillAutograd(const Tensor& student, const Tensor& 
   return {out[0], out[1]};
 }
 
+// The loss with its gradient is not recorded: nothing flows back through it.
+std::tuple<Tensor, Tensor> DistillGradAutograd(const Tensor& student, const Tensor& values,
+                                               const Tensor& indices, const OptTensor& row_scale,
+                                               const OptTensor& lse, double temperature) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  static auto op = Op<decltype(DistillGradCuda)>("muon_ascend950::distill_topk_grad");
+  return op.call(student, values, indices, row_scale, lse, temperature);
+}
+
 class ResidualNormFunction : public torch::autograd::Function<ResidualNormFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& block_out, const Tensor& residual,
@@ -473,9 +504,8 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
                                const OptTensor& scale, double eps) {
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = Op<decltype(ResidualNormCuda)>("muon_ascend950::residual_norm");
-    auto [hidden, normed, rstd_post, rstd_pre] = op.call(block_out, residual, post, pre, gate, scale, eps);
-    ctx->save_for_backward({block_out, residual, Given(post), Given(pre), Given(gate), Given(scale),
-                            rstd_post, rstd_pre});
+    auto [hidden, normed, rstd] = op.call(block_out, residual, post, pre, gate, scale, eps);
+    ctx->save_for_backward({block_out, residual, Given(post), Given(pre), Given(gate), Given(scale), rstd});
     ctx->saved_data["eps"] = eps;
     const Tensor* inputs[6] = {&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)};
     int64_t wanted = 0;  // a bit for each input that takes a gradient
@@ -483,8 +513,11 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
       if (inputs[i]->defined() && inputs[i]->requires_grad()) wanted |= int64_t{1} << i;
     ctx->saved_data["wanted"] = wanted;
     ctx->set_materialize_grads(false);
-    ctx->mark_non_differentiable({rstd_post, rstd_pre});
-    return {hidden, normed, rstd_post, rstd_pre};
+    if (Given(pre).defined())
+      ctx->mark_non_differentiable({rstd});
+    else
+      ctx->mark_non_differentiable({normed, rstd});
+    return {hidden, normed, rstd};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     NoSecondOrder("residual_norm");
@@ -496,7 +529,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
     static auto op = Op<decltype(ResidualNormBackwardCuda)>("muon_ascend950::residual_norm_backward");
     const OptTensor dn = s[3].defined() ? opt(grads[1]) : OptTensor();
     auto [d0, d1, d2, d3, d4, d5] = op.call(opt(grads[0]), dn, s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]),
-                                            opt(s[5]), s[6], s[7], ctx->saved_data["eps"].toDouble(), wanted);
+                                            opt(s[5]), s[6], ctx->saved_data["eps"].toDouble(), wanted);
     const Tensor all[6] = {d0, d1, d2, d3, d4, d5};
     variable_list out(7);
     for (size_t i = 0; i < 6; ++i)
@@ -505,7 +538,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> ResidualNormAutograd(
+std::tuple<Tensor, Tensor, Tensor> ResidualNormAutograd(
     const Tensor& block_out, const Tensor& residual, const OptTensor& post, const OptTensor& pre,
     const OptTensor& gate, const OptTensor& scale, double eps) {
   if (!Recorded({&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)})) {
@@ -514,7 +547,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> ResidualNormAutograd(
     return op.call(block_out, residual, post, pre, gate, scale, eps);
   }
   auto out = ResidualNormFunction::apply(block_out, residual, post, pre, gate, scale, eps);
-  return {out[0], out[1], out[2], out[3]};
+  return {out[0], out[1], out[2]};
 }
 
 class RouteFunction : public torch::autograd::Function<RouteFunction> {
@@ -530,6 +563,7 @@ class RouteFunction : public torch::autograd::Function<RouteFunction> {
     ctx->saved_data["score"] = score;
     ctx->saved_data["renormalize"] = renormalize;
     ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({indices, counts});
     return {weights, indices, counts};
   }
@@ -568,11 +602,10 @@ TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
   m.def("distill_topk_grad(Tensor student_logits, Tensor teacher_logits, Tensor teacher_indices, "
         "Tensor? row_scale, Tensor? teacher_lse, float temperature) -> (Tensor loss, Tensor grad)");
   m.def("residual_norm(Tensor block_out, Tensor residual, Tensor? post_weight, Tensor? pre_weight, "
-        "Tensor? gate, Tensor? residual_scale, float eps) -> (Tensor hidden, Tensor normed, "
-        "Tensor rstd_post, Tensor rstd_pre)");
+        "Tensor? gate, Tensor? residual_scale, float eps) -> (Tensor hidden, Tensor normed, Tensor rstd)");
   m.def("residual_norm_backward(Tensor? grad_hidden, Tensor? grad_normed, Tensor block_out, "
         "Tensor residual, Tensor? post_weight, Tensor? pre_weight, Tensor? gate, "
-        "Tensor? residual_scale, Tensor rstd_post, Tensor rstd_pre, float eps, bool[6] wanted) -> "
+        "Tensor? residual_scale, Tensor rstd, float eps, bool[6] wanted) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("route_experts(Tensor logits, Tensor? bias, int k, int score, int groups, int top_groups, "
         "int group_top, bool renormalize, float scale) -> (Tensor weights, Tensor indices, Tensor counts)");
@@ -592,6 +625,7 @@ TORCH_LIBRARY_IMPL(muon_ascend950, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(muon_ascend950, Autograd, m) {
   m.impl("distill_topk", &DistillAutograd);
+  m.impl("distill_topk_grad", &DistillGradAutograd);
   m.impl("residual_norm", &ResidualNormAutograd);
   m.impl("route_experts", &RouteAutograd);
 }

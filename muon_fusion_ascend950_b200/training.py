@@ -22,6 +22,9 @@ import torch
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _SCORES = {"softmax": 0, "sigmoid": 1}
+_OPTIONAL = frozenset(("teacher_lse", "row_scale", "post_weight", "pre_weight", "gate", "residual_scale",
+                       "bias"))
+_ops = torch.ops.muon_ascend950
 
 
 def _check(name: str, t, floats: bool = True) -> None:
@@ -33,7 +36,21 @@ def _check(name: str, t, floats: bool = True) -> None:
         raise TypeError(f"{name} must use torch.float32, bfloat16 or float16, got {t.dtype}")
 
 
-def _distill_args(student_logits, teacher_logits, teacher_indices, rows, rows_name):
+def _tensors(**named) -> None:
+    """What must hold before the native operator can be called; it checks
+    shapes, types and devices itself (and the functions below do, where only
+    shapes are traced)."""
+    for name, t in named.items():
+        if t is None and name in _OPTIONAL:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
+
+
+# ------------------------------------------------- checks of traced calls
+def check_distill(student_logits, teacher_logits, teacher_indices, temperature, **rows) -> None:
     _check("student_logits", student_logits)
     _check("teacher_logits", teacher_logits)
     _check("teacher_indices", teacher_indices, floats=False)
@@ -47,20 +64,77 @@ def _distill_args(student_logits, teacher_logits, teacher_indices, rows, rows_na
         raise ValueError("teacher_logits and teacher_indices must both have shape "
                          f"{tuple(lead) + ('top',)}, got {tuple(teacher_logits.shape)} and "
                          f"{tuple(teacher_indices.shape)}")
-    for name, t in zip(rows_name, rows):
+    if not temperature > 0.0:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    for name, t in rows.items():
         if t is not None:
             _check(name, t)
             if t.shape != lead:
                 raise ValueError(f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
-    if student_logits.ndim == 2:
-        return (student_logits, teacher_logits, teacher_indices, *rows)
-    top = teacher_logits.shape[-1]
-    count = lead.numel()
-    return (student_logits.reshape(count, student_logits.shape[-1]),
-            teacher_logits.reshape(count, top), teacher_indices.reshape(count, top),
-            *(t if t is None else t.reshape(count) for t in rows))
 
 
+def gate_rows(gate: torch.Tensor, shape: torch.Size) -> int:
+    """Rows of a gate whose leading sizes are ``shape``'s up to some axis and 1
+    from there on, or which is one row."""
+    if gate.ndim >= 1 and gate.shape[-1] == shape[-1]:
+        lead = tuple(gate.shape[:-1])
+        if all(n == 1 for n in lead):
+            return 1
+        if len(lead) == len(shape) - 1:
+            same = 0
+            while same < len(lead) and lead[same] == shape[same]:
+                same += 1
+            if all(n == 1 for n in lead[same:]):
+                return gate.shape[:-1].numel()
+    raise ValueError(f"gate must have shape [{shape[-1]}] or {tuple(shape)} with trailing leading sizes "
+                     f"of 1, got {tuple(gate.shape)}")
+
+
+def check_norm(block_out, residual, post_weight, pre_weight, gate, residual_scale, eps) -> None:
+    _check("block_out", block_out)
+    _check("residual", residual)
+    if residual.dtype != block_out.dtype:
+        raise TypeError(f"residual must use block_out's {block_out.dtype}, got {residual.dtype}")
+    shape = block_out.shape
+    if block_out.ndim < 1 or shape[-1] < 1:
+        raise ValueError(f"block_out must have shape [..., width], got {tuple(shape)}")
+    if residual.shape != shape:
+        raise ValueError(f"residual must have block_out's shape {tuple(shape)}, got {tuple(residual.shape)}")
+    width = shape[-1]
+    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if w is not None:
+            _check(name, w)
+            if w.shape != (width,):
+                raise ValueError(f"{name} must have shape ({width},), got {tuple(w.shape)}")
+    if gate is not None:
+        _check("gate", gate)
+        gate_rows(gate, shape)
+    if residual_scale is not None:
+        _check("residual_scale", residual_scale)
+        if residual_scale.numel() != 1 and residual_scale.shape != (width,):
+            raise ValueError(f"residual_scale must have one element or shape ({width},), "
+                             f"got {tuple(residual_scale.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+
+
+def check_route(logits, bias, k, groups, top_groups) -> None:
+    _check("logits", logits)
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape [..., experts], got {tuple(logits.shape)}")
+    experts = logits.shape[-1]
+    if bias is not None:
+        _check("bias", bias)
+        if bias.shape != (experts,):
+            raise ValueError(f"bias must have shape ({experts},), got {tuple(bias.shape)}")
+    if groups < 1 or experts % groups or not 1 <= top_groups <= groups:
+        raise ValueError(f"groups must divide the {experts} experts and top_groups be 1 to groups, "
+                         f"got {groups} and {top_groups}")
+    if not 1 <= k <= top_groups * (experts // groups):
+        raise ValueError(f"k must be 1 to the experts of the chosen groups, got {k}")
+
+
+# -------------------------------------------------------------- entry points
 def distill_topk(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
                  teacher_indices: torch.Tensor, *, temperature: float = 1.0,
                  teacher_lse: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -81,10 +155,10 @@ def distill_topk(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
     gradient 0.  Differentiable in ``student_logits``; the teacher's tensors
     are constants.
     """
-    s, t, i, lse = _distill_args(student_logits, teacher_logits, teacher_indices, (teacher_lse,),
-                                 ("teacher_lse",))
-    loss = torch.ops.muon_ascend950.distill_topk(s, t, i, lse, float(temperature))[0]
-    return loss if student_logits.ndim == 2 else loss.reshape(student_logits.shape[:-1])
+    _tensors(student_logits=student_logits, teacher_logits=teacher_logits,
+             teacher_indices=teacher_indices, teacher_lse=teacher_lse)
+    return _ops.distill_topk.default(student_logits, teacher_logits, teacher_indices, teacher_lse,
+                                     float(temperature))[0]
 
 
 def distill_topk_grad(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
@@ -99,31 +173,10 @@ def distill_topk_grad(student_logits: torch.Tensor, teacher_logits: torch.Tensor
     Returns ``(loss, grad)``, the gradient with the logits' shape and type; use
     it as ``student_logits.backward(grad)``.  Not recorded by autograd.
     """
-    with torch.no_grad():
-        s, t, i, scale, lse = _distill_args(student_logits, teacher_logits, teacher_indices,
-                                            (row_scale, teacher_lse), ("row_scale", "teacher_lse"))
-        loss, grad = torch.ops.muon_ascend950.distill_topk_grad(s, t, i, scale, lse, float(temperature))
-        if student_logits.ndim == 2:
-            return loss, grad
-        return loss.reshape(student_logits.shape[:-1]), grad.reshape(student_logits.shape)
-
-
-def _gate_rows(gate: torch.Tensor, shape: torch.Size) -> torch.Tensor:
-    """``gate`` as [gate_rows, width]: its leading sizes are ``shape``'s up to
-    some axis and 1 from there on, or it is one row."""
-    width = shape[-1]
-    if gate.ndim >= 1 and gate.shape[-1] == width:
-        lead = tuple(gate.shape[:-1])
-        if all(n == 1 for n in lead):
-            return gate.reshape(1, width)
-        if len(lead) == len(shape) - 1:
-            same = 0
-            while same < len(lead) and lead[same] == shape[same]:
-                same += 1
-            if all(n == 1 for n in lead[same:]):
-                return gate.reshape(lead and gate.shape[:-1].numel(), width)
-    raise ValueError(f"gate must have shape [{width}] or {tuple(shape)} with trailing leading sizes of 1, "
-                     f"got {tuple(gate.shape)}")
+    _tensors(student_logits=student_logits, teacher_logits=teacher_logits,
+             teacher_indices=teacher_indices, row_scale=row_scale, teacher_lse=teacher_lse)
+    return _ops.distill_topk_grad.default(student_logits, teacher_logits, teacher_indices, row_scale,
+                                          teacher_lse, float(temperature))
 
 
 def residual_norm(block_out: torch.Tensor, residual: torch.Tensor,
@@ -149,39 +202,10 @@ def residual_norm(block_out: torch.Tensor, residual: torch.Tensor,
     it is rounded, and each output is rounded once.  Differentiable in all
     tensor arguments; parameter gradients are summed in a fixed order.
     """
-    _check("block_out", block_out)
-    _check("residual", residual)
-    if residual.dtype != block_out.dtype:
-        raise TypeError(f"residual must use block_out's {block_out.dtype}, got {residual.dtype}")
-    shape = block_out.shape
-    if block_out.ndim < 1 or shape[-1] < 1:
-        raise ValueError(f"block_out must have shape [..., width], got {tuple(shape)}")
-    if residual.shape != shape:
-        raise ValueError(f"residual must have block_out's shape {tuple(shape)}, got {tuple(residual.shape)}")
-    width = shape[-1]
-    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if w is not None:
-            _check(name, w)
-            if w.shape != (width,):
-                raise ValueError(f"{name} must have shape ({width},), got {tuple(w.shape)}")
-    if gate is not None:
-        _check("gate", gate)
-        gate = _gate_rows(gate, shape)
-    if residual_scale is not None:
-        _check("residual_scale", residual_scale)
-        if residual_scale.numel() == 1:
-            residual_scale = residual_scale.reshape(1)
-        elif residual_scale.shape != (width,):
-            raise ValueError(f"residual_scale must have one element or shape ({width},), "
-                             f"got {tuple(residual_scale.shape)}")
-    if block_out.ndim != 2:
-        rows = shape[:-1].numel()
-        block_out, residual = block_out.reshape(rows, width), residual.reshape(rows, width)
-    hidden, normed, _, _ = torch.ops.muon_ascend950.residual_norm(
-        block_out, residual, post_weight, pre_weight, gate, residual_scale, float(eps))
-    if len(shape) != 2:
-        hidden = hidden.reshape(shape)
-        normed = normed.reshape(shape) if pre_weight is not None else None
+    _tensors(block_out=block_out, residual=residual, post_weight=post_weight, pre_weight=pre_weight,
+             gate=gate, residual_scale=residual_scale)
+    hidden, normed, _ = _ops.residual_norm.default(block_out, residual, post_weight, pre_weight, gate,
+                                                   residual_scale, float(eps))
     return hidden, normed if pre_weight is not None else None
 
 
@@ -205,23 +229,10 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax",
     int64 ``[experts]``, how many tokens each expert got.  Differentiable in
     ``logits`` through the weights.
     """
-    _check("logits", logits)
+    _tensors(logits=logits, bias=bias)
     if score not in _SCORES:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
-    if logits.ndim < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must have shape [..., experts], got {tuple(logits.shape)}")
-    if bias is not None:
-        _check("bias", bias)
-        if bias.shape != (logits.shape[-1],):
-            raise ValueError(f"bias must have shape ({logits.shape[-1]},), got {tuple(bias.shape)}")
     if group_top is None:
-        group_top = 2 if score == "sigmoid" and groups > 1 and logits.shape[-1] // groups > 1 else 1
-    shape = logits.shape
-    if len(shape) != 2:
-        logits = logits.reshape(shape[:-1].numel(), shape[-1])
-    weights, indices, counts = torch.ops.muon_ascend950.route_experts(
-        logits, bias, int(k), _SCORES[score], int(groups), int(top_groups), int(group_top),
-        bool(renormalize), float(scale))
-    if len(shape) != 2:
-        weights, indices = (t.reshape(shape[:-1] + (k,)) for t in (weights, indices))
-    return weights, indices, counts
+        group_top = 2 if score == "sigmoid" and 1 < groups < logits.shape[-1] else 1
+    return _ops.route_experts.default(logits, bias, int(k), _SCORES[score], int(groups), int(top_groups),
+                                      int(group_top), bool(renormalize), float(scale))

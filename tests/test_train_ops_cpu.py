@@ -62,7 +62,7 @@ def _distill(**kw):
     dict(rows=-1), dict(vocab=0), dict(ld=7), dict(top=0), dict(top=1025), dict(temperature=0.0),
     dict(temperature=float("nan")), dict(dtype=3), dict(teacher_dtype=-1), dict(index_bytes=2),
     dict(logits=None), dict(teacher_logits=None), dict(teacher_indices=None), dict(loss=None),
-    dict(grad=16, ld_grad=8), dict(grad=32, ld_grad=7)])
+    dict(grad=16, ld_grad=8, stats=16), dict(grad=32, ld_grad=7, stats=16), dict(grad=32, ld_grad=8)])
 def test_distill_refuses(lib, bad):
     args = _distill(**bad)
     assert lib.muon_train_distill_sm100(ctypes.byref(args), None) == -1
@@ -201,15 +201,15 @@ def test_entry_points_check_shapes_and_types():
 
 
 def test_gate_rows_of_every_shape():
-    from muon_fusion_ascend950_b200.training import _gate_rows
+    from muon_fusion_ascend950_b200.training import gate_rows
 
     shape = torch.Size((2, 3, 4, 8))
     for lead, rows in (((), 1), ((1,), 1), ((1, 1, 1), 1), ((2, 1, 1), 2), ((2, 3, 1), 6),
                        ((2, 3, 4), 24)):
-        assert _gate_rows(torch.empty(*lead, 8), shape).shape == (rows, 8)
+        assert gate_rows(torch.empty(*lead, 8), shape) == rows
     for lead in ((3,), (1, 3, 1), (2, 1, 4), (2, 3, 4, 1)):
         with pytest.raises(ValueError):
-            _gate_rows(torch.empty(*lead, 8), shape)
+            gate_rows(torch.empty(*lead, 8), shape)
 
 
 def test_fake_backward_kernels():
@@ -221,9 +221,9 @@ def test_fake_backward_kernels():
         assert stats.shape == (2, 2)
         assert ops.distill_topk_backward(loss, z, t, i, None, stats, 1.0).shape == z.shape
         x, w = _cuda(6, 16), _cuda(16, dtype=torch.float32)
-        h, n, r, rh = ops.residual_norm(x, x, w, None, None, None, 1e-6)
-        assert n.shape == (0, 16) and r.shape == (6,) and rh.shape == (0,)
-        grads = ops.residual_norm_backward(h, None, x, x, w, None, None, None, r, rh, 1e-6,
+        h, n, r = ops.residual_norm(x, x, w, None, None, None, 1e-6)
+        assert n.shape == (0,) and r.shape == (2, 6)
+        grads = ops.residual_norm_backward(h, None, x, x, w, None, None, None, r, 1e-6,
                                            [True, False, True, True, False, False])
         assert [g.shape[0] for g in grads] == [6, 0, 16, 0, 0, 0] and grads[2].dtype == torch.float32
         l = _cuda(4, 8)
