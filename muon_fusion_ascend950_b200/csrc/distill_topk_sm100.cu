@@ -284,20 +284,31 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 4)
 }
 
 // ------------------------------------------------------------ rows through a ring
-// Long rows: one persistent block an SM, or a cluster of them a row.  A
-// producer warp streams the blocks' slices of row after row into a ring of
-// 16 KiB stages with bulk copies, a list warp makes the lists one row ahead,
-// and 512 consumer threads take the statistics from the stages as they land
-// and the gradient from the same stages, which only then are free again.  So
-// the next row is on its way while this one is worked on, and neither the
-// list nor the sums of the row hold up the memory.
-constexpr int kConsumers = 512;
+// Long rows: persistent blocks, two an SM, or clusters of them a row.  A
+// producer warp streams the block's slices of row after row into a ring of
+// stages with bulk copies; eight consumer warps take the statistics from the
+// stages as they land.  For the loss with its gradient the slice is then
+// streamed a second time, from L2, where the first copy asked it to stay.  A
+// list warp makes the lists one row ahead, adds up the block's and the
+// cluster's sums and makes the loss.  So the next stages are on their way while
+// one is worked on, and while one block waits for its sums the other one of
+// the SM computes.
+//
+// Measured for the loss with its gradient, 4096 x 131072 bf16 (333 us at the
+// copy rate): rows in registers of 8-block clusters 783 us (4 blocks an SM
+// 616), slices held in the ring between the passes 504 us, streamed twice
+// 403 us.  8192 x 65536: 390 us.  The loss alone: 174 us of 167.
+constexpr int kConsumers = 256;
 constexpr int kConsumerWarps = kConsumers / 32;
-constexpr int kStageGranules = 2 * kConsumers;
+constexpr int kPerStage = 4;  // granules of a thread in a stage
+constexpr int kBlocksPerSm = 2;
+constexpr int kStageGranules = kPerStage * kConsumers;
 constexpr int kStageBytes = kStageGranules * 16;
-constexpr int kMaxStages = 13;
-constexpr size_t kRingBytes = 224 * 1024;  // of dynamic shared memory
-constexpr double kRowNs = 700.0, kClusterNs = 500.0;
+constexpr int kMaxStages = 6;
+constexpr size_t kRingBytes = 111 * 1024;  // of dynamic shared memory
+// What a row costs a block besides its bytes, and more in a cluster; the bytes
+// of rows in flight that L2 holds until their second reading.
+constexpr double kRowNs = 700.0, kClusterNs = 500.0, kHeldBytes = 60e6;
 
 struct Ring {
   Cut cut;
@@ -309,24 +320,11 @@ __device__ uint32_t g_status = 0;
 // Waits for the phase of `bar`; gives up after the wait limit, or once another
 // thread of the block has: the block then runs on without waiting, and the
 // device status tells.
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(muon_sm100::smem_addr(bar)), "r"(parity) : "memory");
-  return ok != 0;
-}
-template <bool kCluster>
 __device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  const auto done = [&] {
-    return kCluster ? try_wait_cluster(bar, parity) : muon_sm100::mbar_try_wait(bar, parity);
-  };
-  if (done()) return;
+  if (muon_sm100::mbar_try_wait(bar, parity)) return;
   const uint64_t t0 = muon_sm100::global_timer_ns();
   for (uint32_t spins = 1;; ++spins) {
-    if (done()) return;
+    if (muon_sm100::mbar_try_wait(bar, parity)) return;
     if ((spins & 63u) != 0) continue;
     if (*failed) return;
     if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
@@ -335,6 +333,21 @@ __device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, volati
       return;
     }
   }
+}
+
+// Arrives at a named barrier without waiting for the others.
+__device__ __forceinline__ void named_arrive(uint32_t id, uint32_t count) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
+// Bulk copy into shared memory with an L2 eviction policy.
+__device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint32_t bytes, uint64_t* bar,
+                                               uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, "
+      "[%3], %4;" ::"r"(muon_sm100::smem_addr(dst)),
+      "l"(src), "r"(bytes), "r"(muon_sm100::smem_addr(bar)), "l"(policy)
+      : "memory");
 }
 
 // A block's slice of one row.
@@ -354,7 +367,7 @@ struct Slice {
 };
 
 template <typename T, Mode kMode>
-__global__ void __launch_bounds__(kConsumers + 64, 1)
+__global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
     distill_ring_kernel(const __grid_constant__ muon_train_distill_args a, Ring ring) {
   using namespace muon_sm100;
   constexpr int kN = kVec<T>;
@@ -362,6 +375,7 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], heard[2];
   __shared__ float2 warp_part[2][kConsumerWarps];
   __shared__ float2 block_part[2][kMaxCluster];
+  __shared__ float2 row_part[2];  // the row's statistics
   __shared__ float4 row_info[2];  // Q, g, and the statistics of an earlier call
   __shared__ volatile int failed;
   const int parts = ring.cut.parts, stages = ring.stages;
@@ -375,7 +389,7 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kConsumerWarps);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&heard[i], static_cast<uint32_t>(parts));
+    for (int i = 0; i < 2; ++i) mbar_init(&heard[i], 1);
     failed = 0;
     fence_mbar_init();
   }
@@ -390,39 +404,48 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
       phase ^= 1;
     }
   };
-  // The row's statistics from the parts of this block's warps, and of the
-  // cluster's blocks; `turn` counts the worker's rows.  Each block's list warp
-  // tells every block its part, and goes on to the next row only after it has
-  // heard all of them: so no block is ever more than one row ahead of another,
-  // and two slots are enough.
+  // For the list warp: the row's statistics from the parts of this block's
+  // warps, and of the cluster's blocks; `turn` counts the worker's rows.  Each
+  // block sends its part to every block, and goes on to the next row only
+  // after it has heard all of them: so no block is ever more than one row ahead
+  // of another, and two slots are enough.
   const auto statistics = [&](uint32_t turn) {
-    float2 v = lane < kConsumerWarps ? warp_part[turn & 1][lane] : make_float2(-INFINITY, 0.f);
-    v = warp_join(v, c);
+    const uint32_t slot = turn & 1;
+    float2 v = warp_join(lane < kConsumerWarps ? warp_part[slot][lane] : make_float2(-INFINITY, 0.f), c);
     if (parts > 1) {
-      if (warp == kConsumerWarps + 1 && lane < parts) {
+      if (lane == 0) mbar_arrive_expect_tx(&heard[slot], static_cast<uint32_t>(parts * sizeof(float2)));
+      __syncwarp();
+      if (lane < parts) {
         const uint32_t peer = static_cast<uint32_t>(lane);
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
-                         map_to_cta(smem_addr(&block_part[turn & 1][part]), peer)),
-                     "f"(v.x), "f"(v.y) : "memory");
-        mbar_arrive_cluster(map_to_cta(smem_addr(&heard[turn & 1]), peer));
+        asm volatile(
+            "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(
+                map_to_cta(smem_addr(&block_part[slot][part]), peer)),
+            "f"(v.x), "f"(v.y), "r"(map_to_cta(smem_addr(&heard[slot]), peer)) : "memory");
       }
-      ring_wait<true>(&heard[turn & 1], (turn >> 1) & 1, &failed);
-      v = block_part[turn & 1][0];
-      for (int i = 1; i < parts; ++i) v = join(v, block_part[turn & 1][i], c);
+      ring_wait(&heard[slot], (turn >> 1) & 1, &failed);
+      v = block_part[slot][0];
+      for (int i = 1; i < parts; ++i) v = join(v, block_part[slot][i], c);
     }
     return v;
   };
 
   if (warp == kConsumerWarps) {  // producer
+    // with the gradient, what is read again stays in L2, the rest need not
+    [[maybe_unused]] uint64_t keep = 0, drop = 0;
+    if constexpr (kMode == kLossGrad) {
+      asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+      asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(drop));
+    }
     for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers) {
       const Slice<T> slice(a, ring.cut, row, part);
+      for (int pass = 0; pass < (kMode == kLossGrad ? 2 : 1); ++pass)
       for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
         const int g1 = min(slice.last, g0 + kStageGranules);
         // whole granules [lo, hi); at most one more at either end of the row
         const int lo = g0 * kN < slice.shift ? g0 + 1 : g0;
         const int hi = g1 * kN - slice.shift > vocab ? g1 - 1 : g1;
         uint8_t* to = dynamic + stage * kStageBytes;
-        if (lane == 0) ring_wait<false>(&empty[stage], phase ^ 1, &failed);
+        if (lane == 0) ring_wait(&empty[stage], phase ^ 1, &failed);
         __syncwarp();
         if (lane < 2 * kN) {
           const bool left = lane < kN;
@@ -437,8 +460,13 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
         if (lane == 0) {
           const uint32_t bytes = hi > lo ? static_cast<uint32_t>(hi - lo) * 16u : 0u;
           mbar_arrive_expect_tx(&full[stage], bytes);
-          if (bytes > 0)
-            bulk_load(to + (lo - g0) * 16, slice.z + (static_cast<int64_t>(lo) * kN - slice.shift), bytes, &full[stage]);
+          const T* from = slice.z + (static_cast<int64_t>(lo) * kN - slice.shift);
+          if (bytes > 0) {
+            if constexpr (kMode == kLossGrad)
+              bulk_load_hint(to + (lo - g0) * 16, from, bytes, &full[stage], pass == 0 ? keep : drop);
+            else
+              bulk_load(to + (lo - g0) * 16, from, bytes, &full[stage]);
+          }
         }
         advance();
       }
@@ -461,6 +489,11 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
       named_barrier(1, kConsumers + 32);
       if constexpr (kMode != kGradFromStats) {
         const float2 v = statistics(turn);
+        if constexpr (kMode == kLossGrad) {
+          if (lane == 0) row_part[turn & 1] = v;
+          __syncwarp();
+          named_arrive(3, kConsumers + 32);
+        }
         if (part == 0) {
           const float loss = row_loss(list, top, 1.0f / a.temperature, v.x, v.y);
           if (lane == 0) {
@@ -475,13 +508,14 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
     }
   } else {  // consumers
     const float2 cc = make_float2(c, c);
+    const int tid = static_cast<int>(threadIdx.x);
     uint32_t turn = 0;
     for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers, ++turn) {
       const Slice<T> slice(a, ring.cut, row, part);
-      const int row_stage = stage;
-      const uint32_t row_phase = phase;
-      const auto read = [&](int at) {
-        return *reinterpret_cast<const uint4*>(dynamic + stage * kStageBytes + at * 16);
+      uint4 u[kPerStage];
+      const auto at = [&](int i) { return tid + i * kConsumers; };
+      const auto read = [&](int i) {
+        return *reinterpret_cast<const uint4*>(dynamic + stage * kStageBytes + at(i) * 16);
       };
       const auto release = [&] {
         __syncwarp();
@@ -491,29 +525,28 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
         float m = -INFINITY;
         float2 s = make_float2(0.f, 0.f);
         for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
-          ring_wait<false>(&full[stage], phase, &failed);
-          uint4 u[2];
-          bool there[2];
+          ring_wait(&full[stage], phase, &failed);
+          // past the slice's end: -inf
+          if (g0 + kStageGranules <= slice.last) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at = static_cast<int>(threadIdx.x) + i * kConsumers;
-            there[i] = g0 + at < slice.last;
-            u[i] = there[i] ? read(at) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kPerStage; ++i) u[i] = read(i);
+          } else {
+            float none[kN];
+#pragma unroll
+            for (int j = 0; j < kN; ++j) none[j] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPerStage; ++i) u[i] = g0 + at(i) < slice.last ? read(i) : pack<T>(none);
           }
-          if constexpr (kMode == kLoss) release();
+          release();
           float largest = m;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (there[i]) largest = vector_max(u[i], largest, T());
+          for (int i = 0; i < kPerStage; ++i) largest = vector_max(u[i], largest, T());
           const float base = largest == -INFINITY ? 0.f : largest;  // nothing finite yet: a sum of 0
-          if (largest > m) {
-            const float down = fast_exp2((m - base) * c);
-            s = mul2(s, make_float2(down, down));
-            m = largest;
-          }
+          const float down = fast_exp2((m - base) * c);
+          s = mul2(s, make_float2(down, down));
+          m = largest;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!there[i]) continue;
+          for (int i = 0; i < kPerStage; ++i) {
             float e[kN];
             unpack<T>(u[i], e);
 #pragma unroll
@@ -524,40 +557,34 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
         }
         const float2 v = warp_join(make_float2(m, s.x + s.y), c);
         if (lane == 0) warp_part[turn & 1][warp] = v;
+        __syncwarp();
       }
-      named_barrier(1, kConsumers + 32);
+      if constexpr (kMode == kLossGrad) {  // the list warp answers
+        named_arrive(1, kConsumers + 32);
+        named_barrier(3, kConsumers + 32);
+      } else {
+        named_barrier(1, kConsumers + 32);
+      }
       if constexpr (kMode != kLoss) {
         const float4 info = row_info[turn & 1];
-        float2 v = make_float2(info.z, info.w);
-        if constexpr (kMode != kGradFromStats) v = statistics(turn);
-        stage = row_stage;
-        phase = row_phase;
+        const float2 v = kMode == kLossGrad ? row_part[turn & 1] : make_float2(info.z, info.w);
         const float g = info.y;
         const bool none = g == 0.f || info.x == 0.f;  // zero whatever the logits hold
         const float p_scale = none ? 0.f : g * info.x / v.y;
         const float2 scale2 = make_float2(p_scale, p_scale), minus_max = make_float2(-v.x, -v.x);
         T* dz = static_cast<T*>(a.grad) + row * a.ld_grad;
         for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
-          if constexpr (kMode == kGradFromStats) ring_wait<false>(&full[stage], phase, &failed);
-          uint4 u[2];
-          bool there[2];
+          ring_wait(&full[stage], phase, &failed);
+          const int element0 = g0 * kN - slice.shift;
+          if (ring.cut.same_phase && !none && g0 + kStageGranules <= slice.last && element0 >= 0 &&
+              element0 + kStageGranules * kN <= vocab) {  // whole vectors throughout
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at = static_cast<int>(threadIdx.x) + i * kConsumers;
-            there[i] = g0 + at < slice.last;
-            u[i] = there[i] ? read(at) : make_uint4(0, 0, 0, 0);
-          }
-          release();
+            for (int i = 0; i < kPerStage; ++i) u[i] = read(i);
+            release();
+            T* to = dz + element0 + tid * kN;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!there[i]) continue;
-            const int granule = g0 + static_cast<int>(threadIdx.x) + i * kConsumers;
-            const int element = granule * kN - slice.shift;
-            float e[kN];
-            if (none) {
-#pragma unroll
-              for (int j = 0; j < kN; ++j) e[j] = 0.f;
-            } else {
+            for (int i = 0; i < kPerStage; ++i) {
+              float e[kN];
               unpack<T>(u[i], e);
 #pragma unroll
               for (int j = 0; j < kN; j += 2) {
@@ -565,14 +592,30 @@ __global__ void __launch_bounds__(kConsumers + 64, 1)
                 e[j] = p.x;
                 e[j + 1] = p.y;
               }
+              uint4* at_vector = reinterpret_cast<uint4*>(to + i * kConsumers * kN);
+              if constexpr (kMode == kLossGrad)
+                __stcs(at_vector, pack<T>(e));
+              else
+                *at_vector = pack<T>(e);
             }
-            if (ring.cut.same_phase && element >= 0 && element + kN <= vocab) {
-              *reinterpret_cast<uint4*>(dz + element) = pack<T>(e);
-            } else {
+          } else {
+            for (int i = 0; i < kPerStage; ++i) {
+              if (g0 + at(i) >= slice.last) break;
+              const int element = element0 + at(i) * kN;
+              float e[kN];
+              unpack<T>(read(i), e);
 #pragma unroll
               for (int j = 0; j < kN; ++j)
-                if (element + j >= 0 && element + j < vocab) dz[element + j] = from_float<T>(e[j]);
+                e[j] = none ? 0.f : p_scale * fast_exp2((e[j] - v.x) * c);
+              if (ring.cut.same_phase && element >= 0 && element + kN <= vocab) {
+                *reinterpret_cast<uint4*>(dz + element) = pack<T>(e);
+              } else {
+#pragma unroll
+                for (int j = 0; j < kN; ++j)
+                  if (element + j >= 0 && element + j < vocab) dz[element + j] = from_float<T>(e[j]);
+              }
             }
+            release();
           }
           advance();
         }
@@ -650,32 +693,26 @@ int run(const muon_train_distill_args& a, Mode mode, void* stream) {
   }
   const int stages = static_cast<int>(
       std::min<size_t>(kMaxStages, (kRingBytes - 2 * List::bytes(a.top)) / kStageBytes));
-  // With the gradient a slice stays in the ring, and two stages are left for
-  // the next row; a longer row's gradient is made by a second pass.
-  const auto slice_stages = [&](int parts) {
-    return ((granules + parts - 1) / parts + kStageGranules - 1) / kStageGranules;
-  };
-  const int most = mode == kLossGrad ? stages - 2 : 1 << 30;
-  if (slice_stages(kMaxCluster) > most) {
-    const int first = run<T>(a, kLoss, stream);
-    return first != MUON_POLAR_OK ? first : run<T>(a, kGradFromStats, stream);
-  }
   // Parts of a row by the smallest estimate: rounds of rows, each of a slice
-  // at an SM's share of the measured copy rate and what a row costs besides.
-  int parts = 0;
+  // at a block's share of the measured copy rate (43 bytes/ns an SM) and what
+  // a row costs besides.
+  const int64_t blocks = static_cast<int64_t>(sms) * kBlocksPerSm;
+  const double passes = mode == kLoss ? 1.0 : 2.0;
+  int parts = 1;
   double least = 0.0;
-  for (int p = 1; p <= kMaxCluster; p *= 2) {
-    if (slice_stages(p) > most) continue;
-    const int64_t workers = std::max<int64_t>(1, sms / p);
+  for (int p = 1; p <= kMaxCluster && p <= blocks; p *= 2) {
+    const int64_t workers = std::min<int64_t>(a.rows, blocks / p);
     const double rounds = static_cast<double>((a.rows + workers - 1) / workers);
-    const double slice_ns = static_cast<double>(granules) * 16.0 / p / 43.0 * (mode == kLossGrad ? 2.0 : mode == kGradFromStats ? 2.0 : 1.0);
+    const double row_bytes = static_cast<double>(granules) * 16.0;
+    const bool again = mode == kLossGrad && static_cast<double>(workers) * row_bytes > kHeldBytes;
+    const double slice_ns = row_bytes / p * kBlocksPerSm / 43.0 * (again ? 2.3 : passes);
     const double estimate = rounds * (slice_ns + kRowNs + (p > 1 && mode != kGradFromStats ? kClusterNs : 0.0));
-    if (parts == 0 || estimate < least) {
+    if (p == 1 || estimate < least) {
       parts = p;
       least = estimate;
     }
   }
-  const int64_t workers = std::min<int64_t>(a.rows, std::max<int64_t>(1, sms / parts));
+  const int64_t workers = std::min<int64_t>(a.rows, blocks / parts);
   if (mode == kLossGrad) return run_ring<T, kLossGrad>(a, parts, stages, workers, stream);
   if (mode == kLoss) return run_ring<T, kLoss>(a, parts, stages, workers, stream);
   return run_ring<T, kGradFromStats>(a, parts, stages, workers, stream);
