@@ -13,10 +13,12 @@
 namespace muon_train {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;  // tokens in flight of a block, one a warp
 constexpr int kThreads = kWarps * 32;
+constexpr int kBlocksPerSm = 2;
 constexpr int kSoftmax = 0;
 constexpr float kTiny = 1e-20f;
+constexpr int kSlots = MUON_TRAIN_MAX_ROUTES / 32;  // chosen experts a lane keeps
 
 __device__ __forceinline__ float sigmoid(float x) {
   return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x)));
@@ -36,159 +38,348 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// Scores of one token in shared memory, by one warp; returns nothing.
-template <typename T>
-__device__ void scores(const T* l, int experts, int score, float* s) {
-  const int lane = threadIdx.x & 31;
-  if (score != kSoftmax) {
-    for (int e = lane; e < experts; e += 32) s[e] = sigmoid(to_float(l[e]));
-  } else {
-    float m = -INFINITY;
-    for (int e = lane; e < experts; e += 32) m = fmaxf(m, to_float(l[e]));
-    m = warp_max(m);
-    double sum = 0.0;
-    for (int e = lane; e < experts; e += 32) {
-      const float x = m == -INFINITY && !(to_float(l[e]) != to_float(l[e]))
-                          ? 0.f
-                          : expf(__fsub_rn(to_float(l[e]), m));
-      s[e] = x;
-      sum += x;
+// A lane has kPer neighbouring experts of a token, lane * kPer the first, so
+// that the lowest lane holds the lowest index.  They are loaded in runs of up
+// to 16 bytes where rows keep that alignment (whole), else one by one.
+template <typename T, int kPer>
+struct Row {
+  static constexpr int kRun = kPer * static_cast<int>(sizeof(T)) > 16 ? 16 / static_cast<int>(sizeof(T)) : kPer;
+  float v[kPer];
+  __device__ __forceinline__ void load(const T* l, int experts, bool whole) {
+    const int e0 = (threadIdx.x & 31) * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; i += kRun) {
+      if (whole && e0 + i < experts) {
+        if constexpr (kRun * sizeof(T) >= 4) {
+          float part[kRun];
+          Elements<T, kRun>::unpack(Elements<T, kRun>::load(l + e0 + i), part);
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) v[i + j] = part[j];
+          continue;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) v[i + j] = e0 + i + j < experts ? to_float(l[e0 + i + j]) : -INFINITY;
     }
-    const float total = static_cast<float>(warp_sum64(sum));
-    for (int e = lane; e < experts; e += 32) s[e] = total == 0.f ? 0.f : __fdiv_rn(s[e], total);
   }
-  __syncwarp();
+};
+
+// Scores of a lane's experts (0 beyond the last).
+template <int kPer>
+__device__ __forceinline__ void scores(const float (&l)[kPer], int experts, int score, float (&s)[kPer]) {
+  const int e0 = (threadIdx.x & 31) * kPer;
+  if (score != kSoftmax) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s[i] = e0 + i < experts ? sigmoid(l[i]) : 0.f;
+    return;
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) m = fmaxf(m, l[i]);
+  m = warp_max(m);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    // a row of -inf has no scores; a NaN stays one
+    s[i] = e0 + i >= experts || (m == -INFINITY && l[i] == l[i]) ? 0.f : expf(__fsub_rn(l[i], m));
+    sum += s[i];
+  }
+  const float total = static_cast<float>(warp_sum64(sum));
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) s[i] = total == 0.f ? 0.f : __fdiv_rn(s[i], total);
 }
 
-// The largest key in s_key[0 .. n) of the warp's lanes: its lowest index, or
-// -1 when all are taken.
-__device__ int best_of(const uint32_t* keys, int n) {
-  const int lane = threadIdx.x & 31;
-  uint32_t best = 0;
-  int at = n;
-  for (int e = lane; e < n; e += 32)
-    if (keys[e] > best) {
-      best = keys[e];
-      at = e;
-    }
-  const uint32_t top = __reduce_max_sync(kFullMask, best);
-  const int index = __reduce_min_sync(kFullMask, best == top ? at : n);
-  return top == 0 ? -1 : index;
+// How a call's rows are laid out and its groups ranked.
+struct Plan {
+  bool whole;         // runs of a row can be loaded at once
+  bool by_logit;      // the logits are the keys
+  int lanes_a_group;  // a power of two, when no lane has experts of two groups; else 0
+};
+
+__device__ __forceinline__ void best_two(float key, float& first, float& second) {
+  if (key > first) {  // a NaN is passed over
+    second = first;
+    first = key;
+  } else if (key > second) {
+    second = key;
+  }
 }
 
-template <typename T>
+// Forward: one warp a token.  The time goes into instructions, not memory
+// (256 sigmoid scores with groups: about 600 a token against 1 KB read), so
+// keys and scores stay in registers, an argmax is one redux of the lanes'
+// best keys, and only the winning lane looks for its next one.
+template <typename T, int kPer>
 __global__ void __launch_bounds__(kThreads)
-    route_kernel(const __grid_constant__ muon_train_route_args a) {
+    route_kernel(const __grid_constant__ muon_train_route_args a, Plan plan) {
   extern __shared__ float smem[];
   const int experts = static_cast<int>(a.experts);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* s = smem + warp * 3 * experts;
-  uint32_t* keys = reinterpret_cast<uint32_t*>(s + experts);
-  uint32_t* group_keys = keys + experts;
-  const bool by_logit = a.score == kSoftmax && a.bias == nullptr &&
-                        (a.groups == 1 || a.group_top == 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * kPer;
+  uint32_t* histogram = reinterpret_cast<uint32_t*>(smem);  // of the block's tokens
+  float* row = smem + experts + warp * (plan.lanes_a_group > 0 ? 1 : 2) * experts;
+  float* row_keys = row + experts;  // without lanes_a_group
+  for (int e = threadIdx.x; e < experts; e += kThreads) histogram[e] = 0;
+  __syncthreads();
+  float bias[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) bias[i] = a.bias != nullptr && e0 + i < experts ? a.bias[e0 + i] : 0.f;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  Row<T, kPer> l;
+  if (token < a.tokens) l.load(static_cast<const T*>(a.logits) + token * a.ld, experts, plan.whole);
+  for (; token < a.tokens; token += step) {
+    float s[kPer], key[kPer];
+    scores(l.v, experts, a.score, s);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      key[i] = plan.by_logit ? l.v[i] : a.bias != nullptr ? __fadd_rn(s[i], bias[i]) : s[i];
+      if (e0 + i < experts) row[e0 + i] = s[i];
+    }
+    if (token + step < a.tokens)
+      l.load(static_cast<const T*>(a.logits) + (token + step) * a.ld, experts, plan.whole);
+    uint32_t taken = 0;  // a bit for each of the lane's experts that cannot be chosen
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (e0 + i >= experts) taken |= 1u << i;
+    if (a.groups > 1) {
+      const int size = experts / a.groups;
+      if (plan.lanes_a_group > 0) {
+        float first = -INFINITY, second = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) best_two(key[i], first, second);
+        for (int o = 1; o < plan.lanes_a_group; o <<= 1) {
+          const float f = __shfl_xor_sync(kFullMask, first, o), g = __shfl_xor_sync(kFullMask, second, o);
+          second = fmaxf(fminf(first, f), fmaxf(second, g));
+          first = fmaxf(first, f);
+        }
+        const uint32_t mine = ordered(a.group_top == 2 ? __fadd_rn(first, second) : first);
+        const int group = lane / plan.lanes_a_group;
+        int better = 0;
+        for (int g = 0; g < a.groups; ++g) {
+          const uint32_t other = __shfl_sync(kFullMask, mine, g * plan.lanes_a_group);
+          better += other > mine || (other == mine && g < group);
+        }
+        if (better >= a.top_groups) taken = 0xffffffffu;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (e0 + i < experts) row_keys[e0 + i] = key[i];
+        __syncwarp();
+        // each lane ranks its groups g = lane, + 32, ..
+        uint32_t mine[MUON_TRAIN_MAX_EXPERTS / 32];
+        const int rounds = (a.groups + 31) / 32;
+        for (int r = 0; r < rounds; ++r) {
+          const int g = r * 32 + lane;
+          float first = -INFINITY, second = -INFINITY;
+          if (g < a.groups)
+            for (int e = g * size; e < (g + 1) * size; ++e) best_two(row_keys[e], first, second);
+          mine[r] = g < a.groups ? ordered(a.group_top == 2 ? __fadd_rn(first, second) : first) : 0u;
+        }
+        __syncwarp();
+        // the best groups one by one; row_keys now says which groups stay
+        for (int g = lane; g < a.groups; g += 32) row_keys[g] = 0.f;
+        __syncwarp();
+        for (int j = 0; j < a.top_groups; ++j) {
+          uint32_t best = 0;
+          int at = 0;
+          for (int r = 0; r < rounds; ++r)
+            if (mine[r] > best) {
+              best = mine[r];
+              at = r;
+            }
+          const uint32_t top = __reduce_max_sync(kFullMask, best);
+          const int g = __reduce_min_sync(kFullMask, best == top ? at * 32 + lane : 0x7fffffff);
+          if ((g & 31) == lane) {
+            mine[g >> 5] = 0;
+            row_keys[g] = 1.f;
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (e0 + i < experts && row_keys[(e0 + i) / size] == 0.f) taken |= 1u << i;
+      }
+    }
+    // the k best: the lanes' best keys, and within the best lane the first
+    uint32_t best;
+    int at;
+    const auto look = [&] {
+      best = 0;
+      at = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t o = (taken >> i) & 1u ? 0u : ordered(key[i]);
+        if (o > best) {
+          best = o;
+          at = i;
+        }
+      }
+    };
+    look();
+    int chosen[kSlots];
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) chosen[i] = 0;
+    for (int j = 0; j < a.k; ++j) {
+      const uint32_t top = __reduce_max_sync(kFullMask, best);
+      const int who = __ffs(__ballot_sync(kFullMask, best == top)) - 1;
+      const int e = __shfl_sync(kFullMask, e0 + at, who);
+      if (lane == (j & 31)) {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i)
+          if (i == (j >> 5)) chosen[i] = e;
+      }
+      if (lane == who) {
+        taken |= 1u << at;
+        look();
+      }
+    }
+    __syncwarp();  // row is written
+    float w[kSlots], total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      w[i] = i * 32 + lane < a.k ? row[chosen[i]] : 0.f;
+      total += w[i];
+    }
+    total = a.renormalize ? warp_sum(total) + kTiny : 1.f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int j = i * 32 + lane;
+      if (j >= a.k) continue;
+      a.weights[token * a.k + j] = (a.renormalize ? __fdiv_rn(w[i], total) : w[i]) * a.scale;
+      a.indices[token * a.k + j] = chosen[i];
+      atomicAdd(&histogram[chosen[i]], 1u);
+    }
+    __syncwarp();  // row is read before the next token's is written
+  }
+  if (a.counts == nullptr) return;
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kThreads) {
+    if (gridDim.x == 1)
+      a.counts[e] = histogram[e];
+    else if (histogram[e] != 0)
+      atomicAdd(reinterpret_cast<unsigned long long*>(a.counts) + e,
+                static_cast<unsigned long long>(histogram[e]));
+  }
+}
+
+// Backward, one warp a token.  The gradient of the sigmoid, and of the
+// softmax when its chosen scores are renormalised, is zero but for the chosen
+// experts and needs only their logits: with the renormalised weights v (the
+// softmax over the chosen) it is scale v_j (g_j - sum g v).  So the row is
+// written with zeros, and then the chosen; kWholeRow is the softmax without
+// renormalisation, which reaches every expert.
+template <typename T, int kPer, bool kWholeRow>
+__global__ void __launch_bounds__(kThreads)
+    route_backward_kernel(const __grid_constant__ muon_train_route_args a, Plan plan,
+                          const float* __restrict__ grad_weights, T* __restrict__ grad) {
+  extern __shared__ float smem[];
+  using Lanes = Row<T, kPer>;
+  const int experts = static_cast<int>(a.experts);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * kPer;
+  float* row = smem + warp * experts;  // kWholeRow: the gradients of the scores
   for (int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp; token < a.tokens;
        token += static_cast<int64_t>(gridDim.x) * kWarps) {
     const T* l = static_cast<const T*>(a.logits) + token * a.ld;
-    scores(l, experts, a.score, s);
-    for (int e = lane; e < experts; e += 32) {
-      const float key = by_logit ? to_float(l[e])
-                                 : (a.bias != nullptr ? __fadd_rn(s[e], a.bias[e]) : s[e]);
-      keys[e] = ordered(key);
+    T* out = grad + token * a.experts;
+    int chosen[kSlots];
+    float g[kSlots];
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int j = i * 32 + lane;
+      chosen[i] = -1;
+      g[i] = 0.f;
+      if (j < a.k) {
+        const int64_t e = a.indices[token * a.k + j];
+        if (e >= 0 && e < experts) {
+          chosen[i] = static_cast<int>(e);
+          g[i] = grad_weights[token * a.k + j];
+        }
+      }
     }
-    __syncwarp();
-    if (a.groups > 1) {
-      const int size = experts / a.groups;
-      for (int g = lane; g < a.groups; g += 32) {
-        float first = -INFINITY, second = -INFINITY;
-        for (int e = g * size; e < (g + 1) * size; ++e) {
-          const float key = by_logit ? to_float(l[e])
-                                     : (a.bias != nullptr ? __fadd_rn(s[e], a.bias[e]) : s[e]);
-          if (key > first) {
-            second = first;
-            first = key;
-          } else if (key > second) {
-            second = key;
+    const auto store_row = [&](const float(&v)[kPer]) {
+#pragma unroll
+      for (int i = 0; i < kPer; i += Lanes::kRun) {
+        if (plan.whole && e0 + i < experts) {
+          if constexpr (Lanes::kRun * sizeof(T) >= 4) {
+            float part[Lanes::kRun];
+#pragma unroll
+            for (int j = 0; j < Lanes::kRun; ++j) part[j] = v[i + j];
+            Elements<T, Lanes::kRun>::store(out + e0 + i, Elements<T, Lanes::kRun>::pack(part));
+            continue;
           }
         }
-        group_keys[g] = ordered(a.group_top == 2 ? __fadd_rn(first, second) : first);
+#pragma unroll
+        for (int j = 0; j < Lanes::kRun; ++j)
+          if (e0 + i + j < experts) out[e0 + i + j] = from_float<T>(v[i + j]);
       }
+    };
+    if constexpr (kWholeRow) {
+      Lanes lanes;
+      lanes.load(l, experts, plan.whole);
+      float s[kPer];
+      scores(lanes.v, experts, a.score, s);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (e0 + i < experts) row[e0 + i] = 0.f;
       __syncwarp();
-      // the chosen groups' keys become 0: taken
-      for (int j = 0; j < a.top_groups; ++j) {
-        const int g = best_of(group_keys, a.groups);
-        __syncwarp();
-        if (lane == 0) group_keys[g] = 0;
-        __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i)
+        if (chosen[i] >= 0) row[chosen[i]] = g[i] * a.scale;
+      __syncwarp();
+      float d[kPer], dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        d[i] = e0 + i < experts ? row[e0 + i] : 0.f;
+        dot = fmaf(d[i], s[i], dot);
       }
-      for (int e = lane; e < experts; e += 32)
-        if (group_keys[e / size] != 0) keys[e] = 0;
+      dot = warp_sum(dot);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) d[i] = s[i] * (d[i] - dot);
+      store_row(d);
       __syncwarp();
-    }
-    float total = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-      const int e = best_of(keys, experts);
-      __syncwarp();
-      if (lane == 0) {
-        keys[e] = 0;
-        a.indices[token * a.k + j] = e;
-        if (a.counts != nullptr)
-          atomicAdd(reinterpret_cast<unsigned long long*>(a.counts) + e, 1ull);
+    } else {
+      float zero[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) zero[i] = 0.f;
+      store_row(zero);
+      float x[kSlots], value[kSlots];
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) x[i] = chosen[i] >= 0 ? to_float(l[chosen[i]]) : -INFINITY;
+      float s[kSlots], total = 0.f;  // the scores, the softmax's to a factor
+      float m = -INFINITY;
+      if (a.score == kSoftmax) {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) m = fmaxf(m, x[i]);
+        m = warp_max(m);
       }
-      total += s[e];
-      __syncwarp();
-      if (!a.renormalize && lane == 0) a.weights[token * a.k + j] = s[e] * a.scale;
-      if (a.renormalize && lane == 0) group_keys[j] = e;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (a.score != kSoftmax)
+          s[i] = chosen[i] >= 0 ? sigmoid(x[i]) : 0.f;
+        else
+          s[i] = m == -INFINITY && x[i] == x[i] ? 0.f : expf(x[i] - m);
+        total += s[i];
+      }
+      float dot = 0.f;
+      if (a.renormalize) {
+        total = warp_sum(total);
+        total = a.score == kSoftmax ? (total == 0.f ? 1.f : total) : total + kTiny;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) dot = fmaf(g[i], __fdiv_rn(s[i], total), dot);
+        dot = warp_sum(dot);
+      } else {
+        total = 1.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        value[i] = a.scale * __fdiv_rn(s[i], total) * (g[i] - dot);
+        if (a.score != kSoftmax) value[i] *= 1.0f - s[i];
+      }
+      __syncwarp();  // the zeros are written
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i)
+        if (chosen[i] >= 0) out[chosen[i]] = from_float<T>(value[i]);
     }
-    __syncwarp();
-    if (a.renormalize)
-      for (int j = lane; j < a.k; j += 32)
-        a.weights[token * a.k + j] = __fdiv_rn(s[group_keys[j]], total + kTiny) * a.scale;
-    __syncwarp();
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    route_backward_kernel(const __grid_constant__ muon_train_route_args a,
-                          const float* __restrict__ grad_weights, T* __restrict__ grad) {
-  extern __shared__ float smem[];
-  const int experts = static_cast<int>(a.experts);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* s = smem + warp * 2 * experts;
-  float* d = s + experts;
-  for (int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp; token < a.tokens;
-       token += static_cast<int64_t>(gridDim.x) * kWarps) {
-    scores(static_cast<const T*>(a.logits) + token * a.ld, experts, a.score, s);
-    for (int e = lane; e < experts; e += 32) d[e] = 0.f;
-    __syncwarp();
-    float total = 0.f, dot = 0.f;  // over the chosen: s, and dw s
-    for (int j = lane; j < a.k; j += 32) {
-      const int64_t e = a.indices[token * a.k + j];
-      if (e < 0 || e >= experts) continue;
-      total += s[e];
-      dot += grad_weights[token * a.k + j] * s[e];
-    }
-    total = warp_sum(total) + kTiny;
-    dot = warp_sum(dot);
-    for (int j = lane; j < a.k; j += 32) {
-      const int64_t e = a.indices[token * a.k + j];
-      if (e < 0 || e >= experts) continue;
-      const float g = grad_weights[token * a.k + j];
-      d[e] = a.scale * (a.renormalize ? (g - dot / total) / total : g);
-    }
-    __syncwarp();
-    float shared = 0.f;  // softmax: sum of d s
-    if (a.score == kSoftmax) {
-      for (int e = lane; e < experts; e += 32) shared += d[e] * s[e];
-      shared = warp_sum(shared);
-    }
-    T* out = grad + token * a.experts;
-    for (int e = lane; e < experts; e += 32) {
-      const float v = a.score == kSoftmax ? s[e] * (d[e] - shared) : d[e] * s[e] * (1.0f - s[e]);
-      out[e] = from_float<T>(v);
-    }
-    __syncwarp();
   }
 }
 
@@ -209,8 +400,8 @@ int check(const muon_train_route_args* a) {
 int grid_for(int64_t tokens, unsigned* grid) {
   int sms = 0;
   const int rc = sm_count(&sms);
-  const int64_t want = (tokens + kWarps - 1) / kWarps;
-  *grid = static_cast<unsigned>(want < sms * 8 ? want : sms * 8);
+  const int64_t want = (tokens + kWarps - 1) / kWarps, most = static_cast<int64_t>(sms) * kBlocksPerSm;
+  *grid = static_cast<unsigned>(want < most ? want : most);
   return rc;
 }
 
@@ -222,25 +413,68 @@ int allow_smem(Kernel kernel, size_t bytes) {
       kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
-template <typename T>
-int forward(const muon_train_route_args& a, void* stream) {
-  unsigned grid = 0;
-  const size_t smem = kWarps * 3 * a.experts * sizeof(float);
-  int rc = grid_for(a.tokens, &grid);
-  if (rc == MUON_POLAR_OK) rc = allow_smem(route_kernel<T>, smem);
-  if (rc != MUON_POLAR_OK) return rc;
-  return launch(route_kernel<T>, dim3(grid), kThreads, smem, 1, stream, a);
+template <typename T, int kPer>
+Plan make_plan(const muon_train_route_args& a, int64_t ld, const void* other) {
+  constexpr int kRun = Row<T, kPer>::kRun;
+  Plan p{};
+  p.whole = a.experts % kRun == 0 && ld % kRun == 0 && aligned16(a.logits) && aligned16(other);
+  p.by_logit = a.score == kSoftmax && a.bias == nullptr && (a.groups == 1 || a.group_top == 1);
+  const int64_t size = a.experts / a.groups, lanes = size / kPer;
+  p.lanes_a_group = a.groups == 1 ? 1 : (size % kPer == 0 && (lanes & (lanes - 1)) == 0) ? static_cast<int>(lanes) : 0;
+  return p;
 }
 
-template <typename T>
+template <typename T, int kPer>
+int forward(const muon_train_route_args& a, void* stream) {
+  unsigned grid = 0;
+  const Plan plan = make_plan<T, kPer>(a, a.tokens > 1 ? a.ld : a.experts, nullptr);
+  const size_t smem = (1 + kWarps * (plan.lanes_a_group > 0 ? 1 : 2)) * a.experts * sizeof(float);
+  int rc = grid_for(a.tokens, &grid);
+  if (rc == MUON_POLAR_OK) rc = allow_smem(route_kernel<T, kPer>, smem);
+  if (rc != MUON_POLAR_OK) return rc;
+  if (a.counts != nullptr && grid > 1) {  // one block writes its counts, more add them up
+    const cudaError_t e = cudaMemsetAsync(a.counts, 0, a.experts * sizeof(int64_t),
+                                          static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  return launch(route_kernel<T, kPer>, dim3(grid), kThreads, smem, 1, stream, a, plan);
+}
+
+template <typename T, int kPer>
 int backward(const muon_train_route_args& a, const float* grad_weights, void* grad, void* stream) {
   unsigned grid = 0;
-  const size_t smem = kWarps * 2 * a.experts * sizeof(float);
+  const Plan plan = make_plan<T, kPer>(a, a.tokens > 1 ? a.ld : a.experts, grad);
   int rc = grid_for(a.tokens, &grid);
-  if (rc == MUON_POLAR_OK) rc = allow_smem(route_backward_kernel<T>, smem);
+  if (a.score == kSoftmax && !a.renormalize) {
+    const size_t smem = kWarps * a.experts * sizeof(float);
+    if (rc == MUON_POLAR_OK) rc = allow_smem(route_backward_kernel<T, kPer, true>, smem);
+    if (rc != MUON_POLAR_OK) return rc;
+    return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, smem, 1, stream, a, plan,
+                  grad_weights, static_cast<T*>(grad));
+  }
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(route_backward_kernel<T>, dim3(grid), kThreads, smem, 1, stream, a, grad_weights,
-                static_cast<T*>(grad));
+  return launch(route_backward_kernel<T, kPer, false>, dim3(grid), kThreads, 0, 1, stream, a, plan,
+                grad_weights, static_cast<T*>(grad));
+}
+
+// kPer: a lane's experts, the power of two that covers them.
+template <typename T>
+int forward(const muon_train_route_args& a, void* stream) {
+  if (a.experts <= 32) return forward<T, 1>(a, stream);
+  if (a.experts <= 64) return forward<T, 2>(a, stream);
+  if (a.experts <= 128) return forward<T, 4>(a, stream);
+  if (a.experts <= 256) return forward<T, 8>(a, stream);
+  if (a.experts <= 512) return forward<T, 16>(a, stream);
+  return forward<T, 32>(a, stream);
+}
+template <typename T>
+int backward(const muon_train_route_args& a, const float* grad_weights, void* grad, void* stream) {
+  if (a.experts <= 32) return backward<T, 1>(a, grad_weights, grad, stream);
+  if (a.experts <= 64) return backward<T, 2>(a, grad_weights, grad, stream);
+  if (a.experts <= 128) return backward<T, 4>(a, grad_weights, grad, stream);
+  if (a.experts <= 256) return backward<T, 8>(a, grad_weights, grad, stream);
+  if (a.experts <= 512) return backward<T, 16>(a, grad_weights, grad, stream);
+  return backward<T, 32>(a, grad_weights, grad, stream);
 }
 
 }  // namespace
@@ -253,12 +487,11 @@ int muon_train_route_sm100(const muon_train_route_args* args, void* stream) {
   const int rc = check(args);
   if (rc != MUON_POLAR_OK) return rc;
   if (args->tokens > 0 && args->weights == nullptr) return MUON_POLAR_ERR_INVALID_ARGUMENT;
-  if (args->counts != nullptr) {
-    const cudaError_t e = cudaMemsetAsync(args->counts, 0, args->experts * sizeof(int64_t),
-                                          static_cast<cudaStream_t>(stream));
-    if (e != cudaSuccess) return static_cast<int>(e);
+  if (args->tokens == 0) {
+    if (args->counts == nullptr) return MUON_POLAR_OK;
+    return static_cast<int>(cudaMemsetAsync(args->counts, 0, args->experts * sizeof(int64_t),
+                                            static_cast<cudaStream_t>(stream)));
   }
-  if (args->tokens == 0) return MUON_POLAR_OK;
   switch (args->dtype) {
     case MUON_TRAIN_F32: return forward<float>(*args, stream);
     case MUON_TRAIN_BF16: return forward<__nv_bfloat16>(*args, stream);
