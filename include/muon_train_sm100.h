@@ -145,7 +145,7 @@ int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
  * The experts are `groups` equal runs.  A group's key is the sum of its
  * group_top (1 or 2) largest keys; the top_groups best groups stay, and the k
  * largest keys among their experts are chosen, in descending order.  Equal
- * keys go to the lowest index, and a NaN key is below every number.
+ * keys go to the lowest index, and a NaN key counts as -inf.
  *   weight_j = scale * s_j / (sum of the chosen s + 1e-20)   (renormalize)
  *   weight_j = scale * s_j                                    (otherwise)
  * A softmax row without a logit above -inf has s = 0.  The bias only chooses:

@@ -62,7 +62,7 @@ CU_SOURCES = {  # source -> the headers it includes
     "muon_update_sm100.cu": ["sm100_ptx.cuh", "muon_polar_sm100.h"],
     "distill_topk_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "residual_norm_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
-    "route_experts_sm100.cu": ["train_common.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "route_experts_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
 }
 OP_SOURCES = {
     "polar_step_op.cpp": ["muon_polar_sm100.h"],

@@ -15,6 +15,8 @@
 
 namespace muon_train {
 
+cudaError_t norm_status(uint32_t* flags, int clear);  // residual_norm_sm100.cu
+
 std::atomic<uint64_t>& launch_counter() {
   static std::atomic<uint64_t> count{0};
   return count;
@@ -314,26 +316,6 @@ struct Ring {
   Cut cut;
   int stages;
 };
-
-__device__ uint32_t g_status = 0;
-
-// Waits for the phase of `bar`; gives up after the wait limit, or once another
-// thread of the block has: the block then runs on without waiting, and the
-// device status tells.
-__device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  if (muon_sm100::mbar_try_wait(bar, parity)) return;
-  const uint64_t t0 = muon_sm100::global_timer_ns();
-  for (uint32_t spins = 1;; ++spins) {
-    if (muon_sm100::mbar_try_wait(bar, parity)) return;
-    if ((spins & 63u) != 0) continue;
-    if (*failed) return;
-    if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
-      *failed = 1;
-      atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
-      return;
-    }
-  }
-}
 
 // Arrives at a named barrier without waiting for the others.
 __device__ __forceinline__ void named_arrive(uint32_t id, uint32_t count) {
@@ -657,9 +639,8 @@ int run_vectors(const muon_train_distill_args& a, Mode mode, int threads, int pa
 template <typename T, Mode kMode>
 int run_ring(const muon_train_distill_args& a, int parts, int stages, int64_t workers, void* stream) {
   const size_t smem = static_cast<size_t>(stages) * kStageBytes + 2 * List::bytes(a.top);
-  static const cudaError_t allowed = cudaFuncSetAttribute(
-      distill_ring_kernel<T, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-  if (allowed != cudaSuccess) return static_cast<int>(allowed);
+  const int rc = allow_smem<distill_ring_kernel<T, kMode>>(kRingBytes);
+  if (rc != MUON_POLAR_OK) return rc;
   const Ring ring{Cut{parts, same_phase(a, sizeof(T))}, stages};
   return launch(distill_ring_kernel<T, kMode>, dim3(static_cast<unsigned>(workers * parts)),
                 kConsumers + 64, smem, kMode == kGradFromStats ? 1 : parts, stream, a, ring);
@@ -750,17 +731,15 @@ uint64_t muon_train_launch_count(void) {
 }
 
 int muon_train_read_device_status(int device, uint32_t* flags, int clear) {
-  using muon_train::g_status;
   if (flags == nullptr) return MUON_POLAR_ERR_INVALID_ARGUMENT;
   int prev = 0;
   cudaError_t e = cudaGetDevice(&prev);
   if (e == cudaSuccess && device != prev) e = cudaSetDevice(device);
   if (e != cudaSuccess) return static_cast<int>(e);
   uint32_t v = 0;
-  const uint32_t zero = 0;
   e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
-  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+  if (e == cudaSuccess) e = muon_train::take_status(&v, clear);
+  if (e == cudaSuccess) e = muon_train::norm_status(&v, clear);
   if (device != prev) cudaSetDevice(prev);
   if (e != cudaSuccess) return static_cast<int>(e);
   *flags = v;

@@ -24,12 +24,16 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x)));
 }
 
-// Order-preserving unsigned image of a key: 0 is kept for "taken", 1 for NaN
-// (below -inf); -0 and +0 are one key.
-__device__ __forceinline__ uint32_t ordered(float key) {
-  if (key != key) return 1u;
-  const uint32_t b = __float_as_uint(key + 0.0f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+// Keys are compared as they are, which makes -0 and +0 one key.  A NaN counts
+// as -inf; NaN itself then marks a key that can no longer be chosen, since a
+// maximum passes over it and it equals nothing.
+__device__ __forceinline__ float number(float key) { return fmaxf(key, -INFINITY); }
+__device__ __forceinline__ float taken() { return __int_as_float(0x7fffffff); }
+
+__device__ __forceinline__ float lanes_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, %2;" : "=f"(m) : "f"(v), "r"(kFullMask));
+  return m;
 }
 
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -96,13 +100,10 @@ struct Plan {
   int lanes_a_group;  // a power of two, when no lane has experts of two groups; else 0
 };
 
+// The two largest of (first, second, key).
 __device__ __forceinline__ void best_two(float key, float& first, float& second) {
-  if (key > first) {  // a NaN is passed over
-    second = first;
-    first = key;
-  } else if (key > second) {
-    second = key;
-  }
+  second = fmaxf(second, fminf(first, key));
+  first = fmaxf(first, key);
 }
 
 // Forward: one warp a token.  The time goes into instructions, not memory
@@ -110,7 +111,7 @@ __device__ __forceinline__ void best_two(float key, float& first, float& second)
 // keys and scores stay in registers, an argmax is one redux of the lanes'
 // best keys, and only the winning lane looks for its next one.
 template <typename T, int kPer>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
     route_kernel(const __grid_constant__ muon_train_route_args a, Plan plan) {
   extern __shared__ float smem[];
   const int experts = static_cast<int>(a.experts);
@@ -132,15 +133,12 @@ __global__ void __launch_bounds__(kThreads)
     scores(l.v, experts, a.score, s);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      key[i] = plan.by_logit ? l.v[i] : a.bias != nullptr ? __fadd_rn(s[i], bias[i]) : s[i];
+      const float k = plan.by_logit ? l.v[i] : a.bias != nullptr ? __fadd_rn(s[i], bias[i]) : s[i];
+      key[i] = e0 + i < experts ? number(k) : taken();
       if (e0 + i < experts) row[e0 + i] = s[i];
     }
     if (token + step < a.tokens)
       l.load(static_cast<const T*>(a.logits) + (token + step) * a.ld, experts, plan.whole);
-    uint32_t taken = 0;  // a bit for each of the lane's experts that cannot be chosen
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (e0 + i >= experts) taken |= 1u << i;
     if (a.groups > 1) {
       const int size = experts / a.groups;
       if (plan.lanes_a_group > 0) {
@@ -152,91 +150,92 @@ __global__ void __launch_bounds__(kThreads)
           second = fmaxf(fminf(first, f), fmaxf(second, g));
           first = fmaxf(first, f);
         }
-        const uint32_t mine = ordered(a.group_top == 2 ? __fadd_rn(first, second) : first);
+        const float mine = number(a.group_top == 2 ? __fadd_rn(first, second) : first);
         const int group = lane / plan.lanes_a_group;
         int better = 0;
         for (int g = 0; g < a.groups; ++g) {
-          const uint32_t other = __shfl_sync(kFullMask, mine, g * plan.lanes_a_group);
+          const float other = __shfl_sync(kFullMask, mine, g * plan.lanes_a_group);
           better += other > mine || (other == mine && g < group);
         }
-        if (better >= a.top_groups) taken = 0xffffffffu;
+        if (better >= a.top_groups) {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) key[i] = taken();
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
           if (e0 + i < experts) row_keys[e0 + i] = key[i];
         __syncwarp();
         // each lane ranks its groups g = lane, + 32, ..
-        uint32_t mine[MUON_TRAIN_MAX_EXPERTS / 32];
+        float mine[MUON_TRAIN_MAX_EXPERTS / 32];
         const int rounds = (a.groups + 31) / 32;
         for (int r = 0; r < rounds; ++r) {
           const int g = r * 32 + lane;
           float first = -INFINITY, second = -INFINITY;
           if (g < a.groups)
             for (int e = g * size; e < (g + 1) * size; ++e) best_two(row_keys[e], first, second);
-          mine[r] = g < a.groups ? ordered(a.group_top == 2 ? __fadd_rn(first, second) : first) : 0u;
+          mine[r] = g < a.groups ? number(a.group_top == 2 ? __fadd_rn(first, second) : first) : taken();
         }
         __syncwarp();
         // the best groups one by one; row_keys now says which groups stay
         for (int g = lane; g < a.groups; g += 32) row_keys[g] = 0.f;
         __syncwarp();
         for (int j = 0; j < a.top_groups; ++j) {
-          uint32_t best = 0;
-          int at = 0;
-          for (int r = 0; r < rounds; ++r)
-            if (mine[r] > best) {
-              best = mine[r];
-              at = r;
-            }
-          const uint32_t top = __reduce_max_sync(kFullMask, best);
-          const int g = __reduce_min_sync(kFullMask, best == top ? at * 32 + lane : 0x7fffffff);
+          float best = taken();
+          for (int r = 0; r < rounds; ++r) best = fmaxf(best, mine[r]);
+          best = lanes_max(best);
+          int g = 0x7fffffff;
+          for (int r = rounds - 1; r >= 0; --r)
+            if (mine[r] == best) g = r * 32 + lane;
+          g = __reduce_min_sync(kFullMask, g);
           if ((g & 31) == lane) {
-            mine[g >> 5] = 0;
+            mine[g >> 5] = taken();
             row_keys[g] = 1.f;
           }
         }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          if (e0 + i < experts && row_keys[(e0 + i) / size] == 0.f) taken |= 1u << i;
+          if (e0 + i < experts && row_keys[(e0 + i) / size] == 0.f) key[i] = taken();
       }
     }
-    // the k best: the lanes' best keys, and within the best lane the first
-    uint32_t best;
-    int at;
-    const auto look = [&] {
-      best = 0;
-      at = 0;
+    // the k best: the lanes' best keys, the lowest lane of equal ones, and in
+    // it the first
+    float best = taken();
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const uint32_t o = (taken >> i) & 1u ? 0u : ordered(key[i]);
-        if (o > best) {
-          best = o;
-          at = i;
-        }
-      }
-    };
-    look();
+    for (int i = 0; i < kPer; ++i) best = fmaxf(best, key[i]);
     int chosen[kSlots];
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) chosen[i] = 0;
     for (int j = 0; j < a.k; ++j) {
-      const uint32_t top = __reduce_max_sync(kFullMask, best);
+      const float top = lanes_max(best);
       const int who = __ffs(__ballot_sync(kFullMask, best == top)) - 1;
-      const int e = __shfl_sync(kFullMask, e0 + at, who);
+      int e = 0;
+      if (lane == who) {
+        int at = 0;
+#pragma unroll
+        for (int i = kPer - 1; i >= 0; --i)
+          if (key[i] == top) at = i;
+        best = taken();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (i == at) key[i] = taken();
+          best = fmaxf(best, key[i]);
+        }
+        e = e0 + at;
+      }
+      e = __shfl_sync(kFullMask, e, who);
       if (lane == (j & 31)) {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i)
           if (i == (j >> 5)) chosen[i] = e;
-      }
-      if (lane == who) {
-        taken |= 1u << at;
-        look();
       }
     }
     __syncwarp();  // row is written
     float w[kSlots], total = 0.f;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
+      if (i * 32 >= a.k) break;
       w[i] = i * 32 + lane < a.k ? row[chosen[i]] : 0.f;
       total += w[i];
     }
@@ -244,6 +243,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
       const int j = i * 32 + lane;
+      if (i * 32 >= a.k) break;
       if (j >= a.k) continue;
       a.weights[token * a.k + j] = (a.renormalize ? __fdiv_rn(w[i], total) : w[i]) * a.scale;
       a.indices[token * a.k + j] = chosen[i];
@@ -405,13 +405,9 @@ int grid_for(int64_t tokens, unsigned* grid) {
   return rc;
 }
 
-// Shared memory above 48 KB needs the kernel's leave.
-template <typename Kernel>
-int allow_smem(Kernel kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return MUON_POLAR_OK;
-  return static_cast<int>(cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-}
+// Shared memory of a block with the most experts; above 48 KB it needs the
+// kernel's leave.
+constexpr size_t kMostSmem = (1 + kWarps * 2) * MUON_TRAIN_MAX_EXPERTS * sizeof(float);
 
 template <typename T, int kPer>
 Plan make_plan(const muon_train_route_args& a, int64_t ld, const void* other) {
@@ -430,7 +426,7 @@ int forward(const muon_train_route_args& a, void* stream) {
   const Plan plan = make_plan<T, kPer>(a, a.tokens > 1 ? a.ld : a.experts, nullptr);
   const size_t smem = (1 + kWarps * (plan.lanes_a_group > 0 ? 1 : 2)) * a.experts * sizeof(float);
   int rc = grid_for(a.tokens, &grid);
-  if (rc == MUON_POLAR_OK) rc = allow_smem(route_kernel<T, kPer>, smem);
+  if (rc == MUON_POLAR_OK && smem > 48 * 1024) rc = allow_smem<route_kernel<T, kPer>>(kMostSmem);
   if (rc != MUON_POLAR_OK) return rc;
   if (a.counts != nullptr && grid > 1) {  // one block writes its counts, more add them up
     const cudaError_t e = cudaMemsetAsync(a.counts, 0, a.experts * sizeof(int64_t),
@@ -447,7 +443,7 @@ int backward(const muon_train_route_args& a, const float* grad_weights, void* gr
   int rc = grid_for(a.tokens, &grid);
   if (a.score == kSoftmax && !a.renormalize) {
     const size_t smem = kWarps * a.experts * sizeof(float);
-    if (rc == MUON_POLAR_OK) rc = allow_smem(route_backward_kernel<T, kPer, true>, smem);
+    if (rc == MUON_POLAR_OK && smem > 48 * 1024) rc = allow_smem<route_backward_kernel<T, kPer, true>>(kMostSmem);
     if (rc != MUON_POLAR_OK) return rc;
     return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, smem, 1, stream, a, plan,
                   grad_weights, static_cast<T*>(grad));

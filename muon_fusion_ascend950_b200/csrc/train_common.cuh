@@ -10,6 +10,7 @@
 #include <atomic>
 
 #include "muon_train_sm100.h"
+#include "sm100_ptx.cuh"
 
 namespace muon_train {
 
@@ -197,23 +198,26 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Two fp32 operations in one instruction, each rounded as alone.
+// Two fp32 operations in one instruction, each rounded as alone.  The pairs
+// pass as 64-bit registers, so that they need not be put together again.
+__device__ __forceinline__ uint64_t bits(float2 v) { return reinterpret_cast<const uint64_t&>(v); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(bits(a)), "l"(bits(b)));
   return d;
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(bits(a)), "l"(bits(b)));
   return d;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The largest element of a vector, joined to m; NaN elements are passed over.
 __device__ __forceinline__ float vector_max(const uint4& u, float m, float) {
@@ -245,6 +249,38 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// ------------------------------------------------------------ bounded waits
+// Each translation unit has its own status word; the read call joins them.
+static __device__ uint32_t g_status = 0;
+
+// Waits for the phase of `bar`; gives up after the wait limit, or once another
+// thread of the block has: the block then runs on without waiting, and the
+// device status tells.
+__device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  if (muon_sm100::mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = muon_sm100::global_timer_ns();
+  for (uint32_t spins = 1;; ++spins) {
+    if (muon_sm100::mbar_try_wait(bar, parity)) return;
+    if ((spins & 63u) != 0) continue;
+    if (*failed) return;
+    if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
+      *failed = 1;
+      atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
+      return;
+    }
+  }
+}
+
+// Joins this translation unit's status to *flags, and zeroes it if asked.
+static inline cudaError_t take_status(uint32_t* flags, int clear) {
+  uint32_t v = 0;
+  const uint32_t zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+  *flags |= v;
+  return e;
+}
+
 // ------------------------------------------------------------ host side
 std::atomic<uint64_t>& launch_counter();
 
@@ -257,6 +293,22 @@ inline int sm_count(int* sms) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
   return e == cudaSuccess ? MUON_POLAR_OK : static_cast<int>(e);
+}
+
+// Lets a kernel have up to `bytes` of dynamic shared memory, once for each
+// device.
+template <auto kKernel>
+int allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return MUON_POLAR_OK;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return MUON_POLAR_OK;
 }
 
 // One launch, as clusters of `cluster` blocks along x when that is over 1.

@@ -3,6 +3,7 @@
 // residual block, routing to experts.  CUDA kernels through the C ABI
 // (include/muon_train_sm100.h); gradients on the Autograd key.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -46,6 +47,12 @@ void CheckDevice(const Tensor& t, const Tensor& like, const char* who, const cha
                     ", got ", t.device());
 }
 
+// An uninitialised contiguous CUDA tensor, without the dispatcher's way there:
+// small calls are bound by the host.
+Tensor Empty(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
+}
+
 void* Ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 const Tensor& Given(const OptTensor& t) {
   static const Tensor none;
@@ -79,12 +86,12 @@ int64_t RowStride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size
 // that the logits' are read in.
 Tensor GradLike(const Tensor& z) {
   const int64_t ld = RowStride(z), rows = z.size(0), cols = z.size(1);
-  if (rows == 0 || ld > 2 * cols) return at::empty({rows, cols}, z.options());
+  if (rows == 0 || ld > 2 * cols) return Empty({rows, cols}, z.scalar_type(), z);
   const int64_t item = z.element_size();
   const int64_t shift = static_cast<int64_t>(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / item;
-  if (ld == cols && shift == 0) return at::empty({rows, cols}, z.options());
+  if (ld == cols && shift == 0) return Empty({rows, cols}, z.scalar_type(), z);
   const int64_t used = (rows - 1) * ld + cols;
-  return at::empty({used + shift}, z.options()).as_strided({rows, cols}, {ld, 1}, shift);
+  return Empty({used + shift}, z.scalar_type(), z).as_strided({rows, cols}, {ld, 1}, shift);
 }
 
 at::IntArrayRef Lead(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
@@ -148,8 +155,7 @@ std::tuple<Tensor, Tensor> DistillCuda(const Tensor& student, const Tensor& valu
   const char* who = "distill_topk";
   DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
   const c10::cuda::CUDAGuard guard(student.device());
-  const auto f32 = student.options().dtype(at::kFloat);
-  Tensor loss = at::empty(Lead(student), f32), stats = at::empty({in.args.rows, 2}, f32);
+  Tensor loss = Empty(Lead(student), at::kFloat, student), stats = Empty({in.args.rows, 2}, at::kFloat, student);
   in.args.loss = static_cast<float*>(Ptr(loss));
   in.args.stats = static_cast<float*>(Ptr(stats));
   CheckStatus(muon_train_distill_sm100(&in.args, Stream(student)), who);
@@ -183,8 +189,7 @@ std::tuple<Tensor, Tensor> DistillGradCuda(const Tensor& student, const Tensor& 
   DistillInputs in = CheckDistill(student, values, indices, teacher_lse, temperature, who);
   const c10::cuda::CUDAGuard guard(student.device());
   const Tensor scale = RowValues(row_scale, student, who, "row_scale");
-  const auto f32 = student.options().dtype(at::kFloat);
-  Tensor loss = at::empty(Lead(student), f32), stats = at::empty({in.args.rows, 2}, f32);
+  Tensor loss = Empty(Lead(student), at::kFloat, student), stats = Empty({in.args.rows, 2}, at::kFloat, student);
   Tensor grad = GradLike(in.student);
   in.args.row_scale = static_cast<const float*>(Ptr(scale));
   in.args.loss = static_cast<float*>(Ptr(loss));
@@ -284,11 +289,11 @@ std::tuple<Tensor, Tensor, Tensor> ResidualNormCuda(
   const char* who = "residual_norm";
   NormInputs in = CheckNorm(block_out, residual, post, pre, gate, scale, eps, who);
   const c10::cuda::CUDAGuard guard(block_out.device());
-  const auto options = in.block_out.options();
+  const auto dtype = block_out.scalar_type();
   const int64_t rows = in.args.rows;
-  Tensor hidden = at::empty(block_out.sizes(), options);
-  Tensor normed = in.pre.defined() ? at::empty(block_out.sizes(), options) : at::empty({0}, options);
-  Tensor rstd = at::empty({2, rows}, options.dtype(at::kFloat));
+  Tensor hidden = Empty(block_out.sizes(), dtype, block_out);
+  Tensor normed = in.pre.defined() ? Empty(block_out.sizes(), dtype, block_out) : Empty({0}, dtype, block_out);
+  Tensor rstd = Empty({2, rows}, at::kFloat, block_out);
   in.args.hidden = Ptr(hidden);
   in.args.normed = in.pre.defined() ? Ptr(normed) : nullptr;
   in.args.rstd_post = static_cast<float*>(Ptr(rstd));
@@ -328,10 +333,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> ResidualNormBackwardC
   const bool none = rows == 0 || (!dh.defined() && !dn.defined());
   for (int i = 0; i < 6; ++i) {
     if (!wanted[i] || !like[i]->defined())
-      out[i] = at::empty({0}, in.block_out.options());
+      out[i] = Empty({0}, block_out.scalar_type(), block_out);
     else
       out[i] = none ? at::zeros(like[i]->sizes(), like[i]->options())
-                    : at::empty(like[i]->sizes(), like[i]->options());
+                    : Empty(like[i]->sizes(), like[i]->scalar_type(), block_out);
   }
   if (!none) {
     muon_train_norm_grads g{};
@@ -341,8 +346,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> ResidualNormBackwardC
                     &g.grad_pre_weight, &g.grad_gate, &g.grad_residual_scale};
     for (int i = 0; i < 6; ++i) *to[i] = wanted[i] && like[i]->defined() ? Ptr(out[i]) : nullptr;
     g.workspace_bytes = muon_train_residual_norm_workspace_bytes(&in.args);
-    const Tensor workspace = at::empty({static_cast<int64_t>(g.workspace_bytes)},
-                                       in.block_out.options().dtype(at::kByte));
+    const Tensor workspace = Empty({static_cast<int64_t>(g.workspace_bytes)}, at::kByte, block_out);
     g.workspace = Ptr(workspace);
     CheckStatus(muon_train_residual_norm_backward_sm100(&in.args, &g, Stream(block_out)), who);
   }
@@ -403,11 +407,10 @@ std::tuple<Tensor, Tensor, Tensor> RouteCuda(const Tensor& logits, const OptTens
     b = bias->to(at::kFloat).contiguous();
     a.bias = static_cast<const float*>(Ptr(b));
   }
-  const auto i64 = logits.options().dtype(at::kLong);
   at::DimVector shape(Lead(logits));
   shape.push_back(k);
-  Tensor weights = at::empty(shape, logits.options().dtype(at::kFloat));
-  Tensor indices = at::empty(shape, i64), counts = at::empty({a.experts}, i64);
+  Tensor weights = Empty(shape, at::kFloat, logits), indices = Empty(shape, at::kLong, logits);
+  Tensor counts = Empty({a.experts}, at::kLong, logits);
   a.weights = static_cast<float*>(Ptr(weights));
   a.indices = static_cast<int64_t*>(Ptr(indices));
   a.counts = static_cast<int64_t*>(Ptr(counts));
@@ -429,7 +432,7 @@ Tensor RouteBackwardCuda(const Tensor& grad_weights, const Tensor& logits, const
   const c10::cuda::CUDAGuard guard(logits.device());
   const Tensor g = grad_weights.to(at::kFloat).contiguous(), chosen = indices.contiguous();
   a.indices = static_cast<int64_t*>(Ptr(chosen));
-  Tensor grad = at::empty(logits.sizes(), logits.options());
+  Tensor grad = Empty(logits.sizes(), logits.scalar_type(), logits);
   CheckStatus(muon_train_route_backward_sm100(&a, static_cast<const float*>(Ptr(g)), Ptr(grad),
                                               Stream(logits)), who);
   return grad;
