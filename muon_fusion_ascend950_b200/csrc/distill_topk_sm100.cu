@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 4)
   __shared__ float2 warp_part[kBlockThreads / 32];
   __shared__ float2 block_part[kMaxCluster];
   const List list(dynamic, static_cast<int>(a.top));
+  begin_kernel();
   const int64_t row = blockIdx.x / cut.parts;
   const int part = static_cast<int>(blockIdx.x - row * cut.parts);
   const int threads = blockDim.x - 32;  // that hold granules
@@ -377,6 +378,7 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
   }
   __syncthreads();
   if (parts > 1) cluster_sync();  // every block has begun, its barriers are there
+  begin_kernel();
 
   int stage = 0;
   uint32_t phase = 0;
@@ -630,10 +632,10 @@ int run_vectors(const muon_train_distill_args& a, Mode mode, int threads, int pa
   const size_t smem = List::bytes(a.top);
   threads += 32;
   if (mode == kGradFromStats)
-    return launch(distill_kernel<T, kVectors, kGradFromStats>, grid, threads, smem, 1, stream, a, cut);
+    return launch(distill_kernel<T, kVectors, kGradFromStats>, grid, threads, smem, 1, true, stream, a, cut);
   if (mode == kLossGrad)
-    return launch(distill_kernel<T, kVectors, kLossGrad>, grid, threads, smem, parts, stream, a, cut);
-  return launch(distill_kernel<T, kVectors, kLoss>, grid, threads, smem, parts, stream, a, cut);
+    return launch(distill_kernel<T, kVectors, kLossGrad>, grid, threads, smem, parts, true, stream, a, cut);
+  return launch(distill_kernel<T, kVectors, kLoss>, grid, threads, smem, parts, true, stream, a, cut);
 }
 
 template <typename T, Mode kMode>
@@ -643,7 +645,7 @@ int run_ring(const muon_train_distill_args& a, int parts, int stages, int64_t wo
   if (rc != MUON_POLAR_OK) return rc;
   const Ring ring{Cut{parts, same_phase(a, sizeof(T))}, stages};
   return launch(distill_ring_kernel<T, kMode>, dim3(static_cast<unsigned>(workers * parts)),
-                kConsumers + 64, smem, kMode == kGradFromStats ? 1 : parts, stream, a, ring);
+                kConsumers + 64, smem, kMode == kGradFromStats ? 1 : parts, true, stream, a, ring);
 }
 
 template <typename T>

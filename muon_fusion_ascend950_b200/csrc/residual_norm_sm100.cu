@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   __shared__ volatile int failed;
   int turn = 0;
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // every block has begun
+  begin_kernel();
   const Place<N, kOwner> place;
   const int width = static_cast<int>(a.width);
   const float inv_width = 1.0f / static_cast<float>(width);
@@ -455,6 +456,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
     norm_row_kernel(const __grid_constant__ muon_train_norm_args a) {
   __shared__ float red[2 * 32];
+  begin_kernel();
   const Params p{a};
   const int64_t row = blockIdx.x, base = row * a.width;
   const int64_t gate_row = a.gate_rows > 0 ? row / (a.rows / a.gate_rows) : 0;
@@ -578,6 +580,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   const float inv_width = 1.0f / static_cast<float>(width);
   int turn = 0;
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // every block has begun
+  begin_kernel();
   const int64_t worker = kOwner == kWarpRow ? blockIdx.x : place.worker;
   const int64_t workers = kOwner == kWarpRow ? gridDim.x : place.workers;
   const int step = kOwner == kWarpRow ? kWarpRowWarps : 1;
@@ -795,6 +798,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
     norm_backward_row_kernel(const __grid_constant__ Backward b) {
   __shared__ float red[3 * 32];
+  begin_kernel();
   const muon_train_norm_args& a = b.a;
   const Params p{a};
   const float width = static_cast<float>(a.width);
@@ -904,6 +908,7 @@ __device__ float warps_sum(float sum, float (*part)[32]) {
 __global__ void __launch_bounds__(kSumWarps * 32)
     norm_sums_kernel(const __grid_constant__ Backward b) {
   __shared__ float part[kSumWarps][32];
+  begin_kernel();
   const muon_train_norm_args& a = b.a;
   const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
   const bool inside = column < a.width, writes = threadIdx.x < 32 && inside;
@@ -1044,7 +1049,7 @@ int launch_forward(const muon_train_norm_args& a, const Layout& l, dim3 grid, si
                    void* stream) {
   const int rc = smem == 0 ? MUON_POLAR_OK : allow_smem<norm_forward_kernel<T, N, kOwner>>(kRingMost);
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(norm_forward_kernel<T, N, kOwner>, grid, l.threads, smem, l.cluster, stream, a, stages);
+  return launch(norm_forward_kernel<T, N, kOwner>, grid, l.threads, smem, l.cluster, true, stream, a, stages);
 }
 
 template <typename T, int N>
@@ -1068,7 +1073,7 @@ int forward(const muon_train_norm_args& a, void* stream) {
   const int rc = sm_count(&sms);
   if (rc != MUON_POLAR_OK) return rc;
   if (l.elements == 0)
-    return launch(norm_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), kThreads, 0, 1, stream, a);
+    return launch(norm_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), kThreads, 0, 1, true, stream, a);
   if (l.elements == kVec<T>) return forward_rows<T, kVec<T>>(a, l, sms, stream);
   if constexpr (sizeof(T) == 2)
     if (l.elements == 2) return forward_rows<T, 2>(a, l, sms, stream);
@@ -1082,7 +1087,7 @@ int launch_backward(const Backward& b, const Layout& l, void* stream) {
   const int rc = smem == 0 ? MUON_POLAR_OK : allow_smem<norm_backward_kernel<T, N, kOwner, kScaleColumns>>(kRingMost);
   if (rc != MUON_POLAR_OK) return rc;
   return launch(norm_backward_kernel<T, N, kOwner, kScaleColumns>,
-                dim3(static_cast<unsigned>(b.plan.blocks * l.cluster)), l.threads, smem, l.cluster, stream, b,
+                dim3(static_cast<unsigned>(b.plan.blocks * l.cluster)), l.threads, smem, l.cluster, true, stream, b,
                 stages);
 }
 
@@ -1103,7 +1108,7 @@ template <typename T>
 int backward(const Backward& b, const Layout& l, void* stream) {
   if (l.elements == 0)
     return launch(norm_backward_row_kernel<T>, dim3(static_cast<unsigned>(b.plan.blocks)), kThreads,
-                  0, 1, stream, b);
+                  0, 1, true, stream, b);
   if (l.elements == kVec<T>) return backward_rows<T, kVec<T>>(b, l, stream);
   if constexpr (sizeof(T) == 2)
     if (l.elements == 2) return backward_rows<T, 2>(b, l, stream);
@@ -1186,7 +1191,7 @@ int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
   const unsigned columns = static_cast<unsigned>((b.a.width + 31) / 32);
   const int64_t gate_rows = want_gate_sums ? b.plan.groups : 0;
   const unsigned what = 3 + static_cast<unsigned>(gate_rows < kGateRowBlocks ? gate_rows : kGateRowBlocks);
-  return launch(norm_sums_kernel, dim3(columns, what), kSumWarps * 32, 0, 1, stream, b);
+  return launch(norm_sums_kernel, dim3(columns, what), kSumWarps * 32, 0, 1, true, stream, b);
 }
 
 }  // extern "C"

@@ -433,7 +433,7 @@ int forward(const muon_train_route_args& a, void* stream) {
                                           static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  return launch(route_kernel<T, kPer>, dim3(grid), kThreads, smem, 1, stream, a, plan);
+  return launch(route_kernel<T, kPer>, dim3(grid), kThreads, smem, 1, false, stream, a, plan);
 }
 
 template <typename T, int kPer>
@@ -445,11 +445,11 @@ int backward(const muon_train_route_args& a, const float* grad_weights, void* gr
     const size_t smem = kWarps * a.experts * sizeof(float);
     if (rc == MUON_POLAR_OK && smem > 48 * 1024) rc = allow_smem<route_backward_kernel<T, kPer, true>>(kMostSmem);
     if (rc != MUON_POLAR_OK) return rc;
-    return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, smem, 1, stream, a, plan,
+    return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, smem, 1, false, stream, a, plan,
                   grad_weights, static_cast<T*>(grad));
   }
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(route_backward_kernel<T, kPer, false>, dim3(grid), kThreads, 0, 1, stream, a, plan,
+  return launch(route_backward_kernel<T, kPer, false>, dim3(grid), kThreads, 0, 1, false, stream, a, plan,
                 grad_weights, static_cast<T*>(grad));
 }
 

@@ -189,6 +189,13 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, const f
     store_run<__half, N>(static_cast<__half*>(p), i, v);
 }
 
+// First in every kernel, by every thread: lets the next kernel of the stream be
+// set up, and waits until the one before has ended and its writes are seen.
+__device__ __forceinline__ void begin_kernel() {
+  muon_sm100::grid_launch_dependents();
+  muon_sm100::grid_dependency_wait();
+}
+
 // ------------------------------------------------------------ arithmetic
 // 2^x in one instruction (ex2.approx: at most 2 ulp; 2^-inf = 0).
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -312,22 +319,28 @@ int allow_smem(size_t bytes) {
 }
 
 // One launch, as clusters of `cluster` blocks along x when that is over 1.
+// With `early`, by programmatic dependent launch: the kernel may be set up
+// while its predecessor in the stream ends, and waits for it (begin_kernel)
+// before it touches memory.
 template <typename Kernel, typename... Args>
-int launch(Kernel kernel, dim3 grid, int threads, size_t smem, int cluster, void* stream,
+int launch(Kernel kernel, dim3 grid, int threads, size_t smem, int cluster, bool early, void* stream,
            Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (cluster > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
   }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return static_cast<int>(e);
