@@ -6,7 +6,9 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <array>
@@ -20,8 +22,7 @@ namespace {
 
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::Variable;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 void CheckStatus(int rc, const char* who) {
@@ -452,43 +453,54 @@ bool Recorded(std::initializer_list<const Tensor*> inputs) {
   return false;
 }
 
-class DistillFunction : public torch::autograd::Function<DistillFunction> {
- public:
-  static variable_list forward(AutogradContext* ctx, const Tensor& student, const Tensor& values,
-                               const Tensor& indices, const OptTensor& lse, double temperature) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = Op<decltype(DistillCuda)>("muon_ascend950::distill_topk");
-    auto [loss, stats] = op.call(student, values, indices, lse, temperature);
-    ctx->save_for_backward({student, values, indices, Given(lse), stats});
-    ctx->saved_data["temperature"] = temperature;
-    ctx->set_materialize_grads(false);
-    ctx->mark_non_differentiable({stats});
-    return {loss, stats};
+// A node of the graph whose next edges are `inputs`, in order.
+template <typename N, typename... Inputs>
+std::shared_ptr<N> MakeNode(const Inputs&... inputs) {
+  auto node = std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
+}
+
+OptTensor Optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+struct DistillBackward : public torch::autograd::Node {
+  SavedVariable student, values, indices, lse, stats;
+  double temperature = 1.0;
+
+  std::string name() const override { return "DistillTopkBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&student, &values, &indices, &lse, &stats}) v->reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     NoSecondOrder("distill_topk");
-    const auto saved = ctx->get_saved_variables();
-    Tensor grad;
-    if (grads[0].defined()) {
-      static auto op = Op<decltype(DistillBackwardCuda)>("muon_ascend950::distill_topk_backward");
-      const OptTensor lse = saved[3].defined() ? OptTensor(saved[3]) : OptTensor();
-      grad = op.call(grads[0], saved[0], saved[1], saved[2], lse, saved[4],
-                     ctx->saved_data["temperature"].toDouble());
-    }
-    return {grad, Tensor(), Tensor(), Tensor(), Tensor()};
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(1);
+    static auto op = Op<decltype(DistillBackwardCuda)>("muon_ascend950::distill_topk_backward");
+    return {op.call(grads[0], student.unpack(), values.unpack(), indices.unpack(), Optional(lse.unpack()),
+                    stats.unpack(), temperature)};
   }
 };
 
 std::tuple<Tensor, Tensor> DistillAutograd(const Tensor& student, const Tensor& values,
                                            const Tensor& indices, const OptTensor& lse,
                                            double temperature) {
-  if (!Recorded({&student})) {
+  static auto op = Op<decltype(DistillCuda)>("muon_ascend950::distill_topk");
+  const auto call = [&] {
     at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = Op<decltype(DistillCuda)>("muon_ascend950::distill_topk");
     return op.call(student, values, indices, lse, temperature);
-  }
-  auto out = DistillFunction::apply(student, values, indices, lse, temperature);
-  return {out[0], out[1]};
+  };
+  if (!Recorded({&student})) return call();
+  auto node = MakeNode<DistillBackward>(student);
+  auto out = call();
+  node->student = SavedVariable(student, false);
+  node->values = SavedVariable(values, false);
+  node->indices = SavedVariable(indices, false);
+  node->lse = SavedVariable(Given(lse), false);
+  node->stats = SavedVariable(std::get<1>(out), false);
+  node->temperature = temperature;
+  torch::autograd::set_history(std::get<0>(out), node);
+  return out;
 }
 
 // The loss with its gradient is not recorded: nothing flows back through it.
@@ -500,43 +512,35 @@ std::tuple<Tensor, Tensor> DistillGradAutograd(const Tensor& student, const Tens
   return op.call(student, values, indices, row_scale, lse, temperature);
 }
 
-class ResidualNormFunction : public torch::autograd::Function<ResidualNormFunction> {
- public:
-  static variable_list forward(AutogradContext* ctx, const Tensor& block_out, const Tensor& residual,
-                               const OptTensor& post, const OptTensor& pre, const OptTensor& gate,
-                               const OptTensor& scale, double eps) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = Op<decltype(ResidualNormCuda)>("muon_ascend950::residual_norm");
-    auto [hidden, normed, rstd] = op.call(block_out, residual, post, pre, gate, scale, eps);
-    ctx->save_for_backward({block_out, residual, Given(post), Given(pre), Given(gate), Given(scale), rstd});
-    ctx->saved_data["eps"] = eps;
-    const Tensor* inputs[6] = {&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)};
-    int64_t wanted = 0;  // a bit for each input that takes a gradient
-    for (int i = 0; i < 6; ++i)
-      if (inputs[i]->defined() && inputs[i]->requires_grad()) wanted |= int64_t{1} << i;
-    ctx->saved_data["wanted"] = wanted;
-    ctx->set_materialize_grads(false);
-    if (Given(pre).defined())
-      ctx->mark_non_differentiable({rstd});
-    else
-      ctx->mark_non_differentiable({normed, rstd});
-    return {hidden, normed, rstd};
+struct ResidualNormBackward : public torch::autograd::Node {
+  std::array<SavedVariable, 6> inputs;
+  SavedVariable rstd;
+  double eps = 0.0;
+
+  std::string name() const override { return "ResidualNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable& v : inputs) v.reset_data();
+    rstd.reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     NoSecondOrder("residual_norm");
-    const auto s = ctx->get_saved_variables();
-    const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-    const int64_t bits = ctx->saved_data["wanted"].toInt();
+    std::lock_guard<std::mutex> lock(mutex_);
+    std::array<Tensor, 6> s;
     std::array<bool, 6> wanted;
-    for (size_t i = 0; i < 6; ++i) wanted[i] = (bits >> i) & 1;
+    for (size_t i = 0; i < 6; ++i) {
+      s[i] = inputs[i].unpack();
+      wanted[i] = s[i].defined() && task_should_compute_output(i);
+    }
+    const OptTensor dn = grads.size() > 1 ? Optional(grads[1]) : OptTensor();
     static auto op = Op<decltype(ResidualNormBackwardCuda)>("muon_ascend950::residual_norm_backward");
-    const OptTensor dn = s[3].defined() ? opt(grads[1]) : OptTensor();
-    auto [d0, d1, d2, d3, d4, d5] = op.call(opt(grads[0]), dn, s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]),
-                                            opt(s[5]), s[6], ctx->saved_data["eps"].toDouble(), wanted);
-    const Tensor all[6] = {d0, d1, d2, d3, d4, d5};
-    variable_list out(7);
+    auto [d0, d1, d2, d3, d4, d5] =
+        op.call(Optional(grads[0]), dn, s[0], s[1], Optional(s[2]), Optional(s[3]), Optional(s[4]),
+                Optional(s[5]), rstd.unpack(), eps, wanted);
+    Tensor* all[6] = {&d0, &d1, &d2, &d3, &d4, &d5};
+    variable_list out(6);
     for (size_t i = 0; i < 6; ++i)
-      if (wanted[i]) out[i] = all[i];
+      if (wanted[i]) out[i] = std::move(*all[i]);
     return out;
   }
 };
@@ -544,55 +548,63 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
 std::tuple<Tensor, Tensor, Tensor> ResidualNormAutograd(
     const Tensor& block_out, const Tensor& residual, const OptTensor& post, const OptTensor& pre,
     const OptTensor& gate, const OptTensor& scale, double eps) {
-  if (!Recorded({&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)})) {
+  static auto op = Op<decltype(ResidualNormCuda)>("muon_ascend950::residual_norm");
+  const auto call = [&] {
     at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = Op<decltype(ResidualNormCuda)>("muon_ascend950::residual_norm");
     return op.call(block_out, residual, post, pre, gate, scale, eps);
-  }
-  auto out = ResidualNormFunction::apply(block_out, residual, post, pre, gate, scale, eps);
-  return {out[0], out[1], out[2]};
+  };
+  const Tensor* inputs[6] = {&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)};
+  if (!Recorded({inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], inputs[5]})) return call();
+  auto node = MakeNode<ResidualNormBackward>(*inputs[0], *inputs[1], *inputs[2], *inputs[3], *inputs[4],
+                                             *inputs[5]);
+  auto out = call();
+  for (size_t i = 0; i < 6; ++i) node->inputs[i] = SavedVariable(*inputs[i], false);
+  node->rstd = SavedVariable(std::get<2>(out), false);
+  node->eps = eps;
+  torch::autograd::set_history(std::get<0>(out), node);
+  if (Given(pre).defined()) torch::autograd::set_history(std::get<1>(out), node);
+  return out;
 }
 
-class RouteFunction : public torch::autograd::Function<RouteFunction> {
- public:
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& bias,
-                               int64_t k, int64_t score, int64_t groups, int64_t top_groups,
-                               int64_t group_top, bool renormalize, double scale) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = Op<decltype(RouteCuda)>("muon_ascend950::route_experts");
-    auto [weights, indices, counts] =
-        op.call(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
-    ctx->save_for_backward({logits, indices});
-    ctx->saved_data["score"] = score;
-    ctx->saved_data["renormalize"] = renormalize;
-    ctx->saved_data["scale"] = scale;
-    ctx->set_materialize_grads(false);
-    ctx->mark_non_differentiable({indices, counts});
-    return {weights, indices, counts};
+struct RouteBackward : public torch::autograd::Node {
+  SavedVariable logits, indices;
+  int64_t score = 0;
+  bool renormalize = true;
+  double scale = 1.0;
+
+  std::string name() const override { return "RouteExpertsBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits.reset_data();
+    indices.reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     NoSecondOrder("route_experts");
-    const auto saved = ctx->get_saved_variables();
-    variable_list out(9);
-    if (grads[0].defined()) {
-      static auto op = Op<decltype(RouteBackwardCuda)>("muon_ascend950::route_experts_backward");
-      out[0] = op.call(grads[0], saved[0], saved[1], ctx->saved_data["score"].toInt(),
-                       ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
-    }
-    return out;
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(1);
+    static auto op = Op<decltype(RouteBackwardCuda)>("muon_ascend950::route_experts_backward");
+    return {op.call(grads[0], logits.unpack(), indices.unpack(), score, renormalize, scale)};
   }
 };
 
 std::tuple<Tensor, Tensor, Tensor> RouteAutograd(const Tensor& logits, const OptTensor& bias, int64_t k,
                                                  int64_t score, int64_t groups, int64_t top_groups,
                                                  int64_t group_top, bool renormalize, double scale) {
-  if (!Recorded({&logits})) {
+  static auto op = Op<decltype(RouteCuda)>("muon_ascend950::route_experts");
+  const auto call = [&] {
     at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = Op<decltype(RouteCuda)>("muon_ascend950::route_experts");
     return op.call(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
-  }
-  auto out = RouteFunction::apply(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
-  return {out[0], out[1], out[2]};
+  };
+  if (!Recorded({&logits})) return call();
+  auto node = MakeNode<RouteBackward>(logits);
+  auto out = call();
+  node->logits = SavedVariable(logits, false);
+  node->indices = SavedVariable(std::get<1>(out), false);
+  node->score = score;
+  node->renormalize = renormalize;
+  node->scale = scale;
+  torch::autograd::set_history(std::get<0>(out), node);
+  return out;
 }
 
 }  // namespace
