@@ -66,13 +66,16 @@ __device__ __forceinline__ float rms_rstd(float sum, float width, float eps) {
 }
 
 // ------------------------------------------------------------ rows in registers
-// A row of up to 16384 elements is held in registers: each thread has 8 of
-// its columns, the same ones in every row, as 8 / N loads of N elements, so
-// that the columns' parameters stay in registers too.  A row belongs to one
-// warp (up to 256 columns, no barrier), to a block of up to 512 threads, or to
-// a cluster of 2 or 4 such blocks, which add up their sums over distributed
-// shared memory.
-constexpr int kElements = 8;       // a thread's columns
+// A row of up to 16384 elements is held in registers: each thread has kE = 8
+// or 16 of its columns, the same ones in every row, as kE / N loads of N
+// elements.  A row belongs to one warp (up to 256 columns, no barrier), to a
+// block of up to 512 threads, or to a cluster of such blocks, which add up
+// their sums over distributed shared memory.  Rows of whole 16-byte vectors
+// have 8 columns a thread up to 4096, 16 above, and a cluster of 2 above
+// 8192: for 16384 x 8192 bf16 backward takes 436 us so, 568 with 8 columns in
+// a cluster, whose barrier holds up every row.  Other rows have 8 columns a
+// thread and clusters of 2 and 4: 16 would not fit the registers (4098
+// columns: 716 us, with 16 a thread 1219).
 constexpr int kMaxThreads = 512;
 constexpr int kWarpRowWarps = 8;   // rows in flight of a block, one a warp
 constexpr int kMaxCluster = 4;
@@ -169,20 +172,20 @@ struct Place {
 };
 
 // A thread's columns of one row, in pairs for the packed fp32 instructions.
-constexpr int kPairs = kElements / 2;
+template <int kE>
 struct Columns {
-  float2 v[kPairs];
+  float2 v[kE / 2];
   __device__ __forceinline__ float& at(int i) { return (i & 1) ? v[i / 2].y : v[i / 2].x; }
   __device__ __forceinline__ float at(int i) const { return (i & 1) ? v[i / 2].y : v[i / 2].x; }
 };
 
 // One parameter's values in a thread's columns; `none` outside the row, and
 // everywhere when there is no such parameter.
-template <int N, typename P>
-__device__ __forceinline__ void load_columns(Columns& v, const P& place, int width, const void* p, int dtype,
+template <int N, int kE, typename P>
+__device__ __forceinline__ void load_columns(Columns<kE>& v, const P& place, int width, const void* p, int dtype,
                                              int64_t offset, float none) {
 #pragma unroll
-  for (int i = 0; i < kElements / N; ++i) {
+  for (int i = 0; i < kE / N; ++i) {
     float part[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) part[j] = none;
@@ -193,23 +196,23 @@ __device__ __forceinline__ void load_columns(Columns& v, const P& place, int wid
   }
 }
 
-template <typename T, int N>
+template <typename T, int N, int kE>
 struct RowVectors {
   using E = Elements<T, N>;
-  typename E::Raw raw[kElements / N];
+  typename E::Raw raw[kE / N];
   template <typename P>
   __device__ __forceinline__ void load(const T* row, const P& place, int width) {
 #pragma unroll
-    for (int i = 0; i < kElements / N; ++i)
+    for (int i = 0; i < kE / N; ++i)
       raw[i] = place.column(i) < width ? E::load(row + place.column(i)) : typename E::Raw();
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < kElements / N; ++i) raw[i] = typename E::Raw();
+    for (int i = 0; i < kE / N; ++i) raw[i] = typename E::Raw();
   }
-  __device__ __forceinline__ void values(Columns& v) const {
+  __device__ __forceinline__ void values(Columns<kE>& v) const {
 #pragma unroll
-    for (int i = 0; i < kElements / N; ++i) {
+    for (int i = 0; i < kE / N; ++i) {
       float part[N];
       E::unpack(raw[i], part);
 #pragma unroll
@@ -217,9 +220,9 @@ struct RowVectors {
     }
   }
   template <typename P>
-  static __device__ __forceinline__ void store(T* row, const P& place, int width, const Columns& v) {
+  static __device__ __forceinline__ void store(T* row, const P& place, int width, const Columns<kE>& v) {
 #pragma unroll
-    for (int i = 0; i < kElements / N; ++i) {
+    for (int i = 0; i < kE / N; ++i) {
       float part[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) part[j] = v.at(i * N + j);
@@ -236,7 +239,7 @@ __device__ __forceinline__ float pair_sum(float2 v) { return v.x + v.y; }
 // registers, which the barrier of the row's sums tells.
 constexpr int kMaxStages = 16;
 constexpr size_t kRingMost = 222 * 1024;  // bytes of an SM's rings
-template <typename T, int N, int kArrays>
+template <typename T, int N, int kE, int kArrays>
 struct Ring {
   uint64_t* full;
   T* data;
@@ -245,7 +248,7 @@ struct Ring {
   uint32_t phase;
 
   __device__ T* at(int stage_, int array, int run) const {
-    return data + ((stage_ * kArrays + array) * kElements / N + run) * static_cast<int>(blockDim.x) * N;
+    return data + ((stage_ * kArrays + array) * kE / N + run) * static_cast<int>(blockDim.x) * N;
   }
   // By one thread: the row's columns of this block from each tensor (not NULL).
   template <typename P>
@@ -256,7 +259,7 @@ struct Ring {
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {  // first the sum of the bytes, then the copies
 #pragma unroll
-      for (int i = 0; i < kElements / N; ++i) {
+      for (int i = 0; i < kE / N; ++i) {
         const int c = (i * place.threads + first) * N;
         const int n = min(span, width - c);
         if (n <= 0) continue;
@@ -275,9 +278,9 @@ struct Ring {
   }
   __device__ void wait() const { ring_wait(&full[stage], phase, failed); }
   template <typename P>
-  __device__ void read(RowVectors<T, N>& v, int array, int width, const P& place) const {
+  __device__ void read(RowVectors<T, N, kE>& v, int array, int width, const P& place) const {
 #pragma unroll
-    for (int i = 0; i < kElements / N; ++i)
+    for (int i = 0; i < kE / N; ++i)
       v.raw[i] = place.column(i) < width
                      ? Elements<T, N>::load(at(stage, array, i) + static_cast<int>(threadIdx.x) * N)
                      : typename Elements<T, N>::Raw();
@@ -295,15 +298,14 @@ __device__ __forceinline__ int64_t gate_row_of(const muon_train_norm_args& a, in
   return a.gate_rows > 1 ? row / (a.rows / a.gate_rows) : 0;
 }
 
-// Forward.  Four rows at a time: their sums share the shuffles and barriers,
+// Forward.  Four rows (of 8 columns a thread) at a time: their sums share the shuffles and barriers,
 // whose latency else held up every row (one row at a time, two blocks an SM:
 // 116 us for 16384 x 4096 bf16, 83 at the copy rate).
-constexpr int kRowsAtOnce = 4;
-
-template <typename T, int N, RowOwner kOwner>
+template <typename T, int N, int kE, RowOwner kOwner>
 __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads,
                                   kOwner == kWarpRow ? 2 : 1)
     norm_forward_kernel(const __grid_constant__ muon_train_norm_args a, int stages) {
+  constexpr int kRowsAtOnce = 32 / kE, kPairs = kE / 2;
   constexpr bool kRing = N * sizeof(T) == 16 && kOwner != kWarpRow;
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SumSlots slots;
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   const float inv_width = 1.0f / static_cast<float>(width);
   const T* y_all = static_cast<const T*>(a.block_out);
   const T* x_all = static_cast<const T*>(a.residual);
-  Ring<T, N, 2> ring{full, reinterpret_cast<T*>(dynamic), &failed, stages, 0, 0};
+  Ring<T, N, kE, 2> ring{full, reinterpret_cast<T*>(dynamic), &failed, stages, 0, 0};
   const T* const tensors[2] = {y_all, x_all};
   if constexpr (kRing) {
     if (threadIdx.x == 0) {
@@ -329,10 +331,10 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     }
     __syncthreads();
   }
-  Columns gain, scale, pre;
+  Columns<kE> gain, scale, pre;
   int64_t gate_row = 0;
   const auto load_gain = [&] {
-    Columns post;
+    Columns<kE> post;
     load_columns<N>(gain, place, width, a.gate, a.gate_dtype, gate_row * width, 1.f);
     load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
 #pragma unroll
@@ -363,9 +365,9 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         }
       }
     };
-    Columns y[kRowsAtOnce], h[kRowsAtOnce];
+    Columns<kE> y[kRowsAtOnce], h[kRowsAtOnce];
     {
-      RowVectors<T, N> ry[kRowsAtOnce], rx[kRowsAtOnce];
+      RowVectors<T, N, kE> ry[kRowsAtOnce], rx[kRowsAtOnce];
 #pragma unroll
       for (int j = 0; j < kRowsAtOnce; ++j) {
         ry[j].clear();
@@ -406,7 +408,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         if (place.tid == 0 && j < rows && a.rstd_post != nullptr) a.rstd_post[first + j * place.workers] = r[j];
       }
     }
-    float sums[4];
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kRowsAtOnce; ++j) {
       const int64_t row = first + j * place.workers;
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         s = fma2(h[j].v[i], h[j].v[i], s);
       }
       sums[j] = pair_sum(s);
-      if (j < rows) RowVectors<T, N>::store(static_cast<T*>(a.hidden) + row * width, place, width, h[j]);
+      if (j < rows) RowVectors<T, N, kE>::store(static_cast<T*>(a.hidden) + row * width, place, width, h[j]);
     }
     if (a.pre_weight == nullptr) {
       if (a.post_weight == nullptr) {
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       if (place.tid == 0 && a.rstd_pre != nullptr) a.rstd_pre[row] = rh;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) h[j].v[i] = mul2(mul2(h[j].v[i], both(rh)), pre.v[i]);
-      RowVectors<T, N>::store(static_cast<T*>(a.normed) + row * width, place, width, h[j]);
+      RowVectors<T, N, kE>::store(static_cast<T*>(a.normed) + row * width, place, width, h[j]);
     }
   }
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed
@@ -543,12 +545,12 @@ __device__ __forceinline__ void chunk_rows(const Backward& b, int64_t chunk, int
 
 // Sums over a block's warps of each warp's columns (kWarpRow), written to a
 // partial row.
-__device__ __forceinline__ void store_warp_columns(float* to, int width, const Columns& v, int n,
-                                                   float (*columns)[32 * kElements]) {
+__device__ __forceinline__ void store_warp_columns(float* to, int width, const Columns<8>& v, int n,
+                                                   float (*columns)[256]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kElements; ++i) columns[warp][((i / n) * 32 + lane) * n + i % n] = v.at(i);
+  for (int i = 0; i < 8; ++i) columns[warp][((i / n) * 32 + lane) * n + i % n] = v.at(i);
   __syncthreads();
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
     float sum = 0.f;
@@ -557,20 +559,61 @@ __device__ __forceinline__ void store_warp_columns(float* to, int width, const C
   }
 }
 
+// Columns that a thread keeps for the whole kernel: in registers with 8 of
+// them, in shared memory, where only the thread itself reads and writes them,
+// with 16.
+template <int kE>
+struct Held {
+  Columns<kE> c;
+  __device__ Held(float4*, int) {}
+  __device__ void set(const Columns<kE>& v) { c = v; }
+  __device__ void pairs(int q, float2 (&p)[2]) const {  // columns 4 q .. 4 q + 3
+    p[0] = c.v[2 * q];
+    p[1] = c.v[2 * q + 1];
+  }
+  __device__ void set_pairs(int q, const float2 (&p)[2]) {
+    c.v[2 * q] = p[0];
+    c.v[2 * q + 1] = p[1];
+  }
+};
+template <>
+struct Held<16> {
+  float4* at;
+  int stride;
+  __device__ Held(float4* area, int index)
+      : at(area + index * 4 * blockDim.x + threadIdx.x), stride(static_cast<int>(blockDim.x)) {}
+  __device__ void set(const Columns<16>& v) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      at[q * stride] = make_float4(v.v[2 * q].x, v.v[2 * q].y, v.v[2 * q + 1].x, v.v[2 * q + 1].y);
+  }
+  __device__ void pairs(int q, float2 (&p)[2]) const {
+    const float4 v = at[q * stride];
+    p[0] = make_float2(v.x, v.y);
+    p[1] = make_float2(v.z, v.w);
+  }
+  __device__ void set_pairs(int q, const float2 (&p)[2]) {
+    at[q * stride] = make_float4(p[0].x, p[0].y, p[1].x, p[1].y);
+  }
+};
+// gain, pre weight, and sums of a residual scale with columns
+__host__ __device__ constexpr int held_columns(bool scale_columns) { return scale_columns ? 3 : 2; }
+
 // Backward.  A worker (block or cluster) takes whole chunks; with one warp a
 // row, the block's warps take every 8th row of the chunk and are added up
 // where the chunk ends.  kScaleColumns: residual_scale has a value for each
 // column (else one value, or none).
-template <typename T, int N, RowOwner kOwner, bool kScaleColumns>
+template <typename T, int N, int kE, RowOwner kOwner, bool kScaleColumns>
 __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads, 1)
     norm_backward_kernel(const __grid_constant__ Backward b, int stages) {
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SumSlots slots;
-  __shared__ float columns[kOwner == kWarpRow ? kWarpRowWarps : 1][32 * kElements];
+  __shared__ float columns[kOwner == kWarpRow ? kWarpRowWarps : 1][256];
   __shared__ uint64_t full[kMaxStages];
   __shared__ volatile int failed;
   // whole vectors come through a ring; else the next row is loaded while this
   // one is worked on where registers allow
+  constexpr int kPairs = kE / 2;
   constexpr bool kRing = N * sizeof(T) == 16 && kOwner != kWarpRow;
   constexpr bool kAhead = !kRing && sizeof(T) == 2 && N > 1;
   constexpr bool kAgain = kRing && sizeof(T) == 2;
@@ -591,7 +634,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   const T* dh_all = static_cast<const T*>(b.g.grad_hidden);
   const T* dn_all = static_cast<const T*>(b.g.grad_normed);
   const bool has_pre = a.pre_weight != nullptr && dn_all != nullptr;
-  RowVectors<T, N> ry, rx, rdh, rdn;
+  RowVectors<T, N, kE> ry, rx, rdh, rdn;
   const auto load_row = [&](int64_t row) {
     ry.load(y_all + row * width, place, width);
     rx.load(x_all + row * width, place, width);
@@ -600,7 +643,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   };
   rdh.clear();
   rdn.clear();
-  Ring<T, N, 4> ring{full, reinterpret_cast<T*>(dynamic), &failed, stages, 0, 0};
+  float4* const held = reinterpret_cast<float4*>(dynamic);
+  Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + (kE == 16 ? held_columns(kScaleColumns) * kE * sizeof(float) * blockDim.x : 0)), &failed, stages, 0, 0};
   const T* const tensors[4] = {y_all, x_all, dh_all, dn_all};
   // thread 0: the row that goes into the ring next
   int64_t ahead_chunk = worker, ahead_row = 0, ahead_end = 0;
@@ -623,11 +667,17 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     __syncthreads();
   }
 
-  Columns gain, pre;  // gain: gate times post weight
-  Columns scale_columns{};
-  float2 scale_one = both(1.f);
-  load_columns<N>(gain, place, width, a.post_weight, a.post_dtype, 0, 1.f);
-  load_columns<N>(pre, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
+  Held<kE> gain(held, 0), pre(held, 1), sum_scale(held, 2);  // gain: gate times post weight
+  Columns<kE> scale_columns{};
+  float2 scale_one = both(1.f), sum_scale_one = both(0.f);
+  {
+    Columns<kE> v;
+    load_columns<N>(v, place, width, a.post_weight, a.post_dtype, 0, 1.f);
+    gain.set(v);
+    load_columns<N>(v, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
+    pre.set(v);
+    if constexpr (kScaleColumns) sum_scale.set(Columns<kE>{});
+  }
   if (!kScaleColumns && a.residual_scale != nullptr)
     scale_one = both(load_any(a.residual_scale, a.scale_dtype, 0));
   const auto scale_of = [&](int i) {
@@ -637,26 +687,24 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       return scale_one;
   };
   const auto load_gain = [&](int64_t gate_row) {
-    Columns post;
-    load_columns<N>(gain, place, width, a.gate, a.gate_dtype, gate_row * width, 1.f);
+    Columns<kE> gate, post;
+    load_columns<N>(gate, place, width, a.gate, a.gate_dtype, gate_row * width, 1.f);
     load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) gain.v[i] = mul2(gain.v[i], post.v[i]);
+    for (int i = 0; i < kPairs; ++i) gate.v[i] = mul2(gate.v[i], post.v[i]);
+    gain.set(gate);
   };
 
-  Columns sum_gain, sum_pre;
-  float2 sum_scale[kScaleColumns ? kPairs : 1];
+  Columns<kE> sum_gain, sum_pre;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) sum_gain.v[i] = sum_pre.v[i] = both(0.f);
-#pragma unroll
-  for (int i = 0; i < (kScaleColumns ? kPairs : 1); ++i) sum_scale[i] = both(0.f);
 
-  const auto store_columns = [&](float* to, const Columns& v) {
+  const auto store_columns = [&](float* to, const Columns<kE>& v) {
     if constexpr (kOwner == kWarpRow) {
       store_warp_columns(to, width, v, N, columns);
     } else {
 #pragma unroll
-      for (int i = 0; i < kElements / N; ++i) {
+      for (int i = 0; i < kE / N; ++i) {
         if (place.column(i) >= width) continue;
 #pragma unroll
         for (int j = 0; j < N; ++j) to[place.column(i) + j] = v.at(i * N + j);
@@ -690,10 +738,10 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       if (b.plan.gate_per_row) load_gain(row);
       const float r = next_r, rh = next_rh;
       load_rstd(row + step);
-      Columns h, u;  // u: dh + rh dn pre
+      Columns<kE> h, u;  // u: dh + rh dn pre
       rdh.values(u);
       float2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
-      Columns y, x, dn;
+      Columns<kE> y, x, dn;
       ry.values(y);
       rx.values(x);
       rdn.values(dn);
@@ -703,13 +751,20 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       if constexpr (kScaleColumns)
         load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        const float2 gy = mul2(gain.v[i], y.v[i]), an = mul2(dn.v[i], pre.v[i]);
-        h.v[i] = fma2(gy, both(r), mul2(scale_of(i), x.v[i]));
-        u.v[i] = fma2(both(rh), an, u.v[i]);
-        s0 = fma2(an, h.v[i], s0);
-        s1 = fma2(gy, u.v[i], s1);
-        s2 = fma2(gy, h.v[i], s2);
+      for (int q = 0; q < kE / 4; ++q) {
+        float2 g[2], p[2];
+        gain.pairs(q, g);
+        pre.pairs(q, p);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = 2 * q + j;
+          const float2 gy = mul2(g[j], y.v[i]), an = mul2(dn.v[i], p[j]);
+          h.v[i] = fma2(gy, both(r), mul2(scale_of(i), x.v[i]));
+          u.v[i] = fma2(both(rh), an, u.v[i]);
+          s0 = fma2(an, h.v[i], s0);
+          s1 = fma2(gy, u.v[i], s1);
+          s2 = fma2(gy, h.v[i], s2);
+        }
       }
       float sums[4] = {pair_sum(s0), pair_sum(s1), pair_sum(s2), 0.f};
       row_sums<kOwner>(sums, slots, turn);
@@ -726,28 +781,38 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         if constexpr (kScaleColumns)
           load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
       }
-      Columns gained;
+      Columns<kE> gained;
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        const float2 d = fma2(both(-k), h.v[i], u.v[i]);
-        gained.v[i] = mul2(d, mul2(y.v[i], both(r)));
-        sum_pre.v[i] = fma2(mul2(dn.v[i], h.v[i]), both(rh), sum_pre.v[i]);
-        float2& sc = sum_scale[kScaleColumns ? i : 0];
-        sc = fma2(d, x.v[i], sc);
-        x.v[i] = mul2(d, scale_of(i));
-        y.v[i] = fma2(both(-ky), y.v[i], mul2(mul2(gain.v[i], both(r)), d));
+      for (int q = 0; q < kE / 4; ++q) {
+        float2 g[2], sc[2];
+        gain.pairs(q, g);
+        if constexpr (kScaleColumns) sum_scale.pairs(q, sc);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = 2 * q + j;
+          const float2 d = fma2(both(-k), h.v[i], u.v[i]);
+          gained.v[i] = mul2(d, mul2(y.v[i], both(r)));
+          sum_pre.v[i] = fma2(mul2(dn.v[i], h.v[i]), both(rh), sum_pre.v[i]);
+          if constexpr (kScaleColumns)
+            sc[j] = fma2(d, x.v[i], sc[j]);
+          else
+            sum_scale_one = fma2(d, x.v[i], sum_scale_one);
+          x.v[i] = mul2(d, scale_of(i));
+          y.v[i] = fma2(both(-ky), y.v[i], mul2(mul2(g[j], both(r)), d));
+        }
+        if constexpr (kScaleColumns) sum_scale.set_pairs(q, sc);
       }
       if (b.g.grad_residual != nullptr)
-        RowVectors<T, N>::store(static_cast<T*>(b.g.grad_residual) + row * width, place, width, x);
+        RowVectors<T, N, kE>::store(static_cast<T*>(b.g.grad_residual) + row * width, place, width, x);
       if (b.g.grad_block_out != nullptr)
-        RowVectors<T, N>::store(static_cast<T*>(b.g.grad_block_out) + row * width, place, width, y);
+        RowVectors<T, N, kE>::store(static_cast<T*>(b.g.grad_block_out) + row * width, place, width, y);
       if (!b.plan.gate_per_row) {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) sum_gain.v[i] = add2(sum_gain.v[i], gained.v[i]);
         continue;
       }
       // a gate row of its own: its gradient leaves with the row
-      Columns gate, post;
+      Columns<kE> gate, post;
       load_columns<N>(gate, place, width, a.gate, a.gate_dtype, row * width, 1.f);
       load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
 #pragma unroll
@@ -757,7 +822,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       }
       if (b.g.grad_gate == nullptr) continue;
 #pragma unroll
-      for (int i = 0; i < kElements / N; ++i) {
+      for (int i = 0; i < kE / N; ++i) {
         if (place.column(i) >= width) continue;
         float part[N];
 #pragma unroll
@@ -774,12 +839,17 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   if (b.pre != nullptr) store_columns(b.pre + worker * width, sum_pre);
   if (b.scale != nullptr) {
     if constexpr (kScaleColumns) {
-      Columns v;
+      Columns<kE> v;
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) v.v[i] = sum_scale[i];
+      for (int q = 0; q < kE / 4; ++q) {
+        float2 sc[2];
+        sum_scale.pairs(q, sc);
+        v.v[2 * q] = sc[0];
+        v.v[2 * q + 1] = sc[1];
+      }
       store_columns(b.scale + worker * width, v);
     } else {  // one value of each block
-      float sum = warp_sum(pair_sum(sum_scale[0]));
+      float sum = warp_sum(pair_sum(sum_scale_one));
       const int warp = threadIdx.x >> 5;
       __syncthreads();
       if ((threadIdx.x & 31) == 0) slots.warp[0][0][warp] = sum;
@@ -982,6 +1052,7 @@ muon_train_norm_args normalised(const muon_train_norm_args& args) {
 struct Layout {
   int elements;  // N: 16 bytes, two 16-bit elements, or one; 0: any width (one block a row)
   RowOwner owner;
+  int columns;   // of a thread: 8 or 16
   int threads, cluster;
   int per_sm;    // blocks that an SM holds: 512 threads of up to 128 registers
 };
@@ -1004,23 +1075,30 @@ Layout make_layout(const muon_train_norm_args& a, const muon_train_norm_grads* g
                                         g->grad_residual, g->grad_gate});
   l.elements = !aligned ? 1 : a.width % vec == 0 ? vec : (vec == 8 && a.width % 2 == 0) ? 2 : 1;
   l.cluster = 1;
-  if (a.width <= 32 * kElements) {
+  l.columns = 8;
+  // With 16 columns a thread, backward's three held arrays and one stage of
+  // four rows have to fit the shared memory: 512 threads of 16-bit types, 480
+  // of fp32.
+  const int most_columns = l.elements == vec ? 16 : 8;
+  const bool wide = a.width > kMaxThreads * 8;
+  const int most_threads =
+      wide && most_columns == 16 && a.dtype == MUON_TRAIN_F32 && g != nullptr ? 480 : kMaxThreads;
+  const int most_cluster = l.elements == vec ? 2 : kMaxCluster;
+  if (a.width <= 32 * 8) {
     l.owner = kWarpRow;
     l.threads = kWarpRowWarps * 32;
-  } else {
-    const int64_t most = kMaxThreads * kElements;
-    l.cluster = a.width <= most ? 1 : a.width <= 2 * most ? 2 : 4;
+  } else if (a.width <= most_cluster * most_threads * most_columns) {
+    if (wide) l.columns = most_columns;
+    while (a.width > l.cluster * most_threads * l.columns) l.cluster *= 2;
     l.owner = l.cluster > 1 ? kClusterRow : kBlockRow;
-    const int64_t each = 32 * kElements * l.cluster;
+    const int64_t each = 32 * l.columns * l.cluster;
     l.threads = static_cast<int>((a.width + each - 1) / each * 32);
-    if (a.width > kMaxCluster * most) {
-      l.elements = 0;
-      l.owner = kBlockRow;
-      l.cluster = 1;
-      l.threads = kThreads;
-    }
+  } else {
+    l.elements = 0;
+    l.owner = kBlockRow;
+    l.threads = kThreads;
   }
-  l.per_sm = kMaxThreads / l.threads;
+  l.per_sm = l.columns == 16 ? 1 : kMaxThreads / l.threads;  // 16: for their shared memory
   return l;
 }
 
@@ -1033,37 +1111,43 @@ int target_workers(const Layout& l, int64_t* target) {
 }
 
 // Shared memory of a ring of `arrays` tensors' rows, and its stages: what the
-// `per_sm` blocks of an SM have between them.
+// `per_sm` blocks of an SM have between them, besides `held` bytes each.
 template <typename T, int N>
-size_t ring_bytes(const Layout& l, int arrays, int per_sm, int* stages) {
+size_t ring_bytes(const Layout& l, int arrays, int per_sm, size_t held, int* stages) {
   *stages = 0;
   if (N * sizeof(T) != 16 || l.owner == kWarpRow) return 0;
-  const size_t stage = static_cast<size_t>(l.threads) * kElements * sizeof(T) * arrays;
-  const size_t most = ((kRingMost + 2048) / per_sm - 2048) / stage;
+  const size_t stage = static_cast<size_t>(l.threads) * l.columns * sizeof(T) * arrays;
+  const size_t most = ((kRingMost + 2048) / per_sm - 2048 - held) / stage;
   *stages = static_cast<int>(most < kMaxStages ? most : kMaxStages);
   return *stages * stage;
 }
 
-template <typename T, int N, RowOwner kOwner>
-int launch_forward(const muon_train_norm_args& a, const Layout& l, dim3 grid, size_t smem, int stages,
-                   void* stream) {
-  const int rc = smem == 0 ? MUON_POLAR_OK : allow_smem<norm_forward_kernel<T, N, kOwner>>(kRingMost);
+template <typename T, int N, int kE, RowOwner kOwner>
+int launch_forward(const muon_train_norm_args& a, const Layout& l, int sms, void* stream) {
+  if (l.columns != kE || l.owner != kOwner) return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not make_layout's
+  const int64_t rows_a_block = kOwner == kWarpRow ? kWarpRowWarps : 1;
+  const int64_t most = static_cast<int64_t>(sms) * l.per_sm / l.cluster;
+  const int64_t want = (a.rows + rows_a_block - 1) / rows_a_block, workers = want < most ? want : most;
+  int stages = 0;
+  const size_t smem = ring_bytes<T, N>(l, 2, l.per_sm, 0, &stages);
+  if (N * sizeof(T) == 16 && kOwner != kWarpRow && stages < 1)
+    return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not with make_layout's sizes
+  const int rc = smem == 0 ? MUON_POLAR_OK : allow_smem<norm_forward_kernel<T, N, kE, kOwner>>(kRingMost);
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(norm_forward_kernel<T, N, kOwner>, grid, l.threads, smem, l.cluster, true, stream, a, stages);
+  return launch(norm_forward_kernel<T, N, kE, kOwner>, dim3(static_cast<unsigned>(workers * l.cluster)),
+                l.threads, smem, l.cluster, true, stream, a, stages);
 }
 
 template <typename T, int N>
 int forward_rows(const muon_train_norm_args& a, const Layout& l, int sms, void* stream) {
-  const int64_t rows_a_block = l.owner == kWarpRow ? kWarpRowWarps : 1;
-  int64_t workers = (a.rows + rows_a_block - 1) / rows_a_block;
-  const int64_t most = static_cast<int64_t>(sms) * l.per_sm / l.cluster;
-  if (workers > most) workers = most;
-  const dim3 grid(static_cast<unsigned>(workers * l.cluster));
-  int stages = 0;
-  const size_t smem = ring_bytes<T, N>(l, 2, l.per_sm, &stages);
-  if (l.owner == kWarpRow) return launch_forward<T, N, kWarpRow>(a, l, grid, smem, stages, stream);
-  if (l.owner == kBlockRow) return launch_forward<T, N, kBlockRow>(a, l, grid, smem, stages, stream);
-  return launch_forward<T, N, kClusterRow>(a, l, grid, smem, stages, stream);
+  if (l.owner == kWarpRow) return launch_forward<T, N, 8, kWarpRow>(a, l, sms, stream);
+  if constexpr (N * sizeof(T) == 16) {
+    if (l.owner == kClusterRow) return launch_forward<T, N, 16, kClusterRow>(a, l, sms, stream);
+    if (l.columns == 16) return launch_forward<T, N, 16, kBlockRow>(a, l, sms, stream);
+  } else {
+    if (l.owner == kClusterRow) return launch_forward<T, N, 8, kClusterRow>(a, l, sms, stream);
+  }
+  return launch_forward<T, N, 8, kBlockRow>(a, l, sms, stream);
 }
 
 template <typename T>
@@ -1080,22 +1164,32 @@ int forward(const muon_train_norm_args& a, void* stream) {
   return forward_rows<T, 1>(a, l, sms, stream);
 }
 
-template <typename T, int N, RowOwner kOwner, bool kScaleColumns>
+template <typename T, int N, int kE, RowOwner kOwner, bool kScaleColumns>
 int launch_backward(const Backward& b, const Layout& l, void* stream) {
+  if (l.columns != kE || l.owner != kOwner) return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not make_layout's
   int stages = 0;
-  const size_t smem = ring_bytes<T, N>(l, 4, l.per_sm, &stages);
-  const int rc = smem == 0 ? MUON_POLAR_OK : allow_smem<norm_backward_kernel<T, N, kOwner, kScaleColumns>>(kRingMost);
+  const size_t held = kE == 16 ? static_cast<size_t>(l.threads) * kE * sizeof(float) * held_columns(kScaleColumns) : 0;
+  const size_t ring = ring_bytes<T, N>(l, 4, l.per_sm, held, &stages), smem = held + ring;
+  if (N * sizeof(T) == 16 && kOwner != kWarpRow && stages < 1)
+    return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not with make_layout's sizes
+  const int rc =
+      smem == 0 ? MUON_POLAR_OK : allow_smem<norm_backward_kernel<T, N, kE, kOwner, kScaleColumns>>(kRingMost);
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(norm_backward_kernel<T, N, kOwner, kScaleColumns>,
-                dim3(static_cast<unsigned>(b.plan.blocks * l.cluster)), l.threads, smem, l.cluster, true, stream, b,
-                stages);
+  return launch(norm_backward_kernel<T, N, kE, kOwner, kScaleColumns>,
+                dim3(static_cast<unsigned>(b.plan.blocks * l.cluster)), l.threads, smem, l.cluster, true, stream,
+                b, stages);
 }
 
 template <typename T, int N, bool kScaleColumns>
 int backward_rows(const Backward& b, const Layout& l, void* stream) {
-  if (l.owner == kWarpRow) return launch_backward<T, N, kWarpRow, kScaleColumns>(b, l, stream);
-  if (l.owner == kBlockRow) return launch_backward<T, N, kBlockRow, kScaleColumns>(b, l, stream);
-  return launch_backward<T, N, kClusterRow, kScaleColumns>(b, l, stream);
+  if (l.owner == kWarpRow) return launch_backward<T, N, 8, kWarpRow, kScaleColumns>(b, l, stream);
+  if constexpr (N * sizeof(T) == 16) {
+    if (l.owner == kClusterRow) return launch_backward<T, N, 16, kClusterRow, kScaleColumns>(b, l, stream);
+    if (l.columns == 16) return launch_backward<T, N, 16, kBlockRow, kScaleColumns>(b, l, stream);
+  } else {
+    if (l.owner == kClusterRow) return launch_backward<T, N, 8, kClusterRow, kScaleColumns>(b, l, stream);
+  }
+  return launch_backward<T, N, 8, kBlockRow, kScaleColumns>(b, l, stream);
 }
 
 template <typename T, int N>
@@ -1143,8 +1237,16 @@ size_t muon_train_residual_norm_workspace_bytes(const muon_train_norm_args* args
   int64_t target = 0;
   if (check(args) != MUON_POLAR_OK || args->rows == 0) return 0;
   const muon_train_norm_args a = normalised(*args);
-  if (target_workers(make_layout(a, nullptr), &target) != MUON_POLAR_OK) return 0;
-  return make_plan(a, target).bytes;
+  // over what the layout may be, which also depends on the gradients' alignment
+  size_t bytes = 0;
+  for (int aligned = 0; aligned < 2; ++aligned) {
+    muon_train_norm_grads g = {};
+    if (!aligned) g.grad_residual = reinterpret_cast<void*>(2);
+    if (target_workers(make_layout(a, &g), &target) != MUON_POLAR_OK) return 0;
+    const size_t b = make_plan(a, target).bytes;
+    if (b > bytes) bytes = b;
+  }
+  return bytes;
 }
 
 int muon_train_residual_norm_backward_sm100(const muon_train_norm_args* args,
