@@ -42,39 +42,49 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// A lane has kPer neighbouring experts of a token, lane * kPer the first, so
-// that the lowest lane holds the lowest index.  They are loaded in runs of up
-// to 16 bytes where rows keep that alignment (whole), else one by one.
+// A lane has up to kPer neighbouring experts of a token, e0 the first, and a
+// higher lane higher ones, so that the lowest lane holds the lowest index.
+// With groups, each group has lanes of its own.
+struct Lanes {
+  int e0, count;
+  __device__ Lanes(int experts, int groups, int lanes_a_group, int per) {
+    const int lane = threadIdx.x & 31, group = lane / lanes_a_group, size = experts / groups;
+    const int inside = (lane % lanes_a_group) * per;
+    e0 = group * size + inside;
+    count = group < groups ? max(0, min(per, size - inside)) : 0;
+  }
+};
+
+// A lane's logits.  They are loaded in runs of up to 16 bytes where rows and
+// groups keep that alignment (whole), else one by one.
 template <typename T, int kPer>
 struct Row {
   static constexpr int kRun = kPer * static_cast<int>(sizeof(T)) > 16 ? 16 / static_cast<int>(sizeof(T)) : kPer;
   float v[kPer];
-  __device__ __forceinline__ void load(const T* l, int experts, bool whole) {
-    const int e0 = (threadIdx.x & 31) * kPer;
+  __device__ __forceinline__ void load(const T* l, const Lanes& at, bool whole) {
 #pragma unroll
     for (int i = 0; i < kPer; i += kRun) {
-      if (whole && e0 + i < experts) {
+      if (whole && i < at.count) {
         if constexpr (kRun * sizeof(T) >= 4) {
           float part[kRun];
-          Elements<T, kRun>::unpack(Elements<T, kRun>::load(l + e0 + i), part);
+          Elements<T, kRun>::unpack(Elements<T, kRun>::load(l + at.e0 + i), part);
 #pragma unroll
           for (int j = 0; j < kRun; ++j) v[i + j] = part[j];
           continue;
         }
       }
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) v[i + j] = e0 + i + j < experts ? to_float(l[e0 + i + j]) : -INFINITY;
+      for (int j = 0; j < kRun; ++j) v[i + j] = i + j < at.count ? to_float(l[at.e0 + i + j]) : -INFINITY;
     }
   }
 };
 
 // Scores of a lane's experts (0 beyond the last).
 template <int kPer>
-__device__ __forceinline__ void scores(const float (&l)[kPer], int experts, int score, float (&s)[kPer]) {
-  const int e0 = (threadIdx.x & 31) * kPer;
+__device__ __forceinline__ void scores(const float (&l)[kPer], const Lanes& at, int score, float (&s)[kPer]) {
   if (score != kSoftmax) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s[i] = e0 + i < experts ? sigmoid(l[i]) : 0.f;
+    for (int i = 0; i < kPer; ++i) s[i] = i < at.count ? sigmoid(l[i]) : 0.f;
     return;
   }
   float m = -INFINITY;
@@ -85,7 +95,7 @@ __device__ __forceinline__ void scores(const float (&l)[kPer], int experts, int 
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     // a row of -inf has no scores; a NaN stays one
-    s[i] = e0 + i >= experts || (m == -INFINITY && l[i] == l[i]) ? 0.f : expf(__fsub_rn(l[i], m));
+    s[i] = i >= at.count || (m == -INFINITY && l[i] == l[i]) ? 0.f : expf(__fsub_rn(l[i], m));
     sum += s[i];
   }
   const float total = static_cast<float>(warp_sum64(sum));
@@ -97,10 +107,11 @@ __device__ __forceinline__ void scores(const float (&l)[kPer], int experts, int 
 struct Plan {
   bool whole;         // runs of a row can be loaded at once
   bool by_logit;      // the logits are the keys
-  int lanes_a_group;  // a power of two, when no lane has experts of two groups; else 0
+  bool ranked;        // each group has lanes of its own; else groups go through shared memory
+  int lanes_a_group;  // a power of two; 32 for one group, and when not ranked
 };
 
-// The two largest of (first, second, key).
+// The two largest of (first, second, key), a number.
 __device__ __forceinline__ void best_two(float key, float& first, float& second) {
   second = fmaxf(second, fminf(first, key));
   first = fmaxf(first, key);
@@ -115,36 +126,36 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
     route_kernel(const __grid_constant__ muon_train_route_args a, Plan plan) {
   extern __shared__ float smem[];
   const int experts = static_cast<int>(a.experts);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * kPer;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Lanes at(experts, plan.ranked ? a.groups : 1, plan.lanes_a_group, kPer);
   uint32_t* histogram = reinterpret_cast<uint32_t*>(smem);  // of the block's tokens
-  float* row = smem + experts + warp * (plan.lanes_a_group > 0 ? 1 : 2) * experts;
-  float* row_keys = row + experts;  // without lanes_a_group
+  float* row = smem + experts + warp * (plan.ranked ? 1 : 2) * experts;
+  float* row_keys = row + experts;  // when not ranked
   for (int e = threadIdx.x; e < experts; e += kThreads) histogram[e] = 0;
   __syncthreads();
   float bias[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) bias[i] = a.bias != nullptr && e0 + i < experts ? a.bias[e0 + i] : 0.f;
+  for (int i = 0; i < kPer; ++i) bias[i] = a.bias != nullptr && i < at.count ? a.bias[at.e0 + i] : 0.f;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
   int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   Row<T, kPer> l;
-  if (token < a.tokens) l.load(static_cast<const T*>(a.logits) + token * a.ld, experts, plan.whole);
+  if (token < a.tokens) l.load(static_cast<const T*>(a.logits) + token * a.ld, at, plan.whole);
   for (; token < a.tokens; token += step) {
     float s[kPer], key[kPer];
-    scores(l.v, experts, a.score, s);
+    scores(l.v, at, a.score, s);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const float k = plan.by_logit ? l.v[i] : a.bias != nullptr ? __fadd_rn(s[i], bias[i]) : s[i];
-      key[i] = e0 + i < experts ? number(k) : taken();
-      if (e0 + i < experts) row[e0 + i] = s[i];
+      key[i] = i < at.count ? number(k) : taken();
+      if (i < at.count) row[at.e0 + i] = s[i];
     }
     if (token + step < a.tokens)
-      l.load(static_cast<const T*>(a.logits) + (token + step) * a.ld, experts, plan.whole);
+      l.load(static_cast<const T*>(a.logits) + (token + step) * a.ld, at, plan.whole);
     if (a.groups > 1) {
-      const int size = experts / a.groups;
-      if (plan.lanes_a_group > 0) {
+      if (plan.ranked) {
         float first = -INFINITY, second = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) best_two(key[i], first, second);
+        for (int i = 0; i < kPer; ++i) best_two(i < at.count ? key[i] : -INFINITY, first, second);
         for (int o = 1; o < plan.lanes_a_group; o <<= 1) {
           const float f = __shfl_xor_sync(kFullMask, first, o), g = __shfl_xor_sync(kFullMask, second, o);
           second = fmaxf(fminf(first, f), fmaxf(second, g));
@@ -162,9 +173,10 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
           for (int i = 0; i < kPer; ++i) key[i] = taken();
         }
       } else {
+        const int size = experts / a.groups;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          if (e0 + i < experts) row_keys[e0 + i] = key[i];
+          if (i < at.count) row_keys[at.e0 + i] = key[i];
         __syncwarp();
         // each lane ranks its groups g = lane, + 32, ..
         float mine[MUON_TRAIN_MAX_EXPERTS / 32];
@@ -196,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          if (e0 + i < experts && row_keys[(e0 + i) / size] == 0.f) key[i] = taken();
+          if (i < at.count && row_keys[(at.e0 + i) / size] == 0.f) key[i] = taken();
       }
     }
     // the k best: the lanes' best keys, the lowest lane of equal ones, and in
@@ -212,17 +224,17 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
       const int who = __ffs(__ballot_sync(kFullMask, best == top)) - 1;
       int e = 0;
       if (lane == who) {
-        int at = 0;
+        int which = 0;
 #pragma unroll
         for (int i = kPer - 1; i >= 0; --i)
-          if (key[i] == top) at = i;
+          if (key[i] == top) which = i;
         best = taken();
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          if (i == at) key[i] = taken();
+          if (i == which) key[i] = taken();
           best = fmaxf(best, key[i]);
         }
-        e = e0 + at;
+        e = at.e0 + which;
       }
       e = __shfl_sync(kFullMask, e, who);
       if (lane == (j & 31)) {
@@ -273,9 +285,10 @@ __global__ void __launch_bounds__(kThreads)
     route_backward_kernel(const __grid_constant__ muon_train_route_args a, Plan plan,
                           const float* __restrict__ grad_weights, T* __restrict__ grad) {
   extern __shared__ float smem[];
-  using Lanes = Row<T, kPer>;
+  using Logits = Row<T, kPer>;
   const int experts = static_cast<int>(a.experts);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * kPer;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Lanes at(experts, 1, 32, kPer);
   float* row = smem + warp * experts;  // kWholeRow: the gradients of the scores
   for (int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp; token < a.tokens;
        token += static_cast<int64_t>(gridDim.x) * kWarps) {
@@ -298,29 +311,29 @@ __global__ void __launch_bounds__(kThreads)
     }
     const auto store_row = [&](const float(&v)[kPer]) {
 #pragma unroll
-      for (int i = 0; i < kPer; i += Lanes::kRun) {
-        if (plan.whole && e0 + i < experts) {
-          if constexpr (Lanes::kRun * sizeof(T) >= 4) {
-            float part[Lanes::kRun];
+      for (int i = 0; i < kPer; i += Logits::kRun) {
+        if (plan.whole && i < at.count) {
+          if constexpr (Logits::kRun * sizeof(T) >= 4) {
+            float part[Logits::kRun];
 #pragma unroll
-            for (int j = 0; j < Lanes::kRun; ++j) part[j] = v[i + j];
-            Elements<T, Lanes::kRun>::store(out + e0 + i, Elements<T, Lanes::kRun>::pack(part));
+            for (int j = 0; j < Logits::kRun; ++j) part[j] = v[i + j];
+            Elements<T, Logits::kRun>::store(out + at.e0 + i, Elements<T, Logits::kRun>::pack(part));
             continue;
           }
         }
 #pragma unroll
-        for (int j = 0; j < Lanes::kRun; ++j)
-          if (e0 + i + j < experts) out[e0 + i + j] = from_float<T>(v[i + j]);
+        for (int j = 0; j < Logits::kRun; ++j)
+          if (i + j < at.count) out[at.e0 + i + j] = from_float<T>(v[i + j]);
       }
     };
     if constexpr (kWholeRow) {
-      Lanes lanes;
-      lanes.load(l, experts, plan.whole);
+      Logits logits;
+      logits.load(l, at, plan.whole);
       float s[kPer];
-      scores(lanes.v, experts, a.score, s);
+      scores(logits.v, at, a.score, s);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (e0 + i < experts) row[e0 + i] = 0.f;
+        if (i < at.count) row[at.e0 + i] = 0.f;
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
@@ -329,7 +342,7 @@ __global__ void __launch_bounds__(kThreads)
       float d[kPer], dot = 0.f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        d[i] = e0 + i < experts ? row[e0 + i] : 0.f;
+        d[i] = i < at.count ? row[at.e0 + i] : 0.f;
         dot = fmaf(d[i], s[i], dot);
       }
       dot = warp_sum(dot);
@@ -409,22 +422,33 @@ int grid_for(int64_t tokens, unsigned* grid) {
 // kernel's leave.
 constexpr size_t kMostSmem = (1 + kWarps * 2) * MUON_TRAIN_MAX_EXPERTS * sizeof(float);
 
-template <typename T, int kPer>
-Plan make_plan(const muon_train_route_args& a, int64_t ld, const void* other) {
-  constexpr int kRun = Row<T, kPer>::kRun;
-  Plan p{};
-  p.whole = a.experts % kRun == 0 && ld % kRun == 0 && aligned16(a.logits) && aligned16(other);
-  p.by_logit = a.score == kSoftmax && a.bias == nullptr && (a.groups == 1 || a.group_top == 1);
-  const int64_t size = a.experts / a.groups, lanes = size / kPer;
-  p.lanes_a_group = a.groups == 1 ? 1 : (size % kPer == 0 && (lanes & (lanes - 1)) == 0) ? static_cast<int>(lanes) : 0;
-  return p;
+// Lanes of each group: the most, a power of two, that all groups can have.
+int lanes_for(int groups) {
+  int lanes = 32;
+  while (lanes > 1 && lanes * groups > 32) lanes /= 2;
+  return lanes;
+}
+// Whether every group can have lanes of its own, up to 32 experts a lane; its
+// experts a lane are then *per, else those of one row of all experts.
+bool ranked_groups(const muon_train_route_args& a, int64_t* per) {
+  const int64_t size = a.experts / a.groups, lanes = lanes_for(a.groups);
+  *per = (size + lanes - 1) / lanes;
+  if (a.groups <= 32 && *per <= 32) return true;
+  *per = (a.experts + 31) / 32;
+  return false;
 }
 
 template <typename T, int kPer>
-int forward(const muon_train_route_args& a, void* stream) {
+int forward(const muon_train_route_args& a, bool ranked, void* stream) {
+  constexpr int kRun = Row<T, kPer>::kRun;
+  const int64_t ld = a.tokens > 1 ? a.ld : a.experts;
+  Plan plan{};
+  plan.ranked = ranked;
+  plan.lanes_a_group = ranked ? lanes_for(a.groups) : 32;
+  plan.whole = (ranked ? a.experts / a.groups : a.experts) % kRun == 0 && ld % kRun == 0 && aligned16(a.logits);
+  plan.by_logit = a.score == kSoftmax && a.bias == nullptr && (a.groups == 1 || a.group_top == 1);
+  const size_t smem = (1 + kWarps * (ranked ? 1 : 2)) * a.experts * sizeof(float);
   unsigned grid = 0;
-  const Plan plan = make_plan<T, kPer>(a, a.tokens > 1 ? a.ld : a.experts, nullptr);
-  const size_t smem = (1 + kWarps * (plan.lanes_a_group > 0 ? 1 : 2)) * a.experts * sizeof(float);
   int rc = grid_for(a.tokens, &grid);
   if (rc == MUON_POLAR_OK && smem > 48 * 1024) rc = allow_smem<route_kernel<T, kPer>>(kMostSmem);
   if (rc != MUON_POLAR_OK) return rc;
@@ -438,8 +462,11 @@ int forward(const muon_train_route_args& a, void* stream) {
 
 template <typename T, int kPer>
 int backward(const muon_train_route_args& a, const float* grad_weights, void* grad, void* stream) {
+  constexpr int kRun = Row<T, kPer>::kRun;
+  const int64_t ld = a.tokens > 1 ? a.ld : a.experts;
+  Plan plan{};
+  plan.whole = a.experts % kRun == 0 && ld % kRun == 0 && aligned16(a.logits) && aligned16(grad);
   unsigned grid = 0;
-  const Plan plan = make_plan<T, kPer>(a, a.tokens > 1 ? a.ld : a.experts, grad);
   int rc = grid_for(a.tokens, &grid);
   if (a.score == kSoftmax && !a.renormalize) {
     const size_t smem = kWarps * a.experts * sizeof(float);
@@ -453,15 +480,17 @@ int backward(const muon_train_route_args& a, const float* grad_weights, void* gr
                 grad_weights, static_cast<T*>(grad));
 }
 
-// kPer: a lane's experts, the power of two that covers them.
+// kPer: the power of two that covers a lane's experts.
 template <typename T>
 int forward(const muon_train_route_args& a, void* stream) {
-  if (a.experts <= 32) return forward<T, 1>(a, stream);
-  if (a.experts <= 64) return forward<T, 2>(a, stream);
-  if (a.experts <= 128) return forward<T, 4>(a, stream);
-  if (a.experts <= 256) return forward<T, 8>(a, stream);
-  if (a.experts <= 512) return forward<T, 16>(a, stream);
-  return forward<T, 32>(a, stream);
+  int64_t per = 0;
+  const bool ranked = ranked_groups(a, &per);
+  if (per <= 1) return forward<T, 1>(a, ranked, stream);
+  if (per <= 2) return forward<T, 2>(a, ranked, stream);
+  if (per <= 4) return forward<T, 4>(a, ranked, stream);
+  if (per <= 8) return forward<T, 8>(a, ranked, stream);
+  if (per <= 16) return forward<T, 16>(a, ranked, stream);
+  return forward<T, 32>(a, ranked, stream);
 }
 template <typename T>
 int backward(const muon_train_route_args& a, const float* grad_weights, void* grad, void* stream) {
