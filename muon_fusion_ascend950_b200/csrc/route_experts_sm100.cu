@@ -355,18 +355,22 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int i = 0; i < kPer; ++i) zero[i] = 0.f;
       store_row(zero);
+      const int slots = (a.k + 31) / 32;  // of chosen experts that a lane has
       float x[kSlots], value[kSlots];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) x[i] = chosen[i] >= 0 ? to_float(l[chosen[i]]) : -INFINITY;
+      for (int i = 0; i < kSlots; ++i)
+        if (i < slots) x[i] = chosen[i] >= 0 ? to_float(l[chosen[i]]) : -INFINITY;
       float s[kSlots], total = 0.f;  // the scores, the softmax's to a factor
       float m = -INFINITY;
       if (a.score == kSoftmax) {
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) m = fmaxf(m, x[i]);
+        for (int i = 0; i < kSlots; ++i)
+          if (i < slots) m = fmaxf(m, x[i]);
         m = warp_max(m);
       }
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
+        if (i >= slots) break;
         if (a.score != kSoftmax)
           s[i] = chosen[i] >= 0 ? sigmoid(x[i]) : 0.f;
         else
@@ -378,20 +382,22 @@ __global__ void __launch_bounds__(kThreads)
         total = warp_sum(total);
         total = a.score == kSoftmax ? (total == 0.f ? 1.f : total) : total + kTiny;
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) dot = fmaf(g[i], __fdiv_rn(s[i], total), dot);
+        for (int i = 0; i < kSlots; ++i)
+          if (i < slots) dot = fmaf(g[i], __fdiv_rn(s[i], total), dot);
         dot = warp_sum(dot);
       } else {
         total = 1.f;
       }
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
+        if (i >= slots) break;
         value[i] = a.scale * __fdiv_rn(s[i], total) * (g[i] - dot);
         if (a.score != kSoftmax) value[i] *= 1.0f - s[i];
       }
       __syncwarp();  // the zeros are written
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
-        if (chosen[i] >= 0) out[chosen[i]] = from_float<T>(value[i]);
+        if (i < slots && chosen[i] >= 0) out[chosen[i]] = from_float<T>(value[i]);
     }
   }
 }
