@@ -309,9 +309,13 @@ constexpr int kStageGranules = kPerStage * kConsumers;
 constexpr int kStageBytes = kStageGranules * 16;
 constexpr int kMaxStages = 6;
 constexpr size_t kRingBytes = 111 * 1024;  // of dynamic shared memory
-// What a row costs a block besides its bytes, and more in a cluster; the bytes
-// of rows in flight that L2 holds until their second reading.
-constexpr double kRowNs = 700.0, kClusterNs = 500.0, kHeldBytes = 60e6;
+// Measured: bytes/ns of an SM at the copy rate; what a row costs a block besides
+// its bytes, and more with every doubling of a cluster; the bytes of rows in
+// flight that L2 holds until their second reading; and what rows in registers
+// reach (600 x 65536 bf16 loss with gradient: 51 us, ring 44; 150 rows: 14 and
+// 26; 600 x 131072: 94, and 145 with a cluster of 4, 83 of 2).
+constexpr double kSmBytesPerNs = 43.0, kRowNs = 1500.0, kClusterNs = 3000.0, kHeldBytes = 60e6;
+constexpr double kRegisterBytesPerNs = 3200.0;
 
 struct Ring {
   Cut cut;
@@ -657,10 +661,33 @@ int run(const muon_train_distill_args& a, Mode mode, void* stream) {
   const bool aligned = aligned16(a.logits) && (a.rows == 1 || a.ld % kVec<T> == 0);
   const int64_t granules = (a.vocab + kVec<T> - 1) / kVec<T> + (aligned ? 0 : 1);
   const int64_t register_row = static_cast<int64_t>(kBlockThreads) * 8;  // of one block
-  if (granules <= register_row || (granules <= kMaxCluster * register_row && a.rows * 2 <= sms)) {
+
+  // The ring's parts of a row by the smallest estimate: rounds of rows, each
+  // of a slice at a block's share of the measured copy rate and what a row
+  // costs besides.
+  const int64_t blocks = static_cast<int64_t>(sms) * kBlocksPerSm;
+  const double row_bytes = static_cast<double>(granules) * 16.0, passes = mode == kLoss ? 1.0 : 2.0;
+  int parts = 1;
+  double ring_ns = 0.0;
+  for (int p = 1, steps = 0; p <= kMaxCluster && p <= blocks; p *= 2, ++steps) {
+    const int64_t workers = std::min<int64_t>(a.rows, blocks / p);
+    const double rounds = static_cast<double>((a.rows + workers - 1) / workers);
+    const bool again = mode == kLossGrad && static_cast<double>(workers) * row_bytes > kHeldBytes;
+    const double slice_ns = row_bytes / p * kBlocksPerSm / kSmBytesPerNs * (again ? 2.7 : passes);
+    const double cluster_ns = mode == kGradFromStats ? 0.0 : mode == kLoss ? kClusterNs / 2 : kClusterNs;
+    const double estimate = rounds * (slice_ns + kRowNs + steps * cluster_ns);
+    if (p == 1 || estimate < ring_ns) {
+      parts = p;
+      ring_ns = estimate;
+    }
+  }
+  // Rows of one block's registers never pay for a ring; longer ones do where
+  // there are rows enough.
+  const double register_ns = row_bytes * static_cast<double>(a.rows) * passes / kRegisterBytesPerNs;
+  if (granules <= register_row || (granules <= kMaxCluster * register_row && register_ns <= ring_ns)) {
     // Parts of a row: as many as keep a thread at 8 vectors; more, down to one
     // vector a thread, while the device is not full.
-    int parts = 1;
+    parts = 1;
     while (parts < kMaxCluster &&
            (granules > parts * register_row || (a.rows * parts < 2 * sms && granules > parts * kBlockThreads)))
       parts *= 2;
@@ -676,25 +703,6 @@ int run(const muon_train_distill_args& a, Mode mode, void* stream) {
   }
   const int stages = static_cast<int>(
       std::min<size_t>(kMaxStages, (kRingBytes - 2 * List::bytes(a.top)) / kStageBytes));
-  // Parts of a row by the smallest estimate: rounds of rows, each of a slice
-  // at a block's share of the measured copy rate (43 bytes/ns an SM) and what
-  // a row costs besides.
-  const int64_t blocks = static_cast<int64_t>(sms) * kBlocksPerSm;
-  const double passes = mode == kLoss ? 1.0 : 2.0;
-  int parts = 1;
-  double least = 0.0;
-  for (int p = 1; p <= kMaxCluster && p <= blocks; p *= 2) {
-    const int64_t workers = std::min<int64_t>(a.rows, blocks / p);
-    const double rounds = static_cast<double>((a.rows + workers - 1) / workers);
-    const double row_bytes = static_cast<double>(granules) * 16.0;
-    const bool again = mode == kLossGrad && static_cast<double>(workers) * row_bytes > kHeldBytes;
-    const double slice_ns = row_bytes / p * kBlocksPerSm / 43.0 * (again ? 2.3 : passes);
-    const double estimate = rounds * (slice_ns + kRowNs + (p > 1 && mode != kGradFromStats ? kClusterNs : 0.0));
-    if (p == 1 || estimate < least) {
-      parts = p;
-      least = estimate;
-    }
-  }
   const int64_t workers = std::min<int64_t>(a.rows, blocks / parts);
   if (mode == kLossGrad) return run_ring<T, kLossGrad>(a, parts, stages, workers, stream);
   if (mode == kLoss) return run_ring<T, kLoss>(a, parts, stages, workers, stream);
