@@ -67,14 +67,23 @@ def load_library() -> None:
         return (student.new_empty(lead, dtype=torch.float32),
                 student.new_empty((lead.numel(), 2), dtype=torch.float32))
 
+    def grad_like(student):
+        """The gradient has the logits' layout where their rows are padded by
+        no more than a row's length, else it is contiguous."""
+        vocab = student.shape[-1]
+        rows = student.reshape(-1, vocab)
+        if rows.shape[0] > 1 and rows.stride(1) == 1 and vocab < rows.stride(0) <= 2 * vocab:
+            return student.new_empty_strided(rows.shape, rows.stride()).view(student.shape)
+        return student.new_empty(student.shape)
+
     def fake_distill_topk_backward(grad_loss, student, values, indices, lse, stats, temperature):
-        return torch.empty_like(student)
+        return grad_like(student)
 
     def fake_distill_topk_grad(student, values, indices, row_scale, lse, temperature):
         from .training import check_distill
 
         check_distill(student, values, indices, temperature, row_scale=row_scale, teacher_lse=lse)
-        return student.new_empty(student.shape[:-1], dtype=torch.float32), torch.empty_like(student)
+        return student.new_empty(student.shape[:-1], dtype=torch.float32), grad_like(student)
 
     def fake_residual_norm(block_out, residual, post, pre, gate, scale, eps):
         from .training import check_norm

@@ -37,30 +37,70 @@ struct List {
 template <typename T>
 __device__ __forceinline__ float logit(const T* row, int64_t i) { return to_float(row[i]); }
 
-// Fills the list and returns Q; one whole warp, each
-// lane its own entries.  The differences to the largest entry are taken
-// before the division by tau, so that entries of the type's lowest value stay
-// finite.
+// An index of 4 or 8 bytes and a value of 2 or 4, without branches on the
+// type: several entries' loads can then be on their way together.
+__device__ __forceinline__ int64_t load_index(const uint8_t* p, int bytes) {
+  const int32_t low = *reinterpret_cast<const int32_t*>(p);
+  const int32_t high = *reinterpret_cast<const int32_t*>(p + (bytes - 4));
+  return bytes == 8 ? static_cast<int64_t>(high) << 32 | static_cast<uint32_t>(low) : static_cast<int64_t>(low);
+}
+__device__ __forceinline__ float load_value(const uint8_t* p, int dtype) {
+  const uint32_t low = *reinterpret_cast<const uint16_t*>(p);
+  const uint32_t high = *reinterpret_cast<const uint16_t*>(p + (dtype == MUON_TRAIN_F32 ? 2 : 0));
+  const float half = __half2float(__ushort_as_half(static_cast<unsigned short>(low)));
+  const float other = __uint_as_float(high << 16 | (dtype == MUON_TRAIN_F32 ? low : 0u));
+  return dtype == MUON_TRAIN_F16 ? half : other;
+}
+
+// A row's list from memory, four entries a lane at a time: the indices and
+// teacher logits first, then the student's logits at the indices, so that four
+// entries wait for memory twice, and not each of them.  Returns the largest
+// counted teacher logit of the lane's.
+template <typename T>
+__device__ __forceinline__ float load_entries(const muon_train_distill_args& a, int64_t row, const T* z,
+                                              const List& list) {
+  constexpr int kBatch = 4;
+  const int lane = threadIdx.x & 31, top = static_cast<int>(a.top), value_bytes = a.teacher_dtype == MUON_TRAIN_F32 ? 4 : 2;
+  const uint8_t* indices = static_cast<const uint8_t*>(a.teacher_indices) + row * a.top * a.index_bytes;
+  const uint8_t* values = static_cast<const uint8_t*>(a.teacher_logits) + row * a.top * value_bytes;
+  float best = -INFINITY;
+  for (int base = lane; base < top; base += 32 * kBatch) {
+    int64_t index[kBatch];
+    float t[kBatch], zi[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int j = min(base + b * 32, top - 1);  // the last entry again, past the end
+      index[b] = load_index(indices + static_cast<int64_t>(j) * a.index_bytes, a.index_bytes);
+      t[b] = load_value(values + static_cast<int64_t>(j) * value_bytes, a.teacher_dtype);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const bool counted = index[b] >= 0 && index[b] < a.vocab && t[b] > -INFINITY;
+      index[b] = counted ? index[b] : -1;
+      zi[b] = logit(z, counted ? index[b] : 0);
+      best = counted ? fmaxf(best, t[b]) : best;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int j = base + b * 32;
+      if (j >= top) break;
+      list.index[j] = static_cast<int>(index[b]);
+      list.log_q[j] = t[b];
+      list.z[j] = zi[b];
+    }
+  }
+  return best;
+}
+
+// Fills the list and returns Q; one whole warp, each lane its own entries.
+// The differences to the largest entry are taken before the division by tau,
+// so that entries of the type's lowest value stay finite.
 template <typename T>
 __device__ float load_list(const muon_train_distill_args& a, int64_t row, const T* z, const List& list) {
   const int lane = threadIdx.x & 31;
   const int top = static_cast<int>(a.top);
   const float inv_tau = 1.0f / a.temperature;
-  const int64_t base = row * a.top;
-  float best = -INFINITY;
-  for (int j = lane; j < top; j += 32) {
-    const int64_t i = a.index_bytes == 8
-                          ? static_cast<const int64_t*>(a.teacher_indices)[base + j]
-                          : static_cast<const int32_t*>(a.teacher_indices)[base + j];
-    const float t = load_any(a.teacher_logits, a.teacher_dtype, base + j);
-    const bool counted = i >= 0 && i < a.vocab && t > -INFINITY;
-    list.index[j] = counted ? static_cast<int>(i) : -1;
-    list.log_q[j] = t;
-    if (counted) {
-      best = fmaxf(best, t);
-      list.z[j] = logit(z, i);
-    }
-  }
+  float best = load_entries(a, row, z, list);
   best = warp_max(best);
   // log q = (t - shift) / tau - log_norm
   float shift = 0.f, log_norm = 0.f;

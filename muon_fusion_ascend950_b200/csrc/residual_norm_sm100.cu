@@ -1236,7 +1236,8 @@ size_t muon_train_residual_norm_workspace_bytes(const muon_train_norm_args* args
   using namespace muon_train;
   int64_t target = 0;
   if (check(args) != MUON_POLAR_OK || args->rows == 0) return 0;
-  const muon_train_norm_args a = normalised(*args);
+  muon_train_norm_args a = normalised(*args);
+  a.hidden = a.normed = nullptr;  // as in the backward call
   // over what the layout may be, which also depends on the gradients' alignment
   size_t bytes = 0;
   for (int aligned = 0; aligned < 2; ++aligned) {

@@ -144,6 +144,16 @@ def test_distill_largest_vocabularies(pkg, rows, vocab, dtype):
     check_distill(pkg, *distill_inputs(rows, vocab, 50, dtype, seed=3))
 
 
+@pytest.mark.parametrize("rows, vocab, dtype, top", [
+    (700, 24000, torch.bfloat16, 33), (300, 60001, torch.float16, 129), (900, 50001, torch.bfloat16, 7),
+    (620, 131072, torch.bfloat16, 20), (89, 111553, torch.float32, 18), (310, 32771, torch.float32, 300),
+    (75, 150001, torch.float32, 1024), (38, 260003, torch.bfloat16, 5)])
+def test_distill_many_long_rows(pkg, rows, vocab, dtype, top):
+    """Several rows for each block and cluster, so that stages, lists and slots
+    come round again, at every alignment of the rows."""
+    check_distill(pkg, *distill_inputs(rows, vocab, top, dtype, torch.int32, seed=rows))
+
+
 @pytest.mark.parametrize("rows", [1, 16, 147, 148, 149, 300, 1200])
 @pytest.mark.parametrize("vocab", [264, 8192, 33000])
 def test_distill_row_counts(pkg, rows, vocab):
@@ -442,6 +452,15 @@ def test_norm_sizes(pkg, rows, width, dtype):
     check_norm(pkg, *norm_inputs((rows, width), dtype, torch.float32, (), width, seed=width))
 
 
+@pytest.mark.parametrize("rows, width, dtype, scale", [
+    (700, 4104, torch.bfloat16, 1), (700, 8192, torch.float16, -1), (320, 12000, torch.bfloat16, -1),
+    (500, 4100, torch.float32, -1), (320, 7684, torch.float32, 1), (320, 15360, torch.float32, -1),
+    (500, 4098, torch.bfloat16, -1), (320, 9001, torch.float16, 1), (320, 15365, torch.float32, 1)])
+def test_norm_many_wide_rows(pkg, rows, width, dtype, scale):
+    """Several rows for each block and cluster of every wide layout."""
+    check_norm(pkg, *norm_inputs((rows, width), dtype, torch.float32, (), width if scale < 0 else scale, seed=rows))
+
+
 @pytest.mark.parametrize("width", [96, 130, 512, 4096])
 @pytest.mark.parametrize("rows", [1, 2, 147, 148, 149, 295, 296, 297, 1000, 3001])
 def test_norm_row_counts(pkg, rows, width):
@@ -552,6 +571,30 @@ def test_norm_gradient_against_differences(pkg):
         size = sum((a.double() * d[n]).abs().sum() for n, a in zip(leaves, grads))
         h = 1e-4
         near(along, (total(h, d) - total(-h, d)) / (2 * h), size * 1e-5 + 1e-5)
+
+
+def test_norm_past_32_bit_offsets(pkg):
+    """More than 2^31 elements: the last rows, and the parameter gradients,
+    are those of a small call when all other rows are zero."""
+    rows, width = 530000, 4096
+    v, dh, dn = norm_inputs((5, width), torch.bfloat16, torch.float32, (), width, seed=39)
+
+    def grads(y, x, gh, gn):
+        y, x = y.requires_grad_(True), x.requires_grad_(True)
+        p = [v[n].detach().requires_grad_(True) for n in NAMES[2:]]
+        ends = pkg.residual_norm(y, x, p[0], p[1], gate=p[2], residual_scale=p[3])
+        return [e.detach()[-5:] for e in ends] + [
+            g[-5:] if g.ndim == 2 else g for g in torch.autograd.grad(ends, [y, x, *p], [gh, gn])]
+
+    def last(t):
+        return torch.cat([torch.zeros(rows - 5, width, dtype=t.dtype, device="cuda"), t])
+
+    small = grads(v["block_out"].clone(), v["residual"].clone(), dh, dn)
+    large = grads(last(v["block_out"]), last(v["residual"]), last(dh), last(dn))
+    for a, b in zip(small[:4], large[:4]):
+        assert torch.equal(a, b)
+    for a, b in zip(small[4:], large[4:]):  # the same five rows, added up in another order
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
 
 
 # =========================================================== routing
@@ -699,7 +742,7 @@ def test_route_masks(pkg, experts, score):
     assert not bool((indices[3] == 3).any()) and (score == "softmax") == bool(weights[3].isnan().all())
     assert torch.equal(indices[4], torch.arange(8, device="cuda"))
     near(weights[4], torch.full((8,), 0.125 if score == "softmax" else 0.0, device="cuda"), 1e-6)
-    assert indices[5, 0] == 0 and float(weights[5, 0]) == 1.0
+    assert indices[5, 0] == 0 and float(weights[5, 0].detach()) == 1.0
     assert torch.equal(indices[6], torch.arange(8, device="cuda")) and weights[6].isnan().all()
     (grad,) = torch.autograd.grad(weights, leaf, torch.ones_like(weights))
     good = [0, 1, 2, 4, 5, 7]
@@ -721,6 +764,22 @@ def test_route_strides_and_shapes(pkg):
     one = pkg.route_experts(x[3], 5)
     assert one[0].shape == (5,) and torch.equal(one[1], base[1][3])
     check_route(pkg, x[:1].expand(30, 70), 5)
+
+
+def test_route_past_32_bit_offsets(pkg):
+    tokens = 2 ** 31 // 256 + 100
+    small = logits(60, 256, torch.bfloat16, seed=40)
+    x = torch.zeros(tokens, 256, dtype=torch.bfloat16, device="cuda")
+    x[-60:] = small
+    up = torch.randn(60, 4, generator=gen(41), device="cuda")
+    grads = []
+    for z, g in ((small.clone(), up), (x, torch.cat([torch.zeros(tokens - 60, 4, device="cuda"), up]))):
+        z.requires_grad_(True)
+        weights, indices, counts = pkg.route_experts(z, 4)
+        grads.append([weights.detach()[-60:], indices[-60:], torch.autograd.grad(weights, z, g)[0][-60:]])
+        assert int(counts.sum()) == 4 * z.shape[0]
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
 
 
 def test_route_no_tokens(pkg):
@@ -848,10 +907,40 @@ def test_compiled_training_step(pkg):
         assert torch.equal(a, b)
 
 
-def test_kernels_are_launched(pkg):
+def test_gradients_only_where_they_are_asked_for(pkg):
+    """Inputs without a gradient get none, and the others the same as ever."""
+    v, dh, dn = norm_inputs((50, 520), torch.bfloat16, torch.float32, (), 520, seed=38)
+
+    def grads(wanted):
+        leaves = {n: t.detach().requires_grad_(n in wanted) for n, t in v.items()}
+        ends = pkg.residual_norm(*(leaves[n] for n in NAMES[:4]), gate=leaves["gate"],
+                                 residual_scale=leaves["residual_scale"])
+        return torch.autograd.grad(ends, [leaves[n] for n in wanted], [dh, dn])
+
+    everything = dict(zip(NAMES, grads(NAMES)))
+    for name in NAMES:
+        assert torch.equal(grads([name])[0], everything[name])
+    # saved for one backward pass, or as many as are kept
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    loss = pkg.route_experts(x, 2)[0][:, 0].sum()
+    first = torch.autograd.grad(loss, x, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(loss, x)[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, x)
+    # a saved input that was changed since is noticed
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    y = x * 1
+    out = pkg.route_experts(y, 2)[0]
+    y.add_(1)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+
+
+def test_kernels_are_launched_and_end(pkg):
     from muon_fusion_ascend950_b200.capi import capi
 
     api = capi()
     before = api.train_launch_count()
     pkg.route_experts(logits(4, 8), 2)
-    assert api.train_launch_count() > before
+    assert api.train_launch_count() == before + 1
+    assert api.train_device_status(torch.cuda.current_device()) == 0  # no wait has run out so far

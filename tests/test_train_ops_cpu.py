@@ -231,6 +231,17 @@ def test_fake_backward_kernels():
         assert ops.route_experts_backward(weights, l, indices, 0, True, 1.0).shape == l.shape
 
 
+def test_fake_gradient_of_padded_logits_keeps_their_layout():
+    with _fake():
+        i = _cuda(2, 3, dtype=torch.int64)
+        for pad, stride in ((8, 8), (10, 10), (16, 16), (17, 8)):
+            z = _cuda(2, pad)[:, :8]
+            assert pkg.distill_topk_grad(z, _cuda(2, 3), i)[1].stride() == (stride, 1)
+        z = _cuda(2, 1, 10)[..., :8]
+        grad = pkg.distill_topk_grad(z, _cuda(2, 1, 3), i.view(2, 1, 3))[1]
+        assert grad.shape == z.shape and grad.stride(0) == 10
+
+
 def test_measured_cases_stay_in_their_ranges():
     spec = importlib.util.spec_from_file_location("perf_operators", REPO / "perf" / "operators.py")
     cases = importlib.util.module_from_spec(spec)
