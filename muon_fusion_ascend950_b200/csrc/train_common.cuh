@@ -295,11 +295,18 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool valid_dtype(int d) { return d >= MUON_TRAIN_F32 && d <= MUON_TRAIN_F16; }
 inline size_t dtype_size(int d) { return d == MUON_TRAIN_F32 ? 4 : 2; }
 
+// SMs of the current device, asked once for each.
 inline int sm_count(int* sms) {
+  static std::atomic<int> known[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  return e == cudaSuccess ? MUON_POLAR_OK : static_cast<int>(e);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const bool kept = dev >= 0 && dev < 64;
+  *sms = kept ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (*sms > 0) return MUON_POLAR_OK;
+  e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && kept) known[dev].store(*sms, std::memory_order_relaxed);
+  return static_cast<int>(e);
 }
 
 // Lets a kernel have up to `bytes` of dynamic shared memory, once for each

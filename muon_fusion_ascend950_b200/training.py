@@ -10,8 +10,8 @@ step beside them that are bound by memory, each with its gradient:
 * ``route_experts`` -- the routing of tokens to the experts whose batched
   matrices ``Muon`` updates.
 
-They are the operators ``torch.ops.muon_ascend950.*`` of the same names with
-the arguments' shapes and types checked here, run on the current stream, and
+They are the operators ``torch.ops.muon_ascend950.*`` of the same names, which
+check their arguments (ValueError, TypeError), run on the current stream and
 take part in autograd (gradients of gradients are refused).
 """
 from __future__ import annotations
@@ -24,7 +24,10 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _OPTIONAL = frozenset(("teacher_lse", "row_scale", "post_weight", "pre_weight", "gate", "residual_scale",
                        "bias"))
-_ops = torch.ops.muon_ascend950
+_distill_topk = torch.ops.muon_ascend950.distill_topk.default
+_distill_topk_grad = torch.ops.muon_ascend950.distill_topk_grad.default
+_residual_norm = torch.ops.muon_ascend950.residual_norm.default
+_route_experts = torch.ops.muon_ascend950.route_experts.default
 
 
 def _check(name: str, t, floats: bool = True) -> None:
@@ -36,10 +39,11 @@ def _check(name: str, t, floats: bool = True) -> None:
         raise TypeError(f"{name} must use torch.float32, bfloat16 or float16, got {t.dtype}")
 
 
-def _tensors(**named) -> None:
-    """What must hold before the native operator can be called; it checks
-    shapes, types and devices itself (and the functions below do, where only
-    shapes are traced)."""
+# The native operators check their arguments themselves.  Only when a call has
+# failed is it looked at here, so that what the dispatcher refuses before the
+# operator sees it (no tensor, no CUDA tensor) gets the package's own error:
+# small calls are bound by the host.
+def _explain(**named) -> None:
     for name, t in named.items():
         if t is None and name in _OPTIONAL:
             continue
@@ -155,10 +159,12 @@ def distill_topk(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
     gradient 0.  Differentiable in ``student_logits``; the teacher's tensors
     are constants.
     """
-    _tensors(student_logits=student_logits, teacher_logits=teacher_logits,
-             teacher_indices=teacher_indices, teacher_lse=teacher_lse)
-    return _ops.distill_topk.default(student_logits, teacher_logits, teacher_indices, teacher_lse,
-                                     float(temperature))[0]
+    try:
+        return _distill_topk(student_logits, teacher_logits, teacher_indices, teacher_lse, temperature)[0]
+    except Exception:
+        _explain(student_logits=student_logits, teacher_logits=teacher_logits,
+                 teacher_indices=teacher_indices, teacher_lse=teacher_lse)
+        raise
 
 
 def distill_topk_grad(student_logits: torch.Tensor, teacher_logits: torch.Tensor,
@@ -173,10 +179,13 @@ def distill_topk_grad(student_logits: torch.Tensor, teacher_logits: torch.Tensor
     Returns ``(loss, grad)``, the gradient with the logits' shape and type; use
     it as ``student_logits.backward(grad)``.  Not recorded by autograd.
     """
-    _tensors(student_logits=student_logits, teacher_logits=teacher_logits,
-             teacher_indices=teacher_indices, row_scale=row_scale, teacher_lse=teacher_lse)
-    return _ops.distill_topk_grad.default(student_logits, teacher_logits, teacher_indices, row_scale,
-                                          teacher_lse, float(temperature))
+    try:
+        return _distill_topk_grad(student_logits, teacher_logits, teacher_indices, row_scale, teacher_lse,
+                                  temperature)
+    except Exception:
+        _explain(student_logits=student_logits, teacher_logits=teacher_logits,
+                 teacher_indices=teacher_indices, row_scale=row_scale, teacher_lse=teacher_lse)
+        raise
 
 
 def residual_norm(block_out: torch.Tensor, residual: torch.Tensor,
@@ -202,10 +211,13 @@ def residual_norm(block_out: torch.Tensor, residual: torch.Tensor,
     it is rounded, and each output is rounded once.  Differentiable in all
     tensor arguments; parameter gradients are summed in a fixed order.
     """
-    _tensors(block_out=block_out, residual=residual, post_weight=post_weight, pre_weight=pre_weight,
-             gate=gate, residual_scale=residual_scale)
-    hidden, normed, _ = _ops.residual_norm.default(block_out, residual, post_weight, pre_weight, gate,
-                                                   residual_scale, float(eps))
+    try:
+        hidden, normed, _ = _residual_norm(block_out, residual, post_weight, pre_weight, gate, residual_scale,
+                                           eps)
+    except Exception:
+        _explain(block_out=block_out, residual=residual, post_weight=post_weight, pre_weight=pre_weight,
+                 gate=gate, residual_scale=residual_scale)
+        raise
     return hidden, normed if pre_weight is not None else None
 
 
@@ -229,10 +241,12 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax",
     int64 ``[experts]``, how many tokens each expert got.  Differentiable in
     ``logits`` through the weights.
     """
-    _tensors(logits=logits, bias=bias)
-    if score not in _SCORES:
-        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
     if group_top is None:
-        group_top = 2 if score == "sigmoid" and 1 < groups < logits.shape[-1] else 1
-    return _ops.route_experts.default(logits, bias, int(k), _SCORES[score], int(groups), int(top_groups),
-                                      int(group_top), bool(renormalize), float(scale))
+        group_top = 2 if groups > 1 and score == "sigmoid" and groups < logits.shape[-1] else 1
+    try:
+        return _route_experts(logits, bias, k, _SCORES[score], groups, top_groups, group_top, renormalize, scale)
+    except Exception:
+        if score not in _SCORES:
+            raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}") from None
+        _explain(logits=logits, bias=bias)
+        raise
