@@ -179,21 +179,73 @@ struct Columns {
   __device__ __forceinline__ float at(int i) const { return (i & 1) ? v[i / 2].y : v[i / 2].x; }
 };
 
-// One parameter's values in a thread's columns; `none` outside the row, and
-// everywhere when there is no such parameter.
+// One parameter's values in a thread's columns, on their way: N elements are
+// loaded as two halves of the bytes that N fp32 have; of 16-bit types the
+// first half is all of them.  No branch on the type stands between the loads,
+// so that those of several parameters wait for memory together.
+template <int N, int kE>
+struct ParamColumns {
+  using Raw = typename RawOf<2 * N>::type;
+  Raw low[kE / N], high[kE / N];
+  const void* p;
+  int dtype;
+  template <typename P>
+  __device__ __forceinline__ void load(const P& place, int width, const void* param, int type, int64_t offset) {
+    p = param;
+    dtype = type;
+    const int size = type == MUON_TRAIN_F32 ? 4 : 2;
+    const uint8_t* from = static_cast<const uint8_t*>(param) + offset * size;
+#pragma unroll
+    for (int i = 0; i < kE / N; ++i) {
+      const int c = place.column(i);
+      low[i] = high[i] = Raw();
+      if (param != nullptr && c < width) {
+        const uint8_t* at = from + static_cast<int64_t>(c) * size;
+        low[i] = *reinterpret_cast<const Raw*>(at);
+        high[i] = *reinterpret_cast<const Raw*>(at + (size - 2) * N);
+      }
+    }
+  }
+  // `none` outside the row, and everywhere when there is no such parameter
+  template <typename P>
+  __device__ __forceinline__ void values(Columns<kE>& v, const P& place, int width, float none) const {
+#pragma unroll
+    for (int i = 0; i < kE / N; ++i) {
+      const uint16_t* l = reinterpret_cast<const uint16_t*>(&low[i]);
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(&high[i]);
+      const bool there = p != nullptr && place.column(i) < width;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        // 16-bit words 2 j and 2 j + 1 of the N fp32, word j of the N others
+        const uint32_t w0 = 2 * j < N ? l[2 * j] : h[2 * j - N];
+        const uint32_t w1 = 2 * j + 1 < N ? l[2 * j + 1] : h[2 * j + 1 - N];
+        const float f32 = __uint_as_float(w1 << 16 | w0), bf16 = __uint_as_float(static_cast<uint32_t>(l[j]) << 16);
+        const float f16 = __half2float(__ushort_as_half(l[j]));
+        const float value = dtype == MUON_TRAIN_F32 ? f32 : dtype == MUON_TRAIN_BF16 ? bf16 : f16;
+        v.at(i * N + j) = there ? value : none;
+      }
+    }
+  }
+};
 template <int N, int kE, typename P>
 __device__ __forceinline__ void load_columns(Columns<kE>& v, const P& place, int width, const void* p, int dtype,
                                              int64_t offset, float none) {
+  ParamColumns<N, kE> raw;
+  raw.load(place, width, p, dtype, offset);
+  raw.values(v, place, width, none);
+}
+// A gate row times the post weight.
+template <int N, int kE, typename P>
+__device__ __forceinline__ void load_gain(Columns<kE>& v, const P& place, int width, const muon_train_norm_args& a,
+                                          int64_t gate_row) {
+  ParamColumns<N, kE> gate, post;
+  gate.load(place, width, a.gate, a.gate_dtype, gate_row * width);
+  post.load(place, width, a.post_weight, a.post_dtype, 0);
+  Columns<kE> w;
+  gate.values(v, place, width, 1.f);
+  post.values(w, place, width, 1.f);
 #pragma unroll
-  for (int i = 0; i < kE / N; ++i) {
-    float part[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) part[j] = none;
-    const int c = place.column(i);
-    if (p != nullptr && c < width) load_any<N>(p, dtype, offset + c, part);
-#pragma unroll
-    for (int j = 0; j < N; ++j) v.at(i * N + j) = part[j];
-  }
+  for (int i = 0; i < kE / 2; ++i) v.v[i] = mul2(v.v[i], w.v[i]);
 }
 
 template <typename T, int N, int kE>
@@ -332,23 +384,20 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     __syncthreads();
   }
   Columns<kE> gain, scale, pre;
-  int64_t gate_row = 0;
-  const auto load_gain = [&] {
-    Columns<kE> post;
-    load_columns<N>(gain, place, width, a.gate, a.gate_dtype, gate_row * width, 1.f);
-    load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
+  int64_t gate_row = place.worker < a.rows ? gate_row_of(a, place.worker) : 0;
+  {
+    ParamColumns<N, kE> gate_raw, post_raw, pre_raw, scale_raw;
+    gate_raw.load(place, width, a.gate, a.gate_dtype, gate_row * width);
+    post_raw.load(place, width, a.post_weight, a.post_dtype, 0);
+    pre_raw.load(place, width, a.pre_weight, a.pre_dtype, 0);
+    scale_raw.load(place, width, a.scale_count > 1 ? a.residual_scale : nullptr, a.scale_dtype, 0);
+    const float one = a.scale_count == 1 ? load_any(a.residual_scale, a.scale_dtype, 0) : 1.f;
+    gate_raw.values(gain, place, width, 1.f);
+    post_raw.values(scale, place, width, 1.f);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) gain.v[i] = mul2(gain.v[i], post.v[i]);
-  };
-  if (place.worker < a.rows) gate_row = gate_row_of(a, place.worker);
-  load_gain();
-  load_columns<N>(pre, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
-  if (a.scale_count == 1) {
-    const float one = load_any(a.residual_scale, a.scale_dtype, 0);
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) scale.v[i] = both(one);
-  } else {
-    load_columns<N>(scale, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+    for (int i = 0; i < kPairs; ++i) gain.v[i] = mul2(gain.v[i], scale.v[i]);
+    pre_raw.values(pre, place, width, 0.f);
+    scale_raw.values(scale, place, width, one);
   }
   for (int64_t first = place.worker; first < a.rows; first += kRowsAtOnce * place.workers) {
     int64_t left = (a.rows - first + place.workers - 1) / place.workers;  // rows of this worker
@@ -415,7 +464,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       if (j < rows) {
         if (const int64_t g = gate_row_of(a, row); g != gate_row) {
           gate_row = g;
-          load_gain();
+          load_gain<N>(gain, place, width, a, gate_row);
         }
       }
       float2 s = both(0.f);
@@ -686,13 +735,10 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     else
       return scale_one;
   };
-  const auto load_gain = [&](int64_t gate_row) {
-    Columns<kE> gate, post;
-    load_columns<N>(gate, place, width, a.gate, a.gate_dtype, gate_row * width, 1.f);
-    load_columns<N>(post, place, width, a.post_weight, a.post_dtype, 0, 1.f);
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) gate.v[i] = mul2(gate.v[i], post.v[i]);
-    gain.set(gate);
+  const auto hold_gain = [&](int64_t gate_row) {
+    Columns<kE> v;
+    load_gain<N>(v, place, width, a, gate_row);
+    gain.set(v);
   };
 
   Columns<kE> sum_gain, sum_pre;
@@ -715,7 +761,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   for (int64_t chunk = worker; chunk < b.plan.chunks; chunk += workers) {
     int64_t r0, r1, group;
     chunk_rows(b, chunk, &r0, &r1, &group);
-    if (a.gate != nullptr && !b.plan.gate_per_row) load_gain(group);
+    if (a.gate != nullptr && !b.plan.gate_per_row) hold_gain(group);
     if (kAhead && r0 + first < r1) load_row(r0 + first);
     // the statistics of the next row are loaded a row ahead too
     float next_r = 1.f, next_rh = 0.f;
@@ -735,7 +781,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       } else if constexpr (!kAhead) {
         load_row(row);
       }
-      if (b.plan.gate_per_row) load_gain(row);
+      if (b.plan.gate_per_row) hold_gain(row);
       const float r = next_r, rh = next_rh;
       load_rstd(row + step);
       Columns<kE> h, u;  // u: dh + rh dn pre
