@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kThreads)
 // Partial sums in the workspace, fp32:
 //   gain  [chunks][width]  C (times the gate when every row has its own)
 //   pre   [blocks][width]  dp
-//   scale [blocks][width or 1]  ds
+//   scale [blocks][width]  ds, or one fp64 of each block for one value
 struct Plan {
   int64_t groups, chunks_per_group, chunks, blocks;
   int gate_per_row;
@@ -570,9 +570,24 @@ Plan make_plan(const muon_train_norm_args& a, int64_t target) {
   p.gain_off = 0;
   p.pre_off = align(static_cast<size_t>(p.chunks * a.width) * sizeof(float));
   p.scale_off = p.pre_off + align(static_cast<size_t>(p.blocks * a.width) * sizeof(float));
-  // (with one value, one of every block of a cluster: at most kMaxCluster a worker)
-  p.bytes = p.scale_off + align(static_cast<size_t>(p.blocks * (a.width < kMaxCluster ? kMaxCluster : a.width)) * sizeof(float));
+  // (one value: an fp64 of every block of a worker's cluster)
+  const int64_t least = 2 * kMaxCluster;
+  p.bytes = p.scale_off + align(static_cast<size_t>(p.blocks * (a.width < least ? least : a.width)) * sizeof(float));
   return p;
+}
+
+// The block's sum of one value a thread, in a fixed order: of a scalar
+// parameter's gradient, which adds up every element of every row, with both
+// signs, and is held in 64 bits therefore.
+__device__ __forceinline__ void store_block_sum(double v, double* to) {
+  __shared__ double part[32];
+  v = warp_sum64(v);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  double sum = 0.0;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) sum += part[w];
+  *to = sum;
 }
 
 struct Backward {
@@ -718,7 +733,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
 
   Held<kE> gain(held, 0), pre(held, 1), sum_scale(held, 2);  // gain: gate times post weight
   Columns<kE> scale_columns{};
-  float2 scale_one = both(1.f), sum_scale_one = both(0.f);
+  float2 scale_one = both(1.f);
+  double sum_scale_one = 0.0;  // over all of a thread's elements: in 64 bits, an addition a row
   {
     Columns<kE> v;
     load_columns<N>(v, place, width, a.post_weight, a.post_dtype, 0, 1.f);
@@ -828,6 +844,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
           load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
       }
       Columns<kE> gained;
+      float2 row_scale = both(0.f);
 #pragma unroll
       for (int q = 0; q < kE / 4; ++q) {
         float2 g[2], sc[2];
@@ -842,12 +859,13 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
           if constexpr (kScaleColumns)
             sc[j] = fma2(d, x.v[i], sc[j]);
           else
-            sum_scale_one = fma2(d, x.v[i], sum_scale_one);
+            row_scale = fma2(d, x.v[i], row_scale);
           x.v[i] = mul2(d, scale_of(i));
           y.v[i] = fma2(both(-ky), y.v[i], mul2(mul2(g[j], both(r)), d));
         }
         if constexpr (kScaleColumns) sum_scale.set_pairs(q, sc);
       }
+      if constexpr (!kScaleColumns) sum_scale_one += pair_sum(row_scale);
       if (b.g.grad_residual != nullptr)
         RowVectors<T, N, kE>::store(static_cast<T*>(b.g.grad_residual) + row * width, place, width, x);
       if (b.g.grad_block_out != nullptr)
@@ -895,16 +913,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       }
       store_columns(b.scale + worker * width, v);
     } else {  // one value of each block
-      float sum = warp_sum(pair_sum(sum_scale_one));
-      const int warp = threadIdx.x >> 5;
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) slots.warp[0][0][warp] = sum;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        sum = 0.f;
-        for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) sum += slots.warp[0][0][w];
-        b.scale[blockIdx.x] = sum;
-      }
+      store_block_sum(sum_scale_one, reinterpret_cast<double*>(b.scale) + blockIdx.x);
     }
   }
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed
@@ -922,10 +931,10 @@ __global__ void __launch_bounds__(kThreads)
   const T* dn_all = static_cast<const T*>(b.g.grad_normed);
   float* pre = b.pre != nullptr ? b.pre + blockIdx.x * a.width : nullptr;
   float* scale = b.scale != nullptr
-                     ? b.scale + blockIdx.x * (a.scale_count == 1 ? 1 : a.width)
+                     ? b.scale + (a.scale_count == 1 ? 0 : blockIdx.x * a.width)
                      : nullptr;
   bool first_row = true;
-  float scale_sum = 0.f;
+  double scale_sum = 0.0;
   for (int64_t chunk = blockIdx.x; chunk < b.plan.chunks; chunk += gridDim.x) {
     int64_t r0, r1, group;
     chunk_rows(b, chunk, &r0, &r1, &group);
@@ -970,7 +979,7 @@ __global__ void __launch_bounds__(kThreads)
         if (pre != nullptr) pre[c] = (first_row ? 0.f : pre[c]) + dn * h * rh;
         if (scale != nullptr) {
           if (a.scale_count == 1)
-            scale_sum = fmaf(d, xv, scale_sum);
+            scale_sum += d * xv;
           else
             scale[c] = (first_row ? 0.f : scale[c]) + d * xv;
         }
@@ -979,10 +988,7 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   if (scale != nullptr && a.scale_count == 1) {
-    __syncthreads();
-    float sums[1] = {scale_sum};
-    block_sums(sums, red, kThreads);
-    if (threadIdx.x == 0) scale[0] = sums[0];
+    store_block_sum(scale_sum, reinterpret_cast<double*>(b.scale) + blockIdx.x);
   }
 }
 
@@ -1036,6 +1042,15 @@ __global__ void __launch_bounds__(kSumWarps * 32)
     if (writes) store_any(b.g.grad_pre_weight, a.pre_dtype, column, v);
   } else if (what == 1) {
     if (b.scale == nullptr || static_cast<int64_t>(blockIdx.x) * 32 >= a.scale_count) return;
+    if (a.scale_count == 1) {  // by the first warp
+      if (warp != 0) return;
+      const double* from = reinterpret_cast<const double*>(b.scale);
+      double sum = 0.0;
+      for (int64_t i = threadIdx.x; i < b.scale_rows; i += 32) sum += from[i];
+      sum = warp_sum64(sum);
+      if (threadIdx.x == 0) store_any(b.g.grad_residual_scale, a.scale_dtype, 0, static_cast<float>(sum));
+      return;
+    }
     const float v = warps_sum(column < a.scale_count ? rows_sum(b.scale, a.scale_count, column, warp, b.scale_rows, kSumWarps)
                                                      : 0.f, part);
     if (writes && column < a.scale_count)

@@ -36,12 +36,6 @@ __device__ __forceinline__ float lanes_max(float v) {
   return m;
 }
 
-__device__ __forceinline__ double warp_sum64(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-  return v;
-}
-
 // A lane has up to kPer neighbouring experts of a token, e0 the first, and a
 // higher lane higher ones, so that the lowest lane holds the lowest index.
 // With groups, each group has lanes of its own.
