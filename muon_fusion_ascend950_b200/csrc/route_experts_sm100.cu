@@ -18,10 +18,14 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 2;
 constexpr int kSoftmax = 0;
 constexpr float kTiny = 1e-20f;
+// few_best pays from 3 choices on (32768 x 256, one group: 1 of them 23.1 us, by
+// argmaxes 19.0; 2: 23.8 and 22.9; 8: 27 and 40; 16: 34 and 63); with more than
+// half of the lanes chosen from, the bound lets too many keys through.
+constexpr int kFewFrom = 3, kFewTo = 16;
 constexpr int kSlots = MUON_TRAIN_MAX_ROUTES / 32;  // chosen experts a lane keeps
 
 __device__ __forceinline__ float sigmoid(float x) {
-  return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x)));
+  return __frcp_rn(__fadd_rn(1.0f, expf(-x)));
 }
 
 // Keys are compared as they are, which makes -0 and +0 one key.  A NaN counts
@@ -100,6 +104,7 @@ __device__ __forceinline__ void scores(const float (&l)[kPer], const Lanes& at, 
 // How a call's rows are laid out and its groups ranked.
 struct Plan {
   bool whole;         // runs of a row can be loaded at once
+  bool few;           // the best keys may come from few_best
   bool by_logit;      // the logits are the keys
   bool ranked;        // each group has lanes of its own; else groups go through shared memory
   int lanes_a_group;  // a power of two; 32 for one group, and when not ranked
@@ -111,17 +116,70 @@ __device__ __forceinline__ void best_two(float key, float& first, float& second)
   first = fmaxf(first, key);
 }
 
-// Forward: one warp a token.  The time goes into instructions, not memory
-// (256 sigmoid scores with groups: about 600 a token against 1 KB read), so
-// keys and scores stay in registers, an argmax is one redux of the lanes'
-// best keys, and only the winning lane looks for its next one.
-template <typename T, int kPer>
+// The k best keys of a lane's and its warp's, best first, the lowest index of
+// equal ones: lane j < k receives the index of the j-th.  best is the lane's
+// largest key, none a NaN.  The k-th largest of the lanes' best keys is a bound
+// that k keys reach, so only the few keys from it on, the candidates, are put
+// side by side, a lane each, and each counts the better ones.  Returns false
+// with nothing chosen if there are not k such lanes, or too many candidates.
+template <int kPer>
+__device__ __forceinline__ bool few_best(const float (&key)[kPer], float best, const Lanes& at, int k,
+                                         float2* found, int& chosen) {
+  const int lane = threadIdx.x & 31;
+  float bound = taken();
+  for (int j = 0; j < k; ++j) {  // equal ones go at once, which lowers the bound
+    bound = lanes_max(best);
+    if (best == bound) best = taken();
+  }
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) count += key[i] >= bound;
+  int before = count;  // the candidates of this lane and lower ones, then of these alone
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(kFullMask, before, o);
+    if (lane >= o) before += other;
+  }
+  const int total = __shfl_sync(kFullMask, before, 31);
+  if (total < k || total > 32) return false;  // (no bound: no candidate)
+  before -= count;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (key[i] >= bound) found[before++] = make_float2(key[i], __int_as_float(at.e0 + i));
+  __syncwarp();
+  const float2 mine = lane < total ? found[lane] : make_float2(taken(), 0.f);
+  int better = lane < total ? 0 : 32;
+#pragma unroll 4
+  for (int j = 0; j < total; ++j) {
+    const float other = __shfl_sync(kFullMask, mine.x, j);
+    better += other > mine.x || (other == mine.x && j < lane);
+  }
+  __syncwarp();  // found is read
+  int* sorted = reinterpret_cast<int*>(found);
+  if (better < k) sorted[better] = __float_as_int(mine.y);
+  __syncwarp();
+  if (lane < k) chosen = sorted[lane];
+  return true;
+}
+
+// Forward: one warp a token.  The time goes into instructions, not memory (256
+// sigmoid scores in 8 groups: about 840 a token against 1 KB read, 71% of the
+// issue slots used), so keys and scores stay in registers, and kFull, rows of
+// exactly 32 kPer experts, leaves out every check for a lane's last one.  The
+// best keys come from few_best where the plan allows it, else one by one: an
+// argmax is one redux of the lanes' best keys, and only the winning lane looks
+// for its next one.  32768 tokens of 256 experts, 8 of 8 groups' 4 best, fp32:
+// 33 us (45 with argmaxes alone, 53 without kFull too; the bytes take 5.5).
+template <typename T, int kPer, bool kFull>
 __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
     route_kernel(const __grid_constant__ muon_train_route_args a, Plan plan) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   const int experts = static_cast<int>(a.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Lanes at(experts, plan.ranked ? a.groups : 1, plan.lanes_a_group, kPer);
+  Lanes at(experts, plan.ranked ? a.groups : 1, plan.lanes_a_group, kPer);
+  if constexpr (kFull) at.count = kPer;
+  __shared__ float2 candidates[kPer >= 2 ? kWarps : 1][32];
+  float2* found = candidates[kPer >= 2 ? warp : 0];
   uint32_t* histogram = reinterpret_cast<uint32_t*>(smem);  // of the block's tokens
   float* row = smem + experts + warp * (plan.ranked ? 1 : 2) * experts;
   float* row_keys = row + experts;  // when not ranked
@@ -141,7 +199,11 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
     for (int i = 0; i < kPer; ++i) {
       const float k = plan.by_logit ? l.v[i] : a.bias != nullptr ? __fadd_rn(s[i], bias[i]) : s[i];
       key[i] = i < at.count ? number(k) : taken();
-      if (i < at.count) row[at.e0 + i] = s[i];
+      if (kFull && kPer % 4 == 0) {
+        if (i % 4 == 3) *reinterpret_cast<float4*>(row + at.e0 + i - 3) = make_float4(s[i - 3], s[i - 2], s[i - 1], s[i]);
+      } else if (i < at.count) {
+        row[at.e0 + i] = s[i];
+      }
     }
     if (token + step < a.tokens)
       l.load(static_cast<const T*>(a.logits) + (token + step) * a.ld, at, plan.whole);
@@ -205,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
           if (i < at.count && row_keys[(at.e0 + i) / size] == 0.f) key[i] = taken();
       }
     }
-    // the k best: the lanes' best keys, the lowest lane of equal ones, and in
+    // the k best; of equal ones the lowest lane, and in
     // it the first
     float best = taken();
 #pragma unroll
@@ -213,28 +275,34 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
     int chosen[kSlots];
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) chosen[i] = 0;
-    for (int j = 0; j < a.k; ++j) {
-      const float top = lanes_max(best);
-      const int who = __ffs(__ballot_sync(kFullMask, best == top)) - 1;
-      int e = 0;
-      if (lane == who) {
-        int which = 0;
+    bool done = false;
+    if constexpr (kPer >= 2) {
+      if (plan.few) done = few_best<kPer>(key, best, at, a.k, found, chosen[0]);
+    }
+    if (!done) {
+      for (int j = 0; j < a.k; ++j) {
+        const float top = lanes_max(best);
+        const int who = __ffs(__ballot_sync(kFullMask, best == top)) - 1;
+        int e = 0;
+        if (lane == who) {
+          int which = 0;
 #pragma unroll
-        for (int i = kPer - 1; i >= 0; --i)
-          if (key[i] == top) which = i;
-        best = taken();
+          for (int i = kPer - 1; i >= 0; --i)
+            if (key[i] == top) which = i;
+          best = taken();
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (i == which) key[i] = taken();
-          best = fmaxf(best, key[i]);
+          for (int i = 0; i < kPer; ++i) {
+            if (i == which) key[i] = taken();
+            best = fmaxf(best, key[i]);
+          }
+          e = at.e0 + which;
         }
-        e = at.e0 + which;
-      }
-      e = __shfl_sync(kFullMask, e, who);
-      if (lane == (j & 31)) {
+        e = __shfl_sync(kFullMask, e, who);
+        if (lane == (j & 31)) {
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i)
-          if (i == (j >> 5)) chosen[i] = e;
+          for (int i = 0; i < kSlots; ++i)
+            if (i == (j >> 5)) chosen[i] = e;
+        }
       }
     }
     __syncwarp();  // row is written
@@ -278,7 +346,7 @@ template <typename T, int kPer, bool kWholeRow>
 __global__ void __launch_bounds__(kThreads)
     route_backward_kernel(const __grid_constant__ muon_train_route_args a, Plan plan,
                           const float* __restrict__ grad_weights, T* __restrict__ grad) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   using Logits = Row<T, kPer>;
   const int experts = static_cast<int>(a.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -438,26 +506,35 @@ bool ranked_groups(const muon_train_route_args& a, int64_t* per) {
   return false;
 }
 
-template <typename T, int kPer>
-int forward(const muon_train_route_args& a, bool ranked, void* stream) {
+template <typename T, int kPer, bool kFull>
+int forward_as(const muon_train_route_args& a, bool ranked, void* stream) {
   constexpr int kRun = Row<T, kPer>::kRun;
   const int64_t ld = a.tokens > 1 ? a.ld : a.experts;
   Plan plan{};
   plan.ranked = ranked;
   plan.lanes_a_group = ranked ? lanes_for(a.groups) : 32;
   plan.whole = (ranked ? a.experts / a.groups : a.experts) % kRun == 0 && ld % kRun == 0 && aligned16(a.logits);
+  const int64_t size = ranked ? a.experts / a.groups : a.experts;
+  // every choice needs a lane with keys
+  plan.few = a.k >= kFewFrom && a.k <= kFewTo && a.k <= (ranked ? a.top_groups : 1) * ((size + kPer - 1) / kPer);
   plan.by_logit = a.score == kSoftmax && a.bias == nullptr && (a.groups == 1 || a.group_top == 1);
   const size_t smem = (1 + kWarps * (ranked ? 1 : 2)) * a.experts * sizeof(float);
   unsigned grid = 0;
   int rc = grid_for(a.tokens, &grid);
-  if (rc == MUON_POLAR_OK && smem > 48 * 1024) rc = allow_smem<route_kernel<T, kPer>>(kMostSmem);
+  if (rc == MUON_POLAR_OK && smem > 40 * 1024) rc = allow_smem<route_kernel<T, kPer, kFull>>(kMostSmem);
   if (rc != MUON_POLAR_OK) return rc;
   if (a.counts != nullptr && grid > 1) {  // one block writes its counts, more add them up
     const cudaError_t e = cudaMemsetAsync(a.counts, 0, a.experts * sizeof(int64_t),
                                           static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  return launch(route_kernel<T, kPer>, dim3(grid), kThreads, smem, 1, false, stream, a, plan);
+  return launch(route_kernel<T, kPer, kFull>, dim3(grid), kThreads, smem, 1, false, stream, a, plan);
+}
+
+template <typename T, int kPer>
+int forward(const muon_train_route_args& a, bool ranked, void* stream) {
+  if (a.experts == 32 * kPer) return forward_as<T, kPer, true>(a, ranked, stream);
+  return forward_as<T, kPer, false>(a, ranked, stream);
 }
 
 template <typename T, int kPer>
@@ -470,7 +547,7 @@ int backward(const muon_train_route_args& a, const float* grad_weights, void* gr
   int rc = grid_for(a.tokens, &grid);
   if (a.score == kSoftmax && !a.renormalize) {
     const size_t smem = kWarps * a.experts * sizeof(float);
-    if (rc == MUON_POLAR_OK && smem > 48 * 1024) rc = allow_smem<route_backward_kernel<T, kPer, true>>(kMostSmem);
+    if (rc == MUON_POLAR_OK && smem > 40 * 1024) rc = allow_smem<route_backward_kernel<T, kPer, true>>(kMostSmem);
     if (rc != MUON_POLAR_OK) return rc;
     return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, smem, 1, false, stream, a, plan,
                   grad_weights, static_cast<T*>(grad));

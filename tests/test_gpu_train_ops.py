@@ -721,6 +721,36 @@ def test_route_ties_go_to_the_lowest_index(pkg, experts, score):
     assert torch.equal(indices, torch.arange(4, device="cuda").expand(3, 4))
 
 
+@pytest.mark.parametrize("experts", [48, 64, 100, 128, 256, 300, 512, 1000])
+@pytest.mark.parametrize("k", [3, 4, 8, 15, 16, 17])
+def test_route_choice_is_that_of_a_stable_sort(pkg, experts, k):
+    """Logits with some equal ones, the best spread over the row, side by side,
+    few above a floor, or in falling or rising order."""
+    x = torch.randn(400, experts, generator=gen(41), device="cuda")
+    x[100:200] = (x[100:200] * 8).round() / 8
+    x[200:300] = (x[200:300] * 2).round() / 2
+    x[::5] = x[::5].sort(dim=-1, descending=True).values
+    x[1::5] = x[1::5].sort(-1).values
+    x[2::10] = x[2::10].clamp(min=x[2::10].topk(max(1, k // 2), -1).values[:, -1:])
+    for start in (0, 7, experts - 20):
+        x[300 + start % 50::50, start:start + 20] += 8
+    x[399, 5:] = NEG
+    want = x.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+    weights, indices, counts = pkg.route_experts(x, k)
+    assert torch.equal(indices, want)
+    assert torch.equal(counts, torch.bincount(want.reshape(-1), minlength=experts))
+    near(weights, x.double().gather(1, want).softmax(-1), 1e-6)
+    # in four groups, the two with the largest logit
+    lead = x.view(400, 4, -1).amax(-1).sort(dim=-1, descending=True, stable=True).indices[:, :2]
+    stays = torch.zeros(400, 4, dtype=torch.bool, device="cuda").scatter_(1, lead, True)
+    stays = stays.repeat_interleave(experts // 4, 1)
+    order = x.sort(dim=-1, descending=True, stable=True).indices
+    rank = torch.where(stays.gather(1, order), torch.arange(experts, device="cuda"), experts)
+    want = order.gather(1, rank.sort(-1).indices[:, :k])
+    _, indices, _ = pkg.route_experts(x, k, groups=4, top_groups=2, group_top=1)
+    assert torch.equal(indices, want)
+
+
 @pytest.mark.parametrize("experts", [16, 300])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_masks(pkg, experts, score):
