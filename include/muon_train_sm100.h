@@ -77,8 +77,8 @@ typedef struct {
 } muon_train_distill_args;
 
 /* loss, with stats (may be NULL without grad) for a later backward call, and
- * grad (may be NULL): the loss and its gradient from one reading of the
- * logits (two for rows of more than about a million bytes). */
+ * grad (may be NULL): the loss and its gradient in one launch, which reads the
+ * logits once from memory where rows stay in registers or in L2. */
 int muon_train_distill_sm100(const muon_train_distill_args* args, void* stream);
 
 /* grad from the stats of an earlier call on the same inputs (loss unused). */

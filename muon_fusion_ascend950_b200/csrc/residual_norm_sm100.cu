@@ -345,7 +345,7 @@ struct Ring {
   }
 };
 
-// The row's gate row.
+// Which row of the gate a row uses.
 __device__ __forceinline__ int64_t gate_row_of(const muon_train_norm_args& a, int64_t row) {
   return a.gate_rows > 1 ? row / (a.rows / a.gate_rows) : 0;
 }

@@ -172,7 +172,8 @@ def distill_topk_grad(student_logits: torch.Tensor, teacher_logits: torch.Tensor
                       temperature: float = 1.0, teacher_lse: Optional[torch.Tensor] = None
                       ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``distill_topk`` and the gradient of ``sum(row_scale * loss)`` in
-    ``student_logits``, from one reading of the logits.
+    ``student_logits`` in one launch.  The logits come from memory once: rows
+    stay in registers, or in L2 until they are read again.
 
     ``row_scale`` (``[...]``, default 1) is what the rows weigh in the total,
     e.g. one over the number of tokens, or 0 for tokens that do not count.
