@@ -287,7 +287,7 @@ __device__ __forceinline__ float pair_sum(float2 v) { return v.x + v.y; }
 
 // Rows of a block (or of its part of a cluster's rows) on their way through
 // shared memory: bulk copies of kArrays tensors' rows into `stages` stages,
-// issued by one thread.  A stage is free again once every thread has it in
+// issued by the warps' first lanes.  A stage is free again once every thread has it in
 // registers, which the barrier of the row's sums tells.
 constexpr int kMaxStages = 16;
 constexpr size_t kRingMost = 222 * 1024;  // bytes of an SM's rings
@@ -302,30 +302,24 @@ struct Ring {
   __device__ T* at(int stage_, int array, int run) const {
     return data + ((stage_ * kArrays + array) * kE / N + run) * static_cast<int>(blockDim.x) * N;
   }
-  // By one thread: the row's columns of this block from each tensor (not NULL).
+  // By one thread: this block's columns of a row of one tensor.  The stage's
+  // barrier expects one such call for each tensor.
   template <typename P>
-  __device__ void issue(int stage_, const T* const (&from)[kArrays], int64_t row, int width, const P& place) const {
+  __device__ void issue(int stage_, int array, const T* from, int64_t row, int width, const P& place) const {
     const int span = static_cast<int>(blockDim.x) * N;
     const int first = place.tid - static_cast<int>(threadIdx.x);  // the block's first thread of the row
     uint32_t bytes = 0;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {  // first the sum of the bytes, then the copies
+    for (int i = 0; i < kE / N; ++i)
+      bytes += static_cast<uint32_t>(max(0, min(span, width - (i * place.threads + first) * N))) * sizeof(T);
+    muon_sm100::mbar_arrive_expect_tx(&full[stage_], bytes);
 #pragma unroll
-      for (int i = 0; i < kE / N; ++i) {
-        const int c = (i * place.threads + first) * N;
-        const int n = min(span, width - c);
-        if (n <= 0) continue;
-#pragma unroll
-        for (int t = 0; t < kArrays; ++t) {
-          if (from[t] == nullptr) continue;
-          const uint32_t b = static_cast<uint32_t>(n) * sizeof(T);
-          if (pass == 0)
-            bytes += b;
-          else
-            muon_sm100::bulk_load(at(stage_, t, i), from[t] + row * width + c, b, &full[stage_]);
-        }
-      }
-      if (pass == 0) muon_sm100::mbar_arrive_expect_tx(&full[stage_], bytes);
+    for (int i = 0; i < kE / N; ++i) {
+      const int c = (i * place.threads + first) * N;
+      const int n = min(span, width - c);
+      if (n > 0)
+        muon_sm100::bulk_load(at(stage_, array, i), from + row * width + c, static_cast<uint32_t>(n) * sizeof(T),
+                              &full[stage_]);
     }
   }
   __device__ void wait() const { ring_wait(&full[stage], phase, failed); }
@@ -372,16 +366,25 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   const T* y_all = static_cast<const T*>(a.block_out);
   const T* x_all = static_cast<const T*>(a.residual);
   Ring<T, N, kE, 2> ring{full, reinterpret_cast<T*>(dynamic), &failed, stages, 0, 0};
-  const T* const tensors[2] = {y_all, x_all};
+  // `rows` rows from `row` on into the stages from `stage` on; a warp's first
+  // lane issues every so many of the 2 rows copies, since the next sums wait
+  // for the slowest warp
+  const auto issue = [&](int stage, int64_t row, int rows) {
+    if ((threadIdx.x & 31) != 0) return;
+    for (int i = threadIdx.x >> 5; i < 2 * rows; i += blockDim.x >> 5) {
+      const int64_t r = row + (i >> 1) * place.workers;
+      const int to = stage + (i >> 1);
+      if (r < a.rows) ring.issue(to < stages ? to : to - stages, i & 1, (i & 1) == 0 ? y_all : x_all, r, width, place);
+    }
+  };
   if constexpr (kRing) {
     if (threadIdx.x == 0) {
-      for (int i = 0; i < stages; ++i) muon_sm100::mbar_init(&full[i], 1);
+      for (int i = 0; i < stages; ++i) muon_sm100::mbar_init(&full[i], 2);
       failed = 0;
       muon_sm100::fence_mbar_init();
-      for (int i = 0; i < stages && place.worker + i * place.workers < a.rows; ++i)
-        ring.issue(i, tensors, place.worker + i * place.workers, width, place);
     }
     __syncthreads();
+    issue(0, place.worker, stages);
   }
   Columns<kE> gain, scale, pre;
   int64_t gate_row = place.worker < a.rows ? gate_row_of(a, place.worker) : 0;
@@ -405,13 +408,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     // After a barrier that follows the rows' reading: their stages take later ones.
     const auto refill = [&] {
       if constexpr (kRing) {
-        int stage = ring.stage - rows;
-        if (stage < 0) stage += stages;
-        for (int j = 0; j < rows && threadIdx.x == 0; ++j) {
-          const int64_t later = first + (stages + j) * place.workers;
-          if (later < a.rows) ring.issue(stage, tensors, later, width, place);
-          if (++stage == stages) stage = 0;
-        }
+        const int stage = ring.stage - rows;
+        issue(stage < 0 ? stage + stages : stage, first + stages * place.workers, rows);
       }
     };
     Columns<kE> y[kRowsAtOnce], h[kRowsAtOnce];
@@ -709,8 +707,9 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   rdn.clear();
   float4* const held = reinterpret_cast<float4*>(dynamic);
   Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + (kE == 16 ? held_columns(kScaleColumns) * kE * sizeof(float) * blockDim.x : 0)), &failed, stages, 0, 0};
-  const T* const tensors[4] = {y_all, x_all, dh_all, dn_all};
-  // thread 0: the row that goes into the ring next
+  // Each warp's first lane: the row that goes into the ring next.  It issues
+  // every so many of the row's copies, since the next sums wait for the slowest
+  // warp.
   int64_t ahead_chunk = worker, ahead_row = 0, ahead_end = 0;
   const auto issue_next = [&](int stage) {
     while (ahead_row >= ahead_end) {
@@ -719,16 +718,22 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       chunk_rows(b, ahead_chunk, &ahead_row, &ahead_end, &group);
       ahead_chunk += workers;
     }
-    ring.issue(stage, tensors, ahead_row++, width, place);
+    for (int t = threadIdx.x >> 5; t < 4; t += blockDim.x >> 5) {
+      const T* from = t == 0 ? y_all : t == 1 ? x_all : t == 2 ? dh_all : dn_all;
+      if (from != nullptr) ring.issue(stage, t, from, ahead_row, width, place);
+    }
+    ++ahead_row;
   };
   if constexpr (kRing) {
     if (threadIdx.x == 0) {
-      for (int i = 0; i < stages; ++i) muon_sm100::mbar_init(&full[i], 1);
+      for (int i = 0; i < stages; ++i)
+        muon_sm100::mbar_init(&full[i], 2 + (dh_all != nullptr) + (dn_all != nullptr));
       failed = 0;
       muon_sm100::fence_mbar_init();
-      for (int i = 0; i < stages; ++i) issue_next(i);
     }
     __syncthreads();
+    if ((threadIdx.x & 31) == 0 && threadIdx.x < 4 * 32)
+      for (int i = 0; i < stages; ++i) issue_next(i);
   }
 
   Held<kE> gain(held, 0), pre(held, 1), sum_scale(held, 2);  // gain: gate times post weight
@@ -831,7 +836,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       float sums[4] = {pair_sum(s0), pair_sum(s1), pair_sum(s2), 0.f};
       row_sums<kOwner>(sums, slots, turn);
       if constexpr (kRing) {  // every thread has the row in registers
-        if (threadIdx.x == 0) issue_next(ring.stage);
+        if ((threadIdx.x & 31) == 0 && threadIdx.x < 4 * 32) issue_next(ring.stage);
         ring.advance();
       }
       const float k = rh * rh * rh * sums[0] * inv_width;
