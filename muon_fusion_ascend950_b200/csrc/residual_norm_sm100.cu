@@ -638,15 +638,15 @@ struct Held {
     c.v[2 * q + 1] = p[1];
   }
 };
-template <>
-struct Held<16> {
+template <int kE>
+struct SharedHeld {
   float4* at;
   int stride;
-  __device__ Held(float4* area, int index)
-      : at(area + index * 4 * blockDim.x + threadIdx.x), stride(static_cast<int>(blockDim.x)) {}
-  __device__ void set(const Columns<16>& v) {
+  __device__ SharedHeld(float4* area, int index)
+      : at(area + index * (kE / 4) * blockDim.x + threadIdx.x), stride(static_cast<int>(blockDim.x)) {}
+  __device__ void set(const Columns<kE>& v) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < kE / 4; ++q)
       at[q * stride] = make_float4(v.v[2 * q].x, v.v[2 * q].y, v.v[2 * q + 1].x, v.v[2 * q + 1].y);
   }
   __device__ void pairs(int q, float2 (&p)[2]) const {
@@ -658,8 +658,18 @@ struct Held<16> {
     at[q * stride] = make_float4(p[0].x, p[0].y, p[1].x, p[1].y);
   }
 };
-// gain, pre weight, and sums of a residual scale with columns
-__host__ __device__ constexpr int held_columns(bool scale_columns) { return scale_columns ? 3 : 2; }
+template <>
+struct Held<16> : SharedHeld<16> {
+  using SharedHeld<16>::SharedHeld;
+};
+// Floats a thread holds in shared memory: with 16 columns gain, pre weight and
+// the sums of a residual scale with columns; with 8 that scale itself (16384 x
+// 4096 bf16 228 us, loaded for every row 272).  With 16 it would take the
+// ring's second stage, and single elements have no registers for it (2049
+// columns: 377 us, loaded for every row 326).
+__host__ __device__ constexpr int held_floats(int columns, int elements, bool scale_columns) {
+  return columns == 16 ? (scale_columns ? 3 : 2) * 16 : scale_columns && elements > 1 ? 8 : 0;
+}
 
 // Backward.  A worker (block or cluster) takes whole chunks; with one warp a
 // row, the block's warps take every 8th row of the chunk and are added up
@@ -706,7 +716,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   rdh.clear();
   rdn.clear();
   float4* const held = reinterpret_cast<float4*>(dynamic);
-  Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + (kE == 16 ? held_columns(kScaleColumns) * kE * sizeof(float) * blockDim.x : 0)), &failed, stages, 0, 0};
+  Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + held_floats(kE, N, kScaleColumns) * sizeof(float) * blockDim.x), &failed, stages, 0, 0};
   // Each warp's first lane: the row that goes into the ring next.  It issues
   // every so many of the row's copies, since the next sums wait for the slowest
   // warp.
@@ -737,7 +747,9 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   }
 
   Held<kE> gain(held, 0), pre(held, 1), sum_scale(held, 2);  // gain: gate times post weight
+  constexpr bool kHoldScale = kScaleColumns && kE == 8 && N > 1;
   Columns<kE> scale_columns{};
+  SharedHeld<kE> scale_held(held, 0);
   float2 scale_one = both(1.f);
   double sum_scale_one = 0.0;  // over all of a thread's elements: in 64 bits, an addition a row
   {
@@ -747,14 +759,24 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     load_columns<N>(v, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
     pre.set(v);
     if constexpr (kScaleColumns) sum_scale.set(Columns<kE>{});
+    if constexpr (kHoldScale) {
+      load_columns<N>(v, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+      scale_held.set(v);
+    }
   }
   if (!kScaleColumns && a.residual_scale != nullptr)
     scale_one = both(load_any(a.residual_scale, a.scale_dtype, 0));
-  const auto scale_of = [&](int i) {
-    if constexpr (kScaleColumns)
-      return scale_columns.v[i];
-    else
-      return scale_one;
+  const auto load_scale = [&] {
+    if constexpr (kScaleColumns && !kHoldScale)
+      load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+  };
+  const auto scale_pairs = [&](int q, float2 (&p)[2]) {
+    if constexpr (kHoldScale) {
+      scale_held.pairs(q, p);
+    } else {
+      p[0] = kScaleColumns ? scale_columns.v[2 * q] : scale_one;
+      p[1] = kScaleColumns ? scale_columns.v[2 * q + 1] : scale_one;
+    }
   };
   const auto hold_gain = [&](int64_t gate_row) {
     Columns<kE> v;
@@ -815,18 +837,18 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       if constexpr (kAhead) {
         if (row + step < r1) load_row(row + step);
       }
-      if constexpr (kScaleColumns)
-        load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+      load_scale();
 #pragma unroll
       for (int q = 0; q < kE / 4; ++q) {
-        float2 g[2], p[2];
+        float2 g[2], p[2], s[2];
         gain.pairs(q, g);
         pre.pairs(q, p);
+        scale_pairs(q, s);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * q + j;
           const float2 gy = mul2(g[j], y.v[i]), an = mul2(dn.v[i], p[j]);
-          h.v[i] = fma2(gy, both(r), mul2(scale_of(i), x.v[i]));
+          h.v[i] = fma2(gy, both(r), mul2(s[j], x.v[i]));
           u.v[i] = fma2(both(rh), an, u.v[i]);
           s0 = fma2(an, h.v[i], s0);
           s1 = fma2(gy, u.v[i], s1);
@@ -845,15 +867,15 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         ry.values(y);
         rx.values(x);
         rdn.values(dn);
-        if constexpr (kScaleColumns)
-          load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
+        load_scale();
       }
       Columns<kE> gained;
       float2 row_scale = both(0.f);
 #pragma unroll
       for (int q = 0; q < kE / 4; ++q) {
-        float2 g[2], sc[2];
+        float2 g[2], s[2], sc[2];
         gain.pairs(q, g);
+        scale_pairs(q, s);
         if constexpr (kScaleColumns) sum_scale.pairs(q, sc);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -865,7 +887,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
             sc[j] = fma2(d, x.v[i], sc[j]);
           else
             row_scale = fma2(d, x.v[i], row_scale);
-          x.v[i] = mul2(d, scale_of(i));
+          x.v[i] = mul2(d, s[j]);
           y.v[i] = fma2(both(-ky), y.v[i], mul2(mul2(g[j], both(r)), d));
         }
         if constexpr (kScaleColumns) sum_scale.set_pairs(q, sc);
@@ -1234,12 +1256,12 @@ template <typename T, int N, int kE, RowOwner kOwner, bool kScaleColumns>
 int launch_backward(const Backward& b, const Layout& l, void* stream) {
   if (l.columns != kE || l.owner != kOwner) return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not make_layout's
   int stages = 0;
-  const size_t held = kE == 16 ? static_cast<size_t>(l.threads) * kE * sizeof(float) * held_columns(kScaleColumns) : 0;
+  const size_t held = static_cast<size_t>(l.threads) * held_floats(kE, N, kScaleColumns) * sizeof(float);
   const size_t ring = ring_bytes<T, N>(l, 4, l.per_sm, held, &stages), smem = held + ring;
   if (N * sizeof(T) == 16 && kOwner != kWarpRow && stages < 1)
     return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not with make_layout's sizes
   const int rc =
-      smem == 0 ? MUON_POLAR_OK : allow_smem<norm_backward_kernel<T, N, kE, kOwner, kScaleColumns>>(kRingMost);
+      smem <= 32 * 1024 ? MUON_POLAR_OK : allow_smem<norm_backward_kernel<T, N, kE, kOwner, kScaleColumns>>(kRingMost);
   if (rc != MUON_POLAR_OK) return rc;
   return launch(norm_backward_kernel<T, N, kE, kOwner, kScaleColumns>,
                 dim3(static_cast<unsigned>(b.plan.blocks * l.cluster)), l.threads, smem, l.cluster, true, stream,
