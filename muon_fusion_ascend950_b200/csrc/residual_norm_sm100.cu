@@ -663,12 +663,13 @@ struct Held<16> : SharedHeld<16> {
   using SharedHeld<16>::SharedHeld;
 };
 // Floats a thread holds in shared memory: with 16 columns gain, pre weight and
-// the sums of a residual scale with columns; with 8 that scale itself (16384 x
-// 4096 bf16 228 us, loaded for every row 272).  With 16 it would take the
-// ring's second stage, and single elements have no registers for it (2049
-// columns: 377 us, loaded for every row 326).
+// the sums of a residual scale with columns; with 8 that scale and its sums
+// (16384 x 4096 bf16 174 us; the sums in registers 228, and the scale loaded for
+// every row 272).  With 16 the scale would take the ring's second stage, and
+// single elements have no registers for the addresses (2049 columns: 377 us,
+// loaded for every row 326).
 __host__ __device__ constexpr int held_floats(int columns, int elements, bool scale_columns) {
-  return columns == 16 ? (scale_columns ? 3 : 2) * 16 : scale_columns && elements > 1 ? 8 : 0;
+  return columns == 16 ? (scale_columns ? 3 : 2) * 16 : scale_columns && elements > 1 ? 16 : 0;
 }
 
 // Backward.  A worker (block or cluster) takes whole chunks; with one warp a
@@ -746,8 +747,9 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       for (int i = 0; i < stages; ++i) issue_next(i);
   }
 
-  Held<kE> gain(held, 0), pre(held, 1), sum_scale(held, 2);  // gain: gate times post weight
   constexpr bool kHoldScale = kScaleColumns && kE == 8 && N > 1;
+  Held<kE> gain(held, 0), pre(held, 1);  // gain: gate times post weight
+  std::conditional_t<kHoldScale, SharedHeld<kE>, Held<kE>> sum_scale(held, kE == 8 ? 1 : 2);
   Columns<kE> scale_columns{};
   SharedHeld<kE> scale_held(held, 0);
   float2 scale_one = both(1.f);
