@@ -621,10 +621,9 @@ __device__ __forceinline__ void store_warp_columns(float* to, int width, const C
   }
 }
 
-// Columns that a thread keeps for the whole kernel: in registers with 8 of
-// them, in shared memory, where only the thread itself reads and writes them,
-// with 16.
-template <int kE>
+// Columns that a thread keeps for the whole kernel: in registers, or in shared
+// memory, where only the thread itself reads and writes them.
+template <int kE, bool kShared>
 struct Held {
   Columns<kE> c;
   __device__ Held(float4*, int) {}
@@ -639,10 +638,10 @@ struct Held {
   }
 };
 template <int kE>
-struct SharedHeld {
+struct Held<kE, true> {
   float4* at;
   int stride;
-  __device__ SharedHeld(float4* area, int index)
+  __device__ Held(float4* area, int index)
       : at(area + index * (kE / 4) * blockDim.x + threadIdx.x), stride(static_cast<int>(blockDim.x)) {}
   __device__ void set(const Columns<kE>& v) {
 #pragma unroll
@@ -658,19 +657,23 @@ struct SharedHeld {
     at[q * stride] = make_float4(p[0].x, p[0].y, p[1].x, p[1].y);
   }
 };
-template <>
-struct Held<16> : SharedHeld<16> {
-  using SharedHeld<16>::SharedHeld;
+// Which of a thread's held columns are in shared memory, and how many there are.
+// With 16 columns: gain, pre weight and the sums of a residual scale with
+// columns (the scale itself would take the ring's second stage, and is loaded
+// for every row).  With 8 columns registers would do, but the fewer they hold
+// the less a row waits: that scale and its sums (16384 x 4096 bf16 174 us; the
+// sums in registers 228, and the scale loaded for every row 272); of rows
+// through the ring the pre weight (174 us, 178 in registers), of fp32 the gain
+// too (291 us, 334; bf16 181).  Single elements have no registers for the
+// addresses (2049 columns: 377 us, the scale loaded for every row 326).
+template <typename T, int N, int kE, bool kRing, bool kScaleColumns>
+struct Holds {
+  static constexpr bool kScale = kScaleColumns && kE == 8 && N > 1;
+  static constexpr bool kScaleSums = kScaleColumns && (kE == 16 || kScale);
+  static constexpr bool kPre = kE == 16 || kRing;
+  static constexpr bool kGain = kE == 16 || (kRing && sizeof(T) == 4);
+  static constexpr int kFloats = (kScale + kScaleSums + kPre + kGain) * kE;
 };
-// Floats a thread holds in shared memory: with 16 columns gain, pre weight and
-// the sums of a residual scale with columns; with 8 that scale and its sums
-// (16384 x 4096 bf16 174 us; the sums in registers 228, and the scale loaded for
-// every row 272).  With 16 the scale would take the ring's second stage, and
-// single elements have no registers for the addresses (2049 columns: 377 us,
-// loaded for every row 326).
-__host__ __device__ constexpr int held_floats(int columns, int elements, bool scale_columns) {
-  return columns == 16 ? (scale_columns ? 3 : 2) * 16 : scale_columns && elements > 1 ? 16 : 0;
-}
 
 // Backward.  A worker (block or cluster) takes whole chunks; with one warp a
 // row, the block's warps take every 8th row of the chunk and are added up
@@ -690,6 +693,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   constexpr bool kRing = N * sizeof(T) == 16 && kOwner != kWarpRow;
   constexpr bool kAhead = !kRing && sizeof(T) == 2 && N > 1;
   constexpr bool kAgain = kRing && sizeof(T) == 2;
+  using Hold = Holds<T, N, kE, kRing, kScaleColumns>;
   const muon_train_norm_args& a = b.a;
   const Place<N, kOwner> place;
   const int width = static_cast<int>(a.width);
@@ -717,7 +721,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   rdh.clear();
   rdn.clear();
   float4* const held = reinterpret_cast<float4*>(dynamic);
-  Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + held_floats(kE, N, kScaleColumns) * sizeof(float) * blockDim.x), &failed, stages, 0, 0};
+  Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + Hold::kFloats * sizeof(float) * blockDim.x), &failed, stages, 0, 0};
   // Each warp's first lane: the row that goes into the ring next.  It issues
   // every so many of the row's copies, since the next sums wait for the slowest
   // warp.
@@ -747,11 +751,11 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       for (int i = 0; i < stages; ++i) issue_next(i);
   }
 
-  constexpr bool kHoldScale = kScaleColumns && kE == 8 && N > 1;
-  Held<kE> gain(held, 0), pre(held, 1);  // gain: gate times post weight
-  std::conditional_t<kHoldScale, SharedHeld<kE>, Held<kE>> sum_scale(held, kE == 8 ? 1 : 2);
+  Held<kE, Hold::kGain> gain(held, 0);  // gate times post weight
+  Held<kE, Hold::kPre> pre(held, Hold::kGain);
+  Held<kE, Hold::kScaleSums> sum_scale(held, Hold::kGain + Hold::kPre);
+  Held<kE, Hold::kScale> scale_held(held, Hold::kGain + Hold::kPre + Hold::kScaleSums);
   Columns<kE> scale_columns{};
-  SharedHeld<kE> scale_held(held, 0);
   float2 scale_one = both(1.f);
   double sum_scale_one = 0.0;  // over all of a thread's elements: in 64 bits, an addition a row
   {
@@ -761,7 +765,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     load_columns<N>(v, place, width, a.pre_weight, a.pre_dtype, 0, 0.f);
     pre.set(v);
     if constexpr (kScaleColumns) sum_scale.set(Columns<kE>{});
-    if constexpr (kHoldScale) {
+    if constexpr (Hold::kScale) {
       load_columns<N>(v, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
       scale_held.set(v);
     }
@@ -769,11 +773,11 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   if (!kScaleColumns && a.residual_scale != nullptr)
     scale_one = both(load_any(a.residual_scale, a.scale_dtype, 0));
   const auto load_scale = [&] {
-    if constexpr (kScaleColumns && !kHoldScale)
+    if constexpr (kScaleColumns && !Hold::kScale)
       load_columns<N>(scale_columns, place, width, a.residual_scale, a.scale_dtype, 0, 1.f);
   };
   const auto scale_pairs = [&](int q, float2 (&p)[2]) {
-    if constexpr (kHoldScale) {
+    if constexpr (Hold::kScale) {
       scale_held.pairs(q, p);
     } else {
       p[0] = kScaleColumns ? scale_columns.v[2 * q] : scale_one;
@@ -1258,7 +1262,9 @@ template <typename T, int N, int kE, RowOwner kOwner, bool kScaleColumns>
 int launch_backward(const Backward& b, const Layout& l, void* stream) {
   if (l.columns != kE || l.owner != kOwner) return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not make_layout's
   int stages = 0;
-  const size_t held = static_cast<size_t>(l.threads) * held_floats(kE, N, kScaleColumns) * sizeof(float);
+  constexpr bool kRing = N * sizeof(T) == 16 && kOwner != kWarpRow;
+  const size_t held =
+      static_cast<size_t>(l.threads) * Holds<T, N, kE, kRing, kScaleColumns>::kFloats * sizeof(float);
   const size_t ring = ring_bytes<T, N>(l, 4, l.per_sm, held, &stages), smem = held + ring;
   if (N * sizeof(T) == 16 && kOwner != kWarpRow && stages < 1)
     return MUON_POLAR_ERR_INVALID_ARGUMENT;  // not with make_layout's sizes
