@@ -72,10 +72,11 @@ __device__ __forceinline__ float rms_rstd(float sum, float width, float eps) {
 // block of up to 512 threads, or to a cluster of such blocks, which add up
 // their sums over distributed shared memory.  Rows of whole 16-byte vectors
 // have 8 columns a thread up to 4096, 16 above, and a cluster of 2 above
-// 8192: for 16384 x 8192 bf16 backward takes 436 us so, 568 with 8 columns in
-// a cluster, whose barrier holds up every row.  Other rows have 8 columns a
-// thread and clusters of 2 and 4: 16 would not fit the registers (4098
-// columns: 716 us, with 16 a thread 1219).
+// 8192: 16384 x 8192 bf16 backward took 436 us so when it was chosen (404 now),
+// 568 with 8 columns in a cluster, whose barrier holds up every row.  Other
+// rows have 8 columns a thread and clusters of 2 and 4: 16 would not fit the
+// registers (4098 columns: 716 us when it was chosen, with 16 a thread 1219;
+// 588 now).
 constexpr int kMaxThreads = 512;
 constexpr int kWarpRowWarps = 8;   // rows in flight of a block, one a warp
 constexpr int kMaxCluster = 4;
@@ -344,9 +345,10 @@ __device__ __forceinline__ int64_t gate_row_of(const muon_train_norm_args& a, in
   return a.gate_rows > 1 ? row / (a.rows / a.gate_rows) : 0;
 }
 
-// Forward.  Four rows (of 8 columns a thread) at a time: their sums share the shuffles and barriers,
-// whose latency else held up every row (one row at a time, two blocks an SM:
-// 116 us for 16384 x 4096 bf16, 83 at the copy rate).
+// Forward.  Four rows (of 8 columns a thread) at a time: their sums share the
+// shuffles and barriers, whose latency else held up every row.  16384 x 4096
+// bf16: 94 us, 83 at the copy rate (one row at a time, two blocks an SM: 116;
+// with all copies issued by one thread, on whose warp the next sums wait: 103).
 template <typename T, int N, int kE, RowOwner kOwner>
 __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads,
                                   kOwner == kWarpRow ? 2 : 1)
@@ -675,7 +677,11 @@ struct Holds {
   static constexpr int kFloats = (kScale + kScaleSums + kPre + kGain) * kE;
 };
 
-// Backward.  A worker (block or cluster) takes whole chunks; with one warp a
+// Backward.  16384 x 4096 bf16: 173 us, 125 at the copy rate; 60% of the issue
+// slots are used, the rest goes into each row's sums and barrier (two rows at
+// a time, read from their stages again, took 202 against 183 then: more
+// instructions than the waits were worth).
+// A worker (block or cluster) takes whole chunks; with one warp a
 // row, the block's warps take every 8th row of the chunk and are added up
 // where the chunk ends.  kScaleColumns: residual_scale has a value for each
 // column (else one value, or none).
