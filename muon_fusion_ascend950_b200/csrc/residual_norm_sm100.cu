@@ -4,14 +4,15 @@
 //   r = rsqrt(mean y^2 + eps), u = y r w, h = s x + g u,
 //   R = rsqrt(mean h^2 + eps), n = h R p
 //
-// With a = dn p, b0 = g w (dh + R a), A = sum a h, B1 = sum b0 y,
-// B2 = sum g w y h and k = R^3 A / width:
-//   dH = dh + R a - k h         dx = s dH        ds = sum dH x
-//   dy = r g w dH - y r^3 (B1 - k B2) / width
-//   C  = sum dH y r             dg = w C         dw = g C
-//   dp = sum dn h R
+// With the normed rows v = y r and m = h R, a = dn p, A = sum a m,
+// B1 = sum g w v (dh + R a), B2 = sum g w v m and k = R A / width:
+//   dH = dh + R a - k m         dx = s dH        ds = sum dH x
+//   dy = r (g w dH - v (B1 - k B2) / width)
+//   C  = sum dH v               dg = w C         dw = g C
+//   dp = sum dn m
 // so that a row needs one reduction of three sums, and h is made again from
-// x and y instead of being kept.
+// x and y instead of being kept.  No power of r or R is formed: their cubes
+// leave fp32's range from rows of rms 5e12 on, and below 1e-13 when eps allows.
 //
 // Bound by memory: forward reads x, y and writes h, n; backward reads x, y,
 // dh, dn and writes dx, dy.  Parameter gradients: each block adds up its rows
@@ -861,7 +862,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       if (b.plan.gate_per_row) hold_gain(row);
       const float r = next_r, rh = next_rh;
       load_rstd(row + step);
-      Columns<kE> h, u;  // u: dh + rh dn pre
+      Columns<kE> m, u;  // m: hidden, normed; u: dh + rh dn pre
       rdh.values(u);
       float2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
       Columns<kE> y, x, dn;
@@ -881,12 +882,12 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * q + j;
-          const float2 gy = mul2(g[j], y.v[i]), an = mul2(dn.v[i], p[j]);
-          h.v[i] = fma2(gy, both(r), mul2(s[j], x.v[i]));
+          const float2 gv = mul2(g[j], mul2(y.v[i], both(r))), an = mul2(dn.v[i], p[j]);
+          m.v[i] = mul2(fma2(s[j], x.v[i], gv), both(rh));
           u.v[i] = fma2(both(rh), an, u.v[i]);
-          s0 = fma2(an, h.v[i], s0);
-          s1 = fma2(gy, u.v[i], s1);
-          s2 = fma2(gy, h.v[i], s2);
+          s0 = fma2(an, m.v[i], s0);
+          s1 = fma2(gv, u.v[i], s1);
+          s2 = fma2(gv, m.v[i], s2);
         }
       }
       float sums[4] = {pair_sum(s0), pair_sum(s1), pair_sum(s2), 0.f};
@@ -895,8 +896,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         if ((threadIdx.x & 31) == 0 && threadIdx.x < 4 * 32) issue_next(ring.stage);
         ring.advance();
       }
-      const float k = rh * rh * rh * sums[0] * inv_width;
-      const float ky = a.post_weight != nullptr ? r * r * r * (sums[1] - k * sums[2]) * inv_width : 0.f;
+      const float k = rh * (sums[0] * inv_width);
+      const float ky = a.post_weight != nullptr ? r * ((sums[1] - k * sums[2]) * inv_width) : 0.f;
       if constexpr (kAgain) {  // out of the packed registers: fewer are held over the barrier
         ry.values(y);
         rx.values(x);
@@ -914,15 +915,15 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * q + j;
-          const float2 d = fma2(both(-k), h.v[i], u.v[i]);
-          gained.v[i] = mul2(d, mul2(y.v[i], both(r)));
-          sum_pre.v[i] = fma2(mul2(dn.v[i], h.v[i]), both(rh), sum_pre.v[i]);
+          const float2 d = fma2(both(-k), m.v[i], u.v[i]), v = mul2(y.v[i], both(r));
+          gained.v[i] = mul2(d, v);
+          sum_pre.v[i] = fma2(dn.v[i], m.v[i], sum_pre.v[i]);
           if constexpr (kScaleColumns)
             sc[j] = fma2(d, x.v[i], sc[j]);
           else
             row_scale = fma2(d, x.v[i], row_scale);
           x.v[i] = mul2(d, s[j]);
-          y.v[i] = fma2(both(-ky), y.v[i], mul2(mul2(g[j], both(r)), d));
+          y.v[i] = fma2(both(-ky), v, mul2(mul2(g[j], both(r)), d));
         }
         if constexpr (kScaleColumns) sum_scale.set_pairs(q, sc);
       }
@@ -1009,35 +1010,35 @@ __global__ void __launch_bounds__(kThreads)
       const float rh = a.pre_weight != nullptr && dn_all != nullptr ? a.rstd_pre[row] : 0.f;
       float sums[3] = {0.f, 0.f, 0.f};
       for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-        const float yv = to_float(y[c]), gw = p.gate(gate_row, c) * p.post(c);
-        const float h = fmaf(p.scale(c), to_float(x[c]), gw * (yv * r));
+        const float gv = p.gate(gate_row, c) * p.post(c) * (to_float(y[c]) * r);
+        const float m = fmaf(p.scale(c), to_float(x[c]), gv) * rh;
         const float dh = dh_all != nullptr ? to_float(dh_all[base + c]) : 0.f;
         const float an = dn_all != nullptr ? to_float(dn_all[base + c]) * p.pre(c) : 0.f;
-        sums[0] = fmaf(an, h, sums[0]);
-        sums[1] = fmaf(gw * fmaf(rh, an, dh), yv, sums[1]);
-        sums[2] = fmaf(gw * yv, h, sums[2]);
+        sums[0] = fmaf(an, m, sums[0]);
+        sums[1] = fmaf(gv, fmaf(rh, an, dh), sums[1]);
+        sums[2] = fmaf(gv, m, sums[2]);
       }
       __syncthreads();  // the last row's sums have been read
       block_sums(sums, red, kThreads);
-      const float k = rh * rh * rh * sums[0] / width;
-      const float ky = a.post_weight != nullptr ? r * r * r * (sums[1] - k * sums[2]) / width : 0.f;
+      const float k = rh * (sums[0] / width);
+      const float ky = a.post_weight != nullptr ? r * ((sums[1] - k * sums[2]) / width) : 0.f;
       for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-        const float yv = to_float(y[c]), xv = to_float(x[c]);
+        const float v = to_float(y[c]) * r, xv = to_float(x[c]);
         const float gate = p.gate(gate_row, c), post = p.post(c), sc = p.scale(c);
-        const float h = fmaf(sc, xv, gate * post * (yv * r));
+        const float m = fmaf(sc, xv, gate * post * v) * rh;
         const float dh = dh_all != nullptr ? to_float(dh_all[base + c]) : 0.f;
         const float dn = dn_all != nullptr ? to_float(dn_all[base + c]) : 0.f;
-        const float d = fmaf(-k, h, fmaf(rh, dn * p.pre(c), dh));
+        const float d = fmaf(-k, m, fmaf(rh, dn * p.pre(c), dh));
         if (b.g.grad_residual != nullptr)
           static_cast<T*>(b.g.grad_residual)[base + c] = from_float<T>(d * sc);
         if (b.g.grad_block_out != nullptr)
-          static_cast<T*>(b.g.grad_block_out)[base + c] = from_float<T>(fmaf(-ky, yv, r * (gate * post) * d));
-        const float gained = d * (yv * r);
+          static_cast<T*>(b.g.grad_block_out)[base + c] = from_float<T>(fmaf(-ky, v, r * (gate * post) * d));
+        const float gained = d * v;
         if (b.plan.gate_per_row && b.g.grad_gate != nullptr)
           store_any(b.g.grad_gate, a.gate_dtype, base + c, gained * post);
         if (gain != nullptr)
           gain[c] = (row == r0 ? 0.f : gain[c]) + (b.plan.gate_per_row ? gained * gate : gained);
-        if (pre != nullptr) pre[c] = (first_row ? 0.f : pre[c]) + dn * h * rh;
+        if (pre != nullptr) pre[c] = (first_row ? 0.f : pre[c]) + dn * m;
         if (scale != nullptr) {
           if (a.scale_count == 1)
             scale_sum += d * xv;

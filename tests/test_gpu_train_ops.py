@@ -542,6 +542,23 @@ def test_norm_special_rows(pkg):
     check_norm(pkg, keep, dh[good], dn[good])
 
 
+@pytest.mark.parametrize("size, eps", [(1e15, 1e-6), (1e-14, 0.0)])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("rows, width, dtype", [
+    (40, 64, torch.float32), (40, 200, torch.bfloat16), (300, 512, torch.float32), (300, 2048, torch.bfloat16),
+    (20, 2050, torch.bfloat16), (20, 1021, torch.float32), (20, 8192, torch.bfloat16), (20, 12000, torch.float32),
+    (20, 4098, torch.bfloat16), (5, 20000, torch.float32)])
+def test_norm_gradients_of_large_and_small_rows(pkg, rows, width, dtype, size, eps, post):
+    """Rows whose reciprocal roots are in fp32's range and whose cubes are not,
+    in every layout; with the gradient of normed alone, whose projections are
+    then as large as the rest."""
+    v, dh, dn = norm_inputs((rows, width), dtype, torch.float32, (), 1, post=post, seed=42)
+    for name in ("block_out", "residual"):
+        v[name] = (v[name].float() * size).to(dtype)
+    check_norm(pkg, v, dh, dn, eps=eps)
+    check_norm(pkg, v, dh, dn, eps=eps, hidden_used=False)
+
+
 def test_norm_no_rows(pkg):
     x = torch.empty(0, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)
