@@ -63,11 +63,17 @@ void* Stream(const Tensor& t) {
   return static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
 }
 
-// A gradient of a gradient is not computed: say so instead of returning a
-// result that autograd would take for a constant.
-void NoSecondOrder(const char* who) {
+// Tangents are not carried on, nor is a gradient of a gradient computed: say
+// so instead of returning a result that autograd would take for a constant.
+void NoTangents(std::initializer_list<const Tensor*> inputs, const char* who) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), who,
+                                ": forward-mode differentiation (jvp) is not supported");
+}
+void NoSecondOrder(const variable_list& grads, const char* who) {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), who,
                               ": the gradient cannot be differentiated again (create_graph=True)");
+  for (const Tensor& g : grads) NoTangents({&g}, who);
 }
 
 // ------------------------------------------------------------ distillation
@@ -473,7 +479,7 @@ struct DistillBackward : public torch::autograd::Node {
     for (SavedVariable* v : {&student, &values, &indices, &lse, &stats}) v->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
-    NoSecondOrder("distill_topk");
+    NoSecondOrder(grads, "distill_topk");
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(1);
     static auto op = Op<decltype(DistillBackwardCuda)>("muon_ascend950::distill_topk_backward");
@@ -490,6 +496,7 @@ std::tuple<Tensor, Tensor> DistillAutograd(const Tensor& student, const Tensor& 
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(student, values, indices, lse, temperature);
   };
+  NoTangents({&student, &values, &Given(lse)}, "distill_topk");
   if (!Recorded({&student})) return call();
   auto node = MakeNode<DistillBackward>(student);
   auto out = call();
@@ -507,6 +514,7 @@ std::tuple<Tensor, Tensor> DistillAutograd(const Tensor& student, const Tensor& 
 std::tuple<Tensor, Tensor> DistillGradAutograd(const Tensor& student, const Tensor& values,
                                                const Tensor& indices, const OptTensor& row_scale,
                                                const OptTensor& lse, double temperature) {
+  NoTangents({&student, &values, &Given(row_scale), &Given(lse)}, "distill_topk_grad");
   at::AutoDispatchBelowADInplaceOrView guard;
   static auto op = Op<decltype(DistillGradCuda)>("muon_ascend950::distill_topk_grad");
   return op.call(student, values, indices, row_scale, lse, temperature);
@@ -524,7 +532,7 @@ struct ResidualNormBackward : public torch::autograd::Node {
     rstd.reset_data();
   }
   variable_list apply(variable_list&& grads) override {
-    NoSecondOrder("residual_norm");
+    NoSecondOrder(grads, "residual_norm");
     std::lock_guard<std::mutex> lock(mutex_);
     std::array<Tensor, 6> s;
     std::array<bool, 6> wanted;
@@ -554,6 +562,7 @@ std::tuple<Tensor, Tensor, Tensor> ResidualNormAutograd(
     return op.call(block_out, residual, post, pre, gate, scale, eps);
   };
   const Tensor* inputs[6] = {&block_out, &residual, &Given(post), &Given(pre), &Given(gate), &Given(scale)};
+  NoTangents({inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], inputs[5]}, "residual_norm");
   if (!Recorded({inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], inputs[5]})) return call();
   auto node = MakeNode<ResidualNormBackward>(*inputs[0], *inputs[1], *inputs[2], *inputs[3], *inputs[4],
                                              *inputs[5]);
@@ -579,7 +588,7 @@ struct RouteBackward : public torch::autograd::Node {
     indices.reset_data();
   }
   variable_list apply(variable_list&& grads) override {
-    NoSecondOrder("route_experts");
+    NoSecondOrder(grads, "route_experts");
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(1);
     static auto op = Op<decltype(RouteBackwardCuda)>("muon_ascend950::route_experts_backward");
@@ -595,6 +604,7 @@ std::tuple<Tensor, Tensor, Tensor> RouteAutograd(const Tensor& logits, const Opt
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale);
   };
+  NoTangents({&logits, &Given(bias)}, "route_experts");
   if (!Recorded({&logits})) return call();
   auto node = MakeNode<RouteBackward>(logits);
   auto out = call();

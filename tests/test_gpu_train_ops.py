@@ -886,6 +886,19 @@ def test_gradients_of_gradients_are_refused(pkg):
             torch.autograd.grad(value, x, create_graph=True)
 
 
+def test_tangents_of_gradients_are_refused(pkg):
+    """Forward over reverse: a tangent in what flows back."""
+    from torch.autograd import forward_ad
+
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    i = torch.zeros(4, 1, dtype=torch.int64, device="cuda")
+    w = torch.ones(16, device="cuda")
+    for out in (pkg.distill_topk(x, torch.zeros(4, 1, device="cuda"), i), pkg.residual_norm(x, x, w, w)[1],
+                pkg.route_experts(x, 2)[0]):
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
 def test_same_bits_twice_and_on_another_stream(pkg):
     """Every output is deterministic, and follows its own stream's order."""
     def everything():

@@ -200,6 +200,36 @@ def test_entry_points_check_shapes_and_types():
             pkg.route_experts(_cuda(2, 12), 3, bias=_cuda(11))
 
 
+def _calls(z):
+    """Every operator as a function of its floating inputs, and these."""
+    t, i = _cuda(2, 3), _cuda(2, 3, dtype=torch.int64)
+    rows, w = _cuda(2, dtype=torch.float32), _cuda(8)
+    return {
+        "distill_topk": (lambda z, t, n: pkg.distill_topk(z, t, i, teacher_lse=n), (z, t, rows)),
+        "distill_topk_grad": (lambda z, t, r, n: pkg.distill_topk_grad(z, t, i, r, teacher_lse=n),
+                              (z, t, rows, rows.clone())),
+        "residual_norm": (lambda y, x, p, q, g, s: pkg.residual_norm(y, x, p, q, gate=g, residual_scale=s),
+                          (z, z.clone(), w, w.clone(), w.clone(), w.clone())),
+        "route_experts": (lambda l, b: pkg.route_experts(l, 2, bias=b)[0], (z, w.float())),
+    }
+
+
+@pytest.mark.parametrize("name", ["distill_topk", "distill_topk_grad", "residual_norm", "route_experts"])
+def test_forward_mode_is_refused(name):
+    """A tangent in any input, whether gradients are recorded or not."""
+    from torch.autograd import forward_ad
+
+    with _fake():
+        call, inputs = _calls(_cuda(2, 8))[name]
+        for at in range(len(inputs)):
+            with pytest.raises(NotImplementedError):
+                torch.func.jvp(lambda v: call(*inputs[:at], v, *inputs[at + 1:]), (inputs[at],),
+                               (torch.ones_like(inputs[at]),))
+            with forward_ad.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
+                dual = forward_ad.make_dual(inputs[at], torch.ones_like(inputs[at]))
+                call(*inputs[:at], dual, *inputs[at + 1:])
+
+
 def test_gate_rows_of_every_shape():
     from muon_fusion_ascend950_b200.training import gate_rows
 
