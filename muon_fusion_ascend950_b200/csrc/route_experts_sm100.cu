@@ -336,22 +336,24 @@ __global__ void __launch_bounds__(kThreads, kPer <= 8 ? kBlocksPerSm : 1)
   }
 }
 
-// Backward, one warp a token.  The gradient of the sigmoid, and of the
-// softmax when its chosen scores are renormalised, is zero but for the chosen
-// experts and needs only their logits: with the renormalised weights v (the
-// softmax over the chosen) it is scale v_j (g_j - sum g v).  So the row is
-// written with zeros, and then the chosen; kWholeRow is the softmax without
-// renormalisation, which reaches every expert.
+// Backward, one warp a token.  With the renormalised weights v = s / (S + tiny),
+// S the chosen scores' sum, and c = sum g v, a chosen score's gradient is
+// scale (g_j - c) / (S + tiny).  The sigmoid's logits get s (1 - s) times that,
+// the others nothing and are not read: zeros, and then the chosen.  A softmax
+// reaches every expert (kWholeRow): dl = s (ds - sum s ds), whose last sum is
+// scale c tiny / (S + tiny) renormalised, and scale sum g s otherwise.  The
+// whole row's maximum and sum are needed even where the others' part vanishes:
+// a bias may choose experts whose scores vanish beside the row's.
+// 32768 x 256 fp32, 8 chosen: softmax 24.5 us (from the chosen logits alone
+// 17, which is no gradient of such a choice), sigmoid 15.
 template <typename T, int kPer, bool kWholeRow>
 __global__ void __launch_bounds__(kThreads)
     route_backward_kernel(const __grid_constant__ muon_train_route_args a, Plan plan,
                           const float* __restrict__ grad_weights, T* __restrict__ grad) {
-  extern __shared__ __align__(16) float smem[];
   using Logits = Row<T, kPer>;
   const int experts = static_cast<int>(a.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lanes at(experts, 1, 32, kPer);
-  float* row = smem + warp * experts;  // kWholeRow: the gradients of the scores
   for (int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp; token < a.tokens;
        token += static_cast<int64_t>(gridDim.x) * kWarps) {
     const T* l = static_cast<const T*>(a.logits) + token * a.ld;
@@ -388,78 +390,53 @@ __global__ void __launch_bounds__(kThreads)
           if (i + j < at.count) out[at.e0 + i + j] = from_float<T>(v[i + j]);
       }
     };
+    if constexpr (!kWholeRow) store_row({});
+    const int slots = (a.k + 31) / 32;  // of chosen experts that a lane has
+    float s[kSlots], total = 0.f;
+    [[maybe_unused]] float all[kPer];  // the row's scores
     if constexpr (kWholeRow) {
       Logits logits;
       logits.load(l, at, plan.whole);
-      float s[kPer];
-      scores(logits.v, at, a.score, s);
+      scores(logits.v, at, kSoftmax, all);
+    }
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i < at.count) row[at.e0 + i] = 0.f;
-      __syncwarp();
+    for (int i = 0; i < kSlots; ++i) {
+      if (i >= slots) break;
+      s[i] = 0.f;
+      if constexpr (kWholeRow) {  // from the lane that has the expert
+        const int e = max(chosen[i], 0);
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i)
-        if (chosen[i] >= 0) row[chosen[i]] = g[i] * a.scale;
-      __syncwarp();
-      float d[kPer], dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        d[i] = i < at.count ? row[at.e0 + i] : 0.f;
-        dot = fmaf(d[i], s[i], dot);
+        for (int j = 0; j < kPer; ++j) {
+          const float other = __shfl_sync(kFullMask, all[j], e / kPer);
+          if (j == e % kPer && chosen[i] >= 0) s[i] = other;
+        }
+      } else if (chosen[i] >= 0) {
+        s[i] = sigmoid(to_float(l[chosen[i]]));
       }
-      dot = warp_sum(dot);
+      total += s[i];
+    }
+    total = a.renormalize ? warp_sum(total) + kTiny : 1.f;
+    float v[kSlots], c = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) d[i] = s[i] * (d[i] - dot);
-      store_row(d);
-      __syncwarp();
-    } else {
-      float zero[kPer];
+    for (int i = 0; i < kSlots; ++i) {
+      if (i >= slots) break;
+      v[i] = a.renormalize ? __fdiv_rn(s[i], total) : s[i];
+      c = fmaf(g[i], v[i], c);
+    }
+    if (kWholeRow || a.renormalize) c = warp_sum(c);
+    // every expert's part, and what the chosen ones' g is relative to
+    const float others = a.scale * c * (a.renormalize ? kTiny / total : 1.f), base = a.renormalize ? c : 0.f;
+    if constexpr (kWholeRow) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) zero[i] = 0.f;
-      store_row(zero);
-      const int slots = (a.k + 31) / 32;  // of chosen experts that a lane has
-      float x[kSlots], value[kSlots];
+      for (int i = 0; i < kPer; ++i) all[i] = -all[i] * others;
+      store_row(all);
+    }
+    __syncwarp();  // the row is written
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i)
-        if (i < slots) x[i] = chosen[i] >= 0 ? to_float(l[chosen[i]]) : -INFINITY;
-      float s[kSlots], total = 0.f;  // the scores, the softmax's to a factor
-      float m = -INFINITY;
-      if (a.score == kSoftmax) {
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i)
-          if (i < slots) m = fmaxf(m, x[i]);
-        m = warp_max(m);
-      }
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        if (i >= slots) break;
-        if (a.score != kSoftmax)
-          s[i] = chosen[i] >= 0 ? sigmoid(x[i]) : 0.f;
-        else
-          s[i] = m == -INFINITY && x[i] == x[i] ? 0.f : expf(x[i] - m);
-        total += s[i];
-      }
-      float dot = 0.f;
-      if (a.renormalize) {
-        total = warp_sum(total);
-        total = a.score == kSoftmax ? (total == 0.f ? 1.f : total) : total + kTiny;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i)
-          if (i < slots) dot = fmaf(g[i], __fdiv_rn(s[i], total), dot);
-        dot = warp_sum(dot);
-      } else {
-        total = 1.f;
-      }
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        if (i >= slots) break;
-        value[i] = a.scale * __fdiv_rn(s[i], total) * (g[i] - dot);
-        if (a.score != kSoftmax) value[i] *= 1.0f - s[i];
-      }
-      __syncwarp();  // the zeros are written
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i)
-        if (i < slots && chosen[i] >= 0) out[chosen[i]] = from_float<T>(value[i]);
+    for (int i = 0; i < kSlots; ++i) {
+      if (i >= slots || chosen[i] < 0) continue;
+      const float own = a.scale * v[i] * (g[i] - base);
+      out[chosen[i]] = from_float<T>(kWholeRow ? fmaf(-s[i], others, own) : own * (1.0f - s[i]));
     }
   }
 }
@@ -544,15 +521,11 @@ int backward(const muon_train_route_args& a, const float* grad_weights, void* gr
   Plan plan{};
   plan.whole = a.experts % kRun == 0 && ld % kRun == 0 && aligned16(a.logits) && aligned16(grad);
   unsigned grid = 0;
-  int rc = grid_for(a.tokens, &grid);
-  if (a.score == kSoftmax && !a.renormalize) {
-    const size_t smem = kWarps * a.experts * sizeof(float);
-    if (rc == MUON_POLAR_OK && smem > 40 * 1024) rc = allow_smem<route_backward_kernel<T, kPer, true>>(kMostSmem);
-    if (rc != MUON_POLAR_OK) return rc;
-    return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, smem, 1, false, stream, a, plan,
-                  grad_weights, static_cast<T*>(grad));
-  }
+  const int rc = grid_for(a.tokens, &grid);
   if (rc != MUON_POLAR_OK) return rc;
+  if (a.score == kSoftmax)
+    return launch(route_backward_kernel<T, kPer, true>, dim3(grid), kThreads, 0, 1, false, stream, a, plan,
+                  grad_weights, static_cast<T*>(grad));
   return launch(route_backward_kernel<T, kPer, false>, dim3(grid), kThreads, 0, 1, false, stream, a, plan,
                 grad_weights, static_cast<T*>(grad));
 }

@@ -854,6 +854,54 @@ def test_route_gradient_against_differences(pkg):
             near((grad.double() * d).sum(-1), (total(1e-4) - total(-1e-4)) / 2e-4, 1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("experts, k", [(32, 4), (60, 6), (128, 40), (256, 8), (300, 5), (1024, 64)])
+@pytest.mark.parametrize("spread", [0, 30, 45, 60, 90, 120])
+def test_route_bias_for_vanishing_scores(pkg, experts, k, dtype, spread):
+    """A bias that chooses the k experts `spread` below the others: their weights and
+    gradients are those of s / (sum + 1e-20).  An fp32 score is off by a relative `steps`
+    (an exponent of x carries |x| 2^-23) and, where it is subnormal, by 2^-147: `tiny` after
+    the division by the sum."""
+    x = logits(50, experts, seed=43)
+    bias = torch.zeros(experts, device="cuda")
+    bias[::experts // k][:k] = 4.0
+    x[:, bias > 0] -= spread
+    x = x.to(dtype)
+    leaf = x.clone().requires_grad_(True)
+    weights, indices, _ = pkg.route_experts(leaf, k, bias=bias, scale=1.5)
+    assert torch.equal(indices.sort(-1).values, bias.nonzero().view(1, k).expand(50, k))
+    up = torch.randn(50, k, generator=gen(44), device="cuda")
+    (grad,) = torch.autograd.grad(weights, leaf, up)
+    z = x.double().requires_grad_(True)
+    s = z.softmax(-1)
+    chosen = s.gather(1, indices)
+    total = chosen.sum(-1, keepdim=True) + 1e-20
+    want = 1.5 * chosen / total
+    (ref,) = torch.autograd.grad(want, z, up.double(), retain_graph=True)
+    s, chosen, total, want = (t.detach() for t in (s, chosen, total, want))
+    steps = (96 + 8 * float(x.abs().max()) + k) * E32
+    tiny = 1.5 * 2.0 ** -147 / total
+    near(weights, want, steps * want + tiny)
+    size = up.double().abs()
+    mean = (size * chosen / total).sum(-1, keepdim=True)
+    bound = torch.zeros_like(s).scatter(1, indices, 4 * steps * want * (size + mean) + (2 + k) * tiny * size.amax())
+    # the others' part, and the cancellation of the 64-bit sum that it is compared with
+    bound += s * 1.5 * mean * (4 * steps * 1e-20 / total + 2.0 ** -48) + s * k * tiny * size.amax() * 1e-20 / total
+    near(grad, ref, bound + rounded(ref, dtype) + 2.0 ** -126)
+
+
+def test_route_nan_reaches_the_whole_gradient(pkg):
+    """A NaN logit makes a softmax of its row NaN, though it is not chosen."""
+    for renormalize in (True, False):
+        x = logits(6, 40, seed=45)
+        x[2, 7] = math.nan
+        x.requires_grad_(True)
+        weights, indices, _ = pkg.route_experts(x, 4, renormalize=renormalize)
+        assert not bool((indices[2] == 7).any()) and weights[2].isnan().all()
+        (grad,) = torch.autograd.grad(weights, x, torch.ones_like(weights))
+        assert grad[2].isnan().all() and grad[[0, 1, 3, 4, 5]].isfinite().all()
+
+
 # =========================================================== all of them
 def test_refusals_on_the_device(pkg):
     x = torch.zeros(4, 16, device="cuda")
