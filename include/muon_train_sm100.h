@@ -46,6 +46,11 @@ uint64_t muon_train_launch_count(void);
 #define MUON_TRAIN_STATUS_WAIT 0x1u
 int muon_train_read_device_status(int device, uint32_t* flags, int clear);
 
+/* The limit of these kernels' waits on the current device (the largest, where
+ * a setting was cut short).  muon_polar_set_wait_limit_ns sets it, with that of
+ * the library's other kernels.  Waits for the device's default stream. */
+int muon_train_wait_limit_ns(uint64_t* limit_ns);
+
 /* ---- distillation from a teacher's top logits ------------------------------
  * One row has student logits z[vocab] and a list of `top` teacher logits t
  * with their vocabulary indices i.  An entry counts when 0 <= i < vocab and

@@ -140,6 +140,7 @@ TRAIN_SIGNATURES = {
     "muon_train_launch_count": (ctypes.c_uint64, []),
     "muon_train_read_device_status": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_uint32),
                                                      ctypes.c_int]),
+    "muon_train_wait_limit_ns": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint64)]),
     "muon_train_distill_sm100": (ctypes.c_int, [_DISTILL, _VP]),
     "muon_train_distill_backward_sm100": (ctypes.c_int, [_DISTILL, _VP]),
     "muon_train_residual_norm_sm100": (ctypes.c_int, [_NORM, _VP]),
@@ -222,6 +223,12 @@ class CAPI:
         self._check("muon_train_read_device_status",
                     self.lib.muon_train_read_device_status(int(device), ctypes.byref(flags), int(clear)))
         return int(flags.value)
+
+    def train_wait_limit_ns(self) -> int:
+        """Limit of the training-step kernels' waits (set_wait_limit_ns sets it)."""
+        limit = ctypes.c_uint64(0)
+        self._check("muon_train_wait_limit_ns", self.lib.muon_train_wait_limit_ns(ctypes.byref(limit)))
+        return int(limit.value)
 
     def abi_version(self) -> int:
         return int(self.lib.muon_polar_abi_version())

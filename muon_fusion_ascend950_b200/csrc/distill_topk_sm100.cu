@@ -16,6 +16,13 @@
 namespace muon_train {
 
 cudaError_t norm_status(uint32_t* flags, int clear);  // residual_norm_sm100.cu
+cudaError_t norm_put_wait_limit(uint64_t limit_ns);
+cudaError_t norm_get_wait_limit(uint64_t* limit_ns);
+
+cudaError_t set_wait_limit(uint64_t limit_ns) {  // called by muon_polar_set_wait_limit_ns
+  const cudaError_t e = put_wait_limit(limit_ns);
+  return e != cudaSuccess ? e : norm_put_wait_limit(limit_ns);
+}
 
 std::atomic<uint64_t>& launch_counter() {
   static std::atomic<uint64_t> count{0};
@@ -793,6 +800,16 @@ int muon_train_read_device_status(int device, uint32_t* flags, int clear) {
   if (device != prev) cudaSetDevice(prev);
   if (e != cudaSuccess) return static_cast<int>(e);
   *flags = v;
+  return MUON_POLAR_OK;
+}
+
+int muon_train_wait_limit_ns(uint64_t* limit_ns) {
+  if (limit_ns == nullptr) return MUON_POLAR_ERR_INVALID_ARGUMENT;
+  uint64_t distill = 0, norm = 0;
+  cudaError_t e = muon_train::get_wait_limit(&distill);
+  if (e == cudaSuccess) e = muon_train::norm_get_wait_limit(&norm);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  *limit_ns = distill > norm ? distill : norm;
   return MUON_POLAR_OK;
 }
 

@@ -45,6 +45,10 @@
 #include "muon_polar_sm100.h"
 #include "sm100_ptx.cuh"
 
+namespace muon_train {
+cudaError_t set_wait_limit(uint64_t limit_ns);  // distill_topk_sm100.cu: of the training-step kernels
+}
+
 namespace muon_sm100 {
 
 enum Kind : int { kGramBf16 = 0, kGramF32 = 1, kPoly = 2, kApply = 3, kGramT = 4, kApplyT = 5 };
@@ -3477,6 +3481,7 @@ int muon_polar_set_wait_limit_ns(uint64_t limit_ns, uint64_t* previous) {
   uint64_t old = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&old, g_wait_limit_ns, sizeof(old));
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_wait_limit_ns, &limit_ns, sizeof(limit_ns));
+  if (e == cudaSuccess) e = muon_train::set_wait_limit(limit_ns);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (previous != nullptr) *previous = old;
   return MUON_POLAR_OK;

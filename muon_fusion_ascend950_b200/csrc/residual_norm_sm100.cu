@@ -1337,6 +1337,8 @@ int backward(const Backward& b, const Layout& l, void* stream) {
 }  // namespace
 
 cudaError_t norm_status(uint32_t* flags, int clear) { return take_status(flags, clear); }
+cudaError_t norm_put_wait_limit(uint64_t limit_ns) { return put_wait_limit(limit_ns); }
+cudaError_t norm_get_wait_limit(uint64_t* limit_ns) { return get_wait_limit(limit_ns); }
 
 }  // namespace muon_train
 

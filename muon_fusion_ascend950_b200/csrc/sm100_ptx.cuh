@@ -17,7 +17,7 @@ namespace muon_sm100 {
 // default of two seconds only ever trips on a real deadlock.  The host may
 // change it per device (muon_polar_set_wait_limit_ns), e.g. to make a test's
 // wait on a flag that nothing sets give up quickly.  Each translation unit
-// has its own copy; the one the host sets is muon_polar_sm100.cu's.
+// has its own copy; the host sets those of all that wait.
 constexpr uint64_t kDefaultWaitLimitNs = 2000000000ull;
 static __device__ uint64_t g_wait_limit_ns = kDefaultWaitLimitNs;
 

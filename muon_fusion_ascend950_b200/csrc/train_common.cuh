@@ -293,6 +293,14 @@ static inline cudaError_t take_status(uint32_t* flags, int clear) {
   return e;
 }
 
+// This translation unit's wait limit on the current device.
+static inline cudaError_t put_wait_limit(uint64_t limit_ns) {
+  return cudaMemcpyToSymbol(muon_sm100::g_wait_limit_ns, &limit_ns, sizeof(limit_ns));
+}
+static inline cudaError_t get_wait_limit(uint64_t* limit_ns) {
+  return cudaMemcpyFromSymbol(limit_ns, muon_sm100::g_wait_limit_ns, sizeof(*limit_ns));
+}
+
 // ------------------------------------------------------------ host side
 std::atomic<uint64_t>& launch_counter();
 

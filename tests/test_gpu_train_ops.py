@@ -1044,6 +1044,20 @@ def test_gradients_only_where_they_are_asked_for(pkg):
         out.sum().backward()
 
 
+def test_the_wait_limit_reaches_the_training_kernels(pkg):
+    """The library's one setter holds for every kernel of the library."""
+    from muon_fusion_ascend950_b200.capi import capi
+
+    api = capi()
+    before = api.train_wait_limit_ns()
+    previous = api.set_wait_limit_ns(3_000_000_000)
+    try:
+        assert previous == before and api.train_wait_limit_ns() == 3_000_000_000
+    finally:
+        api.set_wait_limit_ns(previous)
+    assert api.train_wait_limit_ns() == before
+
+
 def test_kernels_are_launched_and_end(pkg):
     from muon_fusion_ascend950_b200.capi import capi
 

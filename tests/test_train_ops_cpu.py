@@ -68,6 +68,10 @@ def test_distill_refuses(lib, bad):
     assert lib.muon_train_distill_sm100(ctypes.byref(args), None) == -1
 
 
+def test_wait_limit_refuses_null(lib):
+    assert lib.muon_train_wait_limit_ns(None) == -1
+
+
 def test_distill_refuses_null_and_backward_needs_stats(lib):
     assert lib.muon_train_distill_sm100(None, None) == -1
     args = _distill(grad=32, ld_grad=8)
