@@ -291,16 +291,56 @@ __device__ __forceinline__ float pair_sum(float2 v) { return v.x + v.y; }
 // shared memory: bulk copies of kArrays tensors' rows into `stages` stages,
 // issued by the warps' first lanes.  A stage is free again once every thread has it in
 // registers, which the barrier of the row's sums tells.
+//
+// If a thread's wait ran out, nothing more is issued from the next barrier on:
+// all issuing lanes find it in failed_in[turn], which like the sums of `turn`
+// is written before the barrier and again only after the next but one, and set
+// the other turn's too.  So a stage is armed only when every thread has seen
+// its copies land, and the rows in flight are the next ones of the ring.
 constexpr int kMaxStages = 16;
 constexpr size_t kRingMost = 222 * 1024;  // bytes of an SM's rings
+struct RingState {
+  uint64_t full[kMaxStages];
+  volatile int failed, failed_in[2];
+  // Kept by thread 0: where in the ring the rows in flight begin, and what
+  // tells how many they are (forward: rows left; backward: row and chunk).
+  volatile int stopped, stage, phase;
+  volatile int64_t row, chunk;
+};
 template <typename T, int N, int kE, int kArrays>
 struct Ring {
-  uint64_t* full;
+  RingState* state;
   T* data;
-  volatile int* failed;
   int stages, stage;
   uint32_t phase;
 
+  // By every thread; each barrier expects `copies` arrivals.
+  __device__ void init(uint32_t copies) const {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) muon_sm100::mbar_init(&state->full[i], copies);
+      state->failed = state->failed_in[0] = state->failed_in[1] = state->stopped = 0;
+      muon_sm100::fence_mbar_init();
+    }
+    __syncthreads();
+  }
+  // For an issuing lane after the barrier that follows the waits of `turn`, for
+  // rows from `back` stages ago on: whether it issues no more.
+  __device__ __forceinline__ bool stopped(int turn, int back, int64_t row, int64_t chunk) const {
+    if (!state->failed_in[turn]) return false;
+    state->failed_in[turn ^ 1] = 1;
+    if (threadIdx.x == 0 && !state->stopped) {
+      state->stopped = 1;
+      state->stage = stage < back ? stage - back + stages : stage - back;
+      state->phase = stage < back ? phase ^ 1 : phase;
+      state->row = row;
+      state->chunk = chunk;
+    }
+    return true;
+  }
+  // By thread 0 if it stopped, with the rows that were left: waits for those in flight.
+  __device__ void drain(int64_t left) const {
+    drain_ring(state->full, stages, state->stage, state->phase, static_cast<int>(left < stages ? left : stages));
+  }
   __device__ T* at(int stage_, int array, int run) const {
     return data + ((stage_ * kArrays + array) * kE / N + run) * static_cast<int>(blockDim.x) * N;
   }
@@ -314,17 +354,19 @@ struct Ring {
 #pragma unroll
     for (int i = 0; i < kE / N; ++i)
       bytes += static_cast<uint32_t>(max(0, min(span, width - (i * place.threads + first) * N))) * sizeof(T);
-    muon_sm100::mbar_arrive_expect_tx(&full[stage_], bytes);
+    muon_sm100::mbar_arrive_expect_tx(&state->full[stage_], bytes);
 #pragma unroll
     for (int i = 0; i < kE / N; ++i) {
       const int c = (i * place.threads + first) * N;
       const int n = min(span, width - c);
       if (n > 0)
         muon_sm100::bulk_load(at(stage_, array, i), from + row * width + c, static_cast<uint32_t>(n) * sizeof(T),
-                              &full[stage_]);
+                              &state->full[stage_]);
     }
   }
-  __device__ void wait() const { ring_wait(&full[stage], phase, failed); }
+  __device__ void wait(int turn) const {
+    if (!ring_wait(&state->full[stage], phase, &state->failed)) state->failed_in[turn] = 1;
+  }
   template <typename P>
   __device__ void read(RowVectors<T, N, kE>& v, int array, int width, const P& place) const {
 #pragma unroll
@@ -358,8 +400,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   constexpr bool kRing = N * sizeof(T) == 16 && kOwner != kWarpRow;
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SumSlots slots;
-  __shared__ uint64_t full[kMaxStages];
-  __shared__ volatile int failed;
+  __shared__ RingState ring_state;
   int turn = 0;
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // every block has begun
   begin_kernel();
@@ -377,7 +418,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   const float inv_width = 1.0f / static_cast<float>(width);
   const T* y_all = static_cast<const T*>(a.block_out);
   const T* x_all = static_cast<const T*>(a.residual);
-  Ring<T, N, kE, 2> ring{full, reinterpret_cast<T*>(dynamic), &failed, stages, 0, 0};
+  Ring<T, N, kE, 2> ring{&ring_state, reinterpret_cast<T*>(dynamic), stages, 0, 0};
   // `rows` rows from `row` on into the stages from `stage` on; a warp's first
   // lane issues every so many of the 2 rows copies, since the next sums wait
   // for the slowest warp
@@ -390,12 +431,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     }
   };
   if constexpr (kRing) {
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < stages; ++i) muon_sm100::mbar_init(&full[i], 2);
-      failed = 0;
-      muon_sm100::fence_mbar_init();
-    }
-    __syncthreads();
+    ring.init(2);
     issue(0, begin, stages);
   }
   Columns<kE> gain, scale, pre;
@@ -420,6 +456,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     // After a barrier that follows the rows' reading: their stages take later ones.
     const auto refill = [&] {
       if constexpr (kRing) {
+        if ((threadIdx.x & 31) != 0 || ring.stopped(turn ^ 1, rows, left, 0)) return;
         const int stage = ring.stage - rows;
         issue(stage < 0 ? stage + stages : stage, first + stages * stride, rows);
       }
@@ -433,7 +470,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
         rx[j].clear();
         if (j < rows) {
           if constexpr (kRing) {
-            ring.wait();
+            ring.wait(turn);
             ring.read(ry[j], 0, width, place);
             ring.read(rx[j], 1, width, place);
             ring.advance();
@@ -488,7 +525,10 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     }
     if (a.pre_weight == nullptr) {
       if (a.post_weight == nullptr) {
-        if constexpr (kRing) __syncthreads();
+        if constexpr (kRing) {
+          __syncthreads();
+          turn ^= 1;
+        }
         refill();
       }
       continue;
@@ -506,6 +546,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       RowVectors<T, N, kE>::store(static_cast<T*>(a.normed) + row * width, place, width, h[j]);
     }
   }
+  if constexpr (kRing)
+    if (threadIdx.x == 0 && ring_state.stopped) ring.drain(ring_state.row);
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed
 }
 
@@ -714,8 +756,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ SumSlots slots;
   __shared__ float columns[kOwner == kWarpRow ? kWarpRowWarps : 1][256];
-  __shared__ uint64_t full[kMaxStages];
-  __shared__ volatile int failed;
+  __shared__ RingState ring_state;
   // whole vectors come through a ring; else the next row is loaded while this
   // one is worked on where registers allow
   constexpr int kPairs = kE / 2;
@@ -750,7 +791,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   rdh.clear();
   rdn.clear();
   float4* const held = reinterpret_cast<float4*>(dynamic);
-  Ring<T, N, kE, 4> ring{full, reinterpret_cast<T*>(dynamic + Hold::kFloats * sizeof(float) * blockDim.x), &failed, stages, 0, 0};
+  Ring<T, N, kE, 4> ring{&ring_state, reinterpret_cast<T*>(dynamic + Hold::kFloats * sizeof(float) * blockDim.x),
+                         stages, 0, 0};
   // Each warp's first lane: the row that goes into the ring next.  It issues
   // every so many of the row's copies, since the next sums wait for the slowest
   // warp.
@@ -769,13 +811,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     ++ahead_row;
   };
   if constexpr (kRing) {
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < stages; ++i)
-        muon_sm100::mbar_init(&full[i], 2 + (dh_all != nullptr) + (dn_all != nullptr));
-      failed = 0;
-      muon_sm100::fence_mbar_init();
-    }
-    __syncthreads();
+    ring.init(2 + (dh_all != nullptr) + (dn_all != nullptr));
     if ((threadIdx.x & 31) == 0 && threadIdx.x < 4 * 32)
       for (int i = 0; i < stages; ++i) issue_next(i);
   }
@@ -851,7 +887,7 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
     load_rstd(r0 + first);
     for (int64_t row = r0 + first; row < r1; row += step) {
       if constexpr (kRing) {
-        ring.wait();
+        ring.wait(turn);
         ring.read(ry, 0, width, place);
         ring.read(rx, 1, width, place);
         if (dh_all != nullptr) ring.read(rdh, 2, width, place);
@@ -893,7 +929,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       float sums[4] = {pair_sum(s0), pair_sum(s1), pair_sum(s2), 0.f};
       row_sums<kOwner>(sums, slots, turn);
       if constexpr (kRing) {  // every thread has the row in registers
-        if ((threadIdx.x & 31) == 0 && threadIdx.x < 4 * 32) issue_next(ring.stage);
+        if ((threadIdx.x & 31) == 0 && threadIdx.x < 4 * 32 && !ring.stopped(turn ^ 1, 0, row, chunk))
+          issue_next(ring.stage);
         ring.advance();
       }
       const float k = rh * (sums[0] * inv_width);
@@ -976,6 +1013,16 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       store_columns(b.scale + worker * width, v);
     } else {  // one value of each block
       store_block_sum(sum_scale_one, reinterpret_cast<double*>(b.scale) + blockIdx.x);
+    }
+  }
+  if constexpr (kRing) {
+    if (threadIdx.x == 0 && ring_state.stopped) {
+      int64_t left = 0, from, to, group;
+      for (int64_t chunk = ring_state.chunk; chunk < b.plan.chunks && left < stages; chunk += workers) {
+        chunk_rows(b, chunk, &from, &to, &group);
+        left += to - (chunk == ring_state.chunk ? ring_state.row : from);
+      }
+      ring.drain(left);
     }
   }
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed

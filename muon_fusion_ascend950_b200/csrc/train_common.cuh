@@ -265,20 +265,42 @@ __device__ __forceinline__ float warp_max(float v) {
 // Each translation unit has its own status word; the read call joins them.
 static __device__ uint32_t g_status = 0;
 
-// Waits for the phase of `bar`; gives up after the wait limit, or once another
-// thread of the block has: the block then runs on without waiting, and the
-// device status tells.
-__device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  if (muon_sm100::mbar_try_wait(bar, parity)) return;
+// Waits for the phase of `bar`; false if it gave up after the wait limit, or
+// (unless `alone`) once another thread of the block has.  The device status
+// then tells, and the block runs on without waiting: its results are void.
+// What it gave up on may still be in flight, so its barrier must not be armed
+// again, and the block waits for it (drain_ring) before it ends.
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed,
+                                          bool alone = false) {
+  if (muon_sm100::mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = muon_sm100::global_timer_ns();
-  for (uint32_t spins = 1;; ++spins) {
-    if (muon_sm100::mbar_try_wait(bar, parity)) return;
-    if ((spins & 63u) != 0) continue;
-    if (*failed) return;
-    if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
-      *failed = 1;
-      atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
-      return;
+  for (uint32_t spins = 0;; ++spins) {
+    if ((spins & 63u) == 0) {
+      if (!alone && *failed) return false;
+      if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
+        *failed = 1;
+        atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
+        return false;
+      }
+    }
+    if (muon_sm100::mbar_try_wait(bar, parity)) return true;
+  }
+}
+
+// After a wait was given up: waits for what is in flight to `n` barriers in a
+// row of a ring, from its `stage` with `parity` on, whatever the limit of the
+// other waits is set to.
+__device__ __forceinline__ void drain_ring(uint64_t* bars, int stages, int stage, uint32_t parity, int n) {
+  const uint64_t t0 = muon_sm100::global_timer_ns();
+  while (n > 0) {
+    if (!muon_sm100::mbar_try_wait(&bars[stage], parity)) {
+      if (muon_sm100::global_timer_ns() - t0 > muon_sm100::kDefaultWaitLimitNs) return;
+      continue;
+    }
+    --n;
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
     }
   }
 }
