@@ -344,6 +344,12 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 4)
 // one is worked on, and while one block waits for its sums the other one of
 // the SM computes.
 //
+// Where a wait runs out, no barrier is armed while copies to it are in flight,
+// and none are in flight when the block ends: a consumer warp that gave a stage
+// up releases none any more, so that the producer refills only stages that all
+// have seen land, and comes to a stop; at its end it waits for what it issued.
+// A list warp that gave up neither expects nor sends any more.
+//
 // Measured for the loss with its gradient, 4096 x 131072 bf16 (333 us at the
 // copy rate): rows in registers of 8-block clusters 783 us (4 blocks an SM
 // 616), slices held in the ring between the passes 504 us, streamed twice
@@ -444,10 +450,15 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
   // block sends its part to every block, and goes on to the next row only
   // after it has heard all of them: so no block is ever more than one row ahead
   // of another, and two slots are enough.
+  bool deaf = false;  // it gave up, at this turn
+  uint32_t deaf_turn = 0;
+  const auto drain_heard = [&] {
+    if (lane == 0) drain_ring(&heard[deaf_turn & 1], 1, 0, (deaf_turn >> 1) & 1, 1);
+  };
   const auto statistics = [&](uint32_t turn) {
     const uint32_t slot = turn & 1;
     float2 v = warp_join(lane < kConsumerWarps ? warp_part[slot][lane] : make_float2(-INFINITY, 0.f), c);
-    if (parts > 1) {
+    if (parts > 1 && !deaf) {
       if (lane == 0) mbar_arrive_expect_tx(&heard[slot], static_cast<uint32_t>(parts * sizeof(float2)));
       __syncwarp();
       if (lane < parts) {
@@ -457,7 +468,11 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
                 map_to_cta(smem_addr(&block_part[slot][part]), peer)),
             "f"(v.x), "f"(v.y), "r"(map_to_cta(smem_addr(&heard[slot]), peer)) : "memory");
       }
-      ring_wait(&heard[slot], (turn >> 1) & 1, &failed);
+      deaf = !__all_sync(kFullMask, ring_wait(&heard[slot], (turn >> 1) & 1, &failed, /*alone=*/true));
+      if (deaf) {  // by the time that this takes, what it sent has landed
+        deaf_turn = turn;
+        drain_heard();
+      }
       v = block_part[slot][0];
       for (int i = 1; i < parts; ++i) v = join(v, block_part[slot][i], c);
     }
@@ -471,17 +486,18 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
       asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
       asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(drop));
     }
-    for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers) {
+    bool stopped = false;
+    for (int64_t row = blockIdx.x / parts; row < a.rows && !stopped; row += workers) {
       const Slice<T> slice(a, ring.cut, row, part);
-      for (int pass = 0; pass < (kMode == kLossGrad ? 2 : 1); ++pass)
+      for (int pass = 0; pass < (kMode == kLossGrad ? 2 : 1) && !stopped; ++pass)
       for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
         const int g1 = min(slice.last, g0 + kStageGranules);
         // whole granules [lo, hi); at most one more at either end of the row
         const int lo = g0 * kN < slice.shift ? g0 + 1 : g0;
         const int hi = g1 * kN - slice.shift > vocab ? g1 - 1 : g1;
         uint8_t* to = dynamic + stage * kStageBytes;
-        if (lane == 0) ring_wait(&empty[stage], phase ^ 1, &failed);
-        __syncwarp();
+        stopped = __any_sync(kFullMask, lane == 0 && !ring_wait(&empty[stage], phase ^ 1, &failed));
+        if (stopped) break;
         if (lane < 2 * kN) {
           const bool left = lane < kN;
           const int granule = left ? g0 : g1 - 1, j = lane % kN;
@@ -506,6 +522,8 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
         advance();
       }
     }
+    // the stages' last fillings, from the oldest on: the consumers may have given them up
+    if (lane == 0) drain_ring(full, stages, stage, phase ^ 1, stages);
   } else if (warp == kConsumerWarps + 1) {  // lists
     uint32_t turn = 0;
     for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers, ++turn) {
@@ -545,6 +563,7 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
     const float2 cc = make_float2(c, c);
     const int tid = static_cast<int>(threadIdx.x);
     uint32_t turn = 0;
+    bool lost = false;  // gave a stage up
     for (int64_t row = blockIdx.x / parts; row < a.rows; row += workers, ++turn) {
       const Slice<T> slice(a, ring.cut, row, part);
       uint4 u[kPerStage];
@@ -552,15 +571,18 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
       const auto read = [&](int i) {
         return *reinterpret_cast<const uint4*>(dynamic + stage * kStageBytes + at(i) * 16);
       };
+      const auto wait = [&] {
+        if (!lost) lost = !ring_wait(&full[stage], phase, &failed);
+      };
       const auto release = [&] {
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[stage]);
+        if (lane == 0 && !lost) mbar_arrive(&empty[stage]);
       };
       if constexpr (kMode != kGradFromStats) {
         float m = -INFINITY;
         float2 s = make_float2(0.f, 0.f);
         for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
-          ring_wait(&full[stage], phase, &failed);
+          wait();
           // past the slice's end: -inf
           if (g0 + kStageGranules <= slice.last) {
 #pragma unroll
@@ -609,7 +631,7 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
         const float2 scale2 = make_float2(p_scale, p_scale), minus_max = make_float2(-v.x, -v.x);
         T* dz = static_cast<T*>(a.grad) + row * a.ld_grad;
         for (int g0 = slice.first; g0 < slice.last; g0 += kStageGranules) {
-          ring_wait(&full[stage], phase, &failed);
+          wait();
           const int element0 = g0 * kN - slice.shift;
           if (ring.cut.same_phase && !none && g0 + kStageGranules <= slice.last && element0 >= 0 &&
               element0 + kStageGranules * kN <= vocab) {  // whole vectors throughout
@@ -666,7 +688,10 @@ __global__ void __launch_bounds__(kConsumers + 64, kBlocksPerSm)
     }
   }
   __syncwarp();
-  if (parts > 1) cluster_sync();  // no block leaves while another may still write to it
+  if (parts > 1) {
+    cluster_sync();  // no block leaves while another may still write to it
+    if (deaf) drain_heard();
+  }
 }
 
 // ------------------------------------------------------------ host side

@@ -274,22 +274,21 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volati
                                           bool alone = false) {
   if (muon_sm100::mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = muon_sm100::global_timer_ns();
-  for (uint32_t spins = 0;; ++spins) {
-    if ((spins & 63u) == 0) {
-      if (!alone && *failed) return false;
-      if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
-        *failed = 1;
-        atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
-        return false;
-      }
-    }
+  for (uint32_t spins = 1;; ++spins) {
     if (muon_sm100::mbar_try_wait(bar, parity)) return true;
+    if (!alone && *failed) return false;
+    if ((spins & 63u) != 0) continue;
+    if (muon_sm100::global_timer_ns() - t0 > muon_sm100::g_wait_limit_ns) {
+      *failed = 1;
+      atomicOr(&g_status, MUON_TRAIN_STATUS_WAIT);
+      return false;
+    }
   }
 }
 
-// After a wait was given up: waits for what is in flight to `n` barriers in a
-// row of a ring, from its `stage` with `parity` on, whatever the limit of the
-// other waits is set to.
+// Before a block ends: waits for what is in flight to `n` barriers in a row of a
+// ring, from its `stage` with `parity` on, whatever the limit of the other waits
+// is set to.
 __device__ __forceinline__ void drain_ring(uint64_t* bars, int stages, int stage, uint32_t parity, int n) {
   const uint64_t t0 = muon_sm100::global_timer_ns();
   while (n > 0) {

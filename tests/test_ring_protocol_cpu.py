@@ -101,3 +101,62 @@ def test_norm_ring(rows, stages, threads):
 def test_norm_ring_that_goes_on_issuing_is_caught():
     with pytest.raises(AssertionError, match="in flight"):
         norm_ring(5, 2, 2, mended=False)
+
+
+def distill_ring(uses, stages, warps, mended):
+    """A producer fills stages that all consumer warps have released; each warp
+    waits for a stage and releases it."""
+
+    def moves(state):
+        made, stopped, drained, at, lost, full, empty, failed = state
+        if drained and all(u == uses for u in at):
+            assert not any(bar[2] for bar in full), "the block ended with copies in flight"
+            return
+        for s, bar in enumerate(full):
+            if bar[2]:
+                yield made, stopped, drained, at, lost, put(full, s, land(bar, 1)), empty, failed
+        if made < uses and not stopped:
+            s, round_ = made % stages, made // stages
+            if waited(empty[s], round_ - 1):
+                phase, arrived, flight = full[s]
+                assert phase == round_ and arrived == 0, "armed while copies are in flight"
+                yield made + 1, stopped, drained, at, lost, put(full, s, (phase, 1, flight + 1)), empty, failed
+            elif mended:
+                yield made, True, drained, at, lost, full, empty, True
+            else:
+                phase, arrived, flight = full[s]
+                assert phase == round_ and arrived == 0, "armed while copies are in flight"
+                yield made + 1, stopped, drained, at, lost, put(full, s, (phase, 1, flight + 1)), empty, True
+        elif not drained:
+            if not mended or all(full[u % stages][0] > u // stages for u in range(max(0, made - stages), made)):
+                yield made, stopped, True, at, lost, full, empty, failed
+        for w, use in enumerate(at):
+            if use == uses:
+                continue
+            s = use % stages
+            there, gave_up = put(at, w, use + 1), put(lost, w, True)
+            phase, arrived, _ = empty[s]
+            freed = put(empty, s, (phase + 1, 0, 0) if arrived + 1 == warps else (phase, arrived + 1, 0))
+            if mended and lost[w]:
+                yield made, stopped, drained, there, lost, full, empty, failed
+            elif waited(full[s], use // stages):
+                yield made, stopped, drained, there, lost, full, freed, failed
+            else:
+                yield made, stopped, drained, there, gave_up, full, empty if mended else freed, True
+
+    def ended(state):
+        assert state[2] and all(u == uses for u in state[3]), "a warp waits for good"
+
+    idle = ((0, 0, 0),) * stages
+    return explore((0, False, False, (0,) * warps, (False,) * warps, idle, idle, False), moves, ended)
+
+
+@pytest.mark.parametrize("uses, stages, warps", [(1, 2, 2), (4, 1, 2), (5, 2, 2), (7, 3, 2), (5, 2, 3)])
+def test_distill_ring(uses, stages, warps):
+    states, ends = distill_ring(uses, stages, warps, mended=True)
+    assert states > 10 and ends >= 1
+
+
+def test_distill_ring_that_goes_on_issuing_is_caught():
+    with pytest.raises(AssertionError, match="in flight"):
+        distill_ring(5, 2, 2, mended=False)
