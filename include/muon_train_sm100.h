@@ -42,7 +42,8 @@ uint64_t muon_train_launch_count(void);
 
 /* Device status word (zero: no trouble).  Every wait inside a kernel is
  * bounded; a kernel that gives up a wait sets a bit here, runs on without
- * waiting and returns, its results void.  Synchronises the device. */
+ * waiting and returns, its results void.  Synchronises the device.  The PyTorch
+ * operators read it after each call when MUON_POLAR_DEBUG_SYNC is set. */
 #define MUON_TRAIN_STATUS_WAIT 0x1u
 int muon_train_read_device_status(int device, uint32_t* flags, int clear);
 

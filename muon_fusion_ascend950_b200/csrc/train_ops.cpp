@@ -4,6 +4,7 @@
 // (include/muon_train_sm100.h); gradients on the Autograd key.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -13,6 +14,7 @@
 
 #include <array>
 #include <cmath>
+#include <cstdlib>
 #include <optional>
 #include <tuple>
 
@@ -25,9 +27,17 @@ using OptTensor = std::optional<Tensor>;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
+// Of a launch on the current device.  With MUON_POLAR_DEBUG_SYNC set (read on
+// every call) it also synchronises, and raises if a wait of a kernel ran out.
 void CheckStatus(int rc, const char* who) {
   TORCH_CHECK(rc == MUON_POLAR_OK, who, " failed, status=", rc,
               ", detail=", muon_polar_status_string(rc));
+  if (std::getenv("MUON_POLAR_DEBUG_SYNC") == nullptr) return;
+  uint32_t flags = 0;
+  const int read = muon_train_read_device_status(c10::cuda::current_device(), &flags, /*clear=*/1);
+  TORCH_CHECK(read == MUON_POLAR_OK, who, " failed, status=", read,
+              ", detail=", muon_polar_status_string(read));
+  TORCH_CHECK(flags == 0, who, " gave up on a bounded wait, status word=", flags);
 }
 
 int Dtype(const Tensor& t, const char* who, const char* name) {

@@ -1058,6 +1058,31 @@ def test_the_wait_limit_reaches_the_training_kernels(pkg):
     assert api.train_wait_limit_ns() == before
 
 
+def test_debug_sync_waits_for_every_call(pkg, monkeypatch):
+    """With MUON_POLAR_DEBUG_SYNC set each call, forward and backward, returns
+    only when its kernels have ended and their status word has been read."""
+    z, t, i, w = distill_inputs(4, 64, 3, torch.bfloat16, seed=47)
+    v, dh, dn = norm_inputs((4, 64), torch.bfloat16, torch.float32, (), 1, seed=47)
+    y, up = [v[n] for n in NAMES], torch.ones(4, 2, device="cuda")
+    ops = torch.ops.muon_ascend950
+    stats, rstd = ops.distill_topk(z, t, i, None, 1.0)[1], ops.residual_norm(*y, 1e-6)[2]
+    chosen = ops.route_experts(z, None, 2, 0, 1, 1, 1, True, 1.0)[1]
+    calls = [lambda: ops.distill_topk(z, t, i, None, 1.0), lambda: ops.distill_topk_grad(z, t, i, w, None, 1.0),
+             lambda: ops.distill_topk_backward(w, z, t, i, None, stats, 1.0), lambda: ops.residual_norm(*y, 1e-6),
+             lambda: ops.residual_norm_backward(dh, dn, *y, rstd, 1e-6, [True] * 6),
+             lambda: ops.route_experts(z, None, 2, 0, 1, 1, 1, True, 1.0),
+             lambda: ops.route_experts_backward(up, z, chosen, 0, True, 1.0)]
+    for sync in (False, True):
+        if sync:
+            monkeypatch.setenv("MUON_POLAR_DEBUG_SYNC", "1")
+        for call in calls:
+            call()
+            torch.cuda.synchronize()
+            torch.cuda._sleep(100_000_000)  # some 50 ms before the call's kernels
+            call()
+            assert torch.cuda.current_stream().query() == sync
+
+
 def test_kernels_are_launched_and_end(pkg):
     from muon_fusion_ascend950_b200.capi import capi
 
