@@ -103,7 +103,7 @@ def load_library() -> None:
     def fake_route_experts(logits, bias, k, score, groups, top_groups, group_top, renormalize, scale):
         from .training import check_route
 
-        check_route(logits, bias, k, groups, top_groups)
+        check_route(logits, bias, k, score, groups, top_groups, group_top, scale)
         shape = (*logits.shape[:-1], k)
         return (logits.new_empty(shape, dtype=torch.float32),
                 logits.new_empty(shape, dtype=torch.int64),

@@ -16,11 +16,15 @@ take part in autograd (gradients of gradients are refused).
 """
 from __future__ import annotations
 
+import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+# muon_train_sm100.h: MUON_TRAIN_MAX_TOP, _MAX_EXPERTS, _MAX_ROUTES
+MAX_TOP, MAX_EXPERTS, MAX_ROUTES = 1024, 1024, 64
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _OPTIONAL = frozenset(("teacher_lse", "row_scale", "post_weight", "pre_weight", "gate", "residual_scale",
                        "bias"))
@@ -30,13 +34,29 @@ _residual_norm = torch.ops.muon_ascend950.residual_norm.default
 _route_experts = torch.ops.muon_ascend950.route_experts.default
 
 
-def _check(name: str, t, floats: bool = True) -> None:
+def _check(name: str, t, like: Optional[torch.Tensor] = None, *, floats: bool = True) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
     if floats and t.dtype not in _FLOATS:
         raise TypeError(f"{name} must use torch.float32, bfloat16 or float16, got {t.dtype}")
+
+
+def _check_values(name: str, t, like: torch.Tensor, shape) -> None:
+    """Values that are converted to fp32: of any floating type."""
+    _check(name, t, like, floats=False)
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_floating_point():
+        raise TypeError(f"{name} must be a floating tensor, got {t.dtype}")
+
+
+def _float32(value: float) -> float:
+    """`value` rounded to fp32, infinite beyond it."""
+    return ctypes.c_float(value).value
 
 
 # The native operators check their arguments themselves.  Only when a call has
@@ -56,8 +76,8 @@ def _explain(**named) -> None:
 # ------------------------------------------------- checks of traced calls
 def check_distill(student_logits, teacher_logits, teacher_indices, temperature, **rows) -> None:
     _check("student_logits", student_logits)
-    _check("teacher_logits", teacher_logits)
-    _check("teacher_indices", teacher_indices, floats=False)
+    _check("teacher_logits", teacher_logits, student_logits)
+    _check("teacher_indices", teacher_indices, student_logits, floats=False)
     if teacher_indices.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"teacher_indices must use torch.int64 or int32, got {teacher_indices.dtype}")
     if student_logits.ndim < 1 or student_logits.shape[-1] < 1:
@@ -68,13 +88,14 @@ def check_distill(student_logits, teacher_logits, teacher_indices, temperature, 
         raise ValueError("teacher_logits and teacher_indices must both have shape "
                          f"{tuple(lead) + ('top',)}, got {tuple(teacher_logits.shape)} and "
                          f"{tuple(teacher_indices.shape)}")
-    if not temperature > 0.0:
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 1 <= teacher_logits.shape[-1] <= MAX_TOP:
+        raise ValueError(f"a list must have 1 to {MAX_TOP} entries, got {teacher_logits.shape[-1]}")
+    tau = _float32(temperature)
+    if not (tau > 0.0 and math.isfinite(tau)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
     for name, t in rows.items():
         if t is not None:
-            _check(name, t)
-            if t.shape != lead:
-                raise ValueError(f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+            _check_values(name, t, student_logits, lead)
 
 
 def gate_rows(gate: torch.Tensor, shape: torch.Size) -> int:
@@ -96,7 +117,7 @@ def gate_rows(gate: torch.Tensor, shape: torch.Size) -> int:
 
 def check_norm(block_out, residual, post_weight, pre_weight, gate, residual_scale, eps) -> None:
     _check("block_out", block_out)
-    _check("residual", residual)
+    _check("residual", residual, block_out)
     if residual.dtype != block_out.dtype:
         raise TypeError(f"residual must use block_out's {block_out.dtype}, got {residual.dtype}")
     shape = block_out.shape
@@ -107,35 +128,41 @@ def check_norm(block_out, residual, post_weight, pre_weight, gate, residual_scal
     width = shape[-1]
     for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
         if w is not None:
-            _check(name, w)
+            _check(name, w, block_out)
             if w.shape != (width,):
                 raise ValueError(f"{name} must have shape ({width},), got {tuple(w.shape)}")
     if gate is not None:
-        _check("gate", gate)
+        _check("gate", gate, block_out)
         gate_rows(gate, shape)
     if residual_scale is not None:
-        _check("residual_scale", residual_scale)
+        _check("residual_scale", residual_scale, block_out)
         if residual_scale.numel() != 1 and residual_scale.shape != (width,):
             raise ValueError(f"residual_scale must have one element or shape ({width},), "
                              f"got {tuple(residual_scale.shape)}")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
 
 
-def check_route(logits, bias, k, groups, top_groups) -> None:
+def check_route(logits, bias, k, score, groups, top_groups, group_top, scale) -> None:
     _check("logits", logits)
     if logits.ndim < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must have shape [..., experts], got {tuple(logits.shape)}")
     experts = logits.shape[-1]
+    if experts > MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts are supported, got {experts}")
+    if score not in (0, 1):
+        raise ValueError("score must be 0 (softmax) or 1 (sigmoid)")
     if bias is not None:
-        _check("bias", bias)
-        if bias.shape != (experts,):
-            raise ValueError(f"bias must have shape ({experts},), got {tuple(bias.shape)}")
+        _check_values("bias", bias, logits, (experts,))
     if groups < 1 or experts % groups or not 1 <= top_groups <= groups:
         raise ValueError(f"groups must divide the {experts} experts and top_groups be 1 to groups, "
                          f"got {groups} and {top_groups}")
-    if not 1 <= k <= top_groups * (experts // groups):
-        raise ValueError(f"k must be 1 to the experts of the chosen groups, got {k}")
+    if group_top != 1 and (group_top != 2 or (groups > 1 and experts // groups < 2)):
+        raise ValueError(f"group_top must be 1, or 2 with groups of two experts or more, got {group_top}")
+    if not 1 <= k <= min(MAX_ROUTES, top_groups * (experts // groups)):
+        raise ValueError(f"k must be 1 to {MAX_ROUTES} and at most the experts of the chosen groups, got {k}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
 
 
 # -------------------------------------------------------------- entry points

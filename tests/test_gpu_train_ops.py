@@ -14,6 +14,8 @@ import math
 import pytest
 import torch
 
+from train_calls import CALLS
+
 pytestmark = pytest.mark.gpu
 
 U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
@@ -922,6 +924,16 @@ def test_refusals_on_the_device(pkg):
             pkg.route_experts(x, **kw)
     with pytest.raises(ValueError):
         pkg.route_experts(torch.zeros(1, 1025, device="cuda"), 1)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_calls_are_taken_and_refused(pkg, name):
+    call, error = CALLS[name]
+    if error is None:
+        call()
+    else:
+        with pytest.raises(error):
+            call()
 
 
 def test_gradients_of_gradients_are_refused(pkg):

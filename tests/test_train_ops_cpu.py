@@ -23,6 +23,8 @@ from muon_fusion_ascend950_b200.capi import (
     RouteArgs,
 )
 
+from train_calls import CALLS
+
 REPO = Path(__file__).resolve().parent.parent
 HEADER = REPO / "include" / "muon_train_sm100.h"
 
@@ -232,6 +234,25 @@ def test_forward_mode_is_refused(name):
             with forward_ad.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
                 dual = forward_ad.make_dual(inputs[at], torch.ones_like(inputs[at]))
                 call(*inputs[:at], dual, *inputs[at + 1:])
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_traced_calls_are_taken_and_refused(name):
+    """As test_gpu_train_ops.py asks of the native operators."""
+    call, error = CALLS[name]
+    with _fake():
+        if error is None:
+            call()
+        else:
+            with pytest.raises(error):
+                call()
+
+
+def test_limits_are_the_headers():
+    from muon_fusion_ascend950_b200 import training
+
+    for name, value in (("TOP", training.MAX_TOP), ("EXPERTS", training.MAX_EXPERTS), ("ROUTES", training.MAX_ROUTES)):
+        assert int(re.search(rf"#define MUON_TRAIN_MAX_{name} (\d+)", HEADER.read_text()).group(1)) == value
 
 
 def test_gate_rows_of_every_shape():
