@@ -269,9 +269,10 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax",
     int64 ``[experts]``, how many tokens each expert got.  Differentiable in
     ``logits`` through the weights.
     """
-    if group_top is None:
-        group_top = 2 if groups > 1 and score == "sigmoid" and groups < logits.shape[-1] else 1
     try:
+        if group_top is None:
+            pairs = groups > 1 and score == "sigmoid" and logits.ndim > 0 and groups < logits.shape[-1]
+            group_top = 2 if pairs else 1
         return _route_experts(logits, bias, k, _SCORES[score], groups, top_groups, group_top, renormalize, scale)
     except Exception:
         if score not in _SCORES:

@@ -153,6 +153,15 @@ def test_entry_points_refuse_cpu_tensors_and_wrong_types():
         pkg.route_experts(None, 2)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(groups=2), dict(groups=2, score="sigmoid")])
+def test_route_refuses_what_is_no_tensor(kw):
+    for logits in ([[0.0] * 4], None, 3):
+        with pytest.raises(TypeError, match="logits must be a torch.Tensor"):
+            pkg.route_experts(logits, 2, **kw)
+    with _fake(), pytest.raises(ValueError):
+        pkg.route_experts(_cuda(), 1, **kw)
+
+
 def _fake():
     from torch._subclasses.fake_tensor import FakeTensorMode
 
