@@ -77,7 +77,7 @@ typedef struct {
   void* grad;                  /* [rows][ld_grad], element type dtype */
   int64_t ld_grad;
   int64_t top;                 /* 1 .. MUON_TRAIN_MAX_TOP */
-  float temperature;           /* > 0 */
+  float temperature;           /* >= 2^-126: its reciprocal is taken */
   int dtype, teacher_dtype;    /* MUON_TRAIN_* */
   int index_bytes;             /* 4 or 8 */
 } muon_train_distill_args;

@@ -9,6 +9,7 @@
 // Bound by memory: the vocabulary is read once (and the gradient written
 // once); the lists are a thousandth of it.
 #include <algorithm>
+#include <cfloat>
 
 #include "sm100_ptx.cuh"
 #include "train_common.cuh"
@@ -783,7 +784,7 @@ int run(const muon_train_distill_args& a, Mode mode, void* stream) {
 
 int check(const muon_train_distill_args* a) {
   if (a == nullptr || a->rows < 0 || a->vocab < 1 || a->top < 1 || a->top > MUON_TRAIN_MAX_TOP ||
-      a->rows > 0x7fffffff / 8 || a->vocab > 0x7fffff00 || !(a->temperature > 0.f) ||
+      a->rows > 0x7fffffff / 8 || a->vocab > 0x7fffff00 || !(a->temperature >= FLT_MIN) ||
       (a->rows > 1 && a->ld < a->vocab) || !valid_dtype(a->dtype) ||
       !valid_dtype(a->teacher_dtype) || (a->index_bytes != 4 && a->index_bytes != 8))
     return MUON_POLAR_ERR_INVALID_ARGUMENT;

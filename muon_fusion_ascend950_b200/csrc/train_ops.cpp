@@ -13,6 +13,7 @@
 #include <torch/library.h>
 
 #include <array>
+#include <cfloat>
 #include <cmath>
 #include <cstdlib>
 #include <optional>
@@ -144,8 +145,8 @@ DistillInputs CheckDistill(const Tensor& student, const Tensor& values, const Te
   CheckDevice(indices, student, who, "teacher_indices");
   TORCH_CHECK_TYPE(indices.scalar_type() == at::kLong || indices.scalar_type() == at::kInt, who,
                    ": teacher_indices must be int64 or int32, got ", indices.scalar_type());
-  TORCH_CHECK_VALUE(static_cast<float>(temperature) > 0.f && std::isfinite(static_cast<float>(temperature)), who,
-                    ": temperature must be positive and finite, got ", temperature);
+  TORCH_CHECK_VALUE(static_cast<float>(temperature) >= FLT_MIN && std::isfinite(static_cast<float>(temperature)), who,
+                    ": temperature must be positive (2^-126 or more) and finite, got ", temperature);
   DistillInputs in;
   in.args.dtype = Dtype(student, who, "student_logits");
   in.args.teacher_dtype = Dtype(values, who, "teacher_logits");

@@ -91,8 +91,8 @@ def check_distill(student_logits, teacher_logits, teacher_indices, temperature, 
     if not 1 <= teacher_logits.shape[-1] <= MAX_TOP:
         raise ValueError(f"a list must have 1 to {MAX_TOP} entries, got {teacher_logits.shape[-1]}")
     tau = _float32(temperature)
-    if not (tau > 0.0 and math.isfinite(tau)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not (tau >= 2.0 ** -126 and math.isfinite(tau)):
+        raise ValueError(f"temperature must be positive (2^-126 or more) and finite, got {temperature}")
     for name, t in rows.items():
         if t is not None:
             _check_values(name, t, student_logits, lead)

@@ -283,6 +283,17 @@ def test_distill_zero_scale_gives_zero_gradient(pkg):
     assert bool((grad[1] == 0).all()) and grad.isfinite().all()
 
 
+def test_distill_least_temperature(pkg):
+    """All probability on the largest logit and entry: the loss of a row whose
+    largest entry is its largest logit is 0, and no value is NaN."""
+    z, t, i, w = distill_inputs(5, 700, 6, torch.float32, seed=48)
+    z[:3] = z[:3].scatter(1, i[:3].gather(1, t[:3].argmax(-1, keepdim=True)), 100.0)
+    tau = 2.0 ** -126
+    loss, grad = pkg.distill_topk_grad(z, t, i, torch.zeros_like(w).fill_(tau), temperature=tau)
+    assert bool((loss[:3] == 0).all()) and bool((loss[3:] == math.inf).all())
+    assert int(grad[:3].count_nonzero()) == 0 and grad.isfinite().all()
+
+
 def test_distill_no_rows(pkg):
     z = torch.empty(0, 100, device="cuda", requires_grad=True)
     t, i = torch.empty(0, 4, device="cuda"), torch.empty(0, 4, dtype=torch.int64, device="cuda")

@@ -70,6 +70,11 @@ def test_distill_refuses(lib, bad):
     assert lib.muon_train_distill_sm100(ctypes.byref(args), None) == -1
 
 
+def test_distill_refuses_a_temperature_without_a_reciprocal(lib):
+    assert lib.muon_train_distill_sm100(ctypes.byref(_distill(rows=0, temperature=2.0 ** -127)), None) == -1
+    assert lib.muon_train_distill_sm100(ctypes.byref(_distill(rows=0, temperature=2.0 ** -126)), None) == 0
+
+
 def test_wait_limit_refuses_null(lib):
     assert lib.muon_train_wait_limit_ns(None) == -1
 

@@ -51,6 +51,8 @@ for op in ("distill_topk", "distill_topk_grad"):
             ("infinite temperature", lambda: dict(temperature=math.inf), ValueError),
             ("temperature beyond fp32", lambda: dict(temperature=1e39), ValueError),
             ("temperature below fp32", lambda: dict(temperature=1e-50), ValueError),
+            ("least temperature", lambda: dict(temperature=2.0 ** -126), None),
+            ("subnormal temperature", lambda: dict(temperature=2.0 ** -127), ValueError),
             ("no temperature", lambda: dict(temperature=math.nan), ValueError),
             ("normaliser of fp64", lambda: dict(lse=make(4, dtype=F64)), None),
             ("normaliser of bf16", lambda: dict(lse=make(4, dtype=BF16)), None),
