@@ -12,7 +12,7 @@
 
 Both land next to this file so that they travel with the source tree.  Each
 source compiles to an object under ``_build/`` (all in parallel); what is newer
-than every input is not built again.  Run with
+than every input is not built again, a library without its objects included.  Run with
 ``python -m muon_fusion_ascend950_b200.build`` (``--force`` to rebuild).
 """
 from __future__ import annotations
@@ -70,16 +70,24 @@ OP_SOURCES = {
 }
 
 
+def _inputs(name: str, headers) -> list:
+    return [CSRC / name, Path(__file__)] + [CSRC / h if h.endswith(".cuh") else INCLUDE / h for h in headers]
+
+
+def _up_to_date(out: Path, sources: dict, *more) -> bool:
+    """Whether `out` is newer than every source and header; its objects need not
+    be there, so that a library that came with the tree is not built again."""
+    return _newer(out, [*more, *(i for name, headers in sources.items() for i in _inputs(name, headers))])
+
+
 def _compile(sources: dict, command, force: bool) -> list:
     """Objects of `sources` by `command`, those that are out of date in parallel."""
     BUILD.mkdir(exist_ok=True)
     objects, todo = [], []
     for name, headers in sources.items():
         obj = BUILD / (name + ".o")
-        inputs = [CSRC / name, Path(__file__)]
-        inputs += [CSRC / h if h.endswith(".cuh") else INCLUDE / h for h in headers]
         objects.append(obj)
-        if force or not _newer(obj, inputs):
+        if force or not _newer(obj, _inputs(name, headers)):
             todo.append([*command, "-c", CSRC / name, "-o", obj])
     with ThreadPoolExecutor(max_workers=len(sources)) as pool:
         list(pool.map(_run, todo))
@@ -89,6 +97,8 @@ def _compile(sources: dict, command, force: bool) -> list:
 def build_library(force: bool = False, verbose_ptxas: bool = False) -> Path:
     """nvcc -> libmuon_polar_sm100.so (kernels + C ABI)."""
     out = PKG / LIB_NAME
+    if not force and _up_to_date(out, CU_SOURCES):
+        return out
     nvcc = _cuda_home() / "bin" / "nvcc"
     cmd = [nvcc, *NVCC_ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", INCLUDE]
     if verbose_ptxas:
@@ -106,6 +116,8 @@ def build_op(force: bool = False) -> Path:
 
     lib = build_library(force=force)
     out = PKG / OP_NAME
+    if not force and _up_to_date(out, OP_SOURCES, lib):
+        return out
     cuda_home = _cuda_home()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     includes = cpp_extension.include_paths() + [str(cuda_home / "include"), str(INCLUDE)]
