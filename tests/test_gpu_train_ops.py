@@ -555,6 +555,34 @@ def test_norm_special_rows(pkg):
     check_norm(pkg, keep, dh[good], dn[good])
 
 
+@pytest.mark.parametrize("pre", [True, False])
+@pytest.mark.parametrize("rows, width, dtype", [
+    (5000, 64, torch.bfloat16), (1000, 130, torch.bfloat16), (3001, 512, torch.float16), (1000, 4096, torch.float32),
+    (700, 4104, torch.bfloat16), (500, 4098, torch.bfloat16), (700, 8192, torch.bfloat16), (320, 9001, torch.float16),
+    (320, 12000, torch.bfloat16), (320, 15360, torch.float32), (320, 15365, torch.float32), (50, 20000, torch.bfloat16)])
+def test_norm_residual_scale_gradient_is_every_term_once(pkg, rows, width, dtype, pre):
+    """With whole numbers and no gradient of normed, the terms dh x and every
+    sum of them are exact, as all stay below 2^24 (a thread's and a column's) or
+    2^53 (all): so must the gradient be, rounded once, whether the terms have one
+    sign or cancel.  A row, block or cluster part left out or taken twice shows."""
+    g = gen(49)
+
+    def whole(low, high, *shape):
+        return torch.randint(low, high + 1, shape, generator=g, device="cuda").to(dtype)
+
+    w = torch.rand(width, generator=g, device="cuda")
+    for low in (1, -3):
+        x, dh = whole(low, 3, rows, width), whole(max(low, -2), 2, rows, width)
+        y = torch.randn(rows, width, generator=g, device="cuda").to(dtype)
+        terms = x.double() * dh.double()
+        for scale in (torch.full((1,), 0.75, device="cuda"), torch.rand(width, generator=g, device="cuda")):
+            scale.requires_grad_(True)
+            hidden, _ = pkg.residual_norm(y, x, w, w if pre else None, residual_scale=scale)
+            (grad,) = torch.autograd.grad(hidden, scale, dh)
+            want = terms.sum().view(1) if scale.numel() == 1 else terms.sum(0)
+            assert torch.equal(grad, want.float())
+
+
 @pytest.mark.parametrize("size, eps", [(1e15, 1e-6), (1e-14, 0.0)])
 @pytest.mark.parametrize("post", [True, False])
 @pytest.mark.parametrize("rows, width, dtype", [
