@@ -107,8 +107,8 @@ typedef struct {
   const void* residual_scale;  /* [scale_count] or NULL */
   void* hidden;                /* [rows][width] */
   void* normed;                /* [rows][width], with pre_weight */
-  float* rstd_post;            /* [rows], with post_weight: may be NULL forward */
-  float* rstd_pre;             /* [rows], with pre_weight: may be NULL forward */
+  float* rstd_post;            /* [rows], 1 without post_weight; may be NULL forward */
+  float* rstd_pre;             /* [rows], 0 without pre_weight; may be NULL forward */
   int64_t rows, width;
   int64_t gate_rows;           /* divides rows; 0 without gate */
   int64_t scale_count;         /* 1 or width; 0 without residual_scale */

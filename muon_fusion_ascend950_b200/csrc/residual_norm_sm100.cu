@@ -546,6 +546,11 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
       RowVectors<T, N, kE>::store(static_cast<T*>(a.normed) + row * width, place, width, h[j]);
     }
   }
+  // the statistics of a norm that there is not
+  if (a.post_weight == nullptr && a.rstd_post != nullptr)
+    for (int64_t row = begin + place.tid * stride; row < end; row += place.threads * stride) a.rstd_post[row] = 1.f;
+  if (a.pre_weight == nullptr && a.rstd_pre != nullptr)
+    for (int64_t row = begin + place.tid * stride; row < end; row += place.threads * stride) a.rstd_pre[row] = 0.f;
   if constexpr (kRing)
     if (threadIdx.x == 0 && ring_state.stopped) ring.drain(ring_state.row);
   if constexpr (kOwner == kClusterRow) muon_sm100::cluster_sync();  // peers' stores have landed
@@ -575,8 +580,8 @@ __global__ void __launch_bounds__(kThreads)
     }
     block_sums(sum, red, kThreads);
     r = rms_rstd(sum[0], width, a.eps);
-    if (threadIdx.x == 0 && a.rstd_post != nullptr) a.rstd_post[row] = r;
   }
+  if (threadIdx.x == 0 && a.rstd_post != nullptr) a.rstd_post[row] = r;
   float sum[1] = {0.f};
   T* hidden = static_cast<T*>(a.hidden) + base;
   for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
@@ -584,7 +589,10 @@ __global__ void __launch_bounds__(kThreads)
     hidden[c] = from_float<T>(h);
     sum[0] = fmaf(h, h, sum[0]);
   }
-  if (a.pre_weight == nullptr) return;
+  if (a.pre_weight == nullptr) {
+    if (threadIdx.x == 0 && a.rstd_pre != nullptr) a.rstd_pre[row] = 0.f;
+    return;
+  }
   block_sums(sum, red + 32, kThreads);
   const float rh = rms_rstd(sum[0], width, a.eps);
   if (threadIdx.x == 0 && a.rstd_pre != nullptr) a.rstd_pre[row] = rh;

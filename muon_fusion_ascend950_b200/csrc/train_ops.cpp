@@ -300,7 +300,7 @@ NormInputs CheckNorm(const Tensor& block_out, const Tensor& residual, const OptT
 }
 
 // (hidden, normed, rstd): rstd holds the two statistics of each row, [2,
-// rows].  Without pre_weight normed is empty.
+// rows], 1 and 0 of a norm that there is not.  Without pre_weight normed is empty.
 std::tuple<Tensor, Tensor, Tensor> ResidualNormCuda(
     const Tensor& block_out, const Tensor& residual, const OptTensor& post, const OptTensor& pre,
     const OptTensor& gate, const OptTensor& scale, double eps) {

@@ -600,6 +600,22 @@ def test_norm_gradients_of_large_and_small_rows(pkg, rows, width, dtype, size, e
     check_norm(pkg, v, dh, dn, eps=eps, hidden_used=False)
 
 
+@pytest.mark.parametrize("rows, width", [(300, 64), (300, 130), (700, 512), (400, 4096), (30, 8192), (20, 12000), (5, 20000)])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("pre", [True, False])
+def test_norm_statistics_are_written_in_every_form(pkg, rows, width, post, pre):
+    """The operator's third output has no value that was there before."""
+    v, _, _ = norm_inputs((rows, width), torch.bfloat16, torch.float32, None, 0, post, pre, seed=50)
+    torch.full((2, rows), math.nan, device="cuda")  # what the allocator gives out next
+    hidden, _, rstd = torch.ops.muon_ascend950.residual_norm(*(v[n] for n in NAMES), 1e-6)
+    out, _, _ = norm_reference(v, 1, None, None)
+    y, h = v["block_out"].double(), out["hidden"]
+    steps = (width / 16 + 96) * E32
+    for got, of, there, without in ((rstd[0], y, post, 1.0), (rstd[1], h, pre, 0.0)):
+        want = (of.square().mean(-1) + 1e-6).rsqrt() if there else torch.full((rows,), without, device="cuda")
+        near(got, want, steps * want.double() if there else 0.0)
+
+
 def test_norm_no_rows(pkg):
     x = torch.empty(0, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)
