@@ -959,6 +959,32 @@ def test_route_nan_reaches_the_whole_gradient(pkg):
         assert grad[2].isnan().all() and grad[[0, 1, 3, 4, 5]].isfinite().all()
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_route_choice_is_the_plain_forms(pkg, seed):
+    """Of the measured cases' ranges: a choice does not depend on how the scores
+    were computed, so that indices and counts equal those of torch operations."""
+    import importlib.util
+    import random
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parent.parent / "perf" / "operators.py"
+    spec = importlib.util.spec_from_file_location("perf_operators", path)
+    cases = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(cases)
+    rng, done = random.Random(seed), 0
+    while done < 25:
+        case = cases.draw(rng)
+        if case["op"] != "route":
+            continue
+        done += 1
+        state = cases.prepare(case, seed)
+        cases.own = False
+        plain = cases.run(state)
+        cases.own = True
+        own = cases.run(state)
+        assert torch.equal(own["indices"], plain["indices"]) and torch.equal(own["counts"], plain["counts"]), case
+
+
 # =========================================================== all of them
 def test_refusals_on_the_device(pkg):
     x = torch.zeros(4, 16, device="cuda")
