@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 4)
 // Measured for the loss with its gradient, 4096 x 131072 bf16 (333 us at the
 // copy rate): rows in registers of 8-block clusters 783 us (4 blocks an SM
 // 616), slices held in the ring between the passes 504 us, streamed twice
-// 403 us.  8192 x 65536: 390 us.  The loss alone: 174 us of 167.
+// 403 us (394 now).  8192 x 65536: 372 us.  The loss alone: 172 us of 167.
 constexpr int kConsumers = 256;
 constexpr int kConsumerWarps = kConsumers / 32;
 constexpr int kPerStage = 4;  // granules of a thread in a stage

@@ -73,11 +73,11 @@ __device__ __forceinline__ float rms_rstd(float sum, float width, float eps) {
 // block of up to 512 threads, or to a cluster of such blocks, which add up
 // their sums over distributed shared memory.  Rows of whole 16-byte vectors
 // have 8 columns a thread up to 4096, 16 above, and a cluster of 2 above
-// 8192: 16384 x 8192 bf16 backward took 436 us so when it was chosen (404 now),
+// 8192: 16384 x 8192 bf16 backward took 436 us so when it was chosen (402 now),
 // 568 with 8 columns in a cluster, whose barrier holds up every row.  Other
 // rows have 8 columns a thread and clusters of 2 and 4: 16 would not fit the
 // registers (4098 columns: 716 us when it was chosen, with 16 a thread 1219;
-// 588 now).
+// 567 now).
 constexpr int kMaxThreads = 512;
 constexpr int kWarpRowWarps = 8;   // rows in flight of a block, one a warp
 constexpr int kMaxCluster = 4;
@@ -390,7 +390,7 @@ __device__ __forceinline__ int64_t gate_row_of(const muon_train_norm_args& a, in
 
 // Forward.  Four rows (of 8 columns a thread) at a time: their sums share the
 // shuffles and barriers, whose latency else held up every row.  16384 x 4096
-// bf16: 94 us, 83 at the copy rate (one row at a time, two blocks an SM: 116;
+// bf16: 93 us, 83 at the copy rate (one row at a time, two blocks an SM: 116;
 // with all copies issued by one thread, on whose warp the next sums wait: 103).
 template <typename T, int N, int kE, RowOwner kOwner>
 __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMaxThreads,
@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(kOwner == kWarpRow ? kWarpRowWarps * 32 : kMax
   begin_kernel();
   const Place<N, kOwner> place;
   // Neighbouring rows, which mostly share a gate row (100 x 150 rows of 4096
-  // with a gate row for each 150: 184 us dealt out in turn, 107 so), and which a
-  // block with 8 columns a thread streams better (2050 columns: 122 and 110);
+  // with a gate row for each 150: 184 us dealt out in turn, 103 so), and which a
+  // block with 8 columns a thread streams better (2050 columns: 122 and 107);
   // other rows are dealt out in turn (200 columns: 8.9 us as neighbours, 7.6 so;
   // 8192 without such a gate: 179 and 170).
   const bool neighbours = (kOwner == kBlockRow && kE == 8) || a.gate_rows > 1;
@@ -624,7 +624,7 @@ Plan make_plan(const muon_train_norm_args& a, int64_t target) {
   // Workers take chunks in rounds: of the counts that fill k rounds the one
   // with the least time in rows, where a chunk costs kChunkRows besides its own
   // (one chunk more than workers, in place of a few less, doubled the time: 5
-  // sequences of 3288 x 2050 with a gate row each: 150 chunks 347 us, 145 190).
+  // sequences of 3288 x 2050 with a gate row each: 150 chunks 347 us, 145 183).
   constexpr int64_t kChunkRows = 2;
   int64_t least_rows = INT64_MAX;
   for (int64_t k = 1; k <= 8; ++k) {
@@ -736,11 +736,12 @@ struct Held<kE, true> {
 // With 16 columns: gain, pre weight and the sums of a residual scale with
 // columns (the scale itself would take the ring's second stage, and is loaded
 // for every row).  With 8 columns registers would do, but the fewer they hold
-// the less a row waits: that scale and its sums (16384 x 4096 bf16 174 us; the
-// sums in registers 228, and the scale loaded for every row 272); of rows
-// through the ring the pre weight (174 us, 178 in registers), of fp32 the gain
-// too (291 us, 334; bf16 181).  Single elements have no registers for the
-// addresses (2049 columns: 377 us, the scale loaded for every row 326).
+// the less a row waits: that scale and its sums (16384 x 4096 bf16 174 us when
+// that was chosen, 179 now; the sums in registers 228, and the scale loaded for
+// every row 272); of rows through the ring the pre weight (174 us then, 178 in
+// registers), of fp32 the gain too (291 us then, 334; bf16 181).  Single
+// elements have no registers for the addresses (2049 columns: 377 us, the scale
+// loaded for every row 326, and 317 now).
 template <typename T, int N, int kE, bool kRing, bool kScaleColumns>
 struct Holds {
   static constexpr bool kScale = kScaleColumns && kE == 8 && N > 1;
@@ -750,7 +751,7 @@ struct Holds {
   static constexpr int kFloats = (kScale + kScaleSums + kPre + kGain) * kE;
 };
 
-// Backward.  16384 x 4096 bf16: 173 us, 125 at the copy rate; 60% of the issue
+// Backward.  16384 x 4096 bf16: 167 us, 125 at the copy rate; 59% of the issue
 // slots are used, the rest goes into each row's sums and barrier (two rows at
 // a time, read from their stages again, took 202 against 183 then: more
 // instructions than the waits were worth).

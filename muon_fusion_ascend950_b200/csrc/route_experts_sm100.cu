@@ -163,7 +163,7 @@ __device__ __forceinline__ bool few_best(const float (&key)[kPer], float best, c
 }
 
 // Forward: one warp a token.  The time goes into instructions, not memory (256
-// sigmoid scores in 8 groups: about 840 a token against 1 KB read, 71% of the
+// sigmoid scores in 8 groups: about 840 a token against 1 KB read, 79% of the
 // issue slots used), so keys and scores stay in registers, and kFull, rows of
 // exactly 32 kPer experts, leaves out every check for a lane's last one.  The
 // best keys come from few_best where the plan allows it, else one by one: an

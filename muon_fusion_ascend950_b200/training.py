@@ -12,7 +12,7 @@ step beside them that are bound by memory, each with its gradient:
 
 They are the operators ``torch.ops.muon_ascend950.*`` of the same names, which
 check their arguments (ValueError, TypeError), run on the current stream and
-take part in autograd (gradients of gradients are refused).
+take part in autograd (gradients of gradients and forward mode are refused).
 """
 from __future__ import annotations
 
