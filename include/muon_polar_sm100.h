@@ -419,7 +419,8 @@ uint64_t muon_polar_tensor_map_encodes(void);
 /* Sets the limit of every bounded wait inside this library's kernels on the
  * current device (default 2 s): a wait that has not ended after `limit_ns`
  * nanoseconds of wall-clock time gives up, sets its watchdog bit
- * (muon_polar_read_device_status) and the kernel drains and returns.  The
+ * (muon_polar_read_device_status; muon_train_read_device_status for the kernels
+ * of muon_train_sm100.h) and the kernel drains and returns.  The
  * previous limit is stored in *previous (may be NULL).  1000 <= limit_ns <=
  * 6e10.  Synchronous with respect to the host (cudaMemcpyToSymbol); call it
  * while no kernel of this library runs on the device.  No counterpart in the
