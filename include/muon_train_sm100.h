@@ -180,6 +180,120 @@ int muon_train_route_sm100(const muon_train_route_args* args, void* stream);
 int muon_train_route_backward_sm100(const muon_train_route_args* args, const float* grad_weights,
                                     void* grad_logits, void* stream);
 
+/* ---- attention -------------------------------------------------------------------
+ * For each head of each sequence, with group = heads / kv_heads and key head
+ * h / group:
+ *   s_ij = scale q_i . k_j       for the keys j that query i sees
+ *   p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij)
+ *   out_i = sum_j p_ij v_j
+ * Query i stands at i + keys - length: both are counted from the end.  With
+ * causal it sees the keys up to its own place; with window > 0 those less than
+ * window places away.  A query that sees no key has out 0, lse -inf and
+ * gradient 0.
+ *   dense:    batch sequences of `length` queries and `keys` keys
+ *   lengths:  of sequence b only the first lengths[b] queries and keys count
+ *             (keys == length); the others are as if they saw nothing
+ *   offsets:  `sequences` sequences one after another in one row of tokens
+ *             (batch 1, keys == length): sequence s is the tokens offsets[s] to
+ *             offsets[s + 1]; tokens outside of all see nothing.  Offsets may
+ *             not descend; ends outside of the row are taken as its ends.
+ * Tokens that do not count are not read into the others' results, whatever
+ * they hold.  Elements of a head are contiguous; strides are in elements and
+ * multiples of 8, and all arrays aligned to 16 bytes.
+ */
+#define MUON_TRAIN_MAX_HEAD_DIM 128
+
+typedef struct {
+  int64_t batch, row, head;
+} muon_train_strides;
+
+typedef struct {
+  const void* q;               /* [batch][length][heads][dim], by its strides */
+  const void* k;               /* [batch][keys][kv_heads][dim] */
+  const void* v;               /* as k */
+  void* out;                   /* [batch][length][heads][dim], contiguous */
+  float* lse;                  /* [heads][batch * length] */
+  const int32_t* lengths;      /* [batch] or NULL */
+  const int32_t* offsets;      /* [sequences + 1] or NULL */
+  muon_train_strides q_stride, k_stride, v_stride;
+  int64_t batch, length, keys, heads, kv_heads;
+  int64_t dim;                 /* 8 .. MUON_TRAIN_MAX_HEAD_DIM, a multiple of 8 */
+  int64_t sequences;
+  int64_t window;              /* 0: none */
+  float scale;                 /* positive */
+  int causal;
+  int dtype;                   /* MUON_TRAIN_BF16 or MUON_TRAIN_F16 */
+} muon_train_attention_args;
+
+int muon_train_attention_sm100(const muon_train_attention_args* args, void* stream);
+
+/* grad_q, grad_k and grad_v are contiguous and all written. */
+typedef struct {
+  const void* grad_out;        /* [batch][length][heads][dim], by its strides */
+  muon_train_strides grad_out_stride;
+  void* grad_q;                /* [batch][length][heads][dim] */
+  void* grad_k;                /* [batch][keys][kv_heads][dim] */
+  void* grad_v;                /* as grad_k */
+  void* workspace;             /* 16-byte aligned */
+  size_t workspace_bytes;
+} muon_train_attention_grads;
+
+/* Bytes of workspace of a backward call on the current device (0 on error). */
+size_t muon_train_attention_workspace_bytes(const muon_train_attention_args* args);
+
+/* args: the forward call's, with its out and lse. */
+int muon_train_attention_backward_sm100(const muon_train_attention_args* args,
+                                        const muon_train_attention_grads* grads, void* stream);
+
+/* ---- rotary positions ----------------------------------------------------------
+ * Turns pairs (a, b) of each head's elements at position n by n f_i:
+ *   (a, b) -> scale (a cos - b sin, b cos + a sin)
+ * a = x[i], b = x[i + pairs], or x[2 i] and x[2 i + 1] when interleaved, for i
+ * below pairs; the elements from 2 pairs on are copied.  Angles are taken in 64
+ * bits.  With inverse the pairs turn back: the gradient.  Up to two tensors
+ * (queries and keys) with the same positions; heads 0: there is none.
+ */
+#define MUON_TRAIN_MAX_ROTARY_DIM 4096
+
+typedef struct {
+  const void* x[2];            /* [batch][length][heads][dim], by strides in elements */
+  void* y[2];                  /* contiguous */
+  int64_t x_batch[2], x_row[2], x_head[2];
+  int64_t heads[2];
+  const void* positions;       /* [position_rows][length], int32 or int64 */
+  const void* frequencies;     /* [pairs], fp32 or fp64: radians a position */
+  int64_t batch, length, dim, pairs;
+  int64_t position_rows;       /* batch, or 1: the same for all */
+  int position_bytes, frequency_bytes; /* 4 or 8 */
+  int interleaved, inverse;
+  float scale;
+  int dtype;                   /* MUON_TRAIN_* */
+} muon_train_rotary_args;
+
+int muon_train_rotary_sm100(const muon_train_rotary_args* args, void* stream);
+
+/* ---- gradient norm and clipping ------------------------------------------------
+ *   norm = sqrt(sum of the squares of all elements of all tensors)  (norm_type 2)
+ *        = their largest magnitude                                  (norm_type 0)
+ *   out  = grad min(1, max_norm / (norm + 1e-6))
+ * Tensors are contiguous and do not overlap; out may be grad itself (of the
+ * same type), and in place tensors within the limit are not written.  Squares
+ * are added up in 64 bits.  A NaN makes the norm and all outputs NaN.
+ */
+typedef struct {
+  const void* grad;            /* [count] */
+  void* out;                   /* [count] */
+  int64_t count;
+  int dtype, out_dtype;        /* MUON_TRAIN_* */
+} muon_train_clip_tensor;
+
+/* Bytes of workspace for a list of `tensors` on the current device (0 on error). */
+size_t muon_train_clip_workspace_bytes(int64_t tensors);
+
+/* `tensors` (host memory) is read before the call returns. */
+int muon_train_clip_sm100(const muon_train_clip_tensor* tensors, int64_t n, double max_norm, int norm_type,
+                          float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,10 +112,43 @@ def load_library() -> None:
     def fake_route_experts_backward(grad_weights, logits, indices, score, renormalize, scale):
         return logits.new_empty(logits.shape)
 
+    def fake_attention(query, key, value, offsets, lengths, causal, window, scale):
+        from .transformer import check_attention
+
+        check_attention(query, key, value, offsets, lengths, window, scale)
+        packed = offsets is not None
+        rows = query.shape[0] if packed else query.shape[0] * query.shape[1]
+        return (query.new_empty(query.shape),
+                query.new_empty((query.shape[-2], rows), dtype=torch.float32))
+
+    def fake_attention_backward(grad_out, query, key, value, out, lse, offsets, lengths, causal, window,
+                                scale):
+        return query.new_empty(query.shape), key.new_empty(key.shape), value.new_empty(value.shape)
+
+    def fake_rotary(query, key, positions, frequencies, interleaved, scale, inverse=False):
+        from .transformer import check_rotary
+
+        check_rotary(query, key, positions, frequencies, scale)
+        return (query.new_empty(query.shape),
+                query.new_empty((0,)) if key is None else key.new_empty(key.shape))
+
+    def fake_clip_gradients_in_place(gradients, max_norm, largest):
+        from .transformer import check_clip
+
+        check_clip(gradients, None, max_norm)
+        return gradients[0].new_empty((), dtype=torch.float32)
+
+    def fake_clip_gradients(gradients, out, max_norm, largest):
+        from .transformer import check_clip
+
+        check_clip(gradients, out, max_norm)
+        return gradients[0].new_empty((), dtype=torch.float32)
+
     # Extensions of this build: polar_step_t (the step of x^T in x's layout)
     # has polar_step's output contract; polar_express returns bf16 of x's
     # shape; muon_update_ mutates its arguments and returns nothing.  The
-    # training-step operators (training.py) return fresh tensors.
+    # training-step operators (training.py, transformer.py) return fresh tensors;
+    # clip_gradients and clip_gradients_ mutate the tensors they are given.
     fakes = (("muon_ascend950::polar_step", fake_polar_step),
              ("muon_ascend950::polar_step_t", fake_polar_step),
              ("muon_ascend950::polar_express", fake_polar_express),
@@ -126,7 +159,13 @@ def load_library() -> None:
              ("muon_ascend950::residual_norm", fake_residual_norm),
              ("muon_ascend950::residual_norm_backward", fake_residual_norm_backward),
              ("muon_ascend950::route_experts", fake_route_experts),
-             ("muon_ascend950::route_experts_backward", fake_route_experts_backward))
+             ("muon_ascend950::route_experts_backward", fake_route_experts_backward),
+             ("muon_ascend950::attention", fake_attention),
+             ("muon_ascend950::attention_backward", fake_attention_backward),
+             ("muon_ascend950::rotary", fake_rotary),
+             ("muon_ascend950::rotary_backward", fake_rotary),
+             ("muon_ascend950::clip_gradients_", fake_clip_gradients_in_place),
+             ("muon_ascend950::clip_gradients", fake_clip_gradients))
     for name, fn in fakes:
         try:
             torch.library.register_fake(name)(fn)

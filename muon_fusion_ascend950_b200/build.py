@@ -5,10 +5,11 @@
   Polar Express step (``muon_polar_sm100.cu``), the Muon update around it
   (``muon_update_sm100.cu``) and the training-step operators declared in
   ``include/muon_train_sm100.h`` (``distill_topk_sm100.cu``,
-  ``residual_norm_sm100.cu``, ``route_experts_sm100.cu``).
+  ``residual_norm_sm100.cu``, ``route_experts_sm100.cu``, ``attention_sm100.cu``,
+  ``rotary_sm100.cu``, ``clip_grads_sm100.cu``).
 * ``_C.so`` -- the PyTorch operators ``muon_ascend950::*`` on the CUDA
-  dispatch key (``polar_step_op.cpp``, ``train_ops.cpp``), linked against the
-  library above (rpath ``$ORIGIN``).
+  dispatch key (``polar_step_op.cpp``, ``train_ops.cpp``, ``block_ops.cpp``),
+  linked against the library above (rpath ``$ORIGIN``).
 
 Both land next to this file so that they travel with the source tree.  Each
 source compiles to an object under ``_build/`` (all in parallel); what is newer
@@ -63,15 +64,19 @@ CU_SOURCES = {  # source -> the headers it includes
     "distill_topk_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "residual_norm_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "route_experts_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "attention_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "rotary_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "clip_grads_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
 }
 OP_SOURCES = {
     "polar_step_op.cpp": ["muon_polar_sm100.h"],
-    "train_ops.cpp": ["muon_train_sm100.h", "muon_polar_sm100.h"],
+    "train_ops.cpp": ["train_ops_common.h", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "block_ops.cpp": ["train_ops_common.h", "muon_train_sm100.h", "muon_polar_sm100.h"],
 }
 
 
 def _inputs(name: str, headers) -> list:
-    return [CSRC / name, Path(__file__)] + [CSRC / h if h.endswith(".cuh") else INCLUDE / h for h in headers]
+    return [CSRC / name, Path(__file__)] + [CSRC / h if (CSRC / h).exists() else INCLUDE / h for h in headers]
 
 
 def _up_to_date(out: Path, sources: dict, *more) -> bool:

@@ -134,8 +134,46 @@ class RouteArgs(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+class Strides(ctypes.Structure):
+    """muon_train_strides"""
+    _fields_ = [("batch", _I64), ("row", _I64), ("head", _I64)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """muon_train_attention_args"""
+    _fields_ = [("q", _VP), ("k", _VP), ("v", _VP), ("out", _VP), ("lse", _VP), ("lengths", _VP),
+                ("offsets", _VP), ("q_stride", Strides), ("k_stride", Strides), ("v_stride", Strides),
+                ("batch", _I64), ("length", _I64), ("keys", _I64), ("heads", _I64), ("kv_heads", _I64),
+                ("dim", _I64), ("sequences", _I64), ("window", _I64), ("scale", ctypes.c_float),
+                ("causal", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class AttentionGrads(ctypes.Structure):
+    """muon_train_attention_grads"""
+    _fields_ = [("grad_out", _VP), ("grad_out_stride", Strides), ("grad_q", _VP), ("grad_k", _VP),
+                ("grad_v", _VP), ("workspace", _VP), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """muon_train_rotary_args"""
+    _fields_ = [("x", _VP * 2), ("y", _VP * 2), ("x_batch", _I64 * 2), ("x_row", _I64 * 2),
+                ("x_head", _I64 * 2), ("heads", _I64 * 2), ("positions", _VP), ("frequencies", _VP),
+                ("batch", _I64), ("length", _I64), ("dim", _I64), ("pairs", _I64),
+                ("position_rows", _I64), ("position_bytes", ctypes.c_int),
+                ("frequency_bytes", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("inverse", ctypes.c_int), ("scale", ctypes.c_float), ("dtype", ctypes.c_int)]
+
+
+class ClipTensor(ctypes.Structure):
+    """muon_train_clip_tensor"""
+    _fields_ = [("grad", _VP), ("out", _VP), ("count", _I64), ("dtype", ctypes.c_int),
+                ("out_dtype", ctypes.c_int)]
+
+
 _DISTILL, _NORM, _GRADS, _ROUTE = (ctypes.POINTER(t) for t in (DistillArgs, NormArgs, NormGrads,
                                                                RouteArgs))
+_ATTENTION, _ATTENTION_GRADS, _ROTARY, _CLIP = (
+    ctypes.POINTER(t) for t in (AttentionArgs, AttentionGrads, RotaryArgs, ClipTensor))
 TRAIN_SIGNATURES = {
     "muon_train_launch_count": (ctypes.c_uint64, []),
     "muon_train_read_device_status": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_uint32),
@@ -148,6 +186,13 @@ TRAIN_SIGNATURES = {
     "muon_train_residual_norm_backward_sm100": (ctypes.c_int, [_NORM, _GRADS, _VP]),
     "muon_train_route_sm100": (ctypes.c_int, [_ROUTE, _VP]),
     "muon_train_route_backward_sm100": (ctypes.c_int, [_ROUTE, _VP, _VP, _VP]),
+    "muon_train_attention_sm100": (ctypes.c_int, [_ATTENTION, _VP]),
+    "muon_train_attention_workspace_bytes": (ctypes.c_size_t, [_ATTENTION]),
+    "muon_train_attention_backward_sm100": (ctypes.c_int, [_ATTENTION, _ATTENTION_GRADS, _VP]),
+    "muon_train_rotary_sm100": (ctypes.c_int, [_ROTARY, _VP]),
+    "muon_train_clip_workspace_bytes": (ctypes.c_size_t, [_I64]),
+    "muon_train_clip_sm100": (ctypes.c_int, [_CLIP, _I64, ctypes.c_double, ctypes.c_int, _VP, _VP,
+                                             ctypes.c_size_t, _VP]),
 }
 
 WATCHDOG_PRODUCER = 0x1

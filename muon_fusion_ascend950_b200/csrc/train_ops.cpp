@@ -2,90 +2,16 @@
 // update: distillation from a teacher's top logits, the norms around a
 // residual block, routing to experts.  CUDA kernels through the C ABI
 // (include/muon_train_sm100.h); gradients on the Autograd key.
-#include <ATen/ATen.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAFunctions.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/library.h>
-
 #include <array>
 #include <cfloat>
 #include <cmath>
-#include <cstdlib>
-#include <optional>
 #include <tuple>
 
-#include "muon_train_sm100.h"
+#include "train_ops_common.h"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-// Of a launch on the current device.  With MUON_POLAR_DEBUG_SYNC set (read on
-// every call) it also synchronises, and raises if a wait of a kernel ran out.
-void CheckStatus(int rc, const char* who) {
-  TORCH_CHECK(rc == MUON_POLAR_OK, who, " failed, status=", rc,
-              ", detail=", muon_polar_status_string(rc));
-  if (std::getenv("MUON_POLAR_DEBUG_SYNC") == nullptr) return;
-  uint32_t flags = 0;
-  const int read = muon_train_read_device_status(c10::cuda::current_device(), &flags, /*clear=*/1);
-  TORCH_CHECK(read == MUON_POLAR_OK, who, " failed, status=", read,
-              ", detail=", muon_polar_status_string(read));
-  TORCH_CHECK(flags == 0, who, " gave up on a bounded wait, status word=", flags);
-}
-
-int Dtype(const Tensor& t, const char* who, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return MUON_TRAIN_F32;
-    case at::kBFloat16: return MUON_TRAIN_BF16;
-    case at::kHalf: return MUON_TRAIN_F16;
-    default: TORCH_CHECK_TYPE(false, who, ": ", name, " must be float32, bfloat16 or float16, got ",
-                              t.scalar_type());
-  }
-}
-
-void CheckCuda(const Tensor& t, const char* who, const char* name) {
-  TORCH_CHECK_VALUE(t.device().is_cuda(), who, ": ", name, " must be a CUDA tensor, got ", t.device());
-}
-void CheckDevice(const Tensor& t, const Tensor& like, const char* who, const char* name) {
-  TORCH_CHECK_VALUE(t.device() == like.device(), who, ": ", name, " must be on ", like.device(),
-                    ", got ", t.device());
-}
-
-// An uninitialised contiguous CUDA tensor, without the dispatcher's way there:
-// small calls are bound by the host.
-Tensor Empty(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
-  return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
-}
-
-void* Ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-const Tensor& Given(const OptTensor& t) {
-  static const Tensor none;
-  return t.has_value() && t->defined() ? *t : none;
-}
-void* Stream(const Tensor& t) {
-  return static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
-}
-
-// Tangents are not carried on, nor is a gradient of a gradient computed: say
-// so instead of returning a result that autograd would take for a constant.
-void NoTangents(std::initializer_list<const Tensor*> inputs, const char* who) {
-  for (const Tensor* t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), who,
-                                ": forward-mode differentiation (jvp) is not supported");
-}
-void NoSecondOrder(const variable_list& grads, const char* who) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), who,
-                              ": the gradient cannot be differentiated again (create_graph=True)");
-  for (const Tensor& g : grads) NoTangents({&g}, who);
-}
+using namespace muon_train_ops;
 
 // ------------------------------------------------------------ distillation
 // [..., n] as [rows, n], read in place when the elements of a row are
@@ -111,8 +37,6 @@ Tensor GradLike(const Tensor& z) {
   const int64_t used = (rows - 1) * ld + cols;
   return Empty({used + shift}, z.scalar_type(), z).as_strided({rows, cols}, {ld, 1}, shift);
 }
-
-at::IntArrayRef Lead(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
 
 // One fp32 value for each row.
 Tensor RowValues(const OptTensor& t, const Tensor& like, const char* who, const char* name) {
@@ -457,29 +381,6 @@ Tensor RouteBackwardCuda(const Tensor& grad_weights, const Tensor& logits, const
 }
 
 // ------------------------------------------------------------ autograd
-template <typename Fn>
-auto Op(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
-}
-
-// Whether autograd records a call: otherwise it goes to the kernels directly.
-bool Recorded(std::initializer_list<const Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : inputs)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
-
-// A node of the graph whose next edges are `inputs`, in order.
-template <typename N, typename... Inputs>
-std::shared_ptr<N> MakeNode(const Inputs&... inputs) {
-  auto node = std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
-  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
-  return node;
-}
-
-OptTensor Optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-
 struct DistillBackward : public torch::autograd::Node {
   SavedVariable student, values, indices, lse, stats;
   double temperature = 1.0;
