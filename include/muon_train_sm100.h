@@ -212,6 +212,7 @@ typedef struct {
   const void* k;               /* [batch][keys][kv_heads][dim] */
   const void* v;               /* as k */
   void* out;                   /* [batch][length][heads][dim], contiguous */
+  void* out_rest;              /* as out, or NULL: what rounding took from out, for the backward call */
   float* lse;                  /* [heads][batch * length] */
   const int32_t* lengths;      /* [batch] or NULL */
   const int32_t* offsets;      /* [sequences + 1] or NULL */
@@ -241,7 +242,8 @@ typedef struct {
 /* Bytes of workspace of a backward call on the current device (0 on error). */
 size_t muon_train_attention_workspace_bytes(const muon_train_attention_args* args);
 
-/* args: the forward call's, with its out and lse. */
+/* args: the forward call's, with its out, lse and out_rest.  Without out_rest
+ * the rounding of out goes into grad_q and grad_k. */
 int muon_train_attention_backward_sm100(const muon_train_attention_args* args,
                                         const muon_train_attention_grads* grads, void* stream);
 

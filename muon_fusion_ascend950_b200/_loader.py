@@ -112,17 +112,18 @@ def load_library() -> None:
     def fake_route_experts_backward(grad_weights, logits, indices, score, renormalize, scale):
         return logits.new_empty(logits.shape)
 
-    def fake_attention(query, key, value, offsets, lengths, causal, window, scale):
+    def fake_attention(query, key, value, offsets, lengths, causal, window, scale, keep):
         from .transformer import check_attention
 
         check_attention(query, key, value, offsets, lengths, window, scale)
         packed = offsets is not None
         rows = query.shape[0] if packed else query.shape[0] * query.shape[1]
         return (query.new_empty(query.shape),
-                query.new_empty((query.shape[-2], rows), dtype=torch.float32))
+                query.new_empty((query.shape[-2], rows), dtype=torch.float32),
+                query.new_empty(query.shape if keep else (0,)))
 
-    def fake_attention_backward(grad_out, query, key, value, out, lse, offsets, lengths, causal, window,
-                                scale):
+    def fake_attention_backward(grad_out, query, key, value, out, lse, rest, offsets, lengths, causal,
+                                window, scale):
         return query.new_empty(query.shape), key.new_empty(key.shape), value.new_empty(value.shape)
 
     def fake_rotary(query, key, positions, frequencies, interleaved, scale, inverse=False):

@@ -64,7 +64,7 @@ CU_SOURCES = {  # source -> the headers it includes
     "distill_topk_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "residual_norm_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "route_experts_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
-    "attention_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "attention_sm100.cu": ["tcgen05_attention.cuh", "train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "rotary_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "clip_grads_sm100.cu": ["train_common.cuh", "sm100_ptx.cuh", "muon_train_sm100.h", "muon_polar_sm100.h"],
 }

@@ -141,8 +141,8 @@ class Strides(ctypes.Structure):
 
 class AttentionArgs(ctypes.Structure):
     """muon_train_attention_args"""
-    _fields_ = [("q", _VP), ("k", _VP), ("v", _VP), ("out", _VP), ("lse", _VP), ("lengths", _VP),
-                ("offsets", _VP), ("q_stride", Strides), ("k_stride", Strides), ("v_stride", Strides),
+    _fields_ = [("q", _VP), ("k", _VP), ("v", _VP), ("out", _VP), ("out_rest", _VP),
+                ("lse", _VP), ("lengths", _VP), ("offsets", _VP), ("q_stride", Strides), ("k_stride", Strides), ("v_stride", Strides),
                 ("batch", _I64), ("length", _I64), ("keys", _I64), ("heads", _I64), ("kv_heads", _I64),
                 ("dim", _I64), ("sequences", _I64), ("window", _I64), ("scale", ctypes.c_float),
                 ("causal", ctypes.c_int), ("dtype", ctypes.c_int)]

@@ -1,4 +1,5 @@
-// attention_sm100.cu -- attention of training sequences, forward and backward.
+// attention_sm100.cu -- attention of training sequences, forward and backward,
+// on the tensor cores.
 //
 //   s_ij = scale q_i . k_j over the keys that query i sees
 //   p_ij = exp(s_ij - lse_i), out_i = sum_j p_ij v_j
@@ -6,198 +7,1082 @@
 //   dq_i = scale sum_j ds_ij k_j, dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij dout_i
 // (dk and dv also over the query heads that share the key head).
 //
-// A warp a row: each lane holds four elements of the head, products are summed
-// over the warp, and the softmax goes by a running maximum and sum.  The
-// backward pass computes the probabilities again from lse: one kernel for the
-// queries' rows, one for the keys' rows, so that no sum needs atomics.
+// Tiles of 128 queries and 128 keys.  All products are tcgen05 ones with fp32
+// results in tensor memory; tiles of the inputs come by TMA into swizzled
+// shared memory.  The scores are read from tensor memory into registers, a row
+// a thread, and the probabilities go back there as 16-bit values, in place of
+// the scores, as the next product's left operand: neither is ever in shared or
+// global memory.  In a block of 320 threads eight warps work on the scores, one
+// loads and one issues the products.
+//
+// The backward pass computes the scores again.  It is two kernels, one for a
+// tile of keys (dk, dv: four products a pair of tiles) and one for a tile of
+// queries (dq: three): seven products in place of five, but every sum is held
+// in tensor memory from its first term to its last, without atomics or partial
+// sums in memory, and its order is fixed.
+//
+// Rounding: p and ds are rounded to the inputs' type as operands of the second
+// products, as the inputs were; everything else is fp32.  delta is taken from
+// the output and from what rounding took from it (out_rest), so that it has the
+// scores' precision.  fp16 operands are scaled by powers of two: p by 2^7
+// (forward; at most 2^15) and 2^10 (backward), so that small ones do not fall
+// below fp16's range, and ds by what the largest |dout| and |v| allow.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "tcgen05_attention.cuh"
 #include "train_common.cuh"
 
 namespace muon_train {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kDims = 4;  // of a lane
+using namespace muon_sm100;
 
-struct Rows {  // a row's sequence: its first row, its length, whether it counts
-  int64_t first;
-  int length;
+constexpr int kTile = 128;     // queries, or keys, of a tile
+constexpr int kThreads = 320;  // warps 0-7: scores, 8: loads, 9: products
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr uint32_t kTmemColumns = 512;
+constexpr int kAtom = kTile * 128;  // bytes of 64 columns of a tile, the swizzle's width
+
+template <typename T>
+constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same_v<T, __half>;
+// Binary exponents that p is raised by.
+template <typename T>
+constexpr float kRaise = kBf16<T> ? 0.0f : 7.0f;
+template <typename T>
+constexpr float kRaiseBack = kBf16<T> ? 0.0f : 10.0f;
+// The running maximum may lag behind by this many binary exponents before the
+// sums so far are scaled again: nearly all rows then keep their first maximum.
+constexpr float kLag = 8.0f;
+
+// ------------------------------------------------------------ sequences
+struct Problem {
+  void* out;                // forward: out; backward: see there
+  void* out2;
+  float* lse;
+  const float* stats;       // backward: [2][heads][rows]: -lse (binary), -delta
+  const float* largest;     // backward, fp16: the largest |dout| and |v|
+  const int32_t* lengths;
+  const int32_t* offsets;
+  int64_t rows;             // batch * length
+  int length, keys, heads, kv_heads, dim, sequences, batch, window, causal;
+  float scale;
 };
 
-// The sequence of row `r` (packed: of all tokens; else of batch entry b).
-__device__ __forceinline__ Rows sequence_of(const muon_train_attention_args& a, int64_t b, int64_t r) {
-  Rows s{0, static_cast<int>(a.length)};
-  if (a.lengths != nullptr) {
-    const int n = a.lengths[b];
-    s.length = n < 0 ? 0 : n < a.length ? n : static_cast<int>(a.length);
+// One tile of rows of one sequence.
+struct Tile {
+  int batch;      // coordinate of the tensors
+  int row0;       // first row of the sequence
+  int first;      // of the tile, in the sequence
+  int stored;     // rows of the sequence that are written
+  int queries;    // rows that count, as queries
+  int keys;       // and as keys
+  bool found;
+};
+
+__device__ __forceinline__ int clamp_int(int v, int low, int high) { return v < low ? low : v > high ? high : v; }
+
+// Tile `index` of the problem's tiles of kSize rows, `rows` a batch entry.
+// Packed: of all sequences, the tokens before the first and behind the last
+// among them as sequences that see nothing; every warp looks for itself.
+template <int kSize>
+__device__ __forceinline__ Tile find_tile(const Problem& p, int index, int rows) {
+  Tile t;
+  t.found = true;
+  if (p.offsets == nullptr) {
+    const int per = (rows + kSize - 1) / kSize;
+    t.batch = index / per;
+    t.first = (index - t.batch * per) * kSize;
+    t.row0 = 0;
+    t.stored = rows;
+    t.queries = p.length;
+    t.keys = p.keys;
+    if (p.lengths != nullptr) t.queries = t.keys = clamp_int(p.lengths[t.batch], 0, p.length);
+    return t;
   }
-  if (a.offsets != nullptr) {
-    int64_t low = 0, high = a.sequences + 1;  // offsets up to r: [0, low)
-    while (low < high) {
-      const int64_t mid = (low + high) / 2;
-      if (a.offsets[mid] <= r)
-        low = mid + 1;
-      else
-        high = mid;
+  const int lane = threadIdx.x % 32;
+  int64_t before = 0;
+  t.batch = 0;
+  for (int base = 0; base < p.sequences + 2; base += 32) {
+    const int s = base + lane;
+    int begin = 0, end = 0;
+    if (s < p.sequences + 2) {
+      begin = s == 0 ? 0 : clamp_int(p.offsets[s - 1], 0, p.length);
+      end = s > p.sequences ? p.length : clamp_int(p.offsets[s], 0, p.length);
+      end = end < begin ? begin : end;
     }
-    s.first = r;
-    s.length = 0;
-    if (low > 0 && low <= a.sequences) {
-      s.first = a.offsets[low - 1] < 0 ? 0 : a.offsets[low - 1];
-      const int64_t end = a.offsets[low] < a.length ? a.offsets[low] : a.length;
-      s.length = static_cast<int>(end - s.first);
+    const int tiles = (end - begin + kSize - 1) / kSize;
+    int64_t sum = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(kFullMask, sum, o);
+      if (lane >= o) sum += v;
     }
+    const unsigned over = __ballot_sync(kFullMask, before + sum > index);
+    if (over != 0) {
+      const int at = __ffs(over) - 1;
+      const int local = static_cast<int>(index - before - (sum - tiles));
+      t.first = __shfl_sync(kFullMask, local, at) * kSize;
+      t.row0 = __shfl_sync(kFullMask, begin, at);
+      t.stored = __shfl_sync(kFullMask, end, at) - t.row0;
+      const int found = base + at;
+      t.queries = t.keys = found > 0 && found <= p.sequences ? t.stored : 0;
+      return t;
+    }
+    before += __shfl_sync(kFullMask, sum, 31);
   }
-  return s;
+  t.found = false;
+  return t;
 }
 
-__device__ __forceinline__ int clip(int64_t v, int high) {
-  return v < 0 ? 0 : v > high ? high : static_cast<int>(v);
+// Keys [low, high) that queries [i0, i1) of the sequence see at least in part.
+__device__ __forceinline__ void keys_of(const Problem& p, const Tile& t, int i0, int i1, int* low, int* high) {
+  const int shift = t.keys - t.queries;
+  *low = 0;
+  *high = i0 < i1 ? t.keys : 0;
+  if (p.causal) *high = min(*high, i1 + shift);
+  if (p.window > 0) {
+    *low = max(0, i0 + shift - p.window + 1);
+    *high = min(*high, i1 - 1 + shift + p.window);
+  }
+  *high = max(*high, 0);
+  *low = min(*low, *high);
+}
+// Queries [low, high) that see keys [j0, j1) at least in part.
+__device__ __forceinline__ void queries_of(const Problem& p, const Tile& t, int j0, int j1, int* low, int* high) {
+  const int shift = t.keys - t.queries;
+  *low = 0;
+  *high = j0 < j1 ? t.queries : 0;
+  if (p.causal) *low = max(0, j0 - shift);
+  if (p.window > 0) {
+    if (!p.causal) *low = max(*low, j0 - shift - p.window + 1);
+    *high = min(*high, j1 - 1 - shift + p.window);
+  }
+  *high = max(*high, 0);
+  *low = min(*low, *high);
+}
+
+// ------------------------------------------------------------ shared pieces
+// All lanes of a warp wait; false for all if one gave up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  return __all_sync(kFullMask, ring_wait(bar, parity, failed));
+}
+
+// Rows from `valid` on of a tile in shared memory become zeros: they belong to
+// another sequence or to padding, and 0 * NaN would reach the sums.
+template <int kCols>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int valid) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int a = 0; a < kCols / 64; ++a)
+    for (int i = valid * 128 + lane * 16; i < kAtom; i += 512)
+      *reinterpret_cast<uint4*>(tile + a * kAtom + i) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Boxes of 64 columns of 128 rows.
+template <int kCols>
+__device__ __forceinline__ void load_tile(uint8_t* to, const CUtensorMap* map, uint64_t* bar, int row, int head,
+                                          int batch) {
+#pragma unroll
+  for (int a = 0; a < kCols / 64; ++a) tma_load_4d(to + a * kAtom, map, bar, a * 64, row, head, batch);
+}
+
+// D[128 x 128] = A B^T over `steps` runs of 16 columns of both tiles.
+__device__ __forceinline__ void scores(uint32_t d, const uint8_t* a, const uint8_t* b, uint32_t idesc, int steps) {
+  const uint32_t pa = smem_addr(a), pb = smem_addr(b);
+  for (int k = 0; k < steps; ++k) {
+    const uint32_t at = (k / 4) * kAtom + (k % 4) * 32;
+    umma_ss(d, smem_desc_sw128(pa + at, 16, 1024), smem_desc_sw128(pb + at, 16, 1024), idesc, k > 0);
+  }
+}
+// D[128 x n] (+)= A[tmem: 128 x 128] B, B's rows summed over; columns 64 to 127
+// of A begin at column `half` of tensor memory.
+__device__ __forceinline__ void weighted(uint32_t d, uint32_t a, int half, const uint8_t* b, uint32_t idesc,
+                                         bool more) {
+  const uint32_t pb = smem_addr(b);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    umma_ts(d, a + (k / 4) * half + (k % 4) * 8, smem_desc_sw128(pb + k * 2048, kAtom, 1024), idesc, more || k > 0);
 }
 
 template <typename T>
-__device__ __forceinline__ void load_dims(const T* p, int dim, float (&v)[kDims]) {
-  const int lane = threadIdx.x % 32;
-  if (lane * kDims < dim) {
-    Elements<T, kDims>::unpack(Elements<T, kDims>::load(p + lane * kDims), v);
+__device__ __forceinline__ uint32_t pack2(float low, float high) {
+  if constexpr (kBf16<T>) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&h);
   } else {
-#pragma unroll
-    for (int i = 0; i < kDims; ++i) v[i] = 0.0f;
+    const __half2 h = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-}
-template <typename T>
-__device__ __forceinline__ void store_dims(T* p, int dim, const float (&v)[kDims], float by) {
-  const int lane = threadIdx.x % 32;
-  if (lane * kDims >= dim) return;
-  float w[kDims];
-#pragma unroll
-  for (int i = 0; i < kDims; ++i) w[i] = v[i] * by;
-  Elements<T, kDims>::store(p + lane * kDims, Elements<T, kDims>::pack(w));
-}
-__device__ __forceinline__ float dot(const float (&a)[kDims], const float (&b)[kDims]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kDims; ++i) s = fmaf(a[i], b[i], s);
-  return warp_sum(s);
 }
 
-template <typename T>
-__device__ __forceinline__ const T* row_of(const void* p, const muon_train_strides& s, int64_t b, int64_t r,
-                                           int64_t h) {
-  return static_cast<const T*>(p) + b * s.batch + r * s.row + h * s.head;
-}
+__device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
 
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-    forward_kernel(const __grid_constant__ muon_train_attention_args a) {
-  begin_kernel();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32, h = blockIdx.y;
-  if (row >= a.batch * a.length) return;
-  const int64_t b = row / a.length, r = row % a.length, kh = h / (a.heads / a.kv_heads);
-  const int dim = static_cast<int>(a.dim);
-  const Rows s = sequence_of(a, b, r);
-  const int keys = a.lengths != nullptr || a.offsets != nullptr ? s.length : static_cast<int>(a.keys);
-  const int64_t i = r - s.first, place = i + keys - s.length;
-  int low = 0, high = i < s.length ? keys : 0;
-  if (a.causal) high = clip(place + 1, high);
-  if (a.window > 0) {
-    low = clip(place - a.window + 1, high);
-    high = clip(place + a.window, high);
-  }
-  float q[kDims], acc[kDims] = {};
-  load_dims(row_of<T>(a.q, a.q_stride, b, r, h), dim, q);
-  float top = -INFINITY, sum = 0.0f;
-  for (int j = low; j < high; ++j) {
-    float k[kDims], v[kDims];
-    load_dims(row_of<T>(a.k, a.k_stride, b, s.first + j, kh), dim, k);
-    load_dims(row_of<T>(a.v, a.v_stride, b, s.first + j, kh), dim, v);
-    const float score = dot(q, k) * a.scale, next = fmaxf(top, score);
-    const float old = expf(top - next), p = expf(score - next);
-    sum = sum * old + p;
-    top = next;
+// A row of a result in tensor memory times `by` to memory; with `rest` also
+// what the rounding took.
+template <typename T, int kCols>
+__device__ __forceinline__ void store_row(T* to, T* rest, uint32_t taddr, int dim, float by, bool write) {
+#pragma unroll 1
+  for (int c = 0; c < kCols; c += 32) {
+    uint32_t r[32];
+    if (c >= dim) return;
+    tmem_ld_32x32b_x32(taddr + c, r);
+    tmem_wait_ld(r);
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) acc[d] = acc[d] * old + p * v[d];
-  }
-  store_dims(static_cast<T*>(a.out) + (row * a.heads + h) * dim, dim, acc, sum > 0.0f ? 1.0f / sum : high > low ? NAN : 0.0f);
-  if (threadIdx.x % 32 == 0) a.lse[h * a.batch * a.length + row] = high > low ? top + logf(sum) : -INFINITY;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-    query_grad_kernel(const __grid_constant__ muon_train_attention_args a,
-                      const __grid_constant__ muon_train_attention_grads g) {
-  begin_kernel();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32, h = blockIdx.y;
-  if (row >= a.batch * a.length) return;
-  const int64_t b = row / a.length, r = row % a.length, kh = h / (a.heads / a.kv_heads);
-  const int dim = static_cast<int>(a.dim);
-  const Rows s = sequence_of(a, b, r);
-  const int keys = a.lengths != nullptr || a.offsets != nullptr ? s.length : static_cast<int>(a.keys);
-  const int64_t i = r - s.first, place = i + keys - s.length;
-  int low = 0, high = i < s.length ? keys : 0;
-  if (a.causal) high = clip(place + 1, high);
-  if (a.window > 0) {
-    low = clip(place - a.window + 1, high);
-    high = clip(place + a.window, high);
-  }
-  float q[kDims], o[kDims], go[kDims], acc[kDims] = {};
-  load_dims(row_of<T>(a.q, a.q_stride, b, r, h), dim, q);
-  load_dims(static_cast<const T*>(a.out) + (row * a.heads + h) * dim, dim, o);
-  load_dims(row_of<T>(g.grad_out, g.grad_out_stride, b, r, h), dim, go);
-  const float delta = dot(o, go), lse = a.lse[h * a.batch * a.length + row];
-  if (threadIdx.x % 32 == 0) static_cast<float*>(g.workspace)[h * a.batch * a.length + row] = delta;
-  for (int j = low; j < high; ++j) {
-    float k[kDims], v[kDims];
-    load_dims(row_of<T>(a.k, a.k_stride, b, s.first + j, kh), dim, k);
-    load_dims(row_of<T>(a.v, a.v_stride, b, s.first + j, kh), dim, v);
-    const float p = expf(dot(q, k) * a.scale - lse), ds = p * (dot(go, v) - delta);
+    for (int j = 0; j < 32; j += 8) {
+      if (!write || c + j >= dim) continue;
+      float v[8];
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) acc[d] = fmaf(ds, k[d], acc[d]);
-  }
-  store_dims(static_cast<T*>(g.grad_q) + (row * a.heads + h) * dim, dim, acc, a.scale);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-    key_grad_kernel(const __grid_constant__ muon_train_attention_args a,
-                    const __grid_constant__ muon_train_attention_grads g) {
-  begin_kernel();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32, kh = blockIdx.y;
-  if (row >= a.batch * a.keys) return;
-  const int64_t b = row / a.keys, r = row % a.keys, group = a.heads / a.kv_heads;
-  const int dim = static_cast<int>(a.dim);
-  const Rows s = sequence_of(a, b, r);
-  const int keys = a.lengths != nullptr || a.offsets != nullptr ? s.length : static_cast<int>(a.keys);
-  const int64_t j = r - s.first, place = j - (keys - s.length);  // the query that stands where this key does
-  int low = 0, high = j < keys ? s.length : 0;
-  if (a.causal) low = clip(place, high);
-  if (a.window > 0) {
-    low = clip(place - a.window + 1 > low ? place - a.window + 1 : low, high);
-    high = clip(place + a.window, high);
-  }
-  float k[kDims], v[kDims], dk[kDims] = {}, dv[kDims] = {};
-  load_dims(row_of<T>(a.k, a.k_stride, b, r, kh), dim, k);
-  load_dims(row_of<T>(a.v, a.v_stride, b, r, kh), dim, v);
-  for (int64_t h = kh * group; h < (kh + 1) * group; ++h) {
-    for (int i = low; i < high; ++i) {
-      const int64_t at = s.first + i, stat = h * a.batch * a.length + b * a.length + at;
-      float q[kDims], go[kDims];
-      load_dims(row_of<T>(a.q, a.q_stride, b, at, h), dim, q);
-      load_dims(row_of<T>(g.grad_out, g.grad_out_stride, b, at, h), dim, go);
-      const float p = expf(dot(q, k) * a.scale - a.lse[stat]);
-      const float ds = p * (dot(go, v) - static_cast<const float*>(g.workspace)[stat]);
+      for (int i = 0; i < 8; ++i) v[i] = as_float(r[j + i]) * by;
+      const uint4 u = pack<T>(v);
+      *reinterpret_cast<uint4*>(to + c + j) = u;
+      if (rest != nullptr) {
+        float w[8];
+        unpack<T>(u, w);
 #pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        dk[d] = fmaf(ds, q[d], dk[d]);
-        dv[d] = fmaf(p, go[d], dv[d]);
+        for (int i = 0; i < 8; ++i) v[i] -= w[i];
+        *reinterpret_cast<uint4*>(rest + c + j) = pack<T>(v);
       }
     }
+    __syncwarp();
   }
-  const int64_t to = (row * a.kv_heads + kh) * dim;
-  store_dims(static_cast<T*>(g.grad_k) + to, dim, dk, a.scale);
-  store_dims(static_cast<T*>(g.grad_v) + to, dim, dv, 1.0f);
+}
+template <typename T>
+__device__ __forceinline__ void zero_row(T* to, int dim) {
+  for (int c = 0; c < dim; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+}
+
+// After a wait that gave up: the copies in flight to the last fills of a ring.
+__device__ __forceinline__ void drain_fills(uint64_t* full, int stages, int fills) {
+  const int first = fills > stages ? fills - stages : 0;
+  drain_ring(full, stages, first % stages, (first / stages) & 1, fills - first);
+}
+
+// The end of a block, by all threads: tensor memory is given back.  After a wait
+// that gave up, only when the copies and products in flight have ended.
+__device__ __forceinline__ void finish(uint32_t tmem, volatile int* failed, int fills, uint64_t* full, int stages,
+                                       uint64_t* once, uint64_t* again, uint64_t* drained) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  tc_fence_before();
+  __syncthreads();
+  if (*failed && warp == kLoadWarp && lane == 0) {
+    drain_fills(full, stages, fills);
+    if (once != nullptr) drain_ring(once, 1, 0, 0, 1);
+    if (again != nullptr) drain_ring(again, 1, 0, 0, 1);
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    if (*failed) {
+      if (lane == 0) umma_commit(drained);
+      __syncwarp();
+      drain_ring(drained, 1, 0, 0, 1);
+      __syncwarp();
+    }
+    tmem_relinquish();
+    tmem_dealloc(tmem, kTmemColumns);
+  }
+}
+
+// ------------------------------------------------------------ forward
+template <int kCols>
+struct Forward {
+  static constexpr int kTileBytes = kTile * kCols * 2;
+  static constexpr int kStages = kCols == 128 ? 5 : 8;  // tiles of keys or values
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + 1024;
+};
+
+// Two tiles of queries a block, which take turns: while the scores of one are
+// worked on, the products of the other run.  Keys and values pass through a
+// ring of tiles, keys j, values j, keys j + 1 and so on.
+template <typename T, int kCols>
+__global__ void __launch_bounds__(kThreads, 1)
+    forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Problem p, int tiles) {
+  using C = Forward<kCols>;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_done[2], drained, full[C::kStages], empty[C::kStages];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed_word;
+  volatile int* failed = &failed_word;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
+  uint8_t* ring = smem + 2 * C::kTileBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kTile);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(&drained, 1);
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    fence_mbar_init();
+    failed_word = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kTmemColumns);
+  tc_fence_before();
+  begin_kernel();
+  // the tiles with the most keys first (causal: the last); heads side by side, so that they share keys in L2
+  const int head = blockIdx.x % p.heads, index = tiles - 1 - static_cast<int>(blockIdx.x) / p.heads;
+  const Tile t = find_tile<2 * kTile>(p, index, p.length);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  // key tiles [from, to) of the two query tiles
+  int from[2], to[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int i0 = t.first + i * kTile;
+    int low = 0, high = 0;
+    if (t.found) keys_of(p, t, min(i0, t.queries), min(i0 + kTile, t.queries), &low, &high);
+    from[i] = low / kTile;
+    to[i] = (high + kTile - 1) / kTile;
+    if (low >= high) from[i] = to[i] = 0;
+  }
+  int first = from[0], last = to[0];
+  if (from[0] == to[0]) first = from[1], last = to[1];
+  if (from[0] < to[0] && from[1] < to[1]) first = min(from[0], from[1]), last = max(to[0], to[1]);
+
+  int fills = 0;
+  if (warp == kLoadWarp) {
+    if (lane == 0 && first < last) {
+      const int kv_head = head / (p.heads / p.kv_heads);
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (from[i] == to[i]) continue;
+        mbar_arrive_expect_tx(&q_full[i], C::kTileBytes);
+        load_tile<kCols>(smem + i * C::kTileBytes, &map_q, &q_full[i], t.row0 + t.first + i * kTile, head, t.batch);
+      }
+      for (int j = first; j < last && ok; ++j) {
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          const int s = fills % C::kStages;
+          if (fills >= C::kStages) ok = ok && ring_wait(&empty[s], (fills / C::kStages - 1) & 1, failed);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[s], C::kTileBytes);
+          load_tile<kCols>(ring + s * C::kTileBytes, which ? &map_v : &map_k, &full[s], t.row0 + j * kTile, kv_head,
+                           t.batch);
+          ++fills;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    const uint32_t id_s = idesc_16bit(kBf16<T>, kTile, 0), id_o = idesc_16bit(kBf16<T>, (p.dim + 15) / 16 * 16, 1);
+    const int steps = (p.dim + 15) / 16;
+    int done[2] = {0, 0};  // key tiles whose scores were asked for
+    bool ok = true;
+    // scores of query tile i with the keys in `slot`
+    const auto ask = [&](int i, int slot) {
+      if (done[i] == 0) ok = ok && warp_wait(&q_full[i], 0, failed);
+      if (!ok) return;
+      if (lane == 0) {
+        scores(tmem + i * kTile, smem + i * C::kTileBytes, ring + slot * C::kTileBytes, id_s, steps);
+        umma_commit(&s_full[i]);
+      }
+      __syncwarp();
+      ++done[i];
+    };
+    int fill = 0;
+    if (first < last) {
+      ok = warp_wait(&full[0], 0, failed);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (ok && from[i] <= first && first < to[i]) ask(i, 0);
+      if (ok && lane == 0) umma_commit(&empty[0]);
+    }
+    for (int j = first; j < last && ok; ++j) {
+      const int v_slot = (fill + 1) % C::kStages, k_slot = (fill + 2) % C::kStages;
+      ok = warp_wait(&full[v_slot], ((fill + 1) / C::kStages) & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      if ((p.offsets != nullptr || p.lengths != nullptr) && (j + 1) * kTile > t.keys)
+        zero_rows<kCols>(ring + v_slot * C::kTileBytes, t.keys - j * kTile);
+      const bool more = j + 1 < last;
+      if (more) ok = warp_wait(&full[k_slot], ((fill + 2) / C::kStages) & 1, failed);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (ok && from[i] <= j && j < to[i]) {
+          const int it = j - from[i];
+          ok = warp_wait(&p_full[i], it & 1, failed);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            weighted(tmem + 2 * kTile + i * kCols, tmem + i * kTile, 32, ring + v_slot * C::kTileBytes, id_o, it > 0);
+            umma_commit(&o_done[i]);
+          }
+          __syncwarp();
+        }
+        if (ok && more && from[i] <= j + 1 && j + 1 < to[i]) ask(i, k_slot);
+      }
+      if (ok && lane == 0) {
+        umma_commit(&empty[v_slot]);
+        if (more) umma_commit(&empty[k_slot]);
+      }
+      __syncwarp();
+      fill += 2;
+    }
+  } else {
+    const int i = warp / 4, row = t.first + threadIdx.x;  // of the sequence: 128 threads a tile
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21);
+    const uint32_t s_at = lanes + i * kTile, o_at = lanes + 2 * kTile + i * kCols;
+    int low = 0, high = 0, all_low = 0, all_high = 0;
+    if (t.found) {
+      keys_of(p, t, min(row, t.queries), min(row + 1, t.queries), &low, &high);
+      // what every row of the tile sees
+      const int i0 = t.first + i * kTile, i1 = min(i0 + kTile, t.queries);
+      int unused;
+      if (i0 < i1) {
+        keys_of(p, t, i1 - 1, i1, &all_low, &unused);
+        keys_of(p, t, i0, i0 + 1, &unused, &all_high);
+      }
+    }
+    const float c = p.scale * kLog2e;
+    float top = -INFINITY, sum = 0.0f;
+    bool ok = true;
+    for (int j = from[i]; j < to[i]; ++j) {
+      const int it = j - from[i];
+      ok = warp_wait(&s_full[i], it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(s_at + q * 32, s[q]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_wait_ld(s[q]);
+      const int k0 = j * kTile;
+      if (k0 < all_low || k0 + kTile > all_high) {
+        const int a = low - k0, b = high - k0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (q * 32 + e < a || q * 32 + e >= b) s[q][e] = 0xff800000u;
+      }
+      float best = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) best = fmaxf(best, as_float(s[q][e]));
+      if (it == 0) {
+        top = best;
+      } else {
+        const bool grow = (best - top) * c > kLag;
+        if (__any_sync(kFullMask, grow)) {
+          const float next = grow ? best : top, by = grow ? fast_exp2((top - next) * c) : 1.0f;
+          sum *= by;
+          top = next;
+          ok = warp_wait(&o_done[i], (it - 1) & 1, failed);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int q = 0; q < kCols; q += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(o_at + q, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(as_float(o[e]) * by);
+            tmem_st_32x32b_x32(o_at + q, o);
+          }
+        }
+      }
+      const float base = top == -INFINITY ? kRaise<T> : kRaise<T> - top * c;
+      float2 sums = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int at = q * 64 + 2 * e;
+          const float2 x = fma2(make_float2(as_float(s[at / 32][at % 32]), as_float(s[at / 32][at % 32 + 1])), both(c),
+                                both(base));
+          const float2 v = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          sums = add2(sums, v);
+          w[e] = pack2<T>(v.x, v.y);
+        }
+        tmem_st_32x32b_x32(s_at + q * 32, w);
+      }
+      sum += sums.x + sums.y;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[i]);
+    }
+    const int n = to[i] - from[i];
+    if (ok && n > 0) ok = warp_wait(&o_done[i], (n - 1) & 1, failed);
+    tc_fence_after();
+    const int64_t at = static_cast<int64_t>(t.batch) * p.length + t.row0 + row;
+    const bool write = ok && t.found && row < t.stored;
+    T* out = static_cast<T*>(p.out) + (at * p.heads + head) * p.dim;
+    T* rest = p.out2 != nullptr ? static_cast<T*>(p.out2) + (at * p.heads + head) * p.dim : nullptr;
+    if (n > 0) {
+      const bool some = low < high;
+      store_row<T, kCols>(out, rest, o_at, p.dim, some ? 1.0f / sum : 0.0f, write && some);
+    }
+    if (write && (n <= 0 || low >= high)) {
+      zero_row(out, p.dim);
+      if (rest != nullptr) zero_row(rest, p.dim);
+    }
+    if (write)
+      p.lse[head * p.rows + at] = low < high ? top * p.scale + logf(sum) - kRaise<T> * 0.6931471805599453f : -INFINITY;
+  }
+  finish(tmem, failed, fills, full, C::kStages, from[0] < to[0] ? &q_full[0] : nullptr, from[1] < to[1] ? &q_full[1] : nullptr, &drained);
+}
+
+// ------------------------------------------------------------ backward: statistics
+// -lse in binary exponents (so that p = 2^(s scale log2 e - it); -inf where
+// nothing is seen: p = 0) and -delta of each row and head; with kLargest also
+// the largest |dout|.  16 lanes a row.
+template <typename T, bool kLargest>
+__global__ void __launch_bounds__(256)
+    stats_kernel(const T* __restrict__ out, const T* __restrict__ rest, const T* __restrict__ grad,
+                 muon_train_strides stride, const float* __restrict__ lse, float* __restrict__ stats,
+                 uint32_t* largest, int64_t rows, int length, int heads, int dim) {
+  begin_kernel();
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+  const int lane = threadIdx.x % 16;
+  const bool inside = item < rows * heads;
+  float d = 0.0f, big = 0.0f;
+  if (inside && lane * 8 < dim) {
+    const int64_t row = item / heads, h = item - row * heads, b = row / length, r = row - b * length;
+    float o[8], e[8] = {}, g[8];
+    unpack<T>(*reinterpret_cast<const uint4*>(out + item * dim + lane * 8), o);
+    if (rest != nullptr) unpack<T>(*reinterpret_cast<const uint4*>(rest + item * dim + lane * 8), e);
+    unpack<T>(*reinterpret_cast<const uint4*>(grad + b * stride.batch + r * stride.row + h * stride.head + lane * 8), g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      d = fmaf(o[i], g[i], d);
+      d = fmaf(e[i], g[i], d);
+      big = fmaxf(big, fabsf(g[i]));
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(kFullMask, d, o);
+  if (inside && lane == 0) {
+    const int64_t row = item / heads, h = item - row * heads, at = h * rows + row;
+    const float l = lse[at];
+    // a row that sees nothing has no gradient, whatever dout holds there
+    const bool none = l == -INFINITY;
+    stats[at] = none ? -INFINITY : kRaiseBack<T> - l * kLog2e;
+    stats[heads * rows + at] = none ? 0.0f : -d;
+  }
+  if constexpr (kLargest) {
+    if (inside && lse[(item % heads) * rows + item / heads] == -INFINITY) big = 0.0f;
+    big = warp_max(big);
+    if (threadIdx.x % 32 == 0 && big > 0.0f) atomicMax(largest, __float_as_uint(big));
+  }
+}
+
+// The largest magnitude of a tensor, NaN aside, padding included: a bound.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    largest_kernel(const T* __restrict__ x, muon_train_strides stride, uint32_t* largest, int64_t rows, int length,
+                   int heads, int dim) {
+  begin_kernel();
+  const int lane = threadIdx.x % 16;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 16;
+  float big = 0.0f;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16; item < rows * heads; item += step) {
+    if (lane * 8 >= dim) continue;
+    const int64_t row = item / heads, h = item - row * heads, b = row / length, r = row - b * length;
+    float v[8];
+    unpack<T>(*reinterpret_cast<const uint4*>(x + b * stride.batch + r * stride.row + h * stride.head + lane * 8), v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(v[i]) < INFINITY) big = fmaxf(big, fabsf(v[i]));
+  }
+  big = warp_max(big);
+  if (threadIdx.x % 32 == 0 && big > 0.0f) atomicMax(largest, __float_as_uint(big));
+}
+
+// The power of two that ds is multiplied by: |dp - delta| <= 2 dim max|dout|
+// max|v|, which this brings to 2^15 at most.
+template <typename T>
+__device__ __forceinline__ float ds_factor(const Problem& p) {
+  if constexpr (kBf16<T>) {
+    return 1.0f;
+  } else {
+    const float bound = 2.0f * p.dim * p.largest[0] * p.largest[1];
+    if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;
+    return scalbnf(1.0f, clamp_int(14 - ilogbf(bound), -100, 100));
+  }
+}
+
+// ------------------------------------------------------------ backward: keys and values
+template <int kCols>
+struct KeyGrads {
+  static constexpr int kTileBytes = kTile * kCols * 2;
+  static constexpr int kStages = kCols == 128 ? 2 : 4;  // a tile of queries and one of dout
+  static constexpr int kBytes = (2 + 2 * kStages) * kTileBytes + 1024;
+};
+
+// One tile of keys a block.  Scores stand the other way round, a key a thread:
+// p^T and ds^T are left operands as they are.  The warps 0-3 take queries 0 to
+// 63 of each tile, 4-7 the others.  While the scores of the next tile are
+// computed ds is worked on, while dp is computed the next p.
+template <typename T, int kCols>
+__global__ void __launch_bounds__(kThreads, 1)
+    key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
+                    const __grid_constant__ Problem p) {
+  using C = KeyGrads<kCols>;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t kv_full, s_full, dp_full, p_done, ds_done, finished, drained, full[C::kStages], empty[C::kStages];
+  __shared__ __align__(16) float stat[C::kStages][2][kTile];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed_word;
+  volatile int* failed = &failed_word;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
+  uint8_t* tile_k = smem;
+  uint8_t* tile_v = smem + C::kTileBytes;
+  uint8_t* ring = smem + 2 * C::kTileBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    mbar_init(&kv_full, 1);
+    mbar_init(&s_full, 1);
+    mbar_init(&dp_full, 1);
+    mbar_init(&p_done, 256);
+    mbar_init(&ds_done, 256);
+    mbar_init(&finished, 1);
+    mbar_init(&drained, 1);
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 33);  // the copies, and each lane's statistics
+      mbar_init(&empty[i], 1);
+    }
+    fence_mbar_init();
+    failed_word = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kTmemColumns);
+  tc_fence_before();
+  begin_kernel();
+  const int kv_head = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
+  const Tile t = find_tile<kTile>(p, blockIdx.x / p.kv_heads, p.keys);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tmem_s = tmem, tmem_dp = tmem + kTile, tmem_dv = tmem + 2 * kTile,
+                 tmem_dk = tmem + 2 * kTile + kCols;
+  int low = 0, high = 0;
+  if (t.found) queries_of(p, t, min(t.first, t.keys), min(t.first + kTile, t.keys), &low, &high);
+  const int from = low / kTile, to = low < high ? (high + kTile - 1) / kTile : from;
+  const int per = to - from, n = per * group;  // tiles of queries, of all heads
+  const bool foreign = p.offsets != nullptr || p.lengths != nullptr;
+
+  int fills = 0;
+  if (warp == kLoadWarp) {
+    bool ok = true;
+    if (n > 0 && lane == 0) {
+      mbar_arrive_expect_tx(&kv_full, 2 * C::kTileBytes);
+      load_tile<kCols>(tile_k, &map_k, &kv_full, t.row0 + t.first, kv_head, t.batch);
+      load_tile<kCols>(tile_v, &map_v, &kv_full, t.row0 + t.first, kv_head, t.batch);
+    }
+    for (int it = 0; it < n; ++it) {
+      const int s = it % C::kStages, head = kv_head * group + it / per, first = (from + it % per) * kTile;
+      if (it >= C::kStages) ok = warp_wait(&empty[s], (it / C::kStages - 1) & 1, failed);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[s], 2 * C::kTileBytes);
+        load_tile<kCols>(ring + 2 * s * C::kTileBytes, &map_q, &full[s], t.row0 + first, head, t.batch);
+        load_tile<kCols>(ring + (2 * s + 1) * C::kTileBytes, &map_g, &full[s], t.row0 + first, head, t.batch);
+      }
+      const int64_t at = head * p.rows + static_cast<int64_t>(t.batch) * p.length + t.row0 + first;
+#pragma unroll
+      for (int i = lane; i < kTile; i += 32) {
+        const bool counts = first + i < t.queries;
+        stat[s][0][i] = counts ? p.stats[at + i] : -INFINITY;
+        stat[s][1][i] = counts ? p.stats[p.heads * p.rows + at + i] : 0.0f;
+      }
+      mbar_arrive(&full[s]);
+      ++fills;
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    const uint32_t id_s = idesc_16bit(kBf16<T>, kTile, 0), id_o = idesc_16bit(kBf16<T>, (p.dim + 15) / 16 * 16, 1);
+    const int steps = (p.dim + 15) / 16;
+    bool ok = n == 0 || warp_wait(&kv_full, 0, failed);
+    // waits for the tiles of iteration `it` and clears what is not the sequence's
+    const auto arrived = [&](int it) {
+      const int s = it % C::kStages;
+      if (!warp_wait(&full[s], (it / C::kStages) & 1, failed)) return false;
+      const int valid = t.queries - (from + it % per) * kTile;
+      if (foreign && valid < kTile) {
+        zero_rows<kCols>(ring + 2 * s * C::kTileBytes, valid);
+        zero_rows<kCols>(ring + (2 * s + 1) * C::kTileBytes, valid);
+      }
+      return true;
+    };
+    if (ok && n > 0) {
+      ok = arrived(0);
+      if (ok && lane == 0) {
+        scores(tmem_s, tile_k, ring, id_s, steps);
+        umma_commit(&s_full);
+        scores(tmem_dp, tile_v, ring + C::kTileBytes, id_s, steps);
+        umma_commit(&dp_full);
+      }
+      __syncwarp();
+    }
+    for (int it = 0; it < n && ok; ++it) {
+      const uint8_t* tile_q = ring + 2 * (it % C::kStages) * C::kTileBytes;
+      const uint8_t* tile_g = tile_q + C::kTileBytes;
+      const uint8_t* next_q = ring + 2 * ((it + 1) % C::kStages) * C::kTileBytes;
+      const bool more = it + 1 < n;
+      ok = warp_wait(&p_done, it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) weighted(tmem_dv, tmem_s, 64, tile_g, id_o, it > 0);
+      __syncwarp();
+      if (more) {
+        ok = arrived(it + 1);
+        if (!ok) break;
+        if (lane == 0) {
+          scores(tmem_s, tile_k, next_q, id_s, steps);
+          umma_commit(&s_full);
+        }
+        __syncwarp();
+      }
+      ok = warp_wait(&ds_done, it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        weighted(tmem_dk, tmem_dp, 64, tile_q, id_o, it > 0);
+        umma_commit(&empty[it % C::kStages]);
+        if (more) {
+          scores(tmem_dp, tile_v, next_q + C::kTileBytes, id_s, steps);
+          umma_commit(&dp_full);
+        } else {
+          umma_commit(&finished);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    const int w = warp / 4, row = t.first + threadIdx.x % 128;  // the thread's key; both halves have all keys
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
+    const float c = p.scale * kLog2e, raise = ds_factor<T>(p) * (kBf16<T> ? 1.0f : 0x1p-10f);
+    int mine_low = 0, mine_high = 0, all_low = 0, all_high = 0;
+    if (t.found) {
+      queries_of(p, t, min(row, t.keys), min(row + 1, t.keys), &mine_low, &mine_high);
+      const int j1 = min(t.first + kTile, t.keys);
+      int unused;
+      if (t.first < j1) {
+        queries_of(p, t, j1 - 1, j1, &all_low, &unused);
+        queries_of(p, t, t.first, t.first + 1, &unused, &all_high);
+      }
+    }
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int s = it % C::kStages, first = (from + it % per) * kTile;
+      const bool partial = first < all_low || first + kTile > all_high;
+      const int a = mine_low - first - w * 64, b = mine_high - first - w * 64;
+      ok = warp_wait(&full[s], (it / C::kStages) & 1, failed) && warp_wait(&s_full, it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[2][32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(tmem_s + lanes + w * 64 + q * 32, x[q]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_wait_ld(x[q]);
+      const float4* l4 = reinterpret_cast<const float4*>(&stat[s][0][w * 64]);
+      uint32_t packed[32];
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        const float4 l = l4[e / 4];
+        const float2 u = fma2(make_float2(as_float(x[e / 32][e % 32]), as_float(x[e / 32][e % 32 + 1])), both(c),
+                              make_float2(l.x, l.y));
+        const float2 v = fma2(make_float2(as_float(x[e / 32][e % 32 + 2]), as_float(x[e / 32][e % 32 + 3])), both(c),
+                              make_float2(l.z, l.w));
+        float r[4] = {fast_exp2(u.x), fast_exp2(u.y), fast_exp2(v.x), fast_exp2(v.y)};
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (e + i < a || e + i >= b) r[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[(e + i) / 32][(e + i) % 32] = __float_as_uint(r[i]);
+        packed[e / 2] = pack2<T>(r[0], r[1]);
+        packed[e / 2 + 1] = pack2<T>(r[2], r[3]);
+      }
+      tmem_st_32x32b_x32(tmem_s + lanes + w * 64, packed);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_done);
+
+      ok = warp_wait(&dp_full, it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t y[2][32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(tmem_dp + lanes + w * 64 + q * 32, y[q]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_wait_ld(y[q]);
+      const float4* d4 = reinterpret_cast<const float4*>(&stat[s][1][w * 64]);
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        const float4 d = d4[e / 4];
+        const auto one = [&](int at, float d0, float d1) {
+          float2 v = add2(make_float2(as_float(y[at / 32][at % 32]), as_float(y[at / 32][at % 32 + 1])),
+                          make_float2(d0, d1));
+          if constexpr (!kBf16<T>) v = mul2(v, both(raise));
+          v = mul2(v, make_float2(as_float(x[at / 32][at % 32]), as_float(x[at / 32][at % 32 + 1])));
+          if (partial) {
+            if (at < a || at >= b) v.x = 0.0f;
+            if (at + 1 < a || at + 1 >= b) v.y = 0.0f;
+          }
+          return pack2<T>(v.x, v.y);
+        };
+        packed[e / 2] = one(e, d.x, d.y);
+        packed[e / 2 + 1] = one(e + 2, d.z, d.w);
+      }
+      tmem_st_32x32b_x32(tmem_dp + lanes + w * 64, packed);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ds_done);
+    }
+    if (ok && n > 0) ok = warp_wait(&finished, 0, failed);
+    tc_fence_after();
+    // the first half writes dv, the other dk
+    const int64_t at = static_cast<int64_t>(t.batch) * p.keys + t.row0 + row;
+    T* grad = static_cast<T*>(w == 0 ? p.out2 : p.out) + (at * p.kv_heads + kv_head) * p.dim;
+    const bool write = ok && t.found && row < t.stored, some = mine_low < mine_high;
+    const float by = w == 0 ? (kBf16<T> ? 1.0f : 0x1p-10f) : p.scale / ds_factor<T>(p);
+    if (n > 0) store_row<T, kCols>(grad, nullptr, (w == 0 ? tmem_dv : tmem_dk) + lanes, p.dim, by, write && some);
+    if (write && (n == 0 || !some)) zero_row(grad, p.dim);
+  }
+  finish(tmem, failed, fills, full, C::kStages, n > 0 ? &kv_full : nullptr, nullptr, &drained);
+}
+
+// ------------------------------------------------------------ backward: queries
+// One tile of queries a block.  Two tiles of scores in tensor memory, one of
+// dp: the products of the next keys run while ds is worked on, which takes the
+// place of its scores.
+template <typename T, int kCols>
+__global__ void __launch_bounds__(kThreads, 1)
+    query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
+                      const __grid_constant__ Problem p, int tiles) {
+  using C = KeyGrads<kCols>;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t q_full, s_full[2], dp_full, dp_read, ds_done, finished, drained, full[C::kStages], empty[C::kStages];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed_word;
+  volatile int* failed = &failed_word;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
+  uint8_t* tile_q = smem;
+  uint8_t* tile_g = smem + C::kTileBytes;
+  uint8_t* ring = smem + 2 * C::kTileBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&dp_full, 1);
+    mbar_init(&dp_read, 256);
+    mbar_init(&ds_done, 256);
+    mbar_init(&finished, 1);
+    mbar_init(&drained, 1);
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    fence_mbar_init();
+    failed_word = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kTmemColumns);
+  tc_fence_before();
+  begin_kernel();
+  const int head = blockIdx.x % p.heads, index = tiles - 1 - static_cast<int>(blockIdx.x) / p.heads;
+  const Tile t = find_tile<kTile>(p, index, p.length);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tmem_dp = tmem + 2 * kTile, tmem_dq = tmem + 3 * kTile;
+  int low = 0, high = 0;
+  if (t.found) keys_of(p, t, min(t.first, t.queries), min(t.first + kTile, t.queries), &low, &high);
+  const int from = low / kTile, to = low < high ? (high + kTile - 1) / kTile : from;
+  const int n = to - from;
+
+  int fills = 0;
+  if (warp == kLoadWarp) {
+    if (lane == 0 && n > 0) {
+      const int kv_head = head / (p.heads / p.kv_heads);
+      bool ok = true;
+      mbar_arrive_expect_tx(&q_full, 2 * C::kTileBytes);
+      load_tile<kCols>(tile_q, &map_q, &q_full, t.row0 + t.first, head, t.batch);
+      load_tile<kCols>(tile_g, &map_g, &q_full, t.row0 + t.first, head, t.batch);
+      for (int it = 0; it < n; ++it) {
+        const int s = it % C::kStages, row = t.row0 + (from + it) * kTile;
+        if (it >= C::kStages) ok = ring_wait(&empty[s], (it / C::kStages - 1) & 1, failed);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&full[s], 2 * C::kTileBytes);
+        load_tile<kCols>(ring + 2 * s * C::kTileBytes, &map_k, &full[s], row, kv_head, t.batch);
+        load_tile<kCols>(ring + (2 * s + 1) * C::kTileBytes, &map_v, &full[s], row, kv_head, t.batch);
+        ++fills;
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    const uint32_t id_s = idesc_16bit(kBf16<T>, kTile, 0), id_o = idesc_16bit(kBf16<T>, (p.dim + 15) / 16 * 16, 1);
+    const int steps = (p.dim + 15) / 16;
+    bool ok = n == 0 || warp_wait(&q_full, 0, failed);
+    const auto arrived = [&](int it) {
+      const int s = it % C::kStages;
+      if (!warp_wait(&full[s], (it / C::kStages) & 1, failed)) return false;
+      const int valid = t.keys - (from + it) * kTile;
+      if ((p.offsets != nullptr || p.lengths != nullptr) && valid < kTile)
+        zero_rows<kCols>(ring + 2 * s * C::kTileBytes, valid);
+      return true;
+    };
+    if (ok && n > 0) {
+      ok = arrived(0);
+      if (ok && lane == 0) {
+        scores(tmem, tile_q, ring, id_s, steps);
+        umma_commit(&s_full[0]);
+        scores(tmem_dp, tile_g, ring + C::kTileBytes, id_s, steps);
+        umma_commit(&dp_full);
+      }
+      __syncwarp();
+    }
+    for (int it = 0; it < n && ok; ++it) {
+      const uint8_t* tile_k = ring + 2 * (it % C::kStages) * C::kTileBytes;
+      const uint8_t* next_k = ring + 2 * ((it + 1) % C::kStages) * C::kTileBytes;
+      const bool more = it + 1 < n;
+      if (more) {
+        ok = arrived(it + 1);
+        if (!ok) break;
+        if (lane == 0) {
+          scores(tmem + ((it + 1) & 1) * kTile, tile_q, next_k, id_s, steps);
+          umma_commit(&s_full[(it + 1) & 1]);
+        }
+        __syncwarp();
+        ok = warp_wait(&dp_read, it & 1, failed);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          scores(tmem_dp, tile_g, next_k + C::kTileBytes, id_s, steps);
+          umma_commit(&dp_full);
+        }
+        __syncwarp();
+      }
+      ok = warp_wait(&ds_done, it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        weighted(tmem_dq, tmem + (it & 1) * kTile, 64, tile_k, id_o, it > 0);
+        umma_commit(&empty[it % C::kStages]);
+        if (!more) umma_commit(&finished);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int w = warp / 4, row = t.first + threadIdx.x % 128;  // both halves have all queries
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
+    const float factor = ds_factor<T>(p), c = p.scale * kLog2e, raise = factor * (kBf16<T> ? 1.0f : 0x1p-10f);
+    int mine_low = 0, mine_high = 0, all_low = 0, all_high = 0;
+    if (t.found) {
+      keys_of(p, t, min(row, t.queries), min(row + 1, t.queries), &mine_low, &mine_high);
+      const int i1 = min(t.first + kTile, t.queries);
+      int unused;
+      if (t.first < i1) {
+        keys_of(p, t, i1 - 1, i1, &all_low, &unused);
+        keys_of(p, t, t.first, t.first + 1, &unused, &all_high);
+      }
+    }
+    const int64_t at = static_cast<int64_t>(t.batch) * p.length + t.row0 + row;
+    float lse = -INFINITY, delta = 0.0f;
+    if (t.found && row < t.queries) {
+      lse = p.stats[head * p.rows + at];
+      delta = p.stats[(p.heads + head) * p.rows + at];
+    }
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int first = (from + it) * kTile;
+      const bool partial = first < all_low || first + kTile > all_high;
+      const int a = mine_low - first - w * 64, b = mine_high - first - w * 64;
+      const uint32_t s_at = tmem + (it & 1) * kTile + lanes + w * 64;
+      ok = warp_wait(&s_full[it & 1], (it / 2) & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[2][32], y[2][32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(s_at + q * 32, x[q]);
+      ok = warp_wait(&dp_full, it & 1, failed);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(tmem_dp + lanes + w * 64 + q * 32, y[q]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_wait_ld(x[q]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_wait_ld(y[q]);
+      tc_fence_before();
+      mbar_arrive(&dp_read);
+      uint32_t packed[32];
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float2 u = fma2(make_float2(as_float(x[e / 32][e % 32]), as_float(x[e / 32][e % 32 + 1])), both(c), both(lse));
+        float2 v = add2(make_float2(as_float(y[e / 32][e % 32]), as_float(y[e / 32][e % 32 + 1])), both(delta));
+        if constexpr (!kBf16<T>) v = mul2(v, both(raise));
+        v = mul2(v, make_float2(fast_exp2(u.x), fast_exp2(u.y)));
+        if (partial) {
+          if (e < a || e >= b) v.x = 0.0f;
+          if (e + 1 < a || e + 1 >= b) v.y = 0.0f;
+        }
+        packed[e / 2] = pack2<T>(v.x, v.y);
+      }
+      tmem_st_32x32b_x32(s_at, packed);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ds_done);
+    }
+    if (ok && n > 0) ok = warp_wait(&finished, 0, failed);
+    tc_fence_after();
+    if (w == 0) {
+      T* grad = static_cast<T*>(p.out) + (at * p.heads + head) * p.dim;
+      const bool write = ok && t.found && row < t.stored, some = mine_low < mine_high;
+      if (n > 0) store_row<T, kCols>(grad, nullptr, tmem_dq + lanes, p.dim, p.scale / factor, write && some);
+      if (write && (n == 0 || !some)) zero_row(grad, p.dim);
+    }
+  }
+  finish(tmem, failed, fills, full, C::kStages, n > 0 ? &q_full : nullptr, nullptr, &drained);
 }
 
 // ------------------------------------------------------------ host side
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<EncodeTiled>(f) : nullptr;
+  }();
+  return fn;
+}
+
+// [dim, rows, heads, batch] in boxes of 64 columns of 128 rows; what is outside
+// reads as zeros.
+int encode(CUtensorMap* map, const void* base, const muon_train_strides& s, int64_t rows, int64_t heads, int64_t batch,
+           int64_t dim, int dtype) {
+  const EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return MUON_POLAR_ERR_DRIVER;
+  // the stride of an axis of one element is never used, but has to be a legal one
+  const auto stride = [](int64_t n, int64_t v) { return static_cast<cuuint64_t>(n > 1 ? v * 2 : 16); };
+  const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads),
+                               static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[3] = {stride(rows, s.row), stride(heads, s.head), stride(batch, s.batch)};
+  const cuuint32_t box[4] = {64, kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, dtype == MUON_TRAIN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        4, const_cast<void*>(base), sizes, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MUON_POLAR_OK : MUON_POLAR_ERR_TENSOR_MAP;
+}
+
 int check(const muon_train_attention_args* a) {
   constexpr int64_t kMost = int64_t{1} << 30;
   if (a == nullptr || a->batch < 0 || a->length < 0 || a->keys < 0 || a->heads < 1 || a->kv_heads < 1 ||
@@ -209,13 +1094,18 @@ int check(const muon_train_attention_args* a) {
       a->batch * a->keys > kMost || a->heads > 65535)
     return MUON_POLAR_ERR_INVALID_ARGUMENT;
   if ((a->lengths != nullptr || a->offsets != nullptr) && a->keys != a->length) return MUON_POLAR_ERR_INVALID_ARGUMENT;
-  if (a->offsets != nullptr &&
-      (a->lengths != nullptr || a->batch != 1 || a->sequences < 0 || a->sequences > kMost))
+  if (a->offsets != nullptr && (a->lengths != nullptr || a->batch != 1 || a->sequences < 0 || a->sequences > kMost))
+    return MUON_POLAR_ERR_INVALID_ARGUMENT;
+  // tiles times heads number the blocks
+  const int64_t most = (a->length > a->keys ? a->length : a->keys) / kTile + 1;
+  if ((most * a->batch + (a->offsets != nullptr ? a->sequences + 2 : 0)) * a->heads >= (int64_t{1} << 31))
     return MUON_POLAR_ERR_INVALID_ARGUMENT;
   return MUON_POLAR_OK;
 }
 bool strided(const void* p, const muon_train_strides& s, int64_t batch, int64_t rows, int64_t heads) {
-  const auto fits = [](int64_t n, int64_t stride) { return n <= 1 || (stride >= 8 && stride % 8 == 0); };
+  const auto fits = [](int64_t n, int64_t stride) {
+    return n <= 1 || (stride >= 8 && stride % 8 == 0 && stride < (int64_t{1} << 38));
+  };
   return p != nullptr && aligned16(p) && fits(batch, s.batch) && fits(rows, s.row) && fits(heads, s.head);
 }
 int check_forward(const muon_train_attention_args& a) {
@@ -223,26 +1113,150 @@ int check_forward(const muon_train_attention_args& a) {
   if (a.batch * a.keys > 0 && (!strided(a.k, a.k_stride, a.batch, a.keys, a.kv_heads) ||
                                !strided(a.v, a.v_stride, a.batch, a.keys, a.kv_heads)))
     return MUON_POLAR_ERR_ALIGNMENT;
-  if (a.batch * a.length > 0 && (a.out == nullptr || !aligned16(a.out) || a.lse == nullptr))
+  if (a.batch * a.length > 0 &&
+      (a.out == nullptr || !aligned16(a.out) || !aligned16(a.out_rest) || a.lse == nullptr))
     return MUON_POLAR_ERR_INVALID_ARGUMENT;
   return MUON_POLAR_OK;
 }
 
-dim3 grid_for(int64_t rows, int64_t heads) {
-  return dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps), static_cast<unsigned>(heads));
+// Tiles of `size` rows of all sequences, at most.
+int64_t tiles_of(const muon_train_attention_args& a, int64_t rows, int64_t size) {
+  if (a.offsets != nullptr) return rows / size + a.sequences + 2;
+  return a.batch * ((rows + size - 1) / size);
+}
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+int encode_inputs(const muon_train_attention_args& a, Maps* m) {
+  // a thread that has made no CUDA call yet (autograd's) has no context, which the encoder needs
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  int rc = encode(&m->q, a.q, a.q_stride, a.length, a.heads, a.batch, a.dim, a.dtype);
+  // without keys no tile of them is loaded: any legal map will do
+  if (a.keys == 0) {
+    m->k = m->v = m->q;
+    return rc;
+  }
+  if (rc == MUON_POLAR_OK) rc = encode(&m->k, a.k, a.k_stride, a.keys, a.kv_heads, a.batch, a.dim, a.dtype);
+  if (rc == MUON_POLAR_OK) rc = encode(&m->v, a.v, a.v_stride, a.keys, a.kv_heads, a.batch, a.dim, a.dtype);
+  return rc;
+}
+
+Problem problem_of(const muon_train_attention_args& a) {
+  Problem p{};
+  p.lse = a.lse;
+  p.lengths = a.lengths;
+  p.offsets = a.offsets;
+  p.rows = a.batch * a.length;
+  p.length = static_cast<int>(a.length);
+  p.keys = static_cast<int>(a.keys);
+  p.heads = static_cast<int>(a.heads);
+  p.kv_heads = static_cast<int>(a.kv_heads);
+  p.dim = static_cast<int>(a.dim);
+  p.sequences = static_cast<int>(a.sequences);
+  p.batch = static_cast<int>(a.batch);
+  // no two places are further apart than there are queries or keys
+  const int64_t span = a.length > a.keys ? a.length : a.keys;
+  p.window = a.window >= span ? 0 : static_cast<int>(a.window);
+  p.causal = a.causal != 0;
+  p.scale = a.scale;
+  return p;
+}
+
+template <typename T, int kCols>
+int forward(const muon_train_attention_args& a, void* stream) {
+  Maps m;
+  int rc = encode_inputs(a, &m);
+  if (rc != MUON_POLAR_OK) return rc;
+  Problem p = problem_of(a);
+  p.out = a.out;
+  p.out2 = a.out_rest;
+  constexpr int kBytes = Forward<kCols>::kBytes;
+  rc = allow_smem<forward_kernel<T, kCols>>(kBytes);
+  if (rc != MUON_POLAR_OK) return rc;
+  const int64_t tiles = tiles_of(a, a.length, 2 * kTile);
+  return launch(forward_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.heads)), kThreads, kBytes, 1, true, stream,
+                m.q, m.k, m.v, p, static_cast<int>(tiles));
+}
+
+template <typename T, int kCols>
+int backward(const muon_train_attention_args& a, const muon_train_attention_grads& g, void* stream) {
+  const int64_t rows = a.batch * a.length;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {  // keys that nothing looks at
+    const size_t bytes = static_cast<size_t>(a.batch * a.keys * a.kv_heads * a.dim) * sizeof(T);
+    if (bytes == 0) return MUON_POLAR_OK;
+    cudaError_t e = cudaMemsetAsync(g.grad_k, 0, bytes, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(g.grad_v, 0, bytes, s);
+    return static_cast<int>(e);
+  }
+  Maps m;
+  CUtensorMap map_g;
+  int rc = encode_inputs(a, &m);
+  if (rc == MUON_POLAR_OK) rc = encode(&map_g, g.grad_out, g.grad_out_stride, a.length, a.heads, a.batch, a.dim, a.dtype);
+  if (rc != MUON_POLAR_OK) return rc;
+  Problem p = problem_of(a);
+  float* stats = static_cast<float*>(g.workspace) + 4;
+  uint32_t* largest = static_cast<uint32_t*>(g.workspace);
+  p.stats = stats;
+  p.largest = static_cast<const float*>(g.workspace);
+  const int length = p.length, heads = p.heads, dim = p.dim;
+  const dim3 grid(static_cast<unsigned>((rows * heads + 15) / 16));
+  if constexpr (!kBf16<T>) {
+    const cudaError_t e = cudaMemsetAsync(largest, 0, 16, s);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (a.keys > 0) {
+      int sms = 0;
+      rc = sm_count(&sms);
+      if (rc != MUON_POLAR_OK) return rc;
+      const int64_t items = a.batch * a.keys * a.kv_heads, blocks = (items + 15) / 16, most = 8 * sms;
+      rc = launch(largest_kernel<T>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), 256, 0, 1, false, stream,
+                  static_cast<const T*>(a.v), a.v_stride, largest + 1, a.batch * a.keys, p.keys, p.kv_heads, dim);
+      if (rc != MUON_POLAR_OK) return rc;
+    }
+  }
+  rc = launch(stats_kernel<T, !kBf16<T>>, grid, 256, 0, 1, true, stream, static_cast<const T*>(a.out),
+              static_cast<const T*>(a.out_rest), static_cast<const T*>(g.grad_out), g.grad_out_stride,
+              static_cast<const float*>(a.lse), stats, largest, rows, length, heads, dim);
+  if (rc != MUON_POLAR_OK) return rc;
+  constexpr int kBytes = KeyGrads<kCols>::kBytes;
+  if (a.keys > 0) {
+    rc = allow_smem<key_grad_kernel<T, kCols>>(kBytes);
+    if (rc != MUON_POLAR_OK) return rc;
+    p.out = g.grad_k;
+    p.out2 = g.grad_v;
+    const int64_t tiles = tiles_of(a, a.keys, kTile);
+    rc = launch(key_grad_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.kv_heads)), kThreads, kBytes, 1, true,
+                stream, m.q, m.k, m.v, map_g, p);
+    if (rc != MUON_POLAR_OK) return rc;
+  }
+  rc = allow_smem<query_grad_kernel<T, kCols>>(kBytes);
+  if (rc != MUON_POLAR_OK) return rc;
+  p.out = g.grad_q;
+  p.out2 = nullptr;
+  const int64_t tiles = tiles_of(a, a.length, kTile);
+  return launch(query_grad_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.heads)), kThreads, kBytes, 1, true,
+                stream, m.q, m.k, m.v, map_g, p, static_cast<int>(tiles));
 }
 
 template <typename T>
+int forward(const muon_train_attention_args& a, void* stream) {
+  return a.dim <= 64 ? forward<T, 64>(a, stream) : forward<T, 128>(a, stream);
+}
+template <typename T>
 int backward(const muon_train_attention_args& a, const muon_train_attention_grads& g, void* stream) {
-  if (a.batch * a.length > 0) {
-    const int rc = launch(query_grad_kernel<T>, grid_for(a.batch * a.length, a.heads), kWarps * 32, 0, 1, true, stream, a, g);
-    if (rc != MUON_POLAR_OK) return rc;
-  }
-  if (a.batch * a.keys == 0) return MUON_POLAR_OK;
-  return launch(key_grad_kernel<T>, grid_for(a.batch * a.keys, a.kv_heads), kWarps * 32, 0, 1, true, stream, a, g);
+  return a.dim <= 64 ? backward<T, 64>(a, g, stream) : backward<T, 128>(a, g, stream);
 }
 
 }  // namespace
+
+cudaError_t attention_status(uint32_t* flags, int clear) { return take_status(flags, clear); }
+cudaError_t attention_put_wait_limit(uint64_t limit_ns) { return put_wait_limit(limit_ns); }
+cudaError_t attention_get_wait_limit(uint64_t* limit_ns) { return get_wait_limit(limit_ns); }
+
 }  // namespace muon_train
 
 extern "C" {
@@ -252,16 +1266,13 @@ int muon_train_attention_sm100(const muon_train_attention_args* args, void* stre
   int rc = check(args);
   if (rc == MUON_POLAR_OK) rc = check_forward(*args);
   if (rc != MUON_POLAR_OK || args->batch * args->length == 0) return rc;
-  const dim3 grid = grid_for(args->batch * args->length, args->heads);
-  return args->dtype == MUON_TRAIN_BF16
-             ? launch(forward_kernel<__nv_bfloat16>, grid, kWarps * 32, 0, 1, true, stream, *args)
-             : launch(forward_kernel<__half>, grid, kWarps * 32, 0, 1, true, stream, *args);
+  return args->dtype == MUON_TRAIN_BF16 ? forward<__nv_bfloat16>(*args, stream) : forward<__half>(*args, stream);
 }
 
 size_t muon_train_attention_workspace_bytes(const muon_train_attention_args* args) {
   using namespace muon_train;
   if (check(args) != MUON_POLAR_OK) return 0;
-  return static_cast<size_t>(args->heads * args->batch * args->length + 4) * sizeof(float);
+  return static_cast<size_t>(2 * args->heads * args->batch * args->length + 4) * sizeof(float);
 }
 
 int muon_train_attention_backward_sm100(const muon_train_attention_args* args,
@@ -280,7 +1291,8 @@ int muon_train_attention_backward_sm100(const muon_train_attention_args* args,
         g.workspace_bytes < muon_train_attention_workspace_bytes(args))
       return MUON_POLAR_ERR_WORKSPACE;
   }
-  if (a.batch * a.keys > 0 && (g.grad_k == nullptr || g.grad_v == nullptr || !aligned16(g.grad_k) || !aligned16(g.grad_v)))
+  if (a.batch * a.keys > 0 &&
+      (g.grad_k == nullptr || g.grad_v == nullptr || !aligned16(g.grad_k) || !aligned16(g.grad_v)))
     return MUON_POLAR_ERR_INVALID_ARGUMENT;
   return a.dtype == MUON_TRAIN_BF16 ? backward<__nv_bfloat16>(a, g, stream) : backward<__half>(a, g, stream);
 }

@@ -110,28 +110,34 @@ AttentionInputs CheckAttention(const Tensor& q, const Tensor& k, const Tensor& v
   return in;
 }
 
-std::tuple<Tensor, Tensor> AttentionCuda(const Tensor& q, const Tensor& k, const Tensor& v,
-                                         const OptTensor& offsets, const OptTensor& lengths, bool causal,
-                                         int64_t window, double scale) {
+// (out, lse, rest): with `keep`, rest is what rounding took from out, for the
+// backward pass; else it is empty.
+std::tuple<Tensor, Tensor, Tensor> AttentionCuda(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                 const OptTensor& offsets, const OptTensor& lengths, bool causal,
+                                                 int64_t window, double scale, bool keep) {
   const char* who = "attention";
   const c10::cuda::OptionalCUDAGuard guard(q.device().is_cuda() ? std::make_optional(q.device()) : std::nullopt);
   AttentionInputs in = CheckAttention(q, k, v, offsets, lengths, causal, window, scale, who);
   Tensor out = Empty(q.sizes(), q.scalar_type(), q);
   Tensor lse = Empty({in.args.heads, in.args.batch * in.args.length}, at::kFloat, q);
+  Tensor rest = keep ? Empty(q.sizes(), q.scalar_type(), q) : Empty({0}, q.scalar_type(), q);
   in.args.out = Ptr(out);
+  in.args.out_rest = keep ? Ptr(rest) : nullptr;
   in.args.lse = static_cast<float*>(Ptr(lse));
   CheckStatus(muon_train_attention_sm100(&in.args, Stream(q)), who);
-  return {out, lse};
+  return {out, lse, rest};
 }
 
 std::tuple<Tensor, Tensor, Tensor> AttentionBackwardCuda(
     const Tensor& grad_out, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-    const Tensor& lse, const OptTensor& offsets, const OptTensor& lengths, bool causal, int64_t window,
+    const Tensor& lse, const Tensor& rest, const OptTensor& offsets, const OptTensor& lengths, bool causal, int64_t window,
     double scale) {
   const char* who = "attention_backward";
   const c10::cuda::OptionalCUDAGuard guard(q.device().is_cuda() ? std::make_optional(q.device()) : std::nullopt);
   AttentionInputs in = CheckAttention(q, k, v, offsets, lengths, causal, window, scale, who);
-  for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{grad_out, "grad_out"}, {out, "out"}}) {
+  for (const auto& [t, name] :
+       {std::pair<const Tensor&, const char*>{grad_out, "grad_out"}, {out, "out"}, {rest, "rest"}}) {
+    if (&t == &rest && t.numel() == 0) continue;
     CheckDevice(t, q, who, name);
     TORCH_CHECK_VALUE(t.sizes() == q.sizes(), who, ": ", name, " must have query's shape ", q.sizes(), ", got ",
                       t.sizes());
@@ -141,9 +147,10 @@ std::tuple<Tensor, Tensor, Tensor> AttentionBackwardCuda(
   TORCH_CHECK_TYPE(lse.scalar_type() == at::kFloat, who, ": lse must be float32");
   TORCH_CHECK_VALUE(lse.dim() == 2 && lse.size(0) == in.args.heads && lse.size(1) == in.args.batch * in.args.length,
                     who, ": lse must have shape [heads, batch * length]");
-  const Tensor kept_out = out.contiguous(), kept_lse = lse.contiguous();
+  const Tensor kept_out = out.contiguous(), kept_lse = lse.contiguous(), kept_rest = rest.contiguous();
   const Tensor g = Heads4d(in.offsets.defined() ? grad_out.unsqueeze(0) : grad_out);
   in.args.out = Ptr(kept_out);
+  in.args.out_rest = kept_rest.numel() > 0 ? Ptr(kept_rest) : nullptr;
   in.args.lse = static_cast<float*>(Ptr(kept_lse));
   Tensor dq = Empty(q.sizes(), q.scalar_type(), q), dk = Empty(k.sizes(), q.scalar_type(), q);
   Tensor dv = Empty(v.sizes(), q.scalar_type(), q);
@@ -315,7 +322,7 @@ Tensor ClipOutCuda(at::TensorList grads, at::TensorList out, double max_norm, bo
 
 // ------------------------------------------------------------ autograd
 struct AttentionBackward : public torch::autograd::Node {
-  SavedVariable q, k, v, out, lse, offsets, lengths;
+  SavedVariable q, k, v, out, lse, rest, offsets, lengths;
   bool causal = false;
   int64_t window = 0;
   double scale = 1.0;
@@ -323,7 +330,7 @@ struct AttentionBackward : public torch::autograd::Node {
   std::string name() const override { return "AttentionBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* s : {&q, &k, &v, &out, &lse, &offsets, &lengths}) s->reset_data();
+    for (SavedVariable* s : {&q, &k, &v, &out, &lse, &rest, &offsets, &lengths}) s->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     NoSecondOrder(grads, "attention");
@@ -331,8 +338,8 @@ struct AttentionBackward : public torch::autograd::Node {
     if (!grads[0].defined()) return variable_list(3);
     static auto op = Op<decltype(AttentionBackwardCuda)>("muon_ascend950::attention_backward");
     auto [dq, dk, dv] = op.call(grads[0], q.unpack(), k.unpack(), v.unpack(), out.unpack(shared_from_this()),
-                                lse.unpack(), Optional(offsets.unpack()), Optional(lengths.unpack()), causal,
-                                window, scale);
+                                lse.unpack(), rest.unpack(), Optional(offsets.unpack()),
+                                Optional(lengths.unpack()), causal, window, scale);
     variable_list all(3);
     Tensor* made[3] = {&dq, &dk, &dv};
     for (size_t i = 0; i < 3; ++i)
@@ -341,22 +348,24 @@ struct AttentionBackward : public torch::autograd::Node {
   }
 };
 
-std::tuple<Tensor, Tensor> AttentionAutograd(const Tensor& q, const Tensor& k, const Tensor& v,
-                                             const OptTensor& offsets, const OptTensor& lengths, bool causal,
-                                             int64_t window, double scale) {
+std::tuple<Tensor, Tensor, Tensor> AttentionAutograd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                     const OptTensor& offsets, const OptTensor& lengths, bool causal,
+                                                     int64_t window, double scale, bool keep) {
   static auto op = Op<decltype(AttentionCuda)>("muon_ascend950::attention");
+  const bool recorded = Recorded({&q, &k, &v});
   const auto call = [&] {
     at::AutoDispatchBelowADInplaceOrView guard;
-    return op.call(q, k, v, offsets, lengths, causal, window, scale);
+    return op.call(q, k, v, offsets, lengths, causal, window, scale, keep || recorded);
   };
   NoTangents({&q, &k, &v}, "attention");
-  if (!Recorded({&q, &k, &v})) return call();
+  if (!recorded) return call();
   auto node = MakeNode<AttentionBackward>(q, k, v);
   auto result = call();
   node->q = SavedVariable(q, false);
   node->k = SavedVariable(k, false);
   node->v = SavedVariable(v, false);
   node->lse = SavedVariable(std::get<1>(result), false);
+  node->rest = SavedVariable(std::get<2>(result), false);
   node->offsets = SavedVariable(Given(offsets), false);
   node->lengths = SavedVariable(Given(lengths), false);
   node->causal = causal;
@@ -425,9 +434,9 @@ std::tuple<Tensor, Tensor> RotaryForwardCuda(const Tensor& q, const OptTensor& k
 
 TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
   m.def("attention(Tensor query, Tensor key, Tensor value, Tensor? offsets, Tensor? lengths, bool causal, "
-        "int window, float scale) -> (Tensor out, Tensor lse)");
+        "int window, float scale, bool keep) -> (Tensor out, Tensor lse, Tensor rest)");
   m.def("attention_backward(Tensor grad_out, Tensor query, Tensor key, Tensor value, Tensor out, Tensor lse, "
-        "Tensor? offsets, Tensor? lengths, bool causal, int window, float scale) -> (Tensor, Tensor, Tensor)");
+        "Tensor rest, Tensor? offsets, Tensor? lengths, bool causal, int window, float scale) -> (Tensor, Tensor, Tensor)");
   m.def("rotary(Tensor query, Tensor? key, Tensor positions, Tensor frequencies, bool interleaved, "
         "float scale) -> (Tensor, Tensor)");
   m.def("rotary_backward(Tensor grad_query, Tensor? grad_key, Tensor positions, Tensor frequencies, "

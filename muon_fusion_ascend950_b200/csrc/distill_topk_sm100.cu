@@ -9,6 +9,7 @@
 // Bound by memory: the vocabulary is read once (and the gradient written
 // once); the lists are a thousandth of it.
 #include <algorithm>
+#include <algorithm>
 #include <cfloat>
 
 #include "sm100_ptx.cuh"
@@ -19,10 +20,14 @@ namespace muon_train {
 cudaError_t norm_status(uint32_t* flags, int clear);  // residual_norm_sm100.cu
 cudaError_t norm_put_wait_limit(uint64_t limit_ns);
 cudaError_t norm_get_wait_limit(uint64_t* limit_ns);
+cudaError_t attention_status(uint32_t* flags, int clear);  // attention_sm100.cu
+cudaError_t attention_put_wait_limit(uint64_t limit_ns);
+cudaError_t attention_get_wait_limit(uint64_t* limit_ns);
 
 cudaError_t set_wait_limit(uint64_t limit_ns) {  // called by muon_polar_set_wait_limit_ns
-  const cudaError_t e = put_wait_limit(limit_ns);
-  return e != cudaSuccess ? e : norm_put_wait_limit(limit_ns);
+  cudaError_t e = put_wait_limit(limit_ns);
+  if (e == cudaSuccess) e = norm_put_wait_limit(limit_ns);
+  return e != cudaSuccess ? e : attention_put_wait_limit(limit_ns);
 }
 
 std::atomic<uint64_t>& launch_counter() {
@@ -823,6 +828,7 @@ int muon_train_read_device_status(int device, uint32_t* flags, int clear) {
   e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = muon_train::take_status(&v, clear);
   if (e == cudaSuccess) e = muon_train::norm_status(&v, clear);
+  if (e == cudaSuccess) e = muon_train::attention_status(&v, clear);
   if (device != prev) cudaSetDevice(prev);
   if (e != cudaSuccess) return static_cast<int>(e);
   *flags = v;
@@ -831,11 +837,12 @@ int muon_train_read_device_status(int device, uint32_t* flags, int clear) {
 
 int muon_train_wait_limit_ns(uint64_t* limit_ns) {
   if (limit_ns == nullptr) return MUON_POLAR_ERR_INVALID_ARGUMENT;
-  uint64_t distill = 0, norm = 0;
-  cudaError_t e = muon_train::get_wait_limit(&distill);
-  if (e == cudaSuccess) e = muon_train::norm_get_wait_limit(&norm);
+  uint64_t limit[3] = {};
+  cudaError_t e = muon_train::get_wait_limit(&limit[0]);
+  if (e == cudaSuccess) e = muon_train::norm_get_wait_limit(&limit[1]);
+  if (e == cudaSuccess) e = muon_train::attention_get_wait_limit(&limit[2]);
   if (e != cudaSuccess) return static_cast<int>(e);
-  *limit_ns = distill > norm ? distill : norm;
+  *limit_ns = std::max({limit[0], limit[1], limit[2]});
   return MUON_POLAR_OK;
 }
 

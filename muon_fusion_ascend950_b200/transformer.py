@@ -163,7 +163,7 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ca
             scale = query.shape[-1] ** -0.5
         if window is not None and window < 1:
             raise ValueError(f"window must be positive, got {window}")
-        return _attention(query, key, value, offsets, lengths, causal, window or 0, scale)[0]
+        return _attention(query, key, value, offsets, lengths, causal, window or 0, scale, False)[0]
     except Exception:
         _explain(query=query, key=key, value=value)
         _explain(**{n: t for n, t in (("offsets", offsets), ("lengths", lengths)) if t is not None})

@@ -690,9 +690,9 @@ def test_debug_sync_waits_for_every_call(pkg, monkeypatch):
     x, weight, at, f, go = step_inputs(pkg)
     q = randn(1, 64, 2, 64, seed=3, dtype=BF16)
     ops = torch.ops.muon_ascend950
-    out, lse = ops.attention(q, q, q, None, None, True, 0, 0.125)
-    calls = [lambda: ops.attention(q, q, q, None, None, True, 0, 0.125),
-             lambda: ops.attention_backward(q, q, q, q, out, lse, None, None, True, 0, 0.125),
+    out, lse, rest = ops.attention(q, q, q, None, None, True, 0, 0.125, True)
+    calls = [lambda: ops.attention(q, q, q, None, None, True, 0, 0.125, False),
+             lambda: ops.attention_backward(q, q, q, q, out, lse, rest, None, None, True, 0, 0.125),
              lambda: ops.rotary(q, None, at[:64], f, False, 1.0),
              lambda: ops.clip_gradients_([q.clone()], 1.0, False)]
     for sync in (False, True):
