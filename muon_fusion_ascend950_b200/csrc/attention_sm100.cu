@@ -12,8 +12,8 @@
 // shared memory.  The scores are read from tensor memory into registers, a row
 // a thread, and the probabilities go back there as 16-bit values, in place of
 // the scores, as the next product's left operand: neither is ever in shared or
-// global memory.  In a block of 320 threads eight warps work on the scores, one
-// loads and one issues the products.
+// global memory.  Eight warps of a block work on the scores, one loads and one issues the
+// products.
 //
 // The backward pass computes the scores again.  It is two kernels, one for a
 // tile of keys (dk, dv: four products a pair of tiles) and one for a tile of
@@ -40,8 +40,12 @@ namespace {
 using namespace muon_sm100;
 
 constexpr int kTile = 128;     // queries, or keys, of a tile
-constexpr int kThreads = 320;  // warps 0-7: scores, 8: loads, 9: products
+constexpr int kThreads = 384;  // warps 0-7: scores, 8: loads, 9: products; 10 and 11 only give registers
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
+// Registers of a thread at launch, and then of the two warpgroups that work on
+// scores and of the third.
+constexpr int kLaunchRegisters = 168, kScoreRegisters = 208, kOtherRegisters = 88;
+static_assert(2 * kScoreRegisters + kOtherRegisters <= 3 * kLaunchRegisters, "no more than there are at launch");
 constexpr uint32_t kTmemColumns = 512;
 constexpr int kAtom = kTile * 128;  // bytes of 64 columns of a tile, the swizzle's width
 
@@ -190,22 +194,43 @@ __device__ __forceinline__ void load_tile(uint8_t* to, const CUtensorMap* map, u
   for (int a = 0; a < kCols / 64; ++a) tma_load_4d(to + a * kAtom, map, bar, a * 64, row, head, batch);
 }
 
-// D[128 x 128] = A B^T over `steps` runs of 16 columns of both tiles.
-__device__ __forceinline__ void scores(uint32_t d, const uint8_t* a, const uint8_t* b, uint32_t idesc, int steps) {
-  const uint32_t pa = smem_addr(a), pb = smem_addr(b);
-  for (int k = 0; k < steps; ++k) {
-    const uint32_t at = (k / 4) * kAtom + (k % 4) * 32;
-    umma_ss(d, smem_desc_sw128(pa + at, 16, 1024), smem_desc_sw128(pb + at, 16, 1024), idesc, k > 0);
+// Operand descriptors of a tile as their two words: the upper one is the same
+// for all tiles, and a step along the summed axis adds to the lower one.  The
+// warp that issues the products shares its scheduler with two that work on
+// scores: behind a branch of one thread, with its operands in plain registers,
+// a product that runs in 64 cycles took 100 to 125 to issue beside busy warps,
+// by a whole warp with the elected lane's predicate 68 to 80.
+struct Operand {
+  uint32_t low, high;
+  __device__ __forceinline__ Operand(const uint8_t* tile, uint32_t lbo) {
+    const uint64_t d = smem_desc_sw128(smem_addr(tile), lbo, 1024);
+    low = static_cast<uint32_t>(d);
+    high = static_cast<uint32_t>(d >> 32);
   }
-}
-// D[128 x n] (+)= A[tmem: 128 x 128] B, B's rows summed over; columns 64 to 127
-// of A begin at column `half` of tensor memory.
-__device__ __forceinline__ void weighted(uint32_t d, uint32_t a, int half, const uint8_t* b, uint32_t idesc,
-                                         bool more) {
-  const uint32_t pb = smem_addr(b);
+  __device__ __forceinline__ uint64_t at(uint32_t bytes) const {
+    return static_cast<uint64_t>(high) << 32 | (low + (bytes >> 4));
+  }
+};
+
+// D[128 x 128] = A B^T over the first `dim` of kCols columns of both tiles.
+template <int kCols>
+__device__ __forceinline__ void scores(uint32_t d, const uint8_t* a, const uint8_t* b, uint32_t idesc, int dim,
+                                       uint32_t el) {
+  const Operand oa(a, 16), ob(b, 16);
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    umma_ts(d, a + (k / 4) * half + (k % 4) * 8, smem_desc_sw128(pb + k * 2048, kAtom, 1024), idesc, more || k > 0);
+  for (int k = 0; k < kCols / 16; ++k)
+    if (k * 16 < dim) {
+      const uint32_t at = (k / 4) * kAtom + (k % 4) * 32;
+      umma_ss(d, oa.at(at), ob.at(at), idesc, k > 0, el);
+    }
+}
+// D[128 x n] (+)= A[tmem: 128 x 64] B, B's rows summed over: four products, of
+// the tile's first 64 rows or its last.
+__device__ __forceinline__ void weighted(uint32_t d, uint32_t a, const uint8_t* b, int half, uint32_t idesc, bool more,
+                                         uint32_t el) {
+  const Operand ob(b + half * 64 * 128, kAtom);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) umma_ts(d, a + k * 8, ob.at(k * 2048), idesc, more || k > 0, el);
 }
 
 template <typename T>
@@ -276,7 +301,7 @@ __device__ __forceinline__ void finish(uint32_t tmem, volatile int* failed, int 
   if (warp == kMmaWarp) {
     tc_fence_after();
     if (*failed) {
-      if (lane == 0) umma_commit(drained);
+      umma_commit(drained, elect_one());
       __syncwarp();
       drain_ring(drained, 1, 0, 0, 1);
       __syncwarp();
@@ -303,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Problem p, int tiles) {
   using C = Forward<kCols>;
   extern __shared__ uint8_t dynamic[];
-  __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_done[2], drained, full[C::kStages], empty[C::kStages];
+  __shared__ uint64_t q_full[2], s_full[2], p_full[2][2], o_done[2], drained, full[C::kStages], empty[C::kStages];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_word;
   volatile int* failed = &failed_word;
@@ -314,7 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kTile);
+      mbar_init(&p_full[i][0], kTile);
+      mbar_init(&p_full[i][1], kTile);
       mbar_init(&o_done[i], 1);
     }
     mbar_init(&drained, 1);
@@ -350,6 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (from[0] < to[0] && from[1] < to[1]) first = min(from[0], from[1]), last = max(to[0], to[1]);
 
   int fills = 0;
+  if (warp >= kLoadWarp) {
+  give_registers<kOtherRegisters>();
   if (warp == kLoadWarp) {
     if (lane == 0 && first < last) {
       const int kv_head = head / (p.heads / p.kv_heads);
@@ -376,19 +404,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kMmaWarp) {
     const uint32_t id_s = idesc_16bit(kBf16<T>, kTile, 0), id_o = idesc_16bit(kBf16<T>, (p.dim + 15) / 16 * 16, 1);
-    const int steps = (p.dim + 15) / 16;
-    int done[2] = {0, 0};  // key tiles whose scores were asked for
-    bool ok = true;
+    const uint32_t el = elect_one();
+    bool asked[2] = {false, false}, ok = true;
     // scores of query tile i with the keys in `slot`
     const auto ask = [&](int i, int slot) {
-      if (done[i] == 0) ok = ok && warp_wait(&q_full[i], 0, failed);
+      if (!asked[i]) ok = ok && warp_wait(&q_full[i], 0, failed);
       if (!ok) return;
-      if (lane == 0) {
-        scores(tmem + i * kTile, smem + i * C::kTileBytes, ring + slot * C::kTileBytes, id_s, steps);
-        umma_commit(&s_full[i]);
-      }
-      __syncwarp();
-      ++done[i];
+      asked[i] = true;
+      scores<kCols>(tmem + i * kTile, smem + i * C::kTileBytes, ring + slot * C::kTileBytes, id_s, p.dim, el);
+      umma_commit(&s_full[i], el);
     };
     int fill = 0;
     if (first < last) {
@@ -396,13 +420,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (ok && from[i] <= first && first < to[i]) ask(i, 0);
-      if (ok && lane == 0) umma_commit(&empty[0]);
+      if (ok) umma_commit(&empty[0], el);
     }
     for (int j = first; j < last && ok; ++j) {
       const int v_slot = (fill + 1) % C::kStages, k_slot = (fill + 2) % C::kStages;
       ok = warp_wait(&full[v_slot], ((fill + 1) / C::kStages) & 1, failed);
       if (!ok) break;
-      tc_fence_after();
       if ((p.offsets != nullptr || p.lengths != nullptr) && (j + 1) * kTile > t.keys)
         zero_rows<kCols>(ring + v_slot * C::kTileBytes, t.keys - j * kTile);
       const bool more = j + 1 < last;
@@ -411,25 +434,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 2; ++i) {
         if (ok && from[i] <= j && j < to[i]) {
           const int it = j - from[i];
-          ok = warp_wait(&p_full[i], it & 1, failed);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            weighted(tmem + 2 * kTile + i * kCols, tmem + i * kTile, 32, ring + v_slot * C::kTileBytes, id_o, it > 0);
-            umma_commit(&o_done[i]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            ok = ok && warp_wait(&p_full[i][half], it & 1, failed);
+            if (!ok) break;
+            tc_fence_after();
+            weighted(tmem + 2 * kTile + i * kCols, tmem + i * kTile + half * 32, ring + v_slot * C::kTileBytes, half, id_o,
+                     it > 0 || half > 0, el);
           }
-          __syncwarp();
+          if (ok) umma_commit(&o_done[i], el);
         }
         if (ok && more && from[i] <= j + 1 && j + 1 < to[i]) ask(i, k_slot);
       }
-      if (ok && lane == 0) {
-        umma_commit(&empty[v_slot]);
-        if (more) umma_commit(&empty[k_slot]);
+      if (ok) {
+        umma_commit(&empty[v_slot], el);
+        if (more) umma_commit(&empty[k_slot], el);
       }
-      __syncwarp();
       fill += 2;
     }
+  }
   } else {
+    take_registers<kScoreRegisters>();
     const int i = warp / 4, row = t.first + threadIdx.x;  // of the sequence: 128 threads a tile
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21);
     const uint32_t s_at = lanes + i * kTile, o_at = lanes + 2 * kTile + i * kCols;
@@ -453,30 +478,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       uint32_t s[4][32];
+      float best[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(s_at + q * 32, s[q]);
+      for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(s_at + q * 32, s[q]);
+      tmem_wait_ld(s[0]);
+      tmem_wait_ld(s[1]);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_wait_ld(s[q]);
-      const int k0 = j * kTile;
-      if (k0 < all_low || k0 + kTile > all_high) {
-        const int a = low - k0, b = high - k0;
+      for (int q = 2; q < 4; ++q) tmem_ld_32x32b_x32(s_at + q * 32, s[q]);
+      const int k0 = j * kTile, a = low - k0, b = high - k0;
+      const bool partial = k0 < all_low || k0 + kTile > all_high;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1) {
+          tmem_wait_ld(s[2]);
+          tmem_wait_ld(s[3]);
+        }
+        if (partial) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (q * 32 + e < a || q * 32 + e >= b) s[q][e] = 0xff800000u;
+          for (int e = 0; e < 64; ++e)
+            if (h * 64 + e < a || h * 64 + e >= b) s[2 * h + e / 32][e % 32] = 0xff800000u;
+        }
+        // the largest in four chains: one is as long as its 128 latencies
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = 2 * h + q / 2, e0 = q % 2 * 16;
+          float m = as_float(s[at][e0]);
+#pragma unroll
+          for (int e = 1; e < 16; ++e) m = fmaxf(m, as_float(s[at][e0 + e]));
+          best[q] = h == 0 ? m : fmaxf(best[q], m);
+        }
       }
-      float best = -INFINITY;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) best = fmaxf(best, as_float(s[q][e]));
+      const float most = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
       if (it == 0) {
-        top = best;
+        top = most;
       } else {
-        const bool grow = (best - top) * c > kLag;
+        const bool grow = (most - top) * c > kLag;
         if (__any_sync(kFullMask, grow)) {
-          const float next = grow ? best : top, by = grow ? fast_exp2((top - next) * c) : 1.0f;
+          const float next = grow ? most : top, by = grow ? fast_exp2((top - next) * c) : 1.0f;
           sum *= by;
           top = next;
           ok = warp_wait(&o_done[i], (it - 1) & 1, failed);
@@ -494,25 +532,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float base = top == -INFINITY ? kRaise<T> : kRaise<T> - top * c;
-      float2 sums = make_float2(0.0f, 0.0f);
+      float2 sums[4] = {};
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int h = 0; h < 2; ++h) {  // 64 keys each: the product of the first begins while the others are worked on
         uint32_t w[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const int at = q * 64 + 2 * e;
+          const int at = h * 64 + 2 * e;
           const float2 x = fma2(make_float2(as_float(s[at / 32][at % 32]), as_float(s[at / 32][at % 32 + 1])), both(c),
                                 both(base));
           const float2 v = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-          sums = add2(sums, v);
+          sums[e % 4] = add2(sums[e % 4], v);
           w[e] = pack2<T>(v.x, v.y);
         }
-        tmem_st_32x32b_x32(s_at + q * 32, w);
+        tmem_st_32x32b_x32(s_at + h * 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[i][h]);
       }
-      sum += sums.x + sums.y;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[i]);
+      const float2 s01 = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+      sum += s01.x + s01.y;
     }
     const int n = to[i] - from[i];
     if (ok && n > 0) ok = warp_wait(&o_done[i], (n - 1) & 1, failed);
@@ -618,8 +657,17 @@ __device__ __forceinline__ float ds_factor(const Problem& p) {
 template <int kCols>
 struct KeyGrads {
   static constexpr int kTileBytes = kTile * kCols * 2;
-  static constexpr int kStages = kCols == 128 ? 2 : 4;  // a tile of queries and one of dout
-  static constexpr int kBytes = (2 + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kStages = kCols == 128 ? 5 : 8;  // tiles
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + 1024;
+};
+// What the kernel for keys has beside the tiles; in dynamic shared memory, so
+// that the tiles begin on their boundary without room to move them there: there
+// is none (232448 bytes, of which seven tiles take 229376).
+struct KeyShared {
+  uint64_t kv_full, s_full, dp_full, p_done[2], ds_done[2], finished, drained, stat_full[2], stat_read[2], full[8], empty[8];
+  __align__(16) float stat[2][2][kTile];  // of two tiles of queries: -lse and -delta
+  uint32_t tmem_slot;
+  int failed_word;
 };
 
 // One tile of keys a block.  Scores stand the other way round, a key a thread:
@@ -632,135 +680,154 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
                     const __grid_constant__ Problem p) {
   using C = KeyGrads<kCols>;
-  extern __shared__ uint8_t dynamic[];
-  __shared__ uint64_t kv_full, s_full, dp_full, p_done, ds_done, finished, drained, full[C::kStages], empty[C::kStages];
-  __shared__ __align__(16) float stat[C::kStages][2][kTile];
-  __shared__ uint32_t tmem_slot;
-  __shared__ int failed_word;
-  volatile int* failed = &failed_word;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
+  extern __shared__ __align__(1024) uint8_t dynamic[];
+  uint8_t* smem = dynamic;
   uint8_t* tile_k = smem;
   uint8_t* tile_v = smem + C::kTileBytes;
   uint8_t* ring = smem + 2 * C::kTileBytes;
+  KeyShared& m = *reinterpret_cast<KeyShared*>(smem + (2 + C::kStages) * C::kTileBytes);
+  volatile int* failed = &m.failed_word;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    mbar_init(&kv_full, 1);
-    mbar_init(&s_full, 1);
-    mbar_init(&dp_full, 1);
-    mbar_init(&p_done, 256);
-    mbar_init(&ds_done, 256);
-    mbar_init(&finished, 1);
-    mbar_init(&drained, 1);
+    mbar_init(&m.kv_full, 1);
+    mbar_init(&m.s_full, 1);
+    mbar_init(&m.dp_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m.p_done[i], 128);
+      mbar_init(&m.ds_done[i], 128);
+    }
+    mbar_init(&m.finished, 1);
+    mbar_init(&m.drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m.stat_full[i], 32);
+      mbar_init(&m.stat_read[i], 8);
+    }
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&full[i], 33);  // the copies, and each lane's statistics
-      mbar_init(&empty[i], 1);
+      mbar_init(&m.full[i], 1);
+      mbar_init(&m.empty[i], 1);
     }
     fence_mbar_init();
-    failed_word = 0;
+    m.failed_word = 0;
   }
-  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kTmemColumns);
+  if (warp == kMmaWarp) tmem_alloc(&m.tmem_slot, kTmemColumns);
   tc_fence_before();
   begin_kernel();
   const int kv_head = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
   const Tile t = find_tile<kTile>(p, blockIdx.x / p.kv_heads, p.keys);
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot, tmem_s = tmem, tmem_dp = tmem + kTile, tmem_dv = tmem + 2 * kTile,
+  const uint32_t tmem = m.tmem_slot, tmem_s = tmem, tmem_dp = tmem + kTile, tmem_dv = tmem + 2 * kTile,
                  tmem_dk = tmem + 2 * kTile + kCols;
   int low = 0, high = 0;
   if (t.found) queries_of(p, t, min(t.first, t.keys), min(t.first + kTile, t.keys), &low, &high);
   const int from = low / kTile, to = low < high ? (high + kTile - 1) / kTile : from;
   const int per = to - from, n = per * group;  // tiles of queries, of all heads
-  const bool foreign = p.offsets != nullptr || p.lengths != nullptr;
+  // fill 2 it of the ring is the queries of iteration `it`, 2 it + 1 their dout
 
   int fills = 0;
+  if (warp >= kLoadWarp) {
+  give_registers<kOtherRegisters>();
   if (warp == kLoadWarp) {
     bool ok = true;
     if (n > 0 && lane == 0) {
-      mbar_arrive_expect_tx(&kv_full, 2 * C::kTileBytes);
-      load_tile<kCols>(tile_k, &map_k, &kv_full, t.row0 + t.first, kv_head, t.batch);
-      load_tile<kCols>(tile_v, &map_v, &kv_full, t.row0 + t.first, kv_head, t.batch);
+      mbar_arrive_expect_tx(&m.kv_full, 2 * C::kTileBytes);
+      load_tile<kCols>(tile_k, &map_k, &m.kv_full, t.row0 + t.first, kv_head, t.batch);
+      load_tile<kCols>(tile_v, &map_v, &m.kv_full, t.row0 + t.first, kv_head, t.batch);
     }
+    int head = kv_head * group, i = from;
     for (int it = 0; it < n; ++it) {
-      const int s = it % C::kStages, head = kv_head * group + it / per, first = (from + it % per) * kTile;
-      if (it >= C::kStages) ok = warp_wait(&empty[s], (it / C::kStages - 1) & 1, failed);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&full[s], 2 * C::kTileBytes);
-        load_tile<kCols>(ring + 2 * s * C::kTileBytes, &map_q, &full[s], t.row0 + first, head, t.batch);
-        load_tile<kCols>(ring + (2 * s + 1) * C::kTileBytes, &map_g, &full[s], t.row0 + first, head, t.batch);
-      }
-      const int64_t at = head * p.rows + static_cast<int64_t>(t.batch) * p.length + t.row0 + first;
+      const int row = t.row0 + i * kTile;
 #pragma unroll
-      for (int i = lane; i < kTile; i += 32) {
-        const bool counts = first + i < t.queries;
-        stat[s][0][i] = counts ? p.stats[at + i] : -INFINITY;
-        stat[s][1][i] = counts ? p.stats[p.heads * p.rows + at + i] : 0.0f;
+      for (int which = 0; which < 2; ++which) {
+        const int s = fills % C::kStages;
+        if (fills >= C::kStages) ok = ok && warp_wait(&m.empty[s], (fills / C::kStages - 1) & 1, failed);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&m.full[s], C::kTileBytes);
+          load_tile<kCols>(ring + s * C::kTileBytes, which ? &map_g : &map_q, &m.full[s], row, head, t.batch);
+        }
+        ++fills;
+        if (which == 0) {
+          if (it >= 2) ok = warp_wait(&m.stat_read[it % 2], (it / 2 - 1) & 1, failed);
+          if (!ok) break;
+          const int64_t at = head * p.rows + static_cast<int64_t>(t.batch) * p.length + row;
+#pragma unroll
+          for (int e = lane; e < kTile; e += 32) {
+            const bool counts = i * kTile + e < t.queries;
+            m.stat[it % 2][0][e] = counts ? p.stats[at + e] : -INFINITY;
+            m.stat[it % 2][1][e] = counts ? p.stats[p.heads * p.rows + at + e] : 0.0f;
+          }
+          mbar_arrive(&m.stat_full[it % 2]);
+        }
       }
-      mbar_arrive(&full[s]);
-      ++fills;
+      if (!ok) break;
+      if (++i == to) i = from, ++head;
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     const uint32_t id_s = idesc_16bit(kBf16<T>, kTile, 0), id_o = idesc_16bit(kBf16<T>, (p.dim + 15) / 16 * 16, 1);
-    const int steps = (p.dim + 15) / 16;
-    bool ok = n == 0 || warp_wait(&kv_full, 0, failed);
-    // waits for the tiles of iteration `it` and clears what is not the sequence's
-    const auto arrived = [&](int it) {
-      const int s = it % C::kStages;
-      if (!warp_wait(&full[s], (it / C::kStages) & 1, failed)) return false;
-      const int valid = t.queries - (from + it % per) * kTile;
-      if (foreign && valid < kTile) {
-        zero_rows<kCols>(ring + 2 * s * C::kTileBytes, valid);
-        zero_rows<kCols>(ring + (2 * s + 1) * C::kTileBytes, valid);
-      }
+    const uint32_t el = elect_one();
+    const bool foreign = p.offsets != nullptr || p.lengths != nullptr;
+    bool ok = n == 0 || warp_wait(&m.kv_full, 0, failed);
+    // waits for fill `f`, a tile from query `first` on, and clears what is not the sequence's
+    const auto arrived = [&](int f, int first) {
+      if (!warp_wait(&m.full[f % C::kStages], (f / C::kStages) & 1, failed)) return false;
+      if (foreign && t.queries - first < kTile) zero_rows<kCols>(ring + f % C::kStages * C::kTileBytes, t.queries - first);
       return true;
     };
     if (ok && n > 0) {
-      ok = arrived(0);
-      if (ok && lane == 0) {
-        scores(tmem_s, tile_k, ring, id_s, steps);
-        umma_commit(&s_full);
-        scores(tmem_dp, tile_v, ring + C::kTileBytes, id_s, steps);
-        umma_commit(&dp_full);
+      ok = arrived(0, from * kTile);
+      if (ok) {
+        scores<kCols>(tmem_s, tile_k, ring, id_s, p.dim, el);
+        umma_commit(&m.s_full, el);
+        ok = arrived(1, from * kTile);
       }
-      __syncwarp();
+      if (ok) {
+        scores<kCols>(tmem_dp, tile_v, ring + C::kTileBytes, id_s, p.dim, el);
+        umma_commit(&m.dp_full, el);
+      }
     }
+    int next = from + 1 == to ? from : from + 1;  // the next iteration's tile of queries
     for (int it = 0; it < n && ok; ++it) {
-      const uint8_t* tile_q = ring + 2 * (it % C::kStages) * C::kTileBytes;
-      const uint8_t* tile_g = tile_q + C::kTileBytes;
-      const uint8_t* next_q = ring + 2 * ((it + 1) % C::kStages) * C::kTileBytes;
+      const int q_slot = 2 * it % C::kStages, g_slot = (2 * it + 1) % C::kStages;
       const bool more = it + 1 < n;
-      ok = warp_wait(&p_done, it & 1, failed);
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) weighted(tmem_dv, tmem_s, 64, tile_g, id_o, it > 0);
-      __syncwarp();
-      if (more) {
-        ok = arrived(it + 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok = ok && warp_wait(&m.p_done[h], it & 1, failed);
         if (!ok) break;
-        if (lane == 0) {
-          scores(tmem_s, tile_k, next_q, id_s, steps);
-          umma_commit(&s_full);
-        }
-        __syncwarp();
+        tc_fence_after();
+        weighted(tmem_dv, tmem_s + h * 64, ring + g_slot * C::kTileBytes, h, id_o, it > 0 || h > 0, el);
       }
-      ok = warp_wait(&ds_done, it & 1, failed);
       if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
-        weighted(tmem_dk, tmem_dp, 64, tile_q, id_o, it > 0);
-        umma_commit(&empty[it % C::kStages]);
-        if (more) {
-          scores(tmem_dp, tile_v, next_q + C::kTileBytes, id_s, steps);
-          umma_commit(&dp_full);
-        } else {
-          umma_commit(&finished);
-        }
+      umma_commit(&m.empty[g_slot], el);
+      if (more) {
+        ok = arrived(2 * it + 2, next * kTile);
+        if (!ok) break;
+        scores<kCols>(tmem_s, tile_k, ring + (2 * it + 2) % C::kStages * C::kTileBytes, id_s, p.dim, el);
+        umma_commit(&m.s_full, el);
       }
-      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok = ok && warp_wait(&m.ds_done[h], it & 1, failed);
+        if (!ok) break;
+        tc_fence_after();
+        weighted(tmem_dk, tmem_dp + h * 64, ring + q_slot * C::kTileBytes, h, id_o, it > 0 || h > 0, el);
+      }
+      if (!ok) break;
+      umma_commit(&m.empty[q_slot], el);
+      if (more) {
+        ok = arrived(2 * it + 3, next * kTile);
+        if (!ok) break;
+        scores<kCols>(tmem_dp, tile_v, ring + (2 * it + 3) % C::kStages * C::kTileBytes, id_s, p.dim, el);
+        umma_commit(&m.dp_full, el);
+        if (++next == to) next = from;
+      } else {
+        umma_commit(&m.finished, el);
+      }
     }
+  }
   } else {
+    take_registers<kScoreRegisters>();
     const int w = warp / 4, row = t.first + threadIdx.x % 128;  // the thread's key; both halves have all keys
     const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
     const float c = p.scale * kLog2e, raise = ds_factor<T>(p) * (kBf16<T> ? 1.0f : 0x1p-10f);
@@ -775,11 +842,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     bool ok = true;
+    int i = from;
     for (int it = 0; it < n; ++it) {
-      const int s = it % C::kStages, first = (from + it % per) * kTile;
+      const int first = i * kTile;
+      if (++i == to) i = from;
       const bool partial = first < all_low || first + kTile > all_high;
       const int a = mine_low - first - w * 64, b = mine_high - first - w * 64;
-      ok = warp_wait(&full[s], (it / C::kStages) & 1, failed) && warp_wait(&s_full, it & 1, failed);
+      ok = warp_wait(&m.stat_full[it % 2], (it / 2) & 1, failed);
+      if (!ok) break;
+      // the statistics are in registers before the scores are there: loads from shared memory wait behind the products'
+      float4 l[16];
+      const float4* l4 = reinterpret_cast<const float4*>(&m.stat[it % 2][0][w * 64]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) l[e] = l4[e];
+      ok = warp_wait(&m.s_full, it & 1, failed);
       if (!ok) break;
       tc_fence_after();
       uint32_t x[2][32];
@@ -787,32 +863,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(tmem_s + lanes + w * 64 + q * 32, x[q]);
 #pragma unroll
       for (int q = 0; q < 2; ++q) tmem_wait_ld(x[q]);
-      const float4* l4 = reinterpret_cast<const float4*>(&stat[s][0][w * 64]);
       uint32_t packed[32];
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        const float4 l = l4[e / 4];
+      for (int e = 0; e < 64; e += 2) {
         const float2 u = fma2(make_float2(as_float(x[e / 32][e % 32]), as_float(x[e / 32][e % 32 + 1])), both(c),
-                              make_float2(l.x, l.y));
-        const float2 v = fma2(make_float2(as_float(x[e / 32][e % 32 + 2]), as_float(x[e / 32][e % 32 + 3])), both(c),
-                              make_float2(l.z, l.w));
-        float r[4] = {fast_exp2(u.x), fast_exp2(u.y), fast_exp2(v.x), fast_exp2(v.y)};
-        if (partial) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (e + i < a || e + i >= b) r[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[(e + i) / 32][(e + i) % 32] = __float_as_uint(r[i]);
-        packed[e / 2] = pack2<T>(r[0], r[1]);
-        packed[e / 2 + 1] = pack2<T>(r[2], r[3]);
+                              e % 4 == 0 ? make_float2(l[e / 4].x, l[e / 4].y) : make_float2(l[e / 4].z, l[e / 4].w));
+        x[e / 32][e % 32] = __float_as_uint(fast_exp2(u.x));
+        x[e / 32][e % 32 + 1] = __float_as_uint(fast_exp2(u.y));
       }
+      if (partial) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < a || e >= b) x[e / 32][e % 32] = 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 64; e += 2)
+        packed[e / 2] = pack2<T>(as_float(x[e / 32][e % 32]), as_float(x[e / 32][e % 32 + 1]));
       tmem_st_32x32b_x32(tmem_s + lanes + w * 64, packed);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_done);
+      mbar_arrive(&m.p_done[w]);
 
-      ok = warp_wait(&dp_full, it & 1, failed);
+      const float4* d4 = reinterpret_cast<const float4*>(&m.stat[it % 2][1][w * 64]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) l[e] = d4[e];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.stat_read[it % 2]);
+      ok = warp_wait(&m.dp_full, it & 1, failed);
       if (!ok) break;
       tc_fence_after();
       uint32_t y[2][32];
@@ -820,30 +897,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(tmem_dp + lanes + w * 64 + q * 32, y[q]);
 #pragma unroll
       for (int q = 0; q < 2; ++q) tmem_wait_ld(y[q]);
-      const float4* d4 = reinterpret_cast<const float4*>(&stat[s][1][w * 64]);
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        const float4 d = d4[e / 4];
-        const auto one = [&](int at, float d0, float d1) {
-          float2 v = add2(make_float2(as_float(y[at / 32][at % 32]), as_float(y[at / 32][at % 32 + 1])),
-                          make_float2(d0, d1));
-          if constexpr (!kBf16<T>) v = mul2(v, both(raise));
-          v = mul2(v, make_float2(as_float(x[at / 32][at % 32]), as_float(x[at / 32][at % 32 + 1])));
-          if (partial) {
-            if (at < a || at >= b) v.x = 0.0f;
-            if (at + 1 < a || at + 1 >= b) v.y = 0.0f;
-          }
-          return pack2<T>(v.x, v.y);
-        };
-        packed[e / 2] = one(e, d.x, d.y);
-        packed[e / 2 + 1] = one(e + 2, d.z, d.w);
+      for (int e = 0; e < 64; e += 2) {
+        float2 v = add2(make_float2(as_float(y[e / 32][e % 32]), as_float(y[e / 32][e % 32 + 1])),
+                        e % 4 == 0 ? make_float2(l[e / 4].x, l[e / 4].y) : make_float2(l[e / 4].z, l[e / 4].w));
+        if constexpr (!kBf16<T>) v = mul2(v, both(raise));
+        v = mul2(v, make_float2(as_float(x[e / 32][e % 32]), as_float(x[e / 32][e % 32 + 1])));
+        y[e / 32][e % 32] = __float_as_uint(v.x);
+        y[e / 32][e % 32 + 1] = __float_as_uint(v.y);
       }
+      if (partial) {  // p is 0 there, but dp may be no number
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < a || e >= b) y[e / 32][e % 32] = 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 64; e += 2)
+        packed[e / 2] = pack2<T>(as_float(y[e / 32][e % 32]), as_float(y[e / 32][e % 32 + 1]));
       tmem_st_32x32b_x32(tmem_dp + lanes + w * 64, packed);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ds_done);
+      mbar_arrive(&m.ds_done[w]);
     }
-    if (ok && n > 0) ok = warp_wait(&finished, 0, failed);
+    if (ok && n > 0) ok = warp_wait(&m.finished, 0, failed);
     tc_fence_after();
     // the first half writes dv, the other dk
     const int64_t at = static_cast<int64_t>(t.batch) * p.keys + t.row0 + row;
@@ -853,13 +929,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (n > 0) store_row<T, kCols>(grad, nullptr, (w == 0 ? tmem_dv : tmem_dk) + lanes, p.dim, by, write && some);
     if (write && (n == 0 || !some)) zero_row(grad, p.dim);
   }
-  finish(tmem, failed, fills, full, C::kStages, n > 0 ? &kv_full : nullptr, nullptr, &drained);
+  finish(tmem, failed, fills, m.full, C::kStages, n > 0 ? &m.kv_full : nullptr, nullptr, &m.drained);
 }
 
 // ------------------------------------------------------------ backward: queries
 // One tile of queries a block.  Two tiles of scores in tensor memory, one of
 // dp: the products of the next keys run while ds is worked on, which takes the
-// place of its scores.
+// place of its scores.  Half of the warps may be done with the next ds before
+// the product with the present one has been issued, so those barriers are two.
 template <typename T, int kCols>
 __global__ void __launch_bounds__(kThreads, 1)
     query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -867,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ Problem p, int tiles) {
   using C = KeyGrads<kCols>;
   extern __shared__ uint8_t dynamic[];
-  __shared__ uint64_t q_full, s_full[2], dp_full, dp_read, ds_done, finished, drained, full[C::kStages], empty[C::kStages];
+  __shared__ uint64_t q_full, s_full[2], dp_full, dp_read, ds_done[2][2], finished, drained, full[C::kStages], empty[C::kStages];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_word;
   volatile int* failed = &failed_word;
@@ -882,7 +959,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s_full[1], 1);
     mbar_init(&dp_full, 1);
     mbar_init(&dp_read, 256);
-    mbar_init(&ds_done, 256);
+    for (int i = 0; i < 4; ++i) mbar_init(&ds_done[i / 2][i % 2], 128);
     mbar_init(&finished, 1);
     mbar_init(&drained, 1);
     for (int i = 0; i < C::kStages; ++i) {
@@ -906,6 +983,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n = to - from;
 
   int fills = 0;
+  if (warp >= kLoadWarp) {
+  give_registers<kOtherRegisters>();
   if (warp == kLoadWarp) {
     if (lane == 0 && n > 0) {
       const int kv_head = head / (p.heads / p.kv_heads);
@@ -913,71 +992,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_expect_tx(&q_full, 2 * C::kTileBytes);
       load_tile<kCols>(tile_q, &map_q, &q_full, t.row0 + t.first, head, t.batch);
       load_tile<kCols>(tile_g, &map_g, &q_full, t.row0 + t.first, head, t.batch);
-      for (int it = 0; it < n; ++it) {
-        const int s = it % C::kStages, row = t.row0 + (from + it) * kTile;
-        if (it >= C::kStages) ok = ring_wait(&empty[s], (it / C::kStages - 1) & 1, failed);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&full[s], 2 * C::kTileBytes);
-        load_tile<kCols>(ring + 2 * s * C::kTileBytes, &map_k, &full[s], row, kv_head, t.batch);
-        load_tile<kCols>(ring + (2 * s + 1) * C::kTileBytes, &map_v, &full[s], row, kv_head, t.batch);
-        ++fills;
+      for (int it = 0; it < n && ok; ++it) {
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          const int s = fills % C::kStages;
+          if (fills >= C::kStages) ok = ok && ring_wait(&empty[s], (fills / C::kStages - 1) & 1, failed);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[s], C::kTileBytes);
+          load_tile<kCols>(ring + s * C::kTileBytes, which ? &map_v : &map_k, &full[s], t.row0 + (from + it) * kTile, kv_head,
+                           t.batch);
+          ++fills;
+        }
       }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     const uint32_t id_s = idesc_16bit(kBf16<T>, kTile, 0), id_o = idesc_16bit(kBf16<T>, (p.dim + 15) / 16 * 16, 1);
-    const int steps = (p.dim + 15) / 16;
+    const uint32_t el = elect_one();
     bool ok = n == 0 || warp_wait(&q_full, 0, failed);
-    const auto arrived = [&](int it) {
-      const int s = it % C::kStages;
-      if (!warp_wait(&full[s], (it / C::kStages) & 1, failed)) return false;
-      const int valid = t.keys - (from + it) * kTile;
-      if ((p.offsets != nullptr || p.lengths != nullptr) && valid < kTile)
-        zero_rows<kCols>(ring + 2 * s * C::kTileBytes, valid);
+    // scores of iteration `it`; its keys' rows that are not the sequence's are cleared: ds is multiplied with them
+    const auto ask = [&](int it) {
+      const int f = 2 * it, valid = t.keys - (from + it) * kTile;
+      uint8_t* tile = ring + f % C::kStages * C::kTileBytes;
+      if (!warp_wait(&full[f % C::kStages], (f / C::kStages) & 1, failed)) return false;
+      if ((p.offsets != nullptr || p.lengths != nullptr) && valid < kTile) zero_rows<kCols>(tile, valid);
+      scores<kCols>(tmem + (it & 1) * kTile, tile_q, tile, id_s, p.dim, el);
+      umma_commit(&s_full[it & 1], el);
       return true;
     };
-    if (ok && n > 0) {
-      ok = arrived(0);
-      if (ok && lane == 0) {
-        scores(tmem, tile_q, ring, id_s, steps);
-        umma_commit(&s_full[0]);
-        scores(tmem_dp, tile_g, ring + C::kTileBytes, id_s, steps);
-        umma_commit(&dp_full);
-      }
-      __syncwarp();
-    }
+    const auto ask_dp = [&](int it) {
+      const int f = 2 * it + 1;
+      if (!warp_wait(&full[f % C::kStages], (f / C::kStages) & 1, failed)) return false;
+      scores<kCols>(tmem_dp, tile_g, ring + f % C::kStages * C::kTileBytes, id_s, p.dim, el);
+      umma_commit(&dp_full, el);
+      umma_commit(&empty[f % C::kStages], el);
+      return true;
+    };
+    if (ok && n > 0) ok = ask(0) && ask_dp(0);
     for (int it = 0; it < n && ok; ++it) {
-      const uint8_t* tile_k = ring + 2 * (it % C::kStages) * C::kTileBytes;
-      const uint8_t* next_k = ring + 2 * ((it + 1) % C::kStages) * C::kTileBytes;
       const bool more = it + 1 < n;
       if (more) {
-        ok = arrived(it + 1);
-        if (!ok) break;
-        if (lane == 0) {
-          scores(tmem + ((it + 1) & 1) * kTile, tile_q, next_k, id_s, steps);
-          umma_commit(&s_full[(it + 1) & 1]);
-        }
-        __syncwarp();
-        ok = warp_wait(&dp_read, it & 1, failed);
+        ok = ask(it + 1) && warp_wait(&dp_read, it & 1, failed);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          scores(tmem_dp, tile_g, next_k + C::kTileBytes, id_s, steps);
-          umma_commit(&dp_full);
-        }
-        __syncwarp();
+        ok = ask_dp(it + 1);
+        if (!ok) break;
       }
-      ok = warp_wait(&ds_done, it & 1, failed);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok = ok && warp_wait(&ds_done[h][it & 1], (it / 2) & 1, failed);
+        if (!ok) break;
+        tc_fence_after();
+        weighted(tmem_dq, tmem + (it & 1) * kTile + h * 64, ring + 2 * it % C::kStages * C::kTileBytes, h, id_o,
+                 it > 0 || h > 0, el);
+      }
       if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
-        weighted(tmem_dq, tmem + (it & 1) * kTile, 64, tile_k, id_o, it > 0);
-        umma_commit(&empty[it % C::kStages]);
-        if (!more) umma_commit(&finished);
-      }
-      __syncwarp();
+      umma_commit(&empty[2 * it % C::kStages], el);
+      if (!more) umma_commit(&finished, el);
     }
+  }
   } else {
+    take_registers<kScoreRegisters>();
     const int w = warp / 4, row = t.first + threadIdx.x % 128;  // both halves have all queries
     const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
     const float factor = ds_factor<T>(p), c = p.scale * kLog2e, raise = factor * (kBf16<T> ? 1.0f : 0x1p-10f);
@@ -1027,16 +1102,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         float2 v = add2(make_float2(as_float(y[e / 32][e % 32]), as_float(y[e / 32][e % 32 + 1])), both(delta));
         if constexpr (!kBf16<T>) v = mul2(v, both(raise));
         v = mul2(v, make_float2(fast_exp2(u.x), fast_exp2(u.y)));
-        if (partial) {
-          if (e < a || e >= b) v.x = 0.0f;
-          if (e + 1 < a || e + 1 >= b) v.y = 0.0f;
-        }
-        packed[e / 2] = pack2<T>(v.x, v.y);
+        y[e / 32][e % 32] = __float_as_uint(v.x);
+        y[e / 32][e % 32 + 1] = __float_as_uint(v.y);
       }
+      if (partial) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < a || e >= b) y[e / 32][e % 32] = 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 64; e += 2)
+        packed[e / 2] = pack2<T>(as_float(y[e / 32][e % 32]), as_float(y[e / 32][e % 32 + 1]));
       tmem_st_32x32b_x32(s_at, packed);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ds_done);
+      mbar_arrive(&ds_done[w][it & 1]);
     }
     if (ok && n > 0) ok = warp_wait(&finished, 0, failed);
     tc_fence_after();
@@ -1166,6 +1246,19 @@ Problem problem_of(const muon_train_attention_args& a) {
   return p;
 }
 
+// Once for each device: lets a kernel have its shared memory, and checks that it
+// is launched with the registers that its warpgroups share out among them, or
+// it would wait for them forever.
+template <auto kKernel>
+int prepare(size_t bytes) {
+  static const bool fits = [] {
+    cudaFuncAttributes attributes;
+    return cudaFuncGetAttributes(&attributes, kKernel) == cudaSuccess && attributes.numRegs == kLaunchRegisters;
+  }();
+  if (!fits) return MUON_POLAR_ERR_UNSUPPORTED_DEVICE;
+  return allow_smem<kKernel>(bytes);
+}
+
 template <typename T, int kCols>
 int forward(const muon_train_attention_args& a, void* stream) {
   Maps m;
@@ -1175,7 +1268,7 @@ int forward(const muon_train_attention_args& a, void* stream) {
   p.out = a.out;
   p.out2 = a.out_rest;
   constexpr int kBytes = Forward<kCols>::kBytes;
-  rc = allow_smem<forward_kernel<T, kCols>>(kBytes);
+  rc = prepare<forward_kernel<T, kCols>>(kBytes);
   if (rc != MUON_POLAR_OK) return rc;
   const int64_t tiles = tiles_of(a, a.length, 2 * kTile);
   return launch(forward_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.heads)), kThreads, kBytes, 1, true, stream,
@@ -1224,7 +1317,8 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
   if (rc != MUON_POLAR_OK) return rc;
   constexpr int kBytes = KeyGrads<kCols>::kBytes;
   if (a.keys > 0) {
-    rc = allow_smem<key_grad_kernel<T, kCols>>(kBytes);
+    constexpr int kBytes = (2 + KeyGrads<kCols>::kStages) * KeyGrads<kCols>::kTileBytes + static_cast<int>(sizeof(KeyShared));
+    rc = prepare<key_grad_kernel<T, kCols>>(kBytes);
     if (rc != MUON_POLAR_OK) return rc;
     p.out = g.grad_k;
     p.out2 = g.grad_v;
@@ -1233,7 +1327,7 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
                 stream, m.q, m.k, m.v, map_g, p);
     if (rc != MUON_POLAR_OK) return rc;
   }
-  rc = allow_smem<query_grad_kernel<T, kCols>>(kBytes);
+  rc = prepare<query_grad_kernel<T, kCols>>(kBytes);
   if (rc != MUON_POLAR_OK) return rc;
   p.out = g.grad_q;
   p.out2 = nullptr;
