@@ -1,16 +1,25 @@
 // clip_grads_sm100.cu -- the norm of many tensors taken as one vector, and the
 // tensors times min(1, max_norm / (norm + 1e-6)).
 //
-// Two launches over the same work, a share of the elements for each block: the
-// first leaves each block's sum of squares (or largest magnitude) in the
-// workspace, the second adds them up, every block in the same order, and
-// scales.  Bound by memory: the gradients are read once for the norm and once
+// Two launches over the same work, chunks of the tensors dealt out to the blocks
+// in turn: the first leaves each block's sum of squares (or largest magnitude)
+// in the workspace, the second adds them up, every block in the same order, and
+// scales.  (With one run of neighbouring elements a block, all the short
+// tensors of a model, which stand together, fell to one of them: 57 us for 40
+// MB.)  Bound by memory: the gradients are read once for the norm and once
 // more to be scaled, where the second pass begins with what the first read
 // last, which L2 still holds.  In place, gradients within the limit would be
 // written back as they are: the second pass then only gives the norm.
 //
-// Squares are added up in 64 bits: those of fp32 gradients leave fp32's range
-// from 10^19 and under 10^-19 on.
+// Squares are added up in fp32 over the elements of one 16-byte load and in 64
+// bits from there on: converting every element to 64 bits is what bounded the
+// first pass before (640 M bf16: 3.8 TB/s).  A load whose sum leaves the range
+// in which that is exact to a few roundings (squares of 10^19, or of 10^-12
+// alone) is added up again in 64 bits.
+//
+// Tensors lie at any element, and so do the outputs: the second pass stores
+// whole aligned vectors and puts each one's elements together from the two
+// aligned 16-byte granules that hold them.
 #include "train_common.cuh"
 
 namespace muon_train {
@@ -18,8 +27,11 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kBlocksPerSm = 2;
-constexpr int64_t kLeast = 8192;  // elements of a block
-constexpr int kUnroll = 4;        // 16-byte loads in flight a thread
+constexpr int kUnroll = 4;     // 16-byte loads in flight a thread that scales
+constexpr int kUnrollSum = 8;  // and one that adds up (4: 228 us for 1.28 GB)
+// Elements of a chunk: as many as a block has in flight, of 16-bit types, or
+// fewer where there are not two for each block.
+constexpr int64_t kMostChunk = kThreads * kUnrollSum * 8, kLeastChunk = kThreads * 4;
 
 // The tensors of one launch travel as a kernel's parameters (at most 32764 bytes).
 constexpr int kMost = 1024;
@@ -27,16 +39,13 @@ template <int kEntries>
 struct Table {
   const void* in[kEntries];
   void* out[kEntries];
-  int64_t end[kEntries];    // elements of the tensors up to and with this one
+  int64_t elements[kEntries];
+  int32_t end[kEntries];    // chunks of the tensors up to and with this one
   uint8_t types[kEntries];  // of in, and 4 times of out
+  int64_t chunk;            // elements of one
   int count;
+  int in_place;             // all of them
 };
-
-// Element at which block `b` begins, in whole runs of 64.
-__device__ __forceinline__ int64_t share(int64_t n, int64_t b, int64_t blocks) {
-  const int64_t at = (n + 63) / 64 * b / blocks * 64;
-  return at < n ? at : n;
-}
 
 // Of the sum of squares, or of the bits of the largest magnitude (those of NaN
 // are above infinity's, so that a NaN stays).
@@ -69,20 +78,24 @@ __device__ __forceinline__ double block_total(double v) {
   return v;
 }
 
+// The tensor that chunk `c` belongs to, from tensor `low` on.
 template <int kEntries>
-__device__ __forceinline__ int64_t begin_of(const Table<kEntries>& t, int i) { return i > 0 ? t.end[i - 1] : 0; }
-// The tensor that holds element `at`.
-template <int kEntries>
-__device__ __forceinline__ int find(const Table<kEntries>& t, int64_t at) {
-  int low = 0, high = t.count - 1;
+__device__ __forceinline__ int find(const Table<kEntries>& t, int c, int low, int high) {
   while (low < high) {
     const int mid = (low + high) / 2;
-    if (t.end[mid] > at)
+    if (t.end[mid] > c)
       high = mid;
     else
       low = mid + 1;
   }
   return low;
+}
+// First element of chunk `c` of tensor `i`, and how many there are.
+template <int kEntries>
+__device__ __forceinline__ int64_t run_of(const Table<kEntries>& t, int i, int c, int64_t* n) {
+  const int64_t from = (c - (i > 0 ? t.end[i - 1] : 0)) * t.chunk, left = t.elements[i] - from;
+  *n = left < t.chunk ? left : t.chunk;
+  return from;
 }
 
 // Elements before the first 16-byte boundary of p, at most n.
@@ -92,6 +105,29 @@ __device__ __forceinline__ int64_t head_of(const T* p, int64_t n) {
   return h < n ? h : n;
 }
 
+// The elements of one load.
+template <typename T, bool kLargest>
+__device__ __forceinline__ void add_load(const uint4& raw, Total<kLargest>& total) {
+  constexpr int kN = kVec<T>;
+  float x[kN];
+  unpack<T>(raw, x);
+  if constexpr (kLargest) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) total.add(x[j]);
+  } else {
+    float2 s = mul2(make_float2(x[0], x[1]), make_float2(x[0], x[1]));
+#pragma unroll
+    for (int j = 2; j < kN; j += 2) s = fma2(make_float2(x[j], x[j + 1]), make_float2(x[j], x[j + 1]), s);
+    const float sum = s.x + s.y;
+    if (sum >= 0x1p-80f && sum <= 0x1p120f) {
+      total.v += static_cast<double>(sum);
+    } else if ((raw.x | raw.y | raw.z | raw.w) != 0) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) total.add(x[j]);
+    }
+  }
+}
+
 template <typename T, bool kLargest>
 __device__ __forceinline__ void total_of(const T* p, int64_t n, Total<kLargest>& total) {
   constexpr int kN = kVec<T>;
@@ -99,72 +135,97 @@ __device__ __forceinline__ void total_of(const T* p, int64_t n, Total<kLargest>&
   for (int64_t i = threadIdx.x; i < head; i += kThreads) total.add(to_float(p[i]));
   for (int64_t i = tail + threadIdx.x; i < n; i += kThreads) total.add(to_float(p[i]));
   const uint4* q = reinterpret_cast<const uint4*>(p + head);
-  for (int64_t v0 = threadIdx.x; v0 < vectors; v0 += kThreads * kUnroll) {
-    uint4 raw[kUnroll];
+  int64_t v = threadIdx.x;
+  for (; v + (kUnrollSum - 1) * kThreads < vectors; v += kThreads * kUnrollSum) {
+    uint4 raw[kUnrollSum];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)  // beyond the end: zeros, which add nothing
-      raw[u] = v0 + u * kThreads < vectors ? q[v0 + u * kThreads] : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < kUnrollSum; ++u) raw[u] = q[v + u * kThreads];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float x[kN];
-      unpack<T>(raw[u], x);
-#pragma unroll
-      for (int j = 0; j < kN; ++j) total.add(x[j]);
-    }
+    for (int u = 0; u < kUnrollSum; ++u) add_load<T>(raw[u], total);
   }
+  for (; v < vectors; v += kThreads) add_load<T>(q[v], total);
 }
 
 template <int kEntries, bool kLargest>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     total_kernel(const __grid_constant__ Table<kEntries> t, double* partial) {
   begin_kernel();
-  const int64_t all = t.end[t.count - 1];
-  int64_t at = share(all, blockIdx.x, gridDim.x);
-  const int64_t end = share(all, blockIdx.x + 1, gridDim.x);
+  const int chunks = t.end[t.count - 1];
   Total<kLargest> total;
-  for (int i = find(t, at); at < end; ++i) {
-    const int64_t begin = begin_of(t, i), stop = t.end[i] < end ? t.end[i] : end;
-    const int64_t from = at - begin, n = stop - at;
+  int i = 0;
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    i = find(t, c, i, t.count - 1);
+    int64_t n;
+    const int64_t from = run_of(t, i, c, &n);
     switch (t.types[i] & 3) {
       case MUON_TRAIN_F32: total_of(static_cast<const float*>(t.in[i]) + from, n, total); break;
       case MUON_TRAIN_BF16: total_of(static_cast<const __nv_bfloat16*>(t.in[i]) + from, n, total); break;
       default: total_of(static_cast<const __half*>(t.in[i]) + from, n, total); break;
     }
-    at = stop;
   }
   const double v = block_total<kLargest>(total.v);
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
+// 16 bytes from byte `shift` (0 to 15, even) on of two granules side by side.
+__device__ __forceinline__ uint4 joined(const uint4& a, const uint4& b, int shift) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (shift & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (shift & 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // out = factor * in, from the end to the beginning.
 template <typename In, typename Out>
-__device__ __forceinline__ void scale_run(const In* p, Out* out, int64_t n, float factor) {
+__device__ __noinline__ void scale_run(const In* p, Out* out, int64_t n, float factor) {
   constexpr int kN = kVec<In>;
-  const int64_t head = head_of(p, n), vectors = (n - head) / kN, tail = head + vectors * kN;
-  constexpr uintptr_t kStore = kN * sizeof(Out) < 16 ? kN * sizeof(Out) : 16;
-  const bool whole = reinterpret_cast<uintptr_t>(out + head) % kStore == 0;
+  constexpr int kStore = kN * sizeof(Out) < 16 ? kN * static_cast<int>(sizeof(Out)) : 16;  // bytes of a store
+  // vectors begin where a store of the output may; those whose input needs two granules stay clear of both ends
+  int64_t head = (kStore - reinterpret_cast<uintptr_t>(out) % kStore) % kStore / sizeof(Out);
+  if (head > n) head = n;
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p + head) % 16);
+  if (shift != 0) head = head + kN < n ? head + kN : n;
+  int64_t vectors = (n - head) / kN;
+  if (shift != 0 && vectors > 0) --vectors;
+  const int64_t tail = head + vectors * kN;
   for (int64_t i = tail + threadIdx.x; i < n; i += kThreads) out[i] = from_float<Out>(to_float(p[i]) * factor);
-  const uint4* q = reinterpret_cast<const uint4*>(p + head);
-  for (int64_t v0 = threadIdx.x; v0 < vectors; v0 += kThreads * kUnroll) {
-    uint4 raw[kUnroll];
+  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p + head) - shift);
+  const auto put = [&](int64_t v, const uint4& raw) {
+    float x[kN];
+    unpack<In>(raw, x);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (v0 + u * kThreads < vectors) raw[u] = q[vectors - 1 - v0 - u * kThreads];
+    for (int j = 0; j < kN; ++j) x[j] *= factor;
+    store_run<Out, kN>(out, head + v * kN, x);
+  };
+  int64_t v = vectors - 1 - threadIdx.x;
+  if (shift == 0) {
+    for (; v >= (kUnroll - 1) * kThreads; v -= kThreads * kUnroll) {
+      uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (v0 + u * kThreads >= vectors) continue;
-      const int64_t i = head + (vectors - 1 - v0 - u * kThreads) * kN;
-      float x[kN];
-      unpack<In>(raw[u], x);
+      for (int u = 0; u < kUnroll; ++u) raw[u] = q[v - u * kThreads];
 #pragma unroll
-      for (int j = 0; j < kN; ++j) x[j] *= factor;
-      if (whole) {
-        store_run<Out, kN>(out, i, x);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kN; ++j) out[i + j] = from_float<Out>(x[j]);
-      }
+      for (int u = 0; u < kUnroll; ++u) put(v - u * kThreads, raw[u]);
     }
+    for (; v >= 0; v -= kThreads) put(v, q[v]);
+  } else {
+    for (; v >= (kUnroll - 1) * kThreads; v -= kThreads * kUnroll) {
+      uint4 a[kUnroll], b[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) a[u] = q[v - u * kThreads], b[u] = q[v - u * kThreads + 1];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) put(v - u * kThreads, joined(a[u], b[u], shift));
+    }
+    for (; v >= 0; v -= kThreads) put(v, joined(q[v], q[v + 1], shift));
   }
   for (int64_t i = threadIdx.x; i < head; i += kThreads) out[i] = from_float<Out>(to_float(p[i]) * factor);
 }
@@ -192,57 +253,67 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const double n = total.norm(), c = max_norm / (n + 1e-6);
   const float factor = c > 1.0 ? 1.0f : static_cast<float>(c);  // NaN stays
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  if (t.count == 0) return;
-  const int64_t all = t.end[t.count - 1];
-  const int64_t first = share(all, blockIdx.x, gridDim.x);
-  int64_t end = share(all, blockIdx.x + 1, gridDim.x);
-  if (first == end) return;
-  for (int i = find(t, end - 1); end > first; --i) {
-    const int64_t begin = begin_of(t, i), at = begin > first ? begin : first;
+  if (t.count == 0 || (t.in_place && factor == 1.0f)) return;
+  int i = t.count - 1;
+  for (int c = t.end[i] - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= static_cast<int>(gridDim.x)) {
+    i = find(t, c, 0, i);
+    int64_t n;
+    const int64_t from = run_of(t, i, c, &n);
     const int in = t.types[i] & 3, out = t.types[i] >> 2;
-    if (!(t.in[i] == t.out[i] && factor == 1.0f)) {
-      if (in == MUON_TRAIN_F32)
-        scale_into<float>(t.in[i], t.out[i], out, at - begin, end - at, factor);
-      else if (in == MUON_TRAIN_BF16)
-        scale_into<__nv_bfloat16>(t.in[i], t.out[i], out, at - begin, end - at, factor);
-      else
-        scale_into<__half>(t.in[i], t.out[i], out, at - begin, end - at, factor);
-    }
-    end = at;
+    if (t.in[i] == t.out[i] && factor == 1.0f) continue;
+    if (in == MUON_TRAIN_F32)
+      scale_into<float>(t.in[i], t.out[i], out, from, n, factor);
+    else if (in == MUON_TRAIN_BF16)
+      scale_into<__nv_bfloat16>(t.in[i], t.out[i], out, from, n, factor);
+    else
+      scale_into<__half>(t.in[i], t.out[i], out, from, n, factor);
   }
 }
 
 // ------------------------------------------------------------ host side
-int blocks_for(int64_t elements, int sms) {
-  const int64_t want = (elements + kLeast - 1) / kLeast, most = static_cast<int64_t>(sms) * kBlocksPerSm;
-  return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
+int blocks_for(int chunks, int sms) {
+  const int most = sms * kBlocksPerSm;
+  return chunks < 1 ? 1 : chunks < most ? chunks : most;
 }
 
-// The next tensors of the list that are not empty, from *at on.
+// Elements of a chunk of tensors of `elements` in all.
+int64_t chunk_for(int64_t elements, int sms) {
+  int64_t chunk = elements / (2 * kBlocksPerSm * sms) / kLeastChunk * kLeastChunk;
+  chunk = chunk < kLeastChunk ? kLeastChunk : chunk < kMostChunk ? chunk : kMostChunk;
+  while (elements / chunk > (int64_t{1} << 30)) chunk *= 2;
+  return chunk;
+}
+
+// The next tensors of the list that are not empty, from *at on; their chunks.
 template <int kEntries>
-int64_t fill(Table<kEntries>* t, const muon_train_clip_tensor* tensors, int64_t n, int64_t* at) {
+int fill(Table<kEntries>* t, const muon_train_clip_tensor* tensors, int64_t n, int64_t* at, int64_t chunk) {
   t->count = 0;
+  t->chunk = chunk;
+  t->in_place = 1;
   int64_t end = 0;
   for (; *at < n && t->count < kEntries; ++*at) {
     const muon_train_clip_tensor& e = tensors[*at];
     if (e.count == 0) continue;
     t->in[t->count] = e.grad;
     t->out[t->count] = e.out;
+    t->elements[t->count] = e.count;
     t->types[t->count] = static_cast<uint8_t>(e.dtype + 4 * e.out_dtype);
-    t->end[t->count++] = end += e.count;
+    t->in_place = t->in_place && e.grad == e.out;
+    end += (e.count + chunk - 1) / chunk;
+    t->end[t->count++] = static_cast<int32_t>(end);
   }
-  return end;
+  return static_cast<int>(end);
 }
 
 template <int kEntries, bool kLargest>
-int run(const muon_train_clip_tensor* tensors, int64_t n, double max_norm, float* norm, double* partial,
+int run(const muon_train_clip_tensor* tensors, int64_t n, int64_t all, double max_norm, float* norm, double* partial,
         size_t slots, int sms, void* stream) {
+  const int64_t chunk = chunk_for(all, sms);
   Table<kEntries> t;
   int partials = 0;
   for (int64_t at = 0; at < n;) {
-    const int64_t elements = fill(&t, tensors, n, &at);
+    const int blocks = blocks_for(fill(&t, tensors, n, &at, chunk), sms);
     if (t.count == 0) break;
-    const int blocks = blocks_for(elements, sms);
     if (partials + static_cast<size_t>(blocks) > slots) return MUON_POLAR_ERR_WORKSPACE;
     const int rc = launch(total_kernel<kEntries, kLargest>, dim3(blocks), kThreads, 0, 1, true, stream, t,
                           partial + partials);
@@ -251,9 +322,9 @@ int run(const muon_train_clip_tensor* tensors, int64_t n, double max_norm, float
   }
   int64_t at = 0;
   do {
-    const int64_t elements = fill(&t, tensors, n, &at);
-    const int rc = launch(scale_kernel<kEntries, kLargest>, dim3(blocks_for(elements, sms)), kThreads, 0, 1, true,
-                          stream, t, static_cast<const double*>(partial), partials, max_norm, norm);
+    const int blocks = blocks_for(fill(&t, tensors, n, &at, chunk), sms);
+    const int rc = launch(scale_kernel<kEntries, kLargest>, dim3(blocks), kThreads, 0, 1, true, stream, t,
+                          static_cast<const double*>(partial), partials, max_norm, norm);
     if (rc != MUON_POLAR_OK) return rc;
     norm = nullptr;
   } while (at < n);
@@ -261,12 +332,12 @@ int run(const muon_train_clip_tensor* tensors, int64_t n, double max_norm, float
 }
 
 template <bool kLargest>
-int run(const muon_train_clip_tensor* tensors, int64_t n, double max_norm, float* norm, double* partial,
+int run(const muon_train_clip_tensor* tensors, int64_t n, int64_t all, double max_norm, float* norm, double* partial,
         size_t slots, int sms, void* stream) {
   // A launch takes longer the more parameters it has.
-  if (n <= 64) return run<64, kLargest>(tensors, n, max_norm, norm, partial, slots, sms, stream);
-  if (n <= 256) return run<256, kLargest>(tensors, n, max_norm, norm, partial, slots, sms, stream);
-  return run<kMost, kLargest>(tensors, n, max_norm, norm, partial, slots, sms, stream);
+  if (n <= 64) return run<64, kLargest>(tensors, n, all, max_norm, norm, partial, slots, sms, stream);
+  if (n <= 256) return run<256, kLargest>(tensors, n, all, max_norm, norm, partial, slots, sms, stream);
+  return run<kMost, kLargest>(tensors, n, all, max_norm, norm, partial, slots, sms, stream);
 }
 
 }  // namespace
@@ -308,8 +379,8 @@ int muon_train_clip_sm100(const muon_train_clip_tensor* tensors, int64_t n, doub
   if (rc != MUON_POLAR_OK) return rc;
   double* partial = static_cast<double*>(workspace);
   const size_t slots = workspace_bytes / sizeof(double);
-  return norm_type == 2 ? run<false>(tensors, n, max_norm, norm, partial, slots, sms, stream)
-                        : run<true>(tensors, n, max_norm, norm, partial, slots, sms, stream);
+  return norm_type == 2 ? run<false>(tensors, n, all, max_norm, norm, partial, slots, sms, stream)
+                        : run<true>(tensors, n, all, max_norm, norm, partial, slots, sms, stream);
 }
 
 }  // extern "C"
