@@ -247,6 +247,43 @@ std::tuple<Tensor, Tensor> RotaryCuda(const Tensor& q, const OptTensor& key, con
 // Whether `t` is a run of memory without gaps, in some order of its axes.
 bool Dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
+// Bytes [begin, end) of memory, in the order of their addresses where they came
+// in that order; sorted on the first question otherwise.
+class Ranges {
+ public:
+  explicit Ranges(size_t n) { ranges_.reserve(n); }
+  void Add(uintptr_t begin, uintptr_t end) {
+    sorted_ = sorted_ && (ranges_.empty() || ranges_.back().first <= begin);
+    ranges_.emplace_back(begin, end);
+  }
+  // Whether two of them have bytes in common.
+  bool Overlap() {
+    Sort();
+    for (size_t i = 1; i < ranges_.size(); ++i)
+      if (ranges_[i - 1].second > ranges_[i].first) return true;
+    return false;
+  }
+  // Whether [begin, end) has bytes in common with one of them; they do not overlap themselves.
+  bool Touches(uintptr_t begin, uintptr_t end) {
+    Sort();
+    // questions come in the order of addresses too, as a rule: the answer is near the last one
+    if (at_ >= ranges_.size() || !(at_ == 0 || ranges_[at_ - 1].first <= begin) || ranges_[at_].first <= begin)
+      at_ = std::upper_bound(ranges_.begin(), ranges_.end(), std::make_pair(begin, UINTPTR_MAX)) - ranges_.begin();
+    return (at_ > 0 && ranges_[at_ - 1].second > begin) || (at_ < ranges_.size() && ranges_[at_].first < end);
+  }
+
+ private:
+  void Sort() {
+    if (!sorted_) std::sort(ranges_.begin(), ranges_.end());
+    sorted_ = true;
+  }
+  std::vector<std::pair<uintptr_t, uintptr_t>> ranges_;
+  bool sorted_ = true;
+  size_t at_ = 0;
+};
+
+// A call with hundreds of tensors is bound by the host: what cannot be wrong is
+// not asked twice.
 Tensor ClipCuda(at::TensorList grads, at::TensorList out, double max_norm, bool largest) {
   const char* who = "clip_gradients";
   TORCH_CHECK_VALUE(!grads.empty(), who, ": no gradients");
@@ -255,52 +292,45 @@ Tensor ClipCuda(at::TensorList grads, at::TensorList out, double max_norm, bool 
   TORCH_CHECK_VALUE(max_norm >= 0.0, who, ": max_norm must not be negative, got ", max_norm);
   CheckCuda(grads[0], who, "gradients");
   const c10::cuda::CUDAGuard guard(grads[0].device());
-  std::vector<muon_train_clip_tensor> list(grads.size());
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  written.reserve(grads.size());
-  bool ascending = true;
-  for (size_t i = 0; i < grads.size(); ++i) {
+  const size_t n = grads.size();
+  std::vector<muon_train_clip_tensor> list(n);
+  Ranges written(n);
+  const auto check = [&](const Tensor& t, const char* name) {
+    CheckDevice(t, grads[0], who, name);
+    if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return;  // never seen by autograd
+    NoTangents({&t}, who);
+    TORCH_CHECK_VALUE(!t.requires_grad(), who,
+                      ": parameters and recorded tensors are not clipped (pass their gradients, detached)");
+  };
+  for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
     const Tensor& o = out.empty() ? g : out[i];
-    CheckDevice(g, grads[0], who, "every gradient");
-    NoTangents({&g, &o}, who);
-    TORCH_CHECK_VALUE(!g.requires_grad() && !o.requires_grad(), who,
-                      ": parameters and recorded tensors are not clipped (pass their gradients, detached)");
+    check(g, "every gradient");
     TORCH_CHECK_VALUE(Dense(g), who, ": gradients must be dense, got strides ", g.strides(), " for ", g.sizes());
     muon_train_clip_tensor& t = list[i];
     t.count = g.numel();
     t.dtype = t.out_dtype = Dtype(g, who, "every gradient");
-    t.grad = g.data_ptr();
-    t.out = t.count > 0 ? o.data_ptr() : nullptr;
     if (!out.empty()) {
-      CheckDevice(o, g, who, "out");
+      check(o, "out");
       TORCH_CHECK_VALUE(o.sizes() == g.sizes() && (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
                         who, ": out must have its gradient's shape and layout, got ", o.sizes(), " for ", g.sizes());
       t.out_dtype = Dtype(o, who, "out");
     }
     if (t.count == 0) continue;
+    t.grad = g.unsafeGetTensorImpl()->data();
+    t.out = out.empty() ? const_cast<void*>(t.grad) : o.unsafeGetTensorImpl()->mutable_data();
     const uintptr_t begin = reinterpret_cast<uintptr_t>(t.out);
-    const uintptr_t end = begin + static_cast<uintptr_t>(t.count) * o.element_size();
-    ascending = ascending && (written.empty() || written.back().second <= begin);
-    written.emplace_back(begin, end);
+    written.Add(begin, begin + static_cast<uintptr_t>(t.count) * o.element_size());
   }
-  if (!ascending) {
-    std::sort(written.begin(), written.end());
-    for (size_t i = 1; i < written.size(); ++i)
-      TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, who,
-                        ": the same memory would be scaled twice (a gradient listed twice, or views of one another)");
-  }
+  TORCH_CHECK_VALUE(!written.Overlap(), who,
+                    ": the same memory would be scaled twice (a gradient listed twice, or views of one another)");
   if (!out.empty()) {  // what is written may not be read as another gradient
     for (const muon_train_clip_tensor& t : list) {
-      if (t.count == 0) continue;
       const uintptr_t begin = reinterpret_cast<uintptr_t>(t.grad);
-      const uintptr_t end = begin + static_cast<uintptr_t>(t.count) * (t.dtype == MUON_TRAIN_F32 ? 4 : 2);
-      const auto next = std::upper_bound(written.begin(), written.end(), std::make_pair(begin, UINTPTR_MAX));
-      const bool before = next != written.begin() && std::prev(next)->second > begin;
-      const bool after = next != written.end() && next->first < end;
       const bool itself = t.grad == t.out && t.dtype == t.out_dtype;
-      TORCH_CHECK_VALUE(itself || (!before && !after), who,
-                        ": out may be its gradient, of the same type, but not overlap one otherwise");
+      TORCH_CHECK_VALUE(t.count == 0 || itself ||
+                            !written.Touches(begin, begin + static_cast<uintptr_t>(t.count) * (t.dtype == MUON_TRAIN_F32 ? 4 : 2)),
+                        who, ": out may be its gradient, of the same type, but not overlap one otherwise");
     }
   }
   Tensor norm = Empty({}, at::kFloat, grads[0]);
