@@ -59,6 +59,30 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar, uint32_t elected) {
       : "memory");
 }
 
+// Asks for a block of this grid that has not begun, to do its work in its place;
+// the 16 bytes of the answer are counted on `bar`.
+__device__ __forceinline__ void try_cancel_block(void* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_addr(answer)),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+// The block's index along x; -1 if there was none left.
+__device__ __forceinline__ int cancelled_block(const void* answer) {
+  uint32_t found, x = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+      : "=r"(found), "+r"(x)
+      : "r"(smem_addr(answer))
+      : "memory");
+  return found != 0 ? static_cast<int>(x) : -1;
+}
+
 // Registers of the threads of a warpgroup from here on, out of those that the
 // block was launched with.
 template <int kRegisters>

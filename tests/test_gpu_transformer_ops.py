@@ -167,6 +167,24 @@ def test_attention_of_long_sequences(pkg, dim):
     check_attention(pkg, q, k, v, go, sequences=whole(1))
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_many_tiles(pkg, causal):
+    """Many rounds of every ring and barrier, over and over: each run gives the
+    same bits, and no wait runs out."""
+    from muon_fusion_ascend950_b200.capi import capi
+
+    q, k, v, go = attention_inputs(1, 8200, 8200, 4, 2, 128, BF16, seed=8, fused=True)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    first = None
+    for _ in range(12):
+        out = pkg.attention(*leaves, causal=causal)
+        got = [out.detach(), *torch.autograd.grad(out, leaves, go)]
+        first = first or got
+        for a, b in zip(got, first):
+            assert torch.equal(a, b)
+    assert capi().train_device_status(torch.cuda.current_device()) == 0
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
