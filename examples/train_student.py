@@ -1,13 +1,15 @@
-"""Trains a small mixture-of-experts student by distillation, with the package's
+"""Trains a small mixture-of-experts transformer by distillation, with the package's
 training-step operators and the ``Muon`` optimizer together:
 
     python examples/train_student.py [--steps 60]
 
-Every block ends in ``residual_norm`` (the post-norm, gate and residual add of
+Queries and keys are turned by ``rotary`` and tokens look back by ``attention``;
+every block ends in ``residual_norm`` (the post-norm, gate and residual add of
 this block and the pre-norm of the next in one pass), tokens go to experts by
 ``route_experts`` with a balancing bias, the loss and its gradient in the logits
-come from ``distill_topk_grad``, and ``Muon`` updates the matrices, the experts'
-[experts, in, out] batches among them.  The teacher is a table of logits for
+come from ``distill_topk_grad``, ``clip_grad_norm`` holds the gradients to a norm,
+and ``Muon`` updates the matrices, the experts' [experts, in, out] batches among
+them.  The teacher is a table of logits for
 each token, of which the student sees the top 16.
 """
 from __future__ import annotations
@@ -24,9 +26,13 @@ sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 from muon_fusion_ascend950_b200 import (  # noqa: E402
     Muon,
+    attention,
+    clip_grad_norm,
     distill_topk,
     distill_topk_grad,
     residual_norm,
+    rotary,
+    rotary_frequencies,
     route_experts,
 )
 
@@ -50,12 +56,30 @@ class Tail(nn.Module):
                              residual_scale=self.scale)
 
 
+class Attention(nn.Module):
+    """Causal attention of query heads that share key heads, at rotary positions."""
+
+    def __init__(self, width, heads=4, kv_heads=2, dim=32):
+        super().__init__()
+        self.heads, self.dim = [heads, kv_heads, kv_heads], dim
+        self.into, self.out = matrix(width, sum(self.heads) * dim), matrix(heads * dim, width)
+        self.register_buffer("frequencies", rotary_frequencies(dim, device="cpu")[0])
+
+    def forward(self, normed):
+        heads = (normed @ self.into.to(normed.dtype)).unflatten(-1, (-1, self.dim))
+        query, key, value = heads.split(self.heads, dim=-2)
+        positions = torch.arange(normed.shape[1], device=normed.device)
+        query, key = rotary(query, key, positions, self.frequencies)
+        return attention(query, key, value, causal=True).flatten(-2) @ self.out.to(normed.dtype)
+
+
 class Block(nn.Module):
-    """A dense layer, then experts, each with its tail."""
+    """Attention, a dense layer, then experts, each with its tail."""
 
     def __init__(self, width, inner, experts, k):
         super().__init__()
         self.k = k
+        self.attention, self.attention_tail = Attention(width), Tail(width)
         self.dense_in, self.dense_out = matrix(width, inner), matrix(inner, width)
         self.router = matrix(width, experts)
         self.experts_in, self.experts_out = matrix(experts, width, inner), matrix(experts, inner, width)
@@ -63,6 +87,7 @@ class Block(nn.Module):
         self.register_buffer("bias", torch.zeros(experts))
 
     def forward(self, hidden, normed):
+        hidden, normed = self.attention_tail(self.attention(normed), hidden)
         out = F.silu(normed @ self.dense_in.to(normed.dtype)) @ self.dense_out.to(normed.dtype)
         hidden, normed = self.dense_tail(out, hidden)
         weights, indices, counts = route_experts(normed.float() @ self.router, self.k, score="sigmoid",
@@ -92,7 +117,7 @@ class Student(nn.Module):
         return normed @ self.head.to(normed.dtype)
 
 
-def train(steps=60, batch=8, length=64, top=16, seed=0, log=None):
+def train(steps=60, batch=8, length=64, top=16, max_norm=1.0, seed=0, log=None):
     """Returns the mean loss a token of each step and of a last evaluation."""
     torch.manual_seed(seed)
     student = Student().cuda()
@@ -115,6 +140,7 @@ def train(steps=60, batch=8, length=64, top=16, seed=0, log=None):
         logits = student(tokens)
         loss, grad = distill_topk_grad(logits, values, indices, counted / counted.sum())
         logits.backward(grad)
+        clip_grad_norm(student.parameters(), max_norm)
         for optimizer in optimizers:
             optimizer.step()
             optimizer.zero_grad(set_to_none=True)
