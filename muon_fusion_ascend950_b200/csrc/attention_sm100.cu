@@ -12,8 +12,8 @@
 // shared memory.  The scores are read from tensor memory into registers, a row
 // a thread, and the probabilities go back there as 16-bit values, in place of
 // the scores, as the next product's left operand: neither is ever in shared or
-// global memory.  Eight warps of a block work on the scores, one loads and one issues the
-// products.
+// global memory.  Eight warps of a block work on the scores, one loads and one
+// issues the products.
 //
 // The backward pass computes the scores again.  It is two kernels, one for a
 // tile of keys (dk, dv: four products a pair of tiles) and one for a tile of
@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   int fills = 0, loads = 0, asked = 0;
   if (warp >= kLoadWarp) {
-  give_registers<kOtherRegisters>();
+    give_registers<kOtherRegisters>();
     if (warp == kLoadWarp) {
       bool ok = true;
       int g = 0;
@@ -1165,7 +1165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   int fills = 0, loads = 0, asked = 0;
   if (warp >= kLoadWarp) {
-  give_registers<kOtherRegisters>();
+    give_registers<kOtherRegisters>();
     if (warp == kLoadWarp) {
       bool ok = true;
       for (int item = blockIdx.x; ok && item >= 0; item = queue.next(&asked, failed)) {
@@ -1341,13 +1341,15 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-                       q == cudaDriverEntryPointSuccess;
-    return found ? reinterpret_cast<EncodeTiled>(f) : nullptr;
-  }();
+  static std::atomic<EncodeTiled> known{nullptr};
+  EncodeTiled fn = known.load(std::memory_order_relaxed);
+  if (fn != nullptr) return fn;
+  void* f = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+      q == cudaDriverEntryPointSuccess)
+    fn = reinterpret_cast<EncodeTiled>(f);
+  known.store(fn, std::memory_order_relaxed);
   return fn;
 }
 
@@ -1452,16 +1454,19 @@ Problem problem_of(const muon_train_attention_args& a) {
   return p;
 }
 
-// Once for each device: lets a kernel have its shared memory, and checks that it
-// is launched with the registers that its warpgroups share out among them, or
-// it would wait for them forever.
+// Lets a kernel have its shared memory, and checks once that it is launched with
+// the registers that its warpgroups share out among them, or it would wait for
+// them forever.
 template <auto kKernel>
 int prepare(size_t bytes) {
-  static const bool fits = [] {
+  static std::atomic<bool> checked{false};
+  if (!checked.load(std::memory_order_relaxed)) {
     cudaFuncAttributes attributes;
-    return cudaFuncGetAttributes(&attributes, kKernel) == cudaSuccess && attributes.numRegs == kLaunchRegisters;
-  }();
-  if (!fits) return MUON_POLAR_ERR_UNSUPPORTED_DEVICE;
+    const cudaError_t e = cudaFuncGetAttributes(&attributes, kKernel);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (attributes.numRegs != kLaunchRegisters) return MUON_POLAR_ERR_UNSUPPORTED_DEVICE;
+    checked.store(true, std::memory_order_relaxed);
+  }
   return allow_smem<kKernel>(bytes);
 }
 

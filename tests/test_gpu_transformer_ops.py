@@ -513,12 +513,28 @@ def some_grads(sizes, dtypes, seed, std=1e-2, shift=0):
 @pytest.mark.parametrize("norm_type", [2.0, math.inf])
 @pytest.mark.parametrize("out_dtype", [None, F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("shift", [0, 1, 3])
-@pytest.mark.parametrize("sizes", [[1], [1000], [0, 5, 0], [8191, 64, 1, 100003], [3] * 70, [257] * 300, [65, 0] * 600,
+@pytest.mark.parametrize("sizes", [[1], [1000], [0, 5, 0], [8191, 64, 1, 100003], [3] * 70, [257] * 300,
                                    [3_000_001, 17, 2_000_000]], ids=lambda s: f"{len(s)}x{s[0]}")
 def test_clip(pkg, sizes, shift, out_dtype, norm_type):
     for dtypes in ([F32], [BF16, F32, F16]):
         for limit in (1e-3, 1e6):
             check_clip(pkg, some_grads(sizes, dtypes, seed=50, shift=shift), limit, norm_type=norm_type, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+def test_clip_of_more_tensors_than_a_launch_takes(pkg, norm_type):
+    for sizes in ([65, 0] * 600, [2] * 2500, [300] * 1025):
+        grads = some_grads(sizes, [F32, BF16], seed=50)
+        check_clip(pkg, grads, 1e-3, norm_type=norm_type, out_dtype=BF16)
+        check_clip(pkg, grads, 1e-3, norm_type=norm_type)
+
+
+@pytest.mark.parametrize("elements", [1, 2 ** 18 - 3, 2 ** 18, 2 ** 18 + 1, 2 ** 18 + 70000])
+def test_clip_in_one_launch_or_two(pkg, elements):
+    for parts in (1, 3, 64, 65):
+        if elements >= parts:
+            sizes = [elements // parts] * (parts - 1) + [elements - elements // parts * (parts - 1)]
+            check_clip(pkg, some_grads(sizes, [BF16], seed=51), 1e-3)
 
 
 def test_clip_of_shapes_and_layouts(pkg):
@@ -686,6 +702,28 @@ def test_steps_in_cuda_graphs(pkg):
     torch.cuda.synchronize()
     for a, b in zip(got[0], want[1]):
         assert torch.equal(a, b)
+
+
+def test_fp16_attention_in_a_graph(pkg):
+    """Its gradients' scale is found on the device, in every replay anew."""
+    q, k, v, go = attention_inputs(2, 200, 200, 2, 1, 64, F16, seed=111)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+
+    def grads():
+        return torch.autograd.grad(pkg.attention(*leaves, causal=True), leaves, go)
+
+    grads()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = grads()
+    for size in (1.0, 1e-3, 500.0):
+        go.mul_(size)
+        want = grads()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
 
 def test_compiled_block(pkg):
