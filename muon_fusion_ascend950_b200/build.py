@@ -8,8 +8,8 @@
   ``residual_norm_sm100.cu``, ``route_experts_sm100.cu``, ``attention_sm100.cu``,
   ``rotary_sm100.cu``, ``clip_grads_sm100.cu``).
 * ``_C.so`` -- the PyTorch operators ``muon_ascend950::*`` on the CUDA
-  dispatch key (``polar_step_op.cpp``, ``train_ops.cpp``, ``block_ops.cpp``),
-  linked against the library above (rpath ``$ORIGIN``).
+  dispatch key (``polar_step_op.cpp``, ``train_ops.cpp``, ``block_ops.cpp``,
+  and ``clip_list.cpp`` beside them), linked against the library above (rpath ``$ORIGIN``).
 
 Both land next to this file so that they travel with the source tree.  Each
 source compiles to an object under ``_build/`` (all in parallel); what is newer
@@ -22,6 +22,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -72,6 +73,7 @@ OP_SOURCES = {
     "polar_step_op.cpp": ["muon_polar_sm100.h"],
     "train_ops.cpp": ["train_ops_common.h", "muon_train_sm100.h", "muon_polar_sm100.h"],
     "block_ops.cpp": ["train_ops_common.h", "muon_train_sm100.h", "muon_polar_sm100.h"],
+    "clip_list.cpp": ["train_ops_common.h", "muon_train_sm100.h", "muon_polar_sm100.h"],
 }
 
 
@@ -125,7 +127,8 @@ def build_op(force: bool = False) -> Path:
         return out
     cuda_home = _cuda_home()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    includes = cpp_extension.include_paths() + [str(cuda_home / "include"), str(INCLUDE)]
+    includes = cpp_extension.include_paths() + [str(cuda_home / "include"), str(INCLUDE),
+                                                sysconfig.get_paths()["include"]]
     objects = _compile(OP_SOURCES, ["g++", "-O2", "-std=c++17", "-fPIC",
                                     f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
                                     *[f"-I{p}" for p in includes]], force)

@@ -753,12 +753,14 @@ __global__ void __launch_bounds__(256, 6) stats_kernel(const __grid_constant__ S
     join(big, a.largest);
     big = 0.0f;
     const int64_t v_items = a.v_rows * a.kv_heads;
-    for (int64_t item = base + threadIdx.x / kLanes; item < v_items; item += static_cast<int64_t>(gridDim.x) * kGroups * kStatRows) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups * kStatRows;
+    for (int64_t item = base + threadIdx.x / kLanes; item < v_items; item += step) {
 #pragma unroll
       for (int u = 0; u < kStatRows; ++u) {
         const int64_t at = item + u * kGroups;
         if (at >= v_items || lane * 8 >= dim) continue;
-        const uint32_t r = static_cast<uint32_t>(at / a.kv_heads), h = static_cast<uint32_t>(at - static_cast<int64_t>(r) * a.kv_heads);
+        const uint32_t r = static_cast<uint32_t>(at / a.kv_heads);
+        const uint32_t h = static_cast<uint32_t>(at - static_cast<int64_t>(r) * a.kv_heads);
         float x[8];
         unpack<T>(*reinterpret_cast<const uint4*>(row_of<T>(a.v, a.v_stride, r, a.keys, h) + lane * 8), x);
 #pragma unroll
@@ -796,7 +798,8 @@ struct KeyGrads {
 // is none (232448 bytes, of which seven tiles take 229376).
 struct KeyShared {
   Items queue;
-  uint64_t kv_full, kv_empty, s_full, dp_full, p_done[2], ds_done[2], finished, drained, stat_full[2], stat_read[2], full[8], empty[8];
+  uint64_t kv_full, kv_empty, s_full, dp_full, p_done[2], ds_done[2], finished, drained;
+  uint64_t stat_full[2], stat_read[2], full[8], empty[8];
   __align__(16) float stat[2][2][kTile];  // of two tiles of queries: -lse and -delta
   uint32_t tmem_slot;
   int failed_word;
@@ -1126,7 +1129,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ Problem p, int tiles) {
   using C = KeyGrads<kCols>;
   extern __shared__ __align__(1024) uint8_t dynamic[];
-  __shared__ uint64_t q_full, q_empty, s_full[2], dp_full, dp_read, ds_done[2][2], finished, drained, full[C::kStages], empty[C::kStages];
+  __shared__ uint64_t q_full, q_empty, s_full[2], dp_full, dp_read, ds_done[2][2], finished, drained;
+  __shared__ uint64_t full[C::kStages], empty[C::kStages];
   __shared__ Items queue;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_word;
@@ -1473,16 +1477,20 @@ int prepare(size_t bytes) {
 // Heads, of all batch entries, of a section: as many as stay in L2 together
 // with `bytes` of streamed tiles each, but enough for a few items a block, so
 // that a section's large items do not come at the end of all.  8192 keys both
-// ways, 32 heads of 4 MB: forward 700 us with 16 a section, 785 with all; 64
-// heads that share 16 of 2 MB, causal: 301 us with all, 366 with one.
+// ways, 32 heads of 4 MB: backward 3400 us with 8 heads a section, 3600 with 16;
+// 37 heads of 4096 causal, 2 MB each: forward 190 us, 212 with one round of the
+// blocks, and a head at a time 366 us where 64 heads together took 301.
 constexpr int64_t kSectionBytes = int64_t{32} << 20;
+constexpr int kSectionRounds = 2;
 int section_of(int64_t heads, int64_t bytes, int64_t tiles, int* section) {
   int sms = 0;
   const int rc = sm_count(&sms);
   int64_t n = kSectionBytes / (bytes > 0 ? bytes : 1);
-  const int64_t least = (4 * static_cast<int64_t>(sms) + tiles - 1) / (tiles > 0 ? tiles : 1);
+  const int64_t least = (kSectionRounds * static_cast<int64_t>(sms) + tiles - 1) / (tiles > 0 ? tiles : 1);
   n = n > least ? n : least;
-  *section = static_cast<int>(n < 1 ? 1 : n < heads ? n : heads);
+  n = n < 1 ? 1 : n;
+  const int64_t sections = (heads + n - 1) / n;  // of about the same size
+  *section = static_cast<int>((heads + sections - 1) / sections);
   return rc;
 }
 
@@ -1501,8 +1509,8 @@ int forward(const muon_train_attention_args& a, void* stream) {
   const int64_t group = a.heads / a.kv_heads, pair_bytes = 2 * a.dim * static_cast<int64_t>(sizeof(T));
   rc = section_of(a.batch * a.heads, a.keys * pair_bytes / group, tiles / a.batch, &p.section);
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(forward_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.heads)), kThreads, kBytes, 1, true, stream, m.q, m.k, m.v, p,
-                static_cast<int>(tiles));
+  return launch(forward_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.heads)), kThreads, kBytes, 1, true,
+                stream, m.q, m.k, m.v, p, static_cast<int>(tiles));
 }
 
 template <typename T, int kCols>
@@ -1533,12 +1541,14 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
   const Stats st{a.out, a.out_rest, g.grad_out, a.v, a.lse, stats, largest, g.grad_out_stride, a.v_stride, rows,
                  a.batch * a.keys, p.length, p.keys, p.heads, p.kv_heads, p.dim};
   const int64_t per = 256 / (kCols / 8) * kStatRows;
-  rc = launch(stats_kernel<T, kCols>, dim3(static_cast<unsigned>((rows * a.heads + per - 1) / per)), 256, 0, 1, true, stream, st);
+  const dim3 grid(static_cast<unsigned>((rows * a.heads + per - 1) / per));
+  rc = launch(stats_kernel<T, kCols>, grid, 256, 0, 1, true, stream, st);
   if (rc != MUON_POLAR_OK) return rc;
   const int64_t group = a.heads / a.kv_heads, pair_bytes = 2 * a.dim * static_cast<int64_t>(sizeof(T));
   constexpr int kBytes = KeyGrads<kCols>::kBytes;
   if (a.keys > 0) {
-    constexpr int kBytes = (2 + KeyGrads<kCols>::kStages) * KeyGrads<kCols>::kTileBytes + static_cast<int>(sizeof(KeyShared));
+    constexpr int kBytes =
+        (2 + KeyGrads<kCols>::kStages) * KeyGrads<kCols>::kTileBytes + static_cast<int>(sizeof(KeyShared));
     rc = prepare<key_grad_kernel<T, kCols>>(kBytes);
     if (rc != MUON_POLAR_OK) return rc;
     p.out = g.grad_k;

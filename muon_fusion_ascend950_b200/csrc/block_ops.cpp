@@ -282,29 +282,33 @@ class Ranges {
   size_t at_ = 0;
 };
 
+}  // namespace
+
 // A call with hundreds of tensors is bound by the host: what cannot be wrong is
 // not asked twice.
-Tensor ClipCuda(at::TensorList grads, at::TensorList out, double max_norm, bool largest) {
+void muon_train_ops::clip_gradients(TensorPointers grads, TensorPointers out, double max_norm, bool largest,
+                                    const Tensor& norm) {
   const char* who = "clip_gradients";
   TORCH_CHECK_VALUE(!grads.empty(), who, ": no gradients");
   TORCH_CHECK_VALUE(out.empty() || out.size() == grads.size(), who, ": out must have a tensor for each gradient, got ",
                     out.size(), " and ", grads.size());
   TORCH_CHECK_VALUE(max_norm >= 0.0, who, ": max_norm must not be negative, got ", max_norm);
-  CheckCuda(grads[0], who, "gradients");
-  const c10::cuda::CUDAGuard guard(grads[0].device());
+  const Tensor& first = *grads[0];
+  CheckCuda(first, who, "gradients");
+  const c10::cuda::CUDAGuard guard(first.device());
   const size_t n = grads.size();
   std::vector<muon_train_clip_tensor> list(n);
   Ranges written(n);
   const auto check = [&](const Tensor& t, const char* name) {
-    CheckDevice(t, grads[0], who, name);
+    CheckDevice(t, first, who, name);
     if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return;  // never seen by autograd
     NoTangents({&t}, who);
     TORCH_CHECK_VALUE(!t.requires_grad(), who,
                       ": parameters and recorded tensors are not clipped (pass their gradients, detached)");
   };
   for (size_t i = 0; i < n; ++i) {
-    const Tensor& g = grads[i];
-    const Tensor& o = out.empty() ? g : out[i];
+    const Tensor& g = *grads[i];
+    const Tensor& o = out.empty() ? g : *out[i];
     check(g, "every gradient");
     TORCH_CHECK_VALUE(Dense(g), who, ": gradients must be dense, got strides ", g.strides(), " for ", g.sizes());
     muon_train_clip_tensor& t = list[i];
@@ -333,20 +337,35 @@ Tensor ClipCuda(at::TensorList grads, at::TensorList out, double max_norm, bool 
                         who, ": out may be its gradient, of the same type, but not overlap one otherwise");
     }
   }
-  Tensor norm = Empty({}, at::kFloat, grads[0]);
-  const size_t bytes = muon_train_clip_workspace_bytes(static_cast<int64_t>(list.size()));
-  const Tensor workspace = Empty({static_cast<int64_t>(bytes)}, at::kByte, grads[0]);
-  CheckStatus(muon_train_clip_sm100(list.data(), static_cast<int64_t>(list.size()), max_norm, largest ? 0 : 2,
-                                    static_cast<float*>(Ptr(norm)), Ptr(workspace), bytes, Stream(grads[0])),
+  TORCH_CHECK_VALUE(norm.device() == first.device() && norm.scalar_type() == at::kFloat && norm.numel() == 1, who,
+                    ": norm must be one float32 element on ", first.device());
+  const size_t bytes = muon_train_clip_workspace_bytes(static_cast<int64_t>(n));
+  const Tensor workspace = Empty({static_cast<int64_t>(bytes)}, at::kByte, first);
+  CheckStatus(muon_train_clip_sm100(list.data(), static_cast<int64_t>(n), max_norm, largest ? 0 : 2,
+                                    static_cast<float*>(Ptr(norm)), Ptr(workspace), bytes, Stream(first)),
               who);
-  for (const Tensor& t : out.empty() ? grads : out)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  for (const Tensor* t : out.empty() ? grads : out)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+namespace {
+
+Tensor ClipCuda(at::TensorList grads, at::TensorList out, double max_norm, bool largest) {
+  TORCH_CHECK_VALUE(!grads.empty(), "clip_gradients: no gradients");
+  CheckCuda(grads[0], "clip_gradients", "gradients");
+  Tensor norm = Empty({}, at::kFloat, grads[0]);
+  std::vector<const Tensor*> g(grads.size()), o(out.size());
+  for (size_t i = 0; i < g.size(); ++i) g[i] = &grads[i];
+  for (size_t i = 0; i < o.size(); ++i) o[i] = &out[i];
+  muon_train_ops::clip_gradients(g, o, max_norm, largest, norm);
   return norm;
 }
 Tensor ClipInPlaceCuda(at::TensorList grads, double max_norm, bool largest) {
   return ClipCuda(grads, {}, max_norm, largest);
 }
 Tensor ClipOutCuda(at::TensorList grads, at::TensorList out, double max_norm, bool largest) {
+  TORCH_CHECK_VALUE(out.size() == grads.size(), "clip_gradients: out must have a tensor for each gradient, got ",
+                    out.size(), " and ", grads.size());
   return ClipCuda(grads, out, max_norm, largest);
 }
 

@@ -108,4 +108,10 @@ std::shared_ptr<N> MakeNode(const Inputs&... inputs) {
 
 inline OptTensor Optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+// Clips `grads` in place, or into `out` where it is not empty; their norm goes to
+// `norm` (one fp32 element).  By pointers: to copy a tensor that Python holds
+// counts its object's references too.  block_ops.cpp
+using TensorPointers = c10::ArrayRef<const Tensor*>;
+void clip_gradients(TensorPointers grads, TensorPointers out, double max_norm, bool largest, const Tensor& norm);
+
 }  // namespace muon_train_ops

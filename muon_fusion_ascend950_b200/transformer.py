@@ -15,11 +15,13 @@ take part in autograd (gradients of gradients and forward mode are refused).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Iterable, Optional, Sequence, Tuple, Union
 
 import torch
 
+from ._loader import _library_path
 from .training import _check, _explain, _float32
 
 # muon_train_sm100.h: MUON_TRAIN_MAX_HEAD_DIM, _MAX_ROTARY_DIM
@@ -29,6 +31,29 @@ _attention = torch.ops.muon_ascend950.attention.default
 _rotary = torch.ops.muon_ascend950.rotary.default
 _clip_in_place = torch.ops.muon_ascend950.clip_gradients_.default
 _clip_out = torch.ops.muon_ascend950.clip_gradients.default
+# The same on Python's own lists (clip_list.cpp), for long ones: the call itself
+# takes longer.  A library set by MUON_ASCEND950_LIBRARY may be without it.
+_library = ctypes.PyDLL(str(_library_path()))
+_clip_list = getattr(_library, "muon_ascend950_clip_list", None)
+if _clip_list is not None:
+    _clip_list.argtypes = [ctypes.py_object, ctypes.c_void_p, ctypes.py_object, ctypes.c_double, ctypes.c_int]
+    _library.muon_ascend950_clip_message.restype = ctypes.c_char_p
+_CLIP_ERRORS = {1: ValueError, 2: TypeError, 3: NotImplementedError, 4: RuntimeError}
+_LONG_LIST = 32
+_PLAIN = {torch.Tensor}
+
+
+def _clip_lists(gradients: list, out: Optional[list], max_norm: float, largest: bool) -> Optional[torch.Tensor]:
+    """The norm; None if the call has to go through the operator."""
+    if set(map(type, gradients)) != _PLAIN or (out is not None and set(map(type, out)) != _PLAIN):
+        return None
+    if not gradients[0].is_cuda:
+        return None
+    norm = torch.empty((), dtype=torch.float32, device=gradients[0].device)
+    status = _clip_list(gradients, None if out is None else id(out), norm, max_norm, largest)
+    if status in _CLIP_ERRORS:
+        raise _CLIP_ERRORS[status](_library.muon_ascend950_clip_message().decode(errors="replace"))
+    return norm if status == 0 else None
 
 
 # ------------------------------------------------- checks of traced calls
@@ -260,9 +285,15 @@ def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, *, norm_t
     if norm_type not in (2, math.inf):
         raise ValueError(f"norm_type must be 2 or infinity, got {norm_type}")
     try:
+        out = None if out is None else list(out)
+        long = len(gradients) + (len(out) if out is not None else 0) > _LONG_LIST
+        if long and _clip_list is not None and not torch.compiler.is_compiling():
+            norm = _clip_lists(gradients, out, max_norm, norm_type != 2)
+            if norm is not None:
+                return norm
         if out is None:
             return _clip_in_place(gradients, max_norm, norm_type != 2)
-        return _clip_out(gradients, list(out), max_norm, norm_type != 2)
+        return _clip_out(gradients, out, max_norm, norm_type != 2)
     except Exception:
         for t in gradients:
             _explain(gradients=t)

@@ -581,6 +581,45 @@ def test_clip_of_parameters(pkg):
     assert pkg.clip_grad_norm([c], 1.0) == 0.0 and pkg.clip_grad_norm(a, math.inf) > 0
 
 
+def test_clip_goes_through_the_operator_where_something_listens(pkg):
+    """Python's lists are read directly; dispatch modes, compilation and other
+    tensor types see the operator, with the same results."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Listen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func)
+            return func(*args, **(kwargs or {}))
+
+    g = some_grads([1000, 17] * 20, [BF16, F32], seed=72)
+    direct, listened, compiled = ([t.clone() for t in g] for _ in range(3))
+    norms = [pkg.clip_gradients(direct, 0.1)]
+    assert not seen
+    with Listen():
+        norms.append(pkg.clip_gradients(listened, 0.1))
+    assert torch.ops.muon_ascend950.clip_gradients_.default in seen
+    norms.append(torch.compile(lambda *t: pkg.clip_gradients(list(t), 0.1), backend="aot_eager", fullgraph=True)(*compiled))
+    for a, b, c in zip(direct, listened, compiled):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert norms[0] == norms[1] == norms[2]
+    buffers = [torch.nn.Buffer(t.clone()) for t in g]  # not of the type torch.Tensor itself
+    assert pkg.clip_gradients(buffers, 0.1) == norms[0] and torch.equal(buffers[0], direct[0])
+    out = [torch.empty_like(t) for t in g]
+    assert pkg.clip_gradients(tuple(g), 0.1, out=tuple(out)) == norms[0] and torch.equal(out[1], direct[1])
+    for wrong, error in ((g[0].cpu(), ValueError), (g[0].long(), TypeError), (3, TypeError), (None, TypeError),
+                         (g[1], ValueError), (g[0].clone().requires_grad_(True), ValueError)):
+        for grads in ([wrong] + g, g + [wrong], [g[1], wrong]):
+            with pytest.raises(error):
+                pkg.clip_gradients(grads, 1.0)
+    for out in ([], g[:39], g[:-1] + [g[0]], [torch.empty_like(t)[:5] for t in g]):
+        with pytest.raises(ValueError):
+            pkg.clip_gradients(g, 1.0, out=out)
+    with pytest.raises(ValueError):
+        pkg.clip_gradients(g, -1.0)
+
+
 def test_clip_refuses_memory_that_would_be_scaled_twice(pkg):
     g = randn(100, seed=69)
     for grads, out in (([g, g], None), ([g[:60], g[40:]], None), ([g, randn(100, seed=70)], [g, g]),
