@@ -131,38 +131,39 @@ __device__ __forceinline__ void add_load(const uint4& raw, Total<kLargest>& tota
   }
 }
 
-template <typename T, bool kLargest>
-__device__ __forceinline__ void total_of(const T* p, int64_t n, Total<kLargest>& total) {
+// By kGroup threads, of which this is thread `rank`.
+template <int kGroup, typename T, bool kLargest>
+__device__ __forceinline__ void total_of(const T* p, int64_t n, int rank, Total<kLargest>& total) {
   constexpr int kN = kVec<T>;
   const int64_t head = head_of(p, n), vectors = (n - head) / kN, tail = head + vectors * kN;
-  for (int64_t i = threadIdx.x; i < head; i += kThreads) total.add(to_float(p[i]));
-  for (int64_t i = tail + threadIdx.x; i < n; i += kThreads) total.add(to_float(p[i]));
+  for (int64_t i = rank; i < head; i += kGroup) total.add(to_float(p[i]));
+  for (int64_t i = tail + rank; i < n; i += kGroup) total.add(to_float(p[i]));
   const uint4* q = reinterpret_cast<const uint4*>(p + head);
-  int64_t v = threadIdx.x;
-  for (; v + (kUnrollSum - 1) * kThreads < vectors; v += kThreads * kUnrollSum) {
+  int64_t v = rank;
+  for (; v + (kUnrollSum - 1) * kGroup < vectors; v += kGroup * kUnrollSum) {
     uint4 raw[kUnrollSum];
 #pragma unroll
-    for (int u = 0; u < kUnrollSum; ++u) raw[u] = q[v + u * kThreads];
+    for (int u = 0; u < kUnrollSum; ++u) raw[u] = q[v + u * kGroup];
 #pragma unroll
     for (int u = 0; u < kUnrollSum; ++u) add_load<T>(raw[u], total);
   }
-  for (; v < vectors; v += kThreads) add_load<T>(q[v], total);
+  for (; v < vectors; v += kGroup) add_load<T>(q[v], total);
 }
 
-// The share of block `block` of `blocks`.
-template <int kEntries, bool kLargest>
-__device__ __forceinline__ double share_total(const Table<kEntries>& t, int block, int blocks) {
+// The share of group `group` of `groups` of kGroup threads.
+template <int kGroup, int kEntries, bool kLargest>
+__device__ __forceinline__ double share_total(const Table<kEntries>& t, int group, int groups, int rank) {
   const int chunks = t.count > 0 ? t.end[t.count - 1] : 0;
   Total<kLargest> total;
   int i = 0;
-  for (int c = block; c < chunks; c += blocks) {
+  for (int c = group; c < chunks; c += groups) {
     i = find(t, c, i, t.count - 1);
     int64_t n;
     const int64_t from = run_of(t, i, c, &n);
     switch (t.types[i] & 3) {
-      case MUON_TRAIN_F32: total_of(static_cast<const float*>(t.in[i]) + from, n, total); break;
-      case MUON_TRAIN_BF16: total_of(static_cast<const __nv_bfloat16*>(t.in[i]) + from, n, total); break;
-      default: total_of(static_cast<const __half*>(t.in[i]) + from, n, total); break;
+      case MUON_TRAIN_F32: total_of<kGroup>(static_cast<const float*>(t.in[i]) + from, n, rank, total); break;
+      case MUON_TRAIN_BF16: total_of<kGroup>(static_cast<const __nv_bfloat16*>(t.in[i]) + from, n, rank, total); break;
+      default: total_of<kGroup>(static_cast<const __half*>(t.in[i]) + from, n, rank, total); break;
     }
   }
   return total.v;
@@ -172,12 +173,12 @@ template <int kEntries, bool kLargest>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     total_kernel(const __grid_constant__ Table<kEntries> t, double* partial) {
   begin_kernel();
-  const double mine = share_total<kEntries, kLargest>(t, blockIdx.x, gridDim.x);
+  const double mine = share_total<kThreads, kEntries, kLargest>(t, blockIdx.x, gridDim.x, threadIdx.x);
   const double v = block_total<kLargest>(mine);
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
-// 16 bytes from byte `shift` (0 to 15, even) on of two granules side by side.
+// A granule's bytes from byte `shift` (even) on of two side by side.
 __device__ __forceinline__ uint4 joined(const uint4& a, const uint4& b, int shift) {
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   if (shift & 8) {
@@ -194,80 +195,98 @@ __device__ __forceinline__ uint4 joined(const uint4& a, const uint4& b, int shif
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+__device__ __forceinline__ uint2 joined(const uint2& a, const uint2& b, int shift) {
+  uint32_t w[4] = {a.x, a.y, b.x, b.y};
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) w[i] = w[i + 1];
+  }
+  if (shift & 2) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint2(w[0], w[1]);
+}
 
-// out = factor * in, from the end to the beginning.
-template <typename In, typename Out>
-__device__ __noinline__ void scale_run(const In* p, Out* out, int64_t n, float factor) {
-  constexpr int kN = kVec<In>;
-  constexpr int kStore = kN * sizeof(Out) < 16 ? kN * static_cast<int>(sizeof(Out)) : 16;  // bytes of a store
+// out = factor * in by kGroup threads, from the end to the beginning, in
+// vectors that are 16 bytes of the wider type: neighbouring threads then load
+// and store neighbouring bytes (16-bit types into fp32 by eight elements a
+// thread stored every other 16 bytes at a time).
+template <int kGroup, typename In, typename Out>
+__device__ __noinline__ void scale_run(const In* p, Out* out, int64_t n, float factor, int rank) {
+  constexpr int kN = 16 / static_cast<int>(sizeof(In) > sizeof(Out) ? sizeof(In) : sizeof(Out));
+  constexpr int kLoad = kN * static_cast<int>(sizeof(In)), kStore = kN * static_cast<int>(sizeof(Out));  // bytes
+  constexpr int kFlight = kLoad == 16 ? kUnroll : 2 * kUnroll;
+  using E = Elements<In, kN>;
+  using Raw = typename E::Raw;
   // vectors begin where a store of the output may; those whose input needs two granules stay clear of both ends
   int64_t head = (kStore - reinterpret_cast<uintptr_t>(out) % kStore) % kStore / sizeof(Out);
   if (head > n) head = n;
-  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p + head) % 16);
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p + head) % kLoad);
   if (shift != 0) head = head + kN < n ? head + kN : n;
   int64_t vectors = (n - head) / kN;
   if (shift != 0 && vectors > 0) --vectors;
   const int64_t tail = head + vectors * kN;
-  for (int64_t i = tail + threadIdx.x; i < n; i += kThreads) out[i] = from_float<Out>(to_float(p[i]) * factor);
-  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p + head) - shift);
-  const auto put = [&](int64_t v, const uint4& raw) {
+  for (int64_t i = tail + rank; i < n; i += kGroup) out[i] = from_float<Out>(to_float(p[i]) * factor);
+  const Raw* q = reinterpret_cast<const Raw*>(reinterpret_cast<uintptr_t>(p + head) - shift);
+  const auto put = [&](int64_t v, const Raw& raw) {
     float x[kN];
-    unpack<In>(raw, x);
+    E::unpack(raw, x);
 #pragma unroll
     for (int j = 0; j < kN; ++j) x[j] *= factor;
-    store_run<Out, kN>(out, head + v * kN, x);
+    Elements<Out, kN>::store(out + head + v * kN, Elements<Out, kN>::pack(x));
   };
-  int64_t v = vectors - 1 - threadIdx.x;
+  int64_t v = vectors - 1 - rank;
   if (shift == 0) {
-    for (; v >= (kUnroll - 1) * kThreads; v -= kThreads * kUnroll) {
-      uint4 raw[kUnroll];
+    for (; v >= (kFlight - 1) * kGroup; v -= kGroup * kFlight) {
+      Raw raw[kFlight];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) raw[u] = q[v - u * kThreads];
+      for (int u = 0; u < kFlight; ++u) raw[u] = q[v - u * kGroup];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) put(v - u * kThreads, raw[u]);
+      for (int u = 0; u < kFlight; ++u) put(v - u * kGroup, raw[u]);
     }
-    for (; v >= 0; v -= kThreads) put(v, q[v]);
+    for (; v >= 0; v -= kGroup) put(v, q[v]);
   } else {
-    for (; v >= (kUnroll - 1) * kThreads; v -= kThreads * kUnroll) {
-      uint4 a[kUnroll], b[kUnroll];
+    for (; v >= (kFlight - 1) * kGroup; v -= kGroup * kFlight) {
+      Raw a[kFlight], b[kFlight];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) a[u] = q[v - u * kThreads], b[u] = q[v - u * kThreads + 1];
+      for (int u = 0; u < kFlight; ++u) a[u] = q[v - u * kGroup], b[u] = q[v - u * kGroup + 1];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) put(v - u * kThreads, joined(a[u], b[u], shift));
+      for (int u = 0; u < kFlight; ++u) put(v - u * kGroup, joined(a[u], b[u], shift));
     }
-    for (; v >= 0; v -= kThreads) put(v, joined(q[v], q[v + 1], shift));
+    for (; v >= 0; v -= kGroup) put(v, joined(q[v], q[v + 1], shift));
   }
-  for (int64_t i = threadIdx.x; i < head; i += kThreads) out[i] = from_float<Out>(to_float(p[i]) * factor);
+  for (int64_t i = rank; i < head; i += kGroup) out[i] = from_float<Out>(to_float(p[i]) * factor);
 }
-template <typename In>
+template <int kGroup, typename In>
 __device__ __forceinline__ void scale_into(const void* in, void* out, int dtype, int64_t from, int64_t n,
-                                           float factor) {
+                                           float factor, int rank) {
   const In* p = static_cast<const In*>(in) + from;
   if (dtype == MUON_TRAIN_F32)
-    scale_run(p, static_cast<float*>(out) + from, n, factor);
+    scale_run<kGroup>(p, static_cast<float*>(out) + from, n, factor, rank);
   else if (dtype == MUON_TRAIN_BF16)
-    scale_run(p, static_cast<__nv_bfloat16*>(out) + from, n, factor);
+    scale_run<kGroup>(p, static_cast<__nv_bfloat16*>(out) + from, n, factor, rank);
   else
-    scale_run(p, static_cast<__half*>(out) + from, n, factor);
+    scale_run<kGroup>(p, static_cast<__half*>(out) + from, n, factor, rank);
 }
 
-// The share of block `block` of `blocks`, from the end on.
-template <int kEntries>
-__device__ __forceinline__ void scale_share(const Table<kEntries>& t, float factor, int block, int blocks) {
+// The share of group `group` of `groups` of kGroup threads, from the end on.
+template <int kGroup, int kEntries>
+__device__ __forceinline__ void scale_share(const Table<kEntries>& t, float factor, int group, int groups, int rank) {
   if (t.count == 0 || (t.in_place && factor == 1.0f)) return;
   int i = t.count - 1;
-  for (int c = t.end[i] - 1 - block; c >= 0; c -= blocks) {
+  for (int c = t.end[i] - 1 - group; c >= 0; c -= groups) {
     i = find(t, c, 0, i);
     int64_t n;
     const int64_t from = run_of(t, i, c, &n);
     const int in = t.types[i] & 3, out = t.types[i] >> 2;
     if (t.in[i] == t.out[i] && factor == 1.0f) continue;
     if (in == MUON_TRAIN_F32)
-      scale_into<float>(t.in[i], t.out[i], out, from, n, factor);
+      scale_into<kGroup, float>(t.in[i], t.out[i], out, from, n, factor, rank);
     else if (in == MUON_TRAIN_BF16)
-      scale_into<__nv_bfloat16>(t.in[i], t.out[i], out, from, n, factor);
+      scale_into<kGroup, __nv_bfloat16>(t.in[i], t.out[i], out, from, n, factor, rank);
     else
-      scale_into<__half>(t.in[i], t.out[i], out, from, n, factor);
+      scale_into<kGroup, __half>(t.in[i], t.out[i], out, from, n, factor, rank);
   }
 }
 __device__ __forceinline__ float factor_of(double norm, double max_norm) {
@@ -286,17 +305,19 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   total.v = block_total<kLargest>(v);
   const double n = total.norm();
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  scale_share(t, factor_of(n, max_norm), blockIdx.x, gridDim.x);
+  scale_share<kThreads>(t, factor_of(n, max_norm), blockIdx.x, gridDim.x, threadIdx.x);
 }
 
-// Both passes by one cluster, whose blocks are the whole grid.
+// Both passes by one cluster, whose blocks are the whole grid; a warp a chunk, so
+// that many tensors are on their way at once.
 constexpr int kCluster = 8;
 template <int kEntries, bool kLargest>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     small_kernel(const __grid_constant__ Table<kEntries> t, double max_norm, float* norm) {
   __shared__ double of_block;
   begin_kernel();
-  const double mine = block_total<kLargest>(share_total<kEntries, kLargest>(t, blockIdx.x, kCluster));
+  const int warp = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const double mine = block_total<kLargest>(share_total<32, kEntries, kLargest>(t, warp, kCluster * kThreads / 32, lane));
   if (threadIdx.x == 0) of_block = mine;
   muon_sm100::cluster_sync();
   Total<kLargest> total;
@@ -312,12 +333,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   muon_sm100::cluster_sync();  // a block's memory stays until all have read it
   const double n = total.norm();
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  scale_share(t, factor_of(n, max_norm), blockIdx.x, kCluster);
+  scale_share<32>(t, factor_of(n, max_norm), warp, kCluster * kThreads / 32, lane);
 }
 
 // ------------------------------------------------------------ host side
-// What one cluster takes: one launch less, but eight blocks have to read it all
-// (24 tensors of 200000 fp32 in all: 12.0 us a call, 13.1 with two launches).
+// What one cluster takes: one launch less, which a call bound by the host notices
+// (24 tensors of 200000 fp32 in all: 5.7 us on the device), but eight blocks have
+// to read it all (500000: 17 us, 7 with two launches).
 constexpr int kFew = 64;
 constexpr int64_t kSmall = int64_t{1} << 18;
 
