@@ -90,15 +90,18 @@ __device__ __forceinline__ int clamp_int(int v, int low, int high) { return v < 
 
 // Item `item`: a tile of kSize rows of one of `heads` heads, of `rows` rows a
 // batch entry; packed, of `tiles` tiles of all sequences, the tokens before the
-// first and behind the last among them as sequences that see nothing (every
-// warp looks for itself).  Heads of all entries go in sections, and those of a
-// section tile by tile, with `backwards` from the last, which has the most keys
-// under a causal mask.
+// first and behind the last among them as sequences that see nothing.  Heads of
+// all entries go in sections, and those of a section tile by tile, with
+// `backwards` from the last, which has the most keys under a causal mask.
+//
+// The tiles of packed sequence s, which begins at token b, are numbered from
+// b / kSize + s on.  That leaves room for all of the sequences before it, and
+// some numbers without a tile, but the sequence of a number is found by
+// bisection.  Every warp looks for itself.
 template <int kSize>
 __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, int heads, int tiles, bool backwards,
                                           int* head) {
   Tile t;
-  t.found = true;
   const int per = p.offsets == nullptr ? (rows + kSize - 1) / kSize : tiles;
   const int section = item / (p.section * per), in_it = item - section * p.section * per;
   const int columns = min(p.section, p.batch * heads - section * p.section);
@@ -106,6 +109,7 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
   const int index = backwards ? per - 1 - rank : rank;
   *head = at % heads;
   if (p.offsets == nullptr) {
+    t.found = true;
     t.batch = at / heads;
     t.first = index * kSize;
     t.row0 = 0;
@@ -115,38 +119,29 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
     if (p.lengths != nullptr) t.queries = t.keys = clamp_int(p.lengths[t.batch], 0, p.length);
     return t;
   }
-  const int lane = threadIdx.x % 32;
-  int64_t before = 0;
-  t.batch = 0;
-  for (int base = 0; base < p.sequences + 2; base += 32) {
-    const int s = base + lane;
-    int begin = 0, end = 0;
-    if (s < p.sequences + 2) {
+  const int lane = threadIdx.x % 32, count = p.sequences + 2;
+  // the last sequence that starts at this index or before, 32 of them at a time
+  int begin, end, low = 0, span = count, step, pick;
+  do {
+    step = (span + 31) / 32;
+    const int s = low + lane * step;
+    const bool in = lane * step < span;
+    begin = end = 0;
+    if (in) {
       begin = s == 0 ? 0 : clamp_int(p.offsets[s - 1], 0, p.length);
-      end = s > p.sequences ? p.length : clamp_int(p.offsets[s], 0, p.length);
-      end = end < begin ? begin : end;
+      end = s == count - 1 ? p.length : clamp_int(p.offsets[s], 0, p.length);
     }
-    const int tiles = (end - begin + kSize - 1) / kSize;
-    int64_t sum = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(kFullMask, sum, o);
-      if (lane >= o) sum += v;
-    }
-    const unsigned over = __ballot_sync(kFullMask, before + sum > index);
-    if (over != 0) {
-      const int at = __ffs(over) - 1;
-      const int local = static_cast<int>(index - before - (sum - tiles));
-      t.first = __shfl_sync(kFullMask, local, at) * kSize;
-      t.row0 = __shfl_sync(kFullMask, begin, at);
-      t.stored = __shfl_sync(kFullMask, end, at) - t.row0;
-      const int found = base + at;
-      t.queries = t.keys = found > 0 && found <= p.sequences ? t.stored : 0;
-      return t;
-    }
-    before += __shfl_sync(kFullMask, sum, 31);
-  }
-  t.found = false;
+    pick = max(__popc(__ballot_sync(kFullMask, in && begin / kSize + s <= index)) - 1, 0);  // below 0: descending offsets
+    low += pick * step;
+    span = min(step, span - pick * step);
+  } while (step > 1);
+  t.batch = 0;
+  t.row0 = __shfl_sync(kFullMask, begin, pick);
+  t.stored = max(__shfl_sync(kFullMask, end, pick) - t.row0, 0);
+  t.queries = t.keys = low > 0 && low < count - 1 ? t.stored : 0;
+  const int local = index - (t.row0 / kSize + low);
+  t.found = local >= 0 && local < (t.stored + kSize - 1) / kSize;
+  t.first = t.found ? local * kSize : 0;
   return t;
 }
 

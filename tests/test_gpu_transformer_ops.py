@@ -245,6 +245,33 @@ def test_attention_of_many_short_sequences(pkg):
     check_attention(pkg, q[0], k[0], v[0], go[0], sequences=sequences, causal=True, offsets=offsets)
 
 
+@pytest.mark.parametrize("shortest,longest", [(0, 3), (100, 300), (0, 600)])
+def test_attention_of_more_sequences_than_a_warp_looks_at(pkg, shortest, longest):
+    """1200 sequences, empty ones and ones of more than a tile among them: each
+    token's results are those of its sequence among few others."""
+    rng = random.Random(5)
+    ends = [7]
+    while len(ends) < 1201:
+        ends.append(ends[-1] + rng.randint(shortest, longest))
+    total = ends[-1] + 200
+    q, k, v, go = attention_inputs(1, total, total, 2, 1, 64, BF16, seed=24)
+
+    def step(first, last):
+        rows = slice(ends[first], ends[last])
+        leaves = [t[0, rows].detach().requires_grad_(True) for t in (q, k, v)]
+        out = pkg.attention(*leaves, causal=True, offsets=torch.tensor(ends[first:last + 1], device="cuda") - ends[first])
+        return [out.detach(), *torch.autograd.grad(out, leaves, go[0, rows])]
+
+    leaves = [t[0].detach().requires_grad_(True) for t in (q, k, v)]
+    out = pkg.attention(*leaves, causal=True, offsets=torch.tensor(ends, device="cuda"))
+    got = [out.detach(), *torch.autograd.grad(out, leaves, go[0])]
+    for t in got:
+        assert not t[:7].any() and not t[ends[-1]:].any()
+    for first in range(0, 1200, 20):
+        for a, b in zip(got, step(first, first + 20)):
+            assert torch.equal(a[ends[first]:ends[first + 20]], b)
+
+
 def test_attention_takes_any_offsets(pkg):
     """Offsets are not looked at on the host: ends outside of the tensor are
     taken as its ends, descending ones make results void, but no access leaves
