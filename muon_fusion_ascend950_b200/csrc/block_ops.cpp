@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <limits>
 #include <tuple>
 #include <vector>
 
@@ -35,7 +36,10 @@ Tensor Counts(const Tensor& t, const Tensor& like, const char* who, const char* 
   CheckDevice(t, like, who, name);
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, who, ": ", name,
                    " must be int32 or int64, got ", t.scalar_type());
-  return t.to(at::kInt).contiguous();
+  if (t.scalar_type() == at::kInt) return t.contiguous();
+  // what is beyond 32 bits is beyond the tensors too, and stays there
+  constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
+  return t.clamp(int64_t{0}, kMost).to(at::kInt).contiguous();
 }
 
 AttentionInputs CheckAttention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets,

@@ -272,6 +272,19 @@ def test_attention_of_more_sequences_than_a_warp_looks_at(pkg, shortest, longest
             assert torch.equal(a[ends[first]:ends[first + 20]], b)
 
 
+def test_counts_beyond_32_bits_are_the_tensors_ends(pkg):
+    q, k, v, _ = attention_inputs(2, 300, 300, 2, 1, 64, BF16, seed=25)
+    most = torch.iinfo(torch.int64).max
+    for far in (most, (1 << 32) + 5, 1 << 31):
+        lengths = torch.tensor([far, 200], device="cuda")
+        clear = torch.tensor([300, 200], device="cuda")
+        assert torch.equal(pkg.attention(q, k, v, lengths=lengths), pkg.attention(q, k, v, lengths=clear))
+        offsets = torch.tensor([-far, 100, far], device="cuda")
+        clear = torch.tensor([0, 100, 300], device="cuda")
+        assert torch.equal(pkg.attention(q[0], k[0], v[0], offsets=offsets),
+                           pkg.attention(q[0], k[0], v[0], offsets=clear))
+
+
 def test_attention_takes_any_offsets(pkg):
     """Offsets are not looked at on the host: ends outside of the tensor are
     taken as its ends, descending ones make results void, but no access leaves
