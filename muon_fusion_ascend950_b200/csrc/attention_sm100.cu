@@ -39,7 +39,7 @@ namespace {
 
 using namespace muon_sm100;
 
-constexpr int kTile = 128;     // queries, or keys, of a tile
+constexpr int kTileShift = 7, kTile = 1 << kTileShift;  // queries, or keys, of a tile
 constexpr int kThreads = 384;  // warps 0-7: scores, 8: loads, 9: products; 10 and 11 only give registers
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 // Registers of a thread at launch, and then of the two warpgroups that work on
@@ -71,7 +71,8 @@ struct Problem {
   const int32_t* offsets;
   int64_t rows;             // batch * length
   int length, keys, heads, kv_heads, dim, sequences, batch, window, causal;
-  int section;              // heads whose tiles are worked on together
+  int section;              // heads (pairs of them: by_heads) whose tiles are worked on together
+  int by_heads;             // forward: 1, pairs of tiles are of two heads; 0, of one
   float scale;
 };
 
@@ -88,21 +89,20 @@ struct Tile {
 
 __device__ __forceinline__ int clamp_int(int v, int low, int high) { return v < low ? low : v > high ? high : v; }
 
-// Item `item`: a tile of kSize rows of one of `heads` heads, of `rows` rows a
+// Item `item`: a tile of 2^shift rows of one of `heads` heads, of `rows` rows a
 // batch entry; packed, of `tiles` tiles of all sequences, the tokens before the
 // first and behind the last among them as sequences that see nothing.  Heads of
 // all entries go in sections, and those of a section tile by tile, with
 // `backwards` from the last, which has the most keys under a causal mask.
 //
 // The tiles of packed sequence s, which begins at token b, are numbered from
-// b / kSize + s on.  That leaves room for all of the sequences before it, and
+// (b >> shift) + s on.  That leaves room for all of the sequences before it, and
 // some numbers without a tile, but the sequence of a number is found by
 // bisection.  Every warp looks for itself.
-template <int kSize>
-__device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, int heads, int tiles, bool backwards,
-                                          int* head) {
+__device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, int heads, int shift, int tiles,
+                                          bool backwards, int* head) {
   Tile t;
-  const int per = p.offsets == nullptr ? (rows + kSize - 1) / kSize : tiles;
+  const int size = 1 << shift, per = p.offsets == nullptr ? (rows + size - 1) >> shift : tiles;
   const int section = item / (p.section * per), in_it = item - section * p.section * per;
   const int columns = min(p.section, p.batch * heads - section * p.section);
   const int rank = in_it / columns, at = section * p.section + in_it - rank * columns;
@@ -111,7 +111,7 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
   if (p.offsets == nullptr) {
     t.found = true;
     t.batch = at / heads;
-    t.first = index * kSize;
+    t.first = index << shift;
     t.row0 = 0;
     t.stored = rows;
     t.queries = p.length;
@@ -131,7 +131,7 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
       begin = s == 0 ? 0 : clamp_int(p.offsets[s - 1], 0, p.length);
       end = s == count - 1 ? p.length : clamp_int(p.offsets[s], 0, p.length);
     }
-    pick = max(__popc(__ballot_sync(kFullMask, in && begin / kSize + s <= index)) - 1, 0);  // below 0: descending offsets
+    pick = max(__popc(__ballot_sync(kFullMask, in && (begin >> shift) + s <= index)) - 1, 0);  // below 0: descending offsets
     low += pick * step;
     span = min(step, span - pick * step);
   } while (step > 1);
@@ -139,9 +139,9 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
   t.row0 = __shfl_sync(kFullMask, begin, pick);
   t.stored = max(__shfl_sync(kFullMask, end, pick) - t.row0, 0);
   t.queries = t.keys = low > 0 && low < count - 1 ? t.stored : 0;
-  const int local = index - (t.row0 / kSize + low);
-  t.found = local >= 0 && local < (t.stored + kSize - 1) / kSize;
-  t.first = t.found ? local * kSize : 0;
+  const int local = index - ((t.row0 >> shift) + low);
+  t.found = local >= 0 && local < (t.stored + size - 1) >> shift;
+  t.first = t.found ? local << shift : 0;
   return t;
 }
 
@@ -293,32 +293,75 @@ __device__ __forceinline__ uint32_t pack2(float low, float high) {
 
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
 
-// A row of a result in tensor memory times `by` to memory; with `rest` also
-// what the rounding took.
-template <typename T, int kCols>
-__device__ __forceinline__ void store_row(T* to, T* rest, uint32_t taddr, int dim, float by, bool write) {
-#pragma unroll 1
-  for (int c = 0; c < kCols; c += 32) {
-    uint32_t r[32];
-    if (c >= dim) return;
-    tmem_ld_32x32b_x32(taddr + c, r);
-    tmem_wait_ld(r);
+// Four vectors of a row a lane, turned among each four lanes: afterwards x[r] is
+// vector (lane % 4) of the row of lane (lane & ~3) + r.
+__device__ __forceinline__ void turn(uint4 (&x)[4]) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (!write || c + j >= dim) continue;
-      float v[8];
+  for (int b = 1; b < 4; b *= 2) {
+    const bool odd = threadIdx.x & b;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = as_float(r[j + i]) * by;
-      const uint4 u = pack<T>(v);
-      *reinterpret_cast<uint4*>(to + c + j) = u;
-      if (rest != nullptr) {
-        float w[8];
-        unpack<T>(u, w);
+    for (int q = 0; q < 4; ++q) {
+      if (q & b) continue;
+      uint32_t *u = &x[q].x, *v = &x[q + b].x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] -= w[i];
-        *reinterpret_cast<uint4*>(rest + c + j) = pack<T>(v);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t got = __shfl_xor_sync(kFullMask, odd ? u[i] : v[i], b);
+        u[i] = odd ? got : u[i];
+        v[i] = odd ? v[i] : got;
       }
     }
+  }
+}
+
+// A warp's rows of a result in tensor memory times `by` to memory, lane by lane
+// at `to` and `stride` elements apart; with `rest` also what the rounding took.
+// kTurned: four lanes write 64 bytes of a row together, eight rows a store;
+// else each lane its own row, 16 bytes and 32 rows a store.  Those stores hold
+// the two tiles of a pair up where rows have 256 bytes: 128 x 256 causal, 16
+// heads of 128 over 4, 191 us with own rows, 121 turned; 8 x 4096 651 and 556.
+// With 128 bytes a row they gain where tiles are full (256: 109 and 100 us;
+// 4096: 423 and 413), and lose by their exchange where sequences end inside
+// (1024 packed ones of 64, 16 heads of 64 over 4: 442 and 462 us; backward 995
+// and 1050).
+template <typename T, int kCols, bool kTurned>
+__device__ __forceinline__ void store_rows(T* to, T* rest, int64_t stride, uint32_t taddr, int dim, float by, bool write) {
+  const unsigned rows = __ballot_sync(kFullMask, write);
+  const int lane = threadIdx.x % 32, m = lane % 4;
+  const auto store = [&](T* own, uint4 (&x)[4], int column) {
+    if constexpr (kTurned) {
+      turn(x);
+      T* row0 = own - m * stride;
+      column += 8 * m;
+      if (column >= dim) return;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (rows >> (lane - m + r) & 1) *reinterpret_cast<uint4*>(row0 + r * stride + column) = x[r];
+    } else if (write) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (column + 8 * q < dim) *reinterpret_cast<uint4*>(own + column + 8 * q) = x[q];
+    }
+  };
+#pragma unroll 1
+  for (int c = 0; c < kCols; c += 32) {
+    if (c >= dim) return;
+    uint32_t t[32];
+    tmem_ld_32x32b_x32(taddr + c, t);
+    tmem_wait_ld(t);
+    uint4 x[4], y[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float v[8], w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = as_float(t[8 * q + i]) * by;
+      x[q] = pack<T>(v);
+      unpack<T>(x[q], w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] -= w[i];
+      y[q] = pack<T>(v);
+    }
+    store(to, x, c);
+    if (rest != nullptr) store(rest, y, c);
     __syncwarp();
   }
 }
@@ -371,20 +414,27 @@ struct Forward {
 };
 
 // An item is two tiles of queries, which take turns: while the scores of one are
-// worked on, the products of the other run.  Keys and values pass through a
+// worked on, the products of the other run.  They are those of two heads at the
+// same rows where an even number of heads shares a key head, else neighbours of
+// one head, of which one has more keys under a causal mask, and a short sequence
+// may have one only (16 heads over 4, 1024 packed sequences of 64 tokens: 667 us
+// with neighbours, 441 with two heads; 8 x 4096 causal of 128: 585 and 562).  Keys and values pass through a
 // ring of tiles, keys j, values j, keys j + 1 and so on.  Loads and products go
 // on to the next item while the results of the last are written.
 struct Pair {
-  int head;
+  int head, heads_on, rows_on;  // of the first tile; from it to the second
   Tile t;
   int from[2], to[2];  // key tiles of the two query tiles
   int first, last;     // of both
 
   __device__ __forceinline__ Pair(const Problem& p, int item, int tiles) {
-    t = find_tile<2 * kTile>(p, item, p.length, p.heads, tiles, true, &head);
+    heads_on = p.by_heads;
+    rows_on = p.by_heads ? 0 : kTile;
+    t = find_tile(p, item, p.length, p.heads >> heads_on, kTileShift + 1 - heads_on, tiles, true, &head);
+    head <<= heads_on;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int i0 = t.first + i * kTile;
+      const int i0 = t.first + i * rows_on;
       int low = 0, high = 0;
       if (t.found) keys_of(p, t, min(i0, t.queries), min(i0 + kTile, t.queries), &low, &high);
       from[i] = low / kTile;
@@ -397,7 +447,7 @@ struct Pair {
   }
 };
 
-template <typename T, int kCols>
+template <typename T, int kCols, bool kTurned>
 __global__ void __launch_bounds__(kThreads, 1)
     forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Problem p, int tiles) {
@@ -453,8 +503,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_full[i], C::kTileBytes);
-            load_tile<kCols>(smem + i * C::kTileBytes, &map_q, &q_full[i], w.t.row0 + w.t.first + i * kTile, w.head,
-                             w.t.batch);
+            load_tile<kCols>(smem + i * C::kTileBytes, &map_q, &q_full[i], w.t.row0 + w.t.first + i * w.rows_on,
+                             w.head + i * w.heads_on, w.t.batch);
           }
           ++loads[i];
         }
@@ -538,18 +588,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     Pair w(p, blockIdx.x, tiles);
     for (int k = 0, item = blockIdx.x; ok && item >= 0; ++k) {
       const Tile t = w.t;
-      const int head = w.head;
-      const int row = t.first + threadIdx.x;  // of the sequence: 128 threads a tile
+      const int head = w.head + i * w.heads_on, first = t.first + i * w.rows_on;
+      const int row = first + threadIdx.x % kTile;  // of the sequence
       const int from = i == 0 ? w.from[0] : w.from[1], to = i == 0 ? w.to[0] : w.to[1];
       int low = 0, high = 0, all_low = 0, all_high = 0;
       if (t.found) {
         keys_of(p, t, min(row, t.queries), min(row + 1, t.queries), &low, &high);
         // what every row of the tile sees
-        const int i0 = t.first + i * kTile, i1 = min(i0 + kTile, t.queries);
+        const int last = min(first + kTile, t.queries) - 1;
         int unused;
-        if (i0 < i1) {
-          keys_of(p, t, i1 - 1, i1, &all_low, &unused);
-          keys_of(p, t, i0, i0 + 1, &unused, &all_high);
+        if (first <= last) {
+          keys_of(p, t, last, last + 1, &all_low, &unused);
+          keys_of(p, t, first, first + 1, &unused, &all_high);
         }
       }
       float top = -INFINITY, sum = 0.0f;
@@ -640,9 +690,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int64_t at = static_cast<int64_t>(t.batch) * p.length + t.row0 + row;
       const bool write = ok && t.found && row < t.stored, some = low < high;
-      T* out = static_cast<T*>(p.out) + (at * p.heads + head) * p.dim;
-      T* rest = p.out2 != nullptr ? static_cast<T*>(p.out2) + (at * p.heads + head) * p.dim : nullptr;
-      if (from < to) store_row<T, kCols>(out, rest, o_at, p.dim, some ? 1.0f / sum : 0.0f, write && some);
+      const int64_t stride = static_cast<int64_t>(p.heads) * p.dim;
+      T* out = static_cast<T*>(p.out) + at * stride + head * p.dim;
+      T* rest = p.out2 != nullptr ? static_cast<T*>(p.out2) + at * stride + head * p.dim : nullptr;
+      if (from < to)
+        store_rows<T, kCols, kTurned>(out, rest, stride, o_at, p.dim, some ? 1.0f / sum : 0.0f, write && some);
       if (write && (from >= to || !some)) {
         zero_row(out, p.dim);
         if (rest != nullptr) zero_row(rest, p.dim);
@@ -807,7 +859,7 @@ struct Keys {
   int from, to, per;  // tiles of queries, of one head
 
   __device__ __forceinline__ Keys(const Problem& p, int item, int tiles) {
-    t = find_tile<kTile>(p, item, p.keys, p.kv_heads, tiles, false, &kv_head);
+    t = find_tile(p, item, p.keys, p.kv_heads, kTileShift, tiles, false, &kv_head);
     int low = 0, high = 0;
     if (t.found) queries_of(p, t, min(t.first, t.keys), min(t.first + kTile, t.keys), &low, &high);
     from = low / kTile;
@@ -1089,7 +1141,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       T* grad = static_cast<T*>(w == 0 ? p.out2 : p.out) + (at * p.kv_heads + item.kv_head) * p.dim;
       const bool write = ok && t.found && row < t.stored, some = mine_low < mine_high;
       const float by = w == 0 ? (kBf16<T> ? 1.0f : 0x1p-10f) : p.scale / factor;
-      if (n > 0) store_row<T, kCols>(grad, nullptr, (w == 0 ? tmem_dv : tmem_dk) + lanes, p.dim, by, write && some);
+      if (n > 0)
+        store_rows<T, kCols, kCols == 128>(grad, nullptr, static_cast<int64_t>(p.kv_heads) * p.dim,
+                                           (w == 0 ? tmem_dv : tmem_dk) + lanes, p.dim, by, write && some);
       if (write && (n == 0 || !some)) zero_row(grad, p.dim);
       __syncwarp();
     }
@@ -1105,7 +1159,7 @@ struct Queries {
   int from, to;  // tiles of keys
 
   __device__ __forceinline__ Queries(const Problem& p, int item, int tiles) {
-    t = find_tile<kTile>(p, item, p.length, p.heads, tiles, true, &head);
+    t = find_tile(p, item, p.length, p.heads, kTileShift, tiles, true, &head);
     int low = 0, high = 0;
     if (t.found) keys_of(p, t, min(t.first, t.queries), min(t.first + kTile, t.queries), &low, &high);
     from = low / kTile;
@@ -1326,7 +1380,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (w == 0) {
         T* grad = static_cast<T*>(p.out) + (at * p.heads + item.head) * p.dim;
         const bool write = ok && t.found && row < t.stored, some = mine_low < mine_high;
-        if (n > 0) store_row<T, kCols>(grad, nullptr, tmem_dq + lanes, p.dim, p.scale / factor, write && some);
+        if (n > 0)
+          store_rows<T, kCols, kCols == 128>(grad, nullptr, static_cast<int64_t>(p.heads) * p.dim, tmem_dq + lanes, p.dim,
+                                             p.scale / factor, write && some);
         if (write && (n == 0 || !some)) zero_row(grad, p.dim);
       }
       __syncwarp();
@@ -1489,7 +1545,7 @@ int section_of(int64_t heads, int64_t bytes, int64_t tiles, int* section) {
   return rc;
 }
 
-template <typename T, int kCols>
+template <typename T, int kCols, bool kTurned>
 int forward(const muon_train_attention_args& a, void* stream) {
   Maps m;
   int rc = encode_inputs(a, &m);
@@ -1498,13 +1554,14 @@ int forward(const muon_train_attention_args& a, void* stream) {
   p.out = a.out;
   p.out2 = a.out_rest;
   constexpr int kBytes = Forward<kCols>::kBytes;
-  rc = prepare<forward_kernel<T, kCols>>(kBytes);
+  rc = prepare<forward_kernel<T, kCols, kTurned>>(kBytes);
   if (rc != MUON_POLAR_OK) return rc;
-  const int64_t tiles = tiles_of(a, a.length, 2 * kTile);
   const int64_t group = a.heads / a.kv_heads, pair_bytes = 2 * a.dim * static_cast<int64_t>(sizeof(T));
-  rc = section_of(a.batch * a.heads, a.keys * pair_bytes / group, tiles / a.batch, &p.section);
+  p.by_heads = group % 2 == 0;
+  const int64_t tiles = tiles_of(a, a.length, p.by_heads ? kTile : 2 * kTile), columns = a.heads >> p.by_heads;
+  rc = section_of(a.batch * columns, a.keys * pair_bytes / (group >> p.by_heads), tiles / a.batch, &p.section);
   if (rc != MUON_POLAR_OK) return rc;
-  return launch(forward_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.heads)), kThreads, kBytes, 1, true,
+  return launch(forward_kernel<T, kCols, kTurned>, dim3(static_cast<unsigned>(tiles * columns)), kThreads, kBytes, 1, true,
                 stream, m.q, m.k, m.v, p, static_cast<int>(tiles));
 }
 
@@ -1568,7 +1625,8 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
 
 template <typename T>
 int forward(const muon_train_attention_args& a, void* stream) {
-  return a.dim <= 64 ? forward<T, 64>(a, stream) : forward<T, 128>(a, stream);
+  if (a.dim > 64) return forward<T, 128, true>(a, stream);
+  return a.offsets == nullptr ? forward<T, 64, true>(a, stream) : forward<T, 64, false>(a, stream);
 }
 template <typename T>
 int backward(const muon_train_attention_args& a, const muon_train_attention_grads& g, void* stream) {

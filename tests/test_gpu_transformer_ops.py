@@ -245,8 +245,9 @@ def test_attention_of_many_short_sequences(pkg):
     check_attention(pkg, q[0], k[0], v[0], go[0], sequences=sequences, causal=True, offsets=offsets)
 
 
+@pytest.mark.parametrize("kv_heads", [1, 2])
 @pytest.mark.parametrize("shortest,longest", [(0, 3), (100, 300), (0, 600)])
-def test_attention_of_more_sequences_than_a_warp_looks_at(pkg, shortest, longest):
+def test_attention_of_more_sequences_than_a_warp_looks_at(pkg, shortest, longest, kv_heads):
     """1200 sequences, empty ones and ones of more than a tile among them: each
     token's results are those of its sequence among few others."""
     rng = random.Random(5)
@@ -254,7 +255,7 @@ def test_attention_of_more_sequences_than_a_warp_looks_at(pkg, shortest, longest
     while len(ends) < 1201:
         ends.append(ends[-1] + rng.randint(shortest, longest))
     total = ends[-1] + 200
-    q, k, v, go = attention_inputs(1, total, total, 2, 1, 64, BF16, seed=24)
+    q, k, v, go = attention_inputs(1, total, total, 2, kv_heads, 64, BF16, seed=24)
 
     def step(first, last):
         rows = slice(ends[first], ends[last])
