@@ -27,6 +27,14 @@
 // scores' precision.  fp16 operands are scaled by powers of two: p by 2^7
 // (forward; at most 2^15) and 2^10 (backward), so that small ones do not fall
 // below fp16's range, and ds by what the largest |dout| and |v| allow.
+//
+// What bounds it (heads of 128, bf16): power for long sequences (2 x 8192 both
+// ways, 16 heads: forward 1000 us, 1100 TFLOP/s; backward 3320, 1160 TFLOP/s of
+// its seven products, at 1.57 GHz), the latency of scores, probabilities and
+// product one after another for shorter ones (4096 causal, 37 heads: 167 and
+// 529 us, 950 and 750 TFLOP/s of the products needed).  With heads of 64 the
+// exponentials and the issue slots come first (2 x 8192, 16 heads: 750 and 2240
+// us, 733 and 614 TFLOP/s).
 #include <cuda.h>
 
 #include <type_traits>
@@ -713,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // largest |dout| of rows that count and the largest |v|, padding included: a
 // bound.  A lane has 8 columns.  The maxima go to kLargestSlots places each, a block's
 // first joined: with one place the atomic operations, one after another, took
-// 40 us of 56 (131056 rows of 64).
+// 40 us of 56 (131056 rows of 64).  Bound by memory: 117 MB in 23 us, cold.
 struct Stats {
   const void* out;
   const void* rest;
@@ -871,7 +879,8 @@ struct Keys {
 // Scores stand the other way round, a key a thread:
 // p^T and ds^T are left operands as they are.  The warps 0-3 take queries 0 to
 // 63 of each tile, 4-7 the others.  While the scores of the next tile are
-// computed ds is worked on, while dp is computed the next p.
+// computed ds is worked on, while dp is computed the next p.  4096 both ways, 37 heads of
+// 128: 492 us alone, with the tensor pipe busy in 67% of the cycles.
 template <typename T, int kCols>
 __global__ void __launch_bounds__(kThreads, 1)
     key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1170,7 +1179,8 @@ struct Queries {
 // Two tiles of scores in tensor memory, one of
 // dp: the products of the next keys run while ds is worked on, which takes the
 // place of its scores.  Half of the warps may be done with the next ds before
-// the product with the present one has been issued, so those barriers are two.
+// the product with the present one has been issued, so those barriers are two.  4096
+// both ways, 37 heads of 128: 447 us alone, tensor pipe 53%.
 template <typename T, int kCols>
 __global__ void __launch_bounds__(kThreads, 1)
     query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

@@ -9,7 +9,9 @@
 // MB.)  Bound by memory: the gradients are read once for the norm and once
 // more to be scaled, where the second pass begins with what the first read
 // last, which L2 still holds.  In place, gradients within the limit would be
-// written back as they are: the second pass then only gives the norm.
+// written back as they are: the second pass then only gives the norm (640 M
+// bf16: 202 to 214 us, 6.0 to 6.3 TB/s).  160 M fp32 into bf16: 253 us for 1.6
+// GB, of which 0.6 are the second reading.
 //
 // A few small tensors take one launch: a cluster of blocks, which exchange their
 // sums through shared memory.
