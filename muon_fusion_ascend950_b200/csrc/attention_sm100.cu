@@ -26,7 +26,8 @@
 // the output and from what rounding took from it (out_rest), so that it has the
 // scores' precision.  fp16 operands are scaled by powers of two: p by 2^7
 // (forward; at most 2^15) and 2^10 (backward), so that small ones do not fall
-// below fp16's range, and ds by what the largest |dout| and |v| allow.
+// below fp16's range, and ds by a factor for each query (dq) or key (dk), of what
+// its own row can reach (ds_exponent).
 //
 // What bounds it (heads of 128, bf16): power for long sequences (2 x 8192 both
 // ways, 16 heads: forward 1000 us, 1100 TFLOP/s; backward 3320, 1160 TFLOP/s of
@@ -74,7 +75,10 @@ struct Problem {
   void* out2;
   float* lse;
   const float* stats;       // backward: [2][heads][rows]: -lse (binary), -delta
-  const float* largest;     // backward, fp16: the largest |dout| and |v|, kLargestSlots places each
+  const float* grad_norm;   // backward, fp16: [rows][heads]: |dout|
+  const float* value_norm;  // [batch * keys][kv_heads]: |v|
+  const float2* query_top;  // the largest |dout| and |delta| of each tile of queries, of the heads that share a key head
+  const float* key_top;     // the largest |v| of each tile of keys
   const int32_t* lengths;
   const int32_t* offsets;
   int64_t rows;             // batch * length
@@ -92,6 +96,7 @@ struct Tile {
   int stored;     // rows of the sequence that are written
   int queries;    // rows that count, as queries
   int keys;       // and as keys
+  int number;     // of the sequence's first tile
   bool found;
 };
 
@@ -121,6 +126,7 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
     t.batch = at / heads;
     t.first = index << shift;
     t.row0 = 0;
+    t.number = 0;
     t.stored = rows;
     t.queries = p.length;
     t.keys = p.keys;
@@ -147,10 +153,18 @@ __device__ __forceinline__ Tile find_tile(const Problem& p, int item, int rows, 
   t.row0 = __shfl_sync(kFullMask, begin, pick);
   t.stored = max(__shfl_sync(kFullMask, end, pick) - t.row0, 0);
   t.queries = t.keys = low > 0 && low < count - 1 ? t.stored : 0;
-  const int local = index - ((t.row0 >> shift) + low);
+  t.number = (t.row0 >> shift) + low;
+  const int local = index - t.number;
   t.found = local >= 0 && local < (t.stored + size - 1) >> shift;
   t.first = t.found ? local << shift : 0;
   return t;
+}
+
+// The place of the first of a key head's tiles of 128 rows in an array of a value
+// a tile: of all sequences' together where they are packed.
+__device__ __forceinline__ int64_t tile_slot(const Problem& p, const Tile& t, int rows, int tiles, int kv_head) {
+  const int per = p.offsets == nullptr ? (rows + kTile - 1) >> kTileShift : tiles;
+  return (static_cast<int64_t>(t.batch) * p.kv_heads + kv_head) * per + t.number;
 }
 
 // Keys [low, high) that queries [i0, i1) of the sequence see at least in part.
@@ -718,10 +732,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ------------------------------------------------------------ backward: statistics
 // -lse in binary exponents (so that p = 2^(s scale log2 e - it); -inf where
 // nothing is seen: p = 0) and -delta of each row and head; for fp16 also the
-// largest |dout| of rows that count and the largest |v|, padding included: a
-// bound.  A lane has 8 columns.  The maxima go to kLargestSlots places each, a block's
-// first joined: with one place the atomic operations, one after another, took
-// 40 us of 56 (131056 rows of 64).  Bound by memory: 117 MB in 23 us, cold.
+// norms of dout's rows, 0 where nothing is seen, and of v's, of their finite
+// elements.  A lane has 8 columns.  Bound by memory: 117 MB in 23 us, cold.
 struct Stats {
   const void* out;
   const void* rest;
@@ -729,13 +741,13 @@ struct Stats {
   const void* v;
   const float* lse;
   float* stats;
-  uint32_t* largest;
+  float* grad_norm;
+  float* value_norm;
   muon_train_strides grad_stride, v_stride;
   int64_t rows, v_rows;
   int length, keys, heads, kv_heads, dim;
 };
 constexpr int kStatRows = 2;  // a thread's, in flight together
-constexpr int kLargestSlots = 32;
 
 template <typename T>
 __device__ __forceinline__ const T* row_of(const void* x, const muon_train_strides& s, uint32_t row, uint32_t length,
@@ -744,19 +756,26 @@ __device__ __forceinline__ const T* row_of(const void* x, const muon_train_strid
   return static_cast<const T*>(x) + b * s.batch + r * s.row + head * s.head;
 }
 
+// x^2 added to n, where it is a number.
+__device__ __forceinline__ float add_square(float x, float n) { return fabsf(x) < INFINITY ? fmaf(x, x, n) : n; }
+
 template <typename T, int kCols>
 __global__ void __launch_bounds__(256, 6) stats_kernel(const __grid_constant__ Stats a) {
   constexpr int kLanes = kCols / 8, kGroups = 256 / kLanes;
-  __shared__ float warp_big[8];
   begin_kernel();
   const int lane = threadIdx.x % kLanes, dim = a.dim;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups * kStatRows;
+  const auto join = [](float v) {  // of a row's lanes
+#pragma unroll
+    for (int q = kLanes / 2; q > 0; q >>= 1) v += __shfl_xor_sync(kFullMask, v, q, kLanes);
+    return v;
+  };
   // items are heads of rows; the first of the block is divided in 64 bits, the others' distances in 32
   const uint32_t heads = a.heads, row0 = static_cast<uint32_t>(base / heads),
                  h0 = static_cast<uint32_t>(base - static_cast<int64_t>(row0) * heads);
   uint32_t row[kStatRows], head[kStatRows];
   uint4 o[kStatRows], e[kStatRows], g[kStatRows];
-  float l[kStatRows], big = 0.0f;
+  float l[kStatRows];
 #pragma unroll
   for (int u = 0; u < kStatRows; ++u) {
     const uint32_t in_it = h0 + u * kGroups + threadIdx.x / kLanes, down = in_it / heads;
@@ -776,7 +795,7 @@ __global__ void __launch_bounds__(256, 6) stats_kernel(const __grid_constant__ S
   for (int u = 0; u < kStatRows; ++u) {
     // a row that sees nothing has no gradient, whatever dout holds there
     const bool none = l[u] == -INFINITY;
-    float x[8], y[8], z[8], d = 0.0f;
+    float x[8], y[8], z[8], d = 0.0f, n = 0.0f;
     unpack<T>(o[u], x);
     unpack<T>(e[u], y);
     unpack<T>(g[u], z);
@@ -784,61 +803,101 @@ __global__ void __launch_bounds__(256, 6) stats_kernel(const __grid_constant__ S
     for (int i = 0; i < 8; ++i) {
       d = fmaf(x[i], z[i], d);
       d = fmaf(y[i], z[i], d);
-      if (!none) big = fmaxf(big, fabsf(z[i]));
+      if constexpr (!kBf16<T>) n = add_square(z[i], n);
     }
-#pragma unroll
-    for (int q = kLanes / 2; q > 0; q >>= 1) d += __shfl_xor_sync(kFullMask, d, q, kLanes);
+    d = join(d);
+    if constexpr (!kBf16<T>) n = join(n);
     if (row[u] < a.rows && lane == 0) {
       const int64_t at = head[u] * a.rows + row[u];
       a.stats[at] = none ? -INFINITY : kRaiseBack<T> - l[u] * kLog2e;
       a.stats[a.heads * a.rows + at] = none ? 0.0f : -d;
+      if constexpr (!kBf16<T>) a.grad_norm[row[u] * static_cast<int64_t>(heads) + head[u]] = none ? 0.0f : sqrtf(n);
     }
   }
   if constexpr (!kBf16<T>) {
-    const auto join = [&](float m, uint32_t* to) {
-      m = warp_max(m);
-      __syncthreads();
-      if (threadIdx.x % 32 == 0) warp_big[threadIdx.x / 32] = m;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) m = fmaxf(m, warp_big[w]);
-        if (m > 0.0f) atomicMax(to + blockIdx.x % kLargestSlots, __float_as_uint(m));
-      }
-    };
-    join(big, a.largest);
-    big = 0.0f;
     const int64_t v_items = a.v_rows * a.kv_heads;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups * kStatRows;
-    for (int64_t item = base + threadIdx.x / kLanes; item < v_items; item += step) {
+    for (int64_t first = base + threadIdx.x / kLanes; first - threadIdx.x / kLanes < v_items; first += step) {
+      uint4 v[kStatRows];
 #pragma unroll
       for (int u = 0; u < kStatRows; ++u) {
-        const int64_t at = item + u * kGroups;
+        const int64_t at = first + u * kGroups;
+        v[u] = make_uint4(0, 0, 0, 0);
         if (at >= v_items || lane * 8 >= dim) continue;
         const uint32_t r = static_cast<uint32_t>(at / a.kv_heads);
         const uint32_t h = static_cast<uint32_t>(at - static_cast<int64_t>(r) * a.kv_heads);
-        float x[8];
-        unpack<T>(*reinterpret_cast<const uint4*>(row_of<T>(a.v, a.v_stride, r, a.keys, h) + lane * 8), x);
+        v[u] = *reinterpret_cast<const uint4*>(row_of<T>(a.v, a.v_stride, r, a.keys, h) + lane * 8);
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (fabsf(x[i]) < INFINITY) big = fmaxf(big, fabsf(x[i]));
+      for (int u = 0; u < kStatRows; ++u) {
+        float x[8], n = 0.0f;
+        unpack<T>(v[u], x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n = add_square(x[i], n);
+        n = join(n);
+        if (first + u * kGroups < v_items && lane == 0) a.value_norm[first + u * kGroups] = sqrtf(n);
       }
     }
-    join(big, a.largest + kLargestSlots);
   }
 }
 
-// The power of two that ds is multiplied by: |dp - delta| <= 2 dim max|dout|
-// max|v|, which this brings to 2^15 at most.
-template <typename T>
-__device__ __forceinline__ float ds_factor(const Problem& p) {
-  if constexpr (kBf16<T>) {
-    return 1.0f;
-  } else {  // by whole warps
-    const int lane = threadIdx.x % 32;
-    const float bound = 2.0f * p.dim * warp_max(p.largest[lane]) * warp_max(p.largest[kLargestSlots + lane]);
-    if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;
-    return scalbnf(1.0f, clamp_int(14 - ilogbf(bound), -100, 100));
+// The largest of a warp's values, none below 0, whose bits are ordered as they are.
+__device__ __forceinline__ float warp_top(float v) {
+  return __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(v)));
+}
+
+// fp16: the largest |dout| and |delta| of each tile of queries, over the heads
+// that share a key head, and the largest |v| of each tile of keys, over the rows
+// that count: what others hold reaches nothing.  A block a tile, a row a thread.
+__global__ void __launch_bounds__(kTile)
+    tops_kernel(const __grid_constant__ Problem p, float2* query_top, float* key_top, uint32_t query_items, int query_tiles,
+                int key_tiles) {
+  __shared__ float2 of_warp[kTile / 32];
+  begin_kernel();
+  const bool queries = blockIdx.x < query_items;
+  const int rows = queries ? p.length : p.keys, tiles = queries ? query_tiles : key_tiles;
+  int kv_head;
+  const Tile t = find_tile(p, static_cast<int>(blockIdx.x - (queries ? 0 : query_items)), rows, p.kv_heads, kTileShift, tiles,
+                           false, &kv_head);
+  if (!t.found) return;
+  const int row = t.first + threadIdx.x;
+  const int64_t at = static_cast<int64_t>(t.batch) * rows + t.row0 + row;
+  float norm = 0.0f, delta = 0.0f;
+  if (!queries) {
+    if (row < t.keys) norm = p.value_norm[at * p.kv_heads + kv_head];
+  } else if (row < t.queries) {
+    const int group = p.heads / p.kv_heads;
+#pragma unroll 4
+    for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
+      norm = fmaxf(norm, p.grad_norm[at * p.heads + head]);
+      const float d = fabsf(p.stats[(p.heads + head) * p.rows + at]);
+      if (d < INFINITY) delta = fmaxf(delta, d);
+    }
   }
+  norm = warp_top(norm);
+  delta = warp_top(delta);
+  if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = make_float2(norm, delta);
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+  for (int w = 1; w < kTile / 32; ++w) norm = fmaxf(norm, of_warp[w].x), delta = fmaxf(delta, of_warp[w].y);
+  const int64_t to = tile_slot(p, t, rows, tiles, kv_head) + (t.first >> kTileShift);
+  if (queries)
+    query_top[to] = make_float2(norm, delta);
+  else
+    key_top[to] = norm;
+}
+
+// The binary exponent that brings ds, of at most `bound` (|dp| <= |dout| |v|), to
+// 2^14 to 2^15.  A ds below fp16's normal range is then off by half of its last
+// place, 2^-25, which is 2^-39 of the bound or less.  Query rows have one each, of
+// the row's own |dout| and |delta| and the largest |v| of the keys' tiles; keys one
+// each, of the key's |v| and the largest |dout| and |delta| of the queries' tiles:
+// what is large elsewhere takes nothing from them.  (One for the whole call, of
+// its largest elements, lost up to all of dq and dk beside large padding or
+// another sequence 10^3 as large.  The bounds cost 8191 packed tokens, 16 heads of
+// 64, window 512: 169 -> 178 us; 4 x 4096, 16 over 4: 981 -> 997.)
+__device__ __forceinline__ int ds_exponent(float bound) {
+  return bound > 0.0f && bound < INFINITY ? clamp_int(14 - ilogbf(bound), -60, 100) : 0;
 }
 
 // ------------------------------------------------------------ backward: keys and values
@@ -1046,13 +1105,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     take_registers<kScoreRegisters>();
     const int w = warp / 4;  // both halves have all keys
     const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
-    const float factor = ds_factor<T>(p), c = p.scale * kLog2e, raise = factor * (kBf16<T> ? 1.0f : 0x1p-10f);
+    const float c = p.scale * kLog2e;
     bool ok = true;
     int g = 0, used = 0;
+    const auto factor_of = [&](const Keys& item) {
+      if constexpr (kBf16<T>) return 1.0f;
+      const float2* top = p.query_top + tile_slot(p, item.t, p.length, tiles, item.kv_head) + item.from;
+      float grad = 0.0f, delta = 0.0f, value = 0.0f;
+      const int row = item.t.first + threadIdx.x % 128;
+      if (item.per > 0 && row < item.t.keys)
+        value = p.value_norm[(static_cast<int64_t>(item.t.batch) * p.keys + item.t.row0 + row) * p.kv_heads + item.kv_head];
+      for (int x = lane; x < item.per; x += 32) {
+        const float2 most = top[x];
+        grad = fmaxf(grad, most.x);
+        delta = fmaxf(delta, most.y);
+      }
+      return scalbnf(1.0f, ds_exponent(warp_top(grad) * value + warp_top(delta)));
+    };
     Keys next(p, blockIdx.x, tiles);
+    float next_factor = factor_of(next);
     for (int k = 0, number = blockIdx.x; ok && number >= 0; ++k) {
       const Keys item = next;
       const Tile& t = item.t;
+      const float factor = next_factor, raise = factor * (kBf16<T> ? 1.0f : 0x1p-10f);
       const int row = t.first + threadIdx.x % 128, n = item.per * group;  // the thread's key
       int mine_low = 0, mine_high = 0, all_low = 0, all_high = 0;
       if (t.found) {
@@ -1142,7 +1217,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&m.ds_done[w]);
       }
       number = ok ? m.queue.take(k, failed) : -1;
-      if (number >= 0) next = Keys(p, number, tiles);
+      if (number >= 0) {
+        next = Keys(p, number, tiles);
+        next_factor = factor_of(next);
+      }
       if (ok && n > 0) ok = warp_wait(&m.finished, used++ & 1, failed);
       tc_fence_after();
       // the first half writes dv, the other dk
@@ -1314,13 +1392,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     take_registers<kScoreRegisters>();
     const int w = warp / 4;  // both halves have all queries
     const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
-    const float factor = ds_factor<T>(p), c = p.scale * kLog2e, raise = factor * (kBf16<T> ? 1.0f : 0x1p-10f);
+    const float c = p.scale * kLog2e;
     bool ok = true;
     int g = 0, used = 0;
+    // the row's -lse, with ds's factor, and -delta; the factor's exponent
+    float next_lse, next_delta;
+    int next_exponent;
+    const auto look_up = [&](const Queries& item) {
+      next_lse = -INFINITY, next_delta = 0.0f, next_exponent = 0;
+      const int64_t at = static_cast<int64_t>(item.t.batch) * p.length + item.t.row0 + item.t.first + threadIdx.x % 128;
+      const bool counts = item.t.found && item.t.first + static_cast<int>(threadIdx.x % 128) < item.t.queries;
+      if (counts) {
+        next_lse = p.stats[item.head * p.rows + at];
+        next_delta = p.stats[(p.heads + item.head) * p.rows + at];
+      }
+      if constexpr (!kBf16<T>) {
+        const float* top = p.key_top + tile_slot(p, item.t, p.keys, tiles, item.head / (p.heads / p.kv_heads)) + item.from;
+        const float grad = counts ? p.grad_norm[at * p.heads + item.head] : 0.0f;
+        float value = 0.0f;
+        for (int x = lane; x < item.to - item.from; x += 32) value = fmaxf(value, top[x]);
+        next_exponent = ds_exponent(grad * warp_top(value) + fabsf(next_delta));
+        next_lse += static_cast<float>(next_exponent) - kRaiseBack<T>;
+      }
+    };
     Queries next(p, blockIdx.x, tiles);
+    look_up(next);
     for (int k = 0, number = blockIdx.x; ok && number >= 0; ++k) {
       const Queries item = next;
       const Tile& t = item.t;
+      const float lse = next_lse, delta = next_delta;
+      const int exponent = next_exponent;
       const int row = t.first + threadIdx.x % 128, n = item.to - item.from;
       int mine_low = 0, mine_high = 0, all_low = 0, all_high = 0;
       if (t.found) {
@@ -1333,11 +1434,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const int64_t at = static_cast<int64_t>(t.batch) * p.length + t.row0 + row;
-      float lse = -INFINITY, delta = 0.0f;
-      if (t.found && row < t.queries) {
-        lse = p.stats[item.head * p.rows + at];
-        delta = p.stats[(p.heads + item.head) * p.rows + at];
-      }
       for (int it = 0; it < n; ++it, ++g) {
         const int first = (item.from + it) * kTile;
         const bool partial = first < all_low || first + kTile > all_high;
@@ -1365,7 +1461,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 64; e += 2) {
           const float2 u = fma2(make_float2(as_float(x[e / 32][e % 32]), as_float(x[e / 32][e % 32 + 1])), both(c), both(lse));
           float2 v = add2(make_float2(as_float(y[e / 32][e % 32]), as_float(y[e / 32][e % 32 + 1])), both(delta));
-          if constexpr (!kBf16<T>) v = mul2(v, both(raise));
           v = mul2(v, make_float2(fast_exp2(u.x), fast_exp2(u.y)));
           y[e / 32][e % 32] = __float_as_uint(v.x);
           y[e / 32][e % 32 + 1] = __float_as_uint(v.y);
@@ -1384,7 +1479,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&ds_done[w][g & 1]);
       }
       number = ok ? queue.take(k, failed) : -1;
-      if (number >= 0) next = Queries(p, number, tiles);
+      if (number >= 0) {
+        next = Queries(p, number, tiles);
+        look_up(next);
+      }
       if (ok && n > 0) ok = warp_wait(&finished, used++ & 1, failed);
       tc_fence_after();
       if (w == 0) {
@@ -1392,7 +1490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool write = ok && t.found && row < t.stored, some = mine_low < mine_high;
         if (n > 0)
           store_rows<T, kCols, kCols == 128>(grad, nullptr, static_cast<int64_t>(p.heads) * p.dim, tmem_dq + lanes, p.dim,
-                                             p.scale / factor, write && some);
+                                             scalbnf(p.scale, -exponent), write && some);
         if (write && (n == 0 || !some)) zero_row(grad, p.dim);
       }
       __syncwarp();
@@ -1476,6 +1574,23 @@ int check_forward(const muon_train_attention_args& a) {
 int64_t tiles_of(const muon_train_attention_args& a, int64_t rows, int64_t size) {
   if (a.offsets != nullptr) return rows / size + a.sequences + 2;
   return a.batch * ((rows + size - 1) / size);
+}
+
+// A backward call's workspace: its arrays' first elements, in floats.
+struct Workspace {
+  int64_t stats, query_top, grad_norm, value_norm, key_top, end;
+};
+Workspace workspace_of(const muon_train_attention_args& a) {
+  const bool half = a.dtype == MUON_TRAIN_F16;
+  const int64_t rows = a.heads * a.batch * a.length;
+  Workspace w;
+  w.stats = 0;
+  w.query_top = w.stats + 2 * rows;  // pairs
+  w.grad_norm = w.query_top + (half ? 2 * a.kv_heads * tiles_of(a, a.length, kTile) : 0);
+  w.value_norm = w.grad_norm + (half ? rows : 0);
+  w.key_top = w.value_norm + (half ? a.kv_heads * a.batch * a.keys : 0);
+  w.end = w.key_top + (half ? a.kv_heads * tiles_of(a, a.keys, kTile) : 0);
+  return w;
 }
 
 struct Maps {
@@ -1592,20 +1707,30 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
   if (rc == MUON_POLAR_OK) rc = encode(&map_g, g.grad_out, g.grad_out_stride, a.length, a.heads, a.batch, a.dim, a.dtype);
   if (rc != MUON_POLAR_OK) return rc;
   Problem p = problem_of(a);
-  float* stats = static_cast<float*>(g.workspace) + 2 * kLargestSlots;
-  uint32_t* largest = static_cast<uint32_t*>(g.workspace);
-  p.stats = stats;
-  p.largest = static_cast<const float*>(g.workspace);
-  if constexpr (!kBf16<T>) {
-    const cudaError_t e = cudaMemsetAsync(largest, 0, 2 * kLargestSlots * sizeof(float), s);
-    if (e != cudaSuccess) return static_cast<int>(e);
-  }
-  const Stats st{a.out, a.out_rest, g.grad_out, a.v, a.lse, stats, largest, g.grad_out_stride, a.v_stride, rows,
-                 a.batch * a.keys, p.length, p.keys, p.heads, p.kv_heads, p.dim};
+  float* workspace = static_cast<float*>(g.workspace);
+  const Workspace w = workspace_of(a);
+  p.stats = workspace + w.stats;
+  p.grad_norm = workspace + w.grad_norm;
+  p.value_norm = workspace + w.value_norm;
+  p.query_top = reinterpret_cast<float2*>(workspace + w.query_top);
+  p.key_top = workspace + w.key_top;
+  const Stats st{a.out, a.out_rest, g.grad_out, a.v, a.lse, workspace + w.stats, workspace + w.grad_norm,
+                 workspace + w.value_norm, g.grad_out_stride, a.v_stride, rows, a.batch * a.keys, p.length, p.keys, p.heads,
+                 p.kv_heads, p.dim};
   const int64_t per = 256 / (kCols / 8) * kStatRows;
   const dim3 grid(static_cast<unsigned>((rows * a.heads + per - 1) / per));
   rc = launch(stats_kernel<T, kCols>, grid, 256, 0, 1, true, stream, st);
   if (rc != MUON_POLAR_OK) return rc;
+  if constexpr (!kBf16<T>) {
+    const int64_t query_tiles = tiles_of(a, a.length, kTile), key_tiles = tiles_of(a, a.keys, kTile);
+    const uint32_t query_items = static_cast<uint32_t>(query_tiles * a.kv_heads),
+                   key_items = static_cast<uint32_t>(key_tiles * a.kv_heads);
+    p.section = static_cast<int>(a.batch * a.kv_heads);  // all
+    rc = launch(tops_kernel, dim3(query_items + key_items), kTile, 0, 1, true, stream, p,
+                reinterpret_cast<float2*>(workspace + w.query_top), workspace + w.key_top, query_items,
+                static_cast<int>(query_tiles), static_cast<int>(key_tiles));
+    if (rc != MUON_POLAR_OK) return rc;
+  }
   const int64_t group = a.heads / a.kv_heads, pair_bytes = 2 * a.dim * static_cast<int64_t>(sizeof(T));
   constexpr int kBytes = KeyGrads<kCols>::kBytes;
   if (a.keys > 0) {
@@ -1664,7 +1789,7 @@ int muon_train_attention_sm100(const muon_train_attention_args* args, void* stre
 size_t muon_train_attention_workspace_bytes(const muon_train_attention_args* args) {
   using namespace muon_train;
   if (check(args) != MUON_POLAR_OK) return 0;
-  return static_cast<size_t>(2 * args->heads * args->batch * args->length + 2 * kLargestSlots) * sizeof(float);
+  return static_cast<size_t>(workspace_of(*args).end) * sizeof(float);
 }
 
 int muon_train_attention_backward_sm100(const muon_train_attention_args* args,

@@ -427,6 +427,89 @@ def test_attention_gives_gradients_where_asked(pkg):
         out.backward(go)
 
 
+@pytest.mark.parametrize("dtype,largest", [(F16, 65504.0), (BF16, 3e38)], ids=str)
+@pytest.mark.parametrize("packed", [False, True])
+def test_attention_gradients_whatever_finite_values_padding_holds(pkg, dtype, largest, packed):
+    """The same bits with zeros and with the type's largest values in tokens that
+    do not count."""
+    counts = [300, 0, 1, 129, 256]
+    q, k, v, go = attention_inputs(5, 300, 300, 4, 2, 64, dtype, seed=31)
+    counted = torch.arange(300, device="cuda") < torch.tensor(counts, device="cuda")[:, None]
+    kw = {"lengths": torch.tensor(counts, device="cuda")}
+    if packed:  # the tokens of one sequence, between those of none
+        q, k, v, go = (t.flatten(0, 1) for t in (q, k, v, go))
+        counted = torch.arange(1500, device="cuda")
+        counted = (counted >= 3) & (counted < 1300)
+        kw = {"offsets": torch.tensor([3, 260, 260, 700, 1300], device="cuda")}
+    results = []
+    for fill in (0.0, largest, -largest):
+        held = [torch.where(counted[..., None, None], t, fill).to(dtype) for t in (q, k, v, go)]
+        leaves = [t.requires_grad_(True) for t in held[:3]]
+        out = pkg.attention(*leaves, causal=True, **kw)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, held[3])])
+    for other in results[1:]:
+        for a, b in zip(other, results[0]):
+            assert torch.equal(a, b)
+
+
+def check_fp16_gradients(pkg, q, k, v, go, sequences, causal, **kw):
+    """ds is held in fp16 under powers of two that bring a bound B on a row's
+    (dq) or a key's (dk) elements to 2^14 at least; an element below fp16's
+    normal range is then off by half a subnormal, 2^-25, which is 2^-39 of B.
+    For dq B is |dout_i| max_j |v_j| + |delta_i|, for dk max_i |dout_i| |v_j| +
+    max_i |delta_i|, over the sequence and the heads that share the key head."""
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = pkg.attention(*leaves, causal=causal, **kw)
+    got = torch.autograd.grad(out, leaves, go)
+    scale, group = q.shape[-1] ** -0.5, q.shape[-2] // k.shape[-2]
+    made = attention_reference(q, k, v, go, causal=causal, window=None, scale=scale, sequences=sequences)
+    # the reference's bound is linear in what a product's terms are off by: add theirs
+    for rows, keys in sequences:
+        for h in range(k.shape[-2]):
+            vn = v[keys][:, h].double().norm(dim=-1)
+            heads = range(h * group, (h + 1) * group)
+            gn = [go[rows][:, i].double().norm(dim=-1) for i in heads]
+            delta = [(go[rows][:, i].double() * made[0][0][rows][:, i]).sum(-1).abs() for i in heads]
+            most, most_delta = max(g.max() for g in gn), max(d.max() for d in delta)
+            see = sees(len(gn[0]), len(vn), causal, None).double()
+            for i, g, d in zip(heads, gn, delta):
+                made[1][1][rows][:, i] += 2.0 ** -39 * scale * (g * vn.max() + d)[:, None] * (see @ k[keys][:, h].abs().double())
+                made[2][1][keys][:, h] += 2.0 ** -39 * scale * (most * vn + most_delta)[:, None] * (
+                    see.T @ q[rows][:, i].abs().double())
+    for name, a, (value, bound) in zip(("dq", "dk", "dv"), got, made[1:]):
+        near(a, value, bound, name)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_fp16_gradients_of_sequences_and_heads_of_different_sizes(pkg, causal):
+    """Values and gradients that differ by 10^3 to 10^5 between sequences and
+    heads: none is lost in the others' range."""
+    q, k, v, go = attention_inputs(4, 1500, 1500, 4, 2, 64, F16, seed=32)
+    v[0, :, 1] *= 2000.0
+    v[3, :, 1] *= 2000.0
+    go *= 0.2
+    go[1] *= 1e4
+    go[:, :, 2] *= 0.01
+    v[2] *= 0.01
+    check_fp16_gradients(pkg, q, k, v, go, whole(4), causal)
+    offsets = torch.tensor([0, 1500, 1700, 4500, 6000], device="cuda")
+    parts = [((slice(a, b),), (slice(a, b),)) for a, b in zip(offsets.tolist(), offsets.tolist()[1:])]
+    check_fp16_gradients(pkg, *(t.flatten(0, 1) for t in (q, k, v, go)), parts, causal, offsets=offsets)
+
+
+def test_fp16_gradients_beside_single_large_rows(pkg):
+    """One token of a sequence with large values, another with a large gradient."""
+    q, k, v, go = attention_inputs(2, 1200, 1200, 4, 2, 128, F16, seed=33)
+    go *= 0.5
+    v[0, 700] *= 1000.0
+    go[1, 300] *= 1000.0
+    check_fp16_gradients(pkg, q, k, v, go, whole(2), True)
+    lengths = torch.tensor([701, 1111], device="cuda")
+    go[0, 701:], go[1, 1111:] = 0, 0
+    check_fp16_gradients(pkg, q, k, v, go, [((b, slice(0, n)), (b, slice(0, n))) for b, n in enumerate(lengths.tolist())],
+                         False, lengths=lengths)
+
+
 # =================================================================== rotary
 def rotary_reference(x, positions, frequencies, interleaved, scale, sign=1.0):
     """(value, bound) in 64 bits."""
