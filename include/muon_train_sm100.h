@@ -281,7 +281,9 @@ int muon_train_rotary_sm100(const muon_train_rotary_args* args, void* stream);
  * Tensors are contiguous and do not overlap; out may be grad itself (of the
  * same type), and in place tensors within the limit are not written.  Squares
  * are added up in fp32 over at most eight elements, then in 64 bits, and in 64
- * bits alone where they leave fp32's range.  A NaN makes the norm and all outputs NaN.
+ * bits alone where they leave fp32's range.  A NaN makes the norm and, under a
+ * finite max_norm, all outputs NaN; an infinite max_norm scales nothing, whatever
+ * the norm is.
  */
 typedef struct {
   const void* grad;            /* [count] */

@@ -291,7 +291,9 @@ __device__ __forceinline__ void scale_share(const Table<kEntries>& t, float fact
       scale_into<kGroup, __half>(t.in[i], t.out[i], out, from, n, factor, rank);
   }
 }
+// Without a limit nothing is scaled, whatever the norm is: inf / inf is none.
 __device__ __forceinline__ float factor_of(double norm, double max_norm) {
+  if (max_norm == static_cast<double>(INFINITY)) return 1.0f;
   const double c = max_norm / (norm + 1e-6);
   return c > 1.0 ? 1.0f : static_cast<float>(c);  // NaN stays
 }

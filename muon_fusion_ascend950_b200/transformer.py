@@ -274,10 +274,11 @@ def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, *, norm_t
     place, or into the tensors of ``out``, of the same shapes and any of the
     three types (gradients accumulated in fp32 go to the parameters' type in
     the same pass).  ``norm_type`` is 2 or infinity (the largest magnitude).
-    ``max_norm=math.inf`` only takes the norm.  Squares are summed in fp32 over
-    the elements of one load and in fp64 from there on, in a fixed order,
-    products are fp32, and each output is rounded once.  A NaN
-    makes the norm and all results NaN.
+    ``max_norm=math.inf`` only takes the norm (and converts, with ``out``),
+    whatever it is.  Squares are summed in fp32 over the elements of one load
+    and in fp64 from there on, in a fixed order, products are fp32, and each
+    output is rounded once.  With a finite limit a NaN makes the norm and all
+    results NaN, and an infinite element makes them 0, its own NaN.
     """
     gradients = list(gradients)
     if not gradients:

@@ -692,6 +692,26 @@ def test_clip_of_values_of_any_size(pkg):
     assert not g.any()
 
 
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("sizes", [[1000, 7], [2 ** 18, 1001], [50] * 40, [300] * 1100], ids=lambda s: f"{len(s)}x{s[0]}")
+def test_without_a_limit_clipping_only_takes_the_norm(pkg, sizes, bad, norm_type):
+    """Whatever the norm is: one launch and two, short lists and long ones."""
+    grads = some_grads(sizes, [F32, BF16, F16], seed=73)
+    grads[-1][5] = bad
+    kept = [g.clone() for g in grads]
+    norms = [pkg.clip_gradients(grads, math.inf, norm_type=norm_type)]
+    for out_dtype in (F32, BF16):
+        out = [torch.full_like(g, 7.0, dtype=out_dtype) for g in grads]
+        norms.append(pkg.clip_gradients(grads, math.inf, norm_type=norm_type, out=out))
+        for o, k in zip(out, kept):
+            assert torch.equal(o.nan_to_num(nan=-3.0), k.to(out_dtype).nan_to_num(nan=-3.0))
+    for g, k in zip(grads, kept):
+        assert torch.equal(g.nan_to_num(nan=-3.0), k.nan_to_num(nan=-3.0))
+    for norm in norms:
+        assert norm.isnan() if math.isnan(bad) else norm == math.inf
+
+
 def test_clip_of_parameters(pkg):
     a, b, c = (torch.nn.Parameter(torch.zeros(50, 20, device="cuda")) for _ in range(3))
     a.grad, b.grad = randn(50, 20, seed=67), randn(50, 20, seed=68)
