@@ -85,6 +85,7 @@ struct Problem {
   int length, keys, heads, kv_heads, dim, sequences, batch, window, causal;
   int section;              // heads (pairs of them: by_heads) whose tiles are worked on together
   int by_heads;             // forward: 1, pairs of tiles are of two heads; 0, of one
+  int blind;                // kernel for keys: queries from the first on that see no key, and that its maps leave out
   float scale;
 };
 
@@ -1015,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             if (lane == 0) {
               mbar_arrive_expect_tx(&m.full[s], C::kTileBytes);
-              load_tile<kCols>(ring + s * C::kTileBytes, which ? &map_g : &map_q, &m.full[s], row, head, w.t.batch);
+              load_tile<kCols>(ring + s * C::kTileBytes, which ? &map_g : &map_q, &m.full[s], row - p.blind, head, w.t.batch);
             }
             ++fills;
             if (which == 0) {
@@ -1743,8 +1744,21 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
     const int64_t tiles = tiles_of(a, a.keys, kTile);
     rc = section_of(a.batch * a.kv_heads, a.length * pair_bytes * group, tiles / a.batch, &p.section);
     if (rc != MUON_POLAR_OK) return rc;
+    // Queries before the first key's place, which see none, share tiles with others: maps that begin behind them
+    // give zeros for what they and their gradients hold.
+    const int64_t blind = a.causal ? a.length - a.keys : a.window > 0 ? a.length - a.keys - a.window + 1 : 0;
+    CUtensorMap seeing_q = m.q, seeing_g = map_g;
+    if (blind > 0 && blind < a.length) {
+      p.blind = static_cast<int>(blind);
+      rc = encode(&seeing_q, static_cast<const T*>(a.q) + blind * a.q_stride.row, a.q_stride, a.length - blind, a.heads,
+                  a.batch, a.dim, a.dtype);
+      if (rc == MUON_POLAR_OK)
+        rc = encode(&seeing_g, static_cast<const T*>(g.grad_out) + blind * g.grad_out_stride.row, g.grad_out_stride,
+                    a.length - blind, a.heads, a.batch, a.dim, a.dtype);
+      if (rc != MUON_POLAR_OK) return rc;
+    }
     rc = launch(key_grad_kernel<T, kCols>, dim3(static_cast<unsigned>(tiles * a.kv_heads)), kThreads, kBytes, 1, true,
-                stream, m.q, m.k, m.v, map_g, p, static_cast<int>(tiles));
+                stream, seeing_q, m.k, m.v, seeing_g, p, static_cast<int>(tiles));
     if (rc != MUON_POLAR_OK) return rc;
   }
   rc = prepare<query_grad_kernel<T, kCols>>(kBytes);

@@ -427,6 +427,25 @@ def test_attention_gives_gradients_where_asked(pkg):
         out.backward(go)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("length,keys,causal,window", [(300, 200, True, None), (300, 7, True, 3), (513, 300, False, 20),
+                                                       (700, 1, True, None), (256, 128, True, None)])
+def test_rows_that_see_nothing_reach_no_gradient(pkg, length, keys, causal, window, dtype):
+    """Queries before the first key's place: whatever they and their gradients hold."""
+    q, k, v, go = attention_inputs(2, length, keys, 4, 2, 64, dtype, seed=34)
+    blind = ~sees(length, keys, causal, window).any(1)
+    assert blind.any() and not blind.all()
+    q[:, blind], go[:, blind] = 0, 0
+    sequences = whole(2)
+    got = check_attention(pkg, q, k, v, go, sequences=sequences, causal=causal, window=window)
+    for bad in (math.nan, math.inf):
+        q[:, blind], go[:, blind] = bad, -bad
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = pkg.attention(*leaves, causal=causal, window=window)
+        for a, b in zip(got, [out.detach(), *torch.autograd.grad(out, leaves, go)]):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype,largest", [(F16, 65504.0), (BF16, 3e38)], ids=str)
 @pytest.mark.parametrize("packed", [False, True])
 def test_attention_gradients_whatever_finite_values_padding_holds(pkg, dtype, largest, packed):
