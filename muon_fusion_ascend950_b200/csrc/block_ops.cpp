@@ -325,11 +325,12 @@ void muon_train_ops::clip_gradients(TensorPointers grads, TensorPointers out, do
       t.out_dtype = Dtype(o, who, "out");
     }
     if (t.count == 0) continue;
-    t.grad = g.unsafeGetTensorImpl()->data();
-    t.out = out.empty() ? const_cast<void*>(t.grad) : o.unsafeGetTensorImpl()->mutable_data();
+    t.out = o.unsafeGetTensorImpl()->mutable_data();  // a lazy clone gets memory of its own here
     const uintptr_t begin = reinterpret_cast<uintptr_t>(t.out);
     written.Add(begin, begin + static_cast<uintptr_t>(t.count) * o.element_size());
   }
+  for (size_t i = 0; i < n; ++i)  // where they are when all that is written has its memory
+    if (list[i].count > 0) list[i].grad = grads[i]->unsafeGetTensorImpl()->data();
   TORCH_CHECK_VALUE(!written.Overlap(), who,
                     ": the same memory would be scaled twice (a gradient listed twice, or views of one another)");
   if (!out.empty()) {  // what is written may not be read as another gradient

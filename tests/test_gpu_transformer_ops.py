@@ -783,6 +783,27 @@ def test_clip_goes_through_the_operator_where_something_listens(pkg):
         pkg.clip_gradients(g, -1.0)
 
 
+@pytest.mark.parametrize("count", [1, 40])
+def test_clipping_in_place_leaves_lazy_clones_alone(pkg, count):
+    """A clone that shares its memory until one of the two is written."""
+    base = [randn(500, seed=74 + i) for i in range(count)]
+    kept = [t.clone() for t in base]
+    clones = [torch._lazy_clone(t) for t in base]
+    norm, want = clip_reference(kept, 0.5, 2.0)
+    near(pkg.clip_gradients(base, 0.5), norm, 6 * E32 * norm)
+    for t, clone, k, w in zip(base, clones, kept, want):
+        near(t, w, 3.2 * E32 * w.abs())
+        assert torch.equal(clone, k)
+    # parts of one buffer, and outputs that are the gradients themselves
+    flat = randn(1000, seed=75)
+    kept, clone = flat.clone(), torch._lazy_clone(flat)
+    parts = list(flat.split(1000 // (2 * count)))
+    norm, want = clip_reference([kept], 0.5, 2.0)
+    pkg.clip_gradients(parts, 0.5, out=parts)
+    near(flat, want[0], 3.2 * E32 * want[0].abs())
+    assert torch.equal(clone, kept)
+
+
 def test_clip_refuses_memory_that_would_be_scaled_twice(pkg):
     g = randn(100, seed=69)
     for grads, out in (([g, g], None), ([g[:60], g[40:]], None), ([g, randn(100, seed=70)], [g, g]),
