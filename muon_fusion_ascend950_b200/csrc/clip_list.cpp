@@ -14,6 +14,8 @@
 
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
+#include <cstddef>
+#include <cstring>
 #include <string>
 #include <vector>
 
@@ -24,7 +26,8 @@ namespace {
 using at::Tensor;
 
 // How torch.Tensor begins (torch/csrc/autograd/python_variable.h, whose other
-// contents would need the Python library).
+// contents would need the Python library).  Other versions of torch may hold the
+// tensor another way: muon_ascend950_clip_reads tells.
 struct PythonTensor {
   PyObject_HEAD Tensor tensor;
 };
@@ -55,6 +58,17 @@ thread_local std::string message;
 enum Status { kDone = 0, kValue = 1, kType = 2, kNotImplemented = 3, kRuntime = 4, kThroughTheOperator = 5 };
 
 }  // namespace
+
+// The word where this file takes the tensor of `object`, of the type torch.Tensor
+// itself, to be; nothing is read through it.  It is the tensor's `_cdata` where the
+// layout is as above, and only then may lists be passed to the entry below.
+static_assert(sizeof(Tensor) == sizeof(uintptr_t), "a tensor is one pointer");
+extern "C" __attribute__((visibility("default"))) uintptr_t muon_ascend950_clip_reads(PyObject* object) {
+  if (static_cast<size_t>(Py_TYPE(object)->tp_basicsize) < sizeof(PythonTensor)) return 0;
+  uintptr_t word;
+  std::memcpy(&word, reinterpret_cast<const char*>(object) + offsetof(PythonTensor, tensor), sizeof(word));
+  return word;
+}
 
 // `gradients` and `out` (or NULL): lists of objects of the type torch.Tensor
 // itself, not empty; `norm`: such a tensor.  Called with the interpreter's lock.

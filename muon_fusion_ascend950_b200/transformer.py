@@ -31,13 +31,26 @@ _attention = torch.ops.muon_ascend950.attention.default
 _rotary = torch.ops.muon_ascend950.rotary.default
 _clip_in_place = torch.ops.muon_ascend950.clip_gradients_.default
 _clip_out = torch.ops.muon_ascend950.clip_gradients.default
-# The same on Python's own lists (clip_list.cpp), for long ones: the call itself
-# takes longer.  A library set by MUON_ASCEND950_LIBRARY may be without it.
+
+
+def _list_entry(library):
+    """The same on Python's own lists (clip_list.cpp), for long ones: the call
+    itself takes longer.  None where the library is without it (one set by
+    MUON_ASCEND950_LIBRARY) or does not find the tensors in this torch's objects."""
+    entry, reads = (getattr(library, "muon_ascend950_clip_" + name, None) for name in ("list", "reads"))
+    if entry is None or reads is None:
+        return None
+    reads.argtypes, reads.restype = [ctypes.py_object], ctypes.c_size_t
+    probes = (torch.empty(shape, device="cpu") for shape in ((), (3, 2)))
+    if any(reads(t) != t._cdata for t in probes):
+        return None
+    entry.argtypes = [ctypes.py_object, ctypes.c_void_p, ctypes.py_object, ctypes.c_double, ctypes.c_int]
+    library.muon_ascend950_clip_message.restype = ctypes.c_char_p
+    return entry
+
+
 _library = ctypes.PyDLL(str(_library_path()))
-_clip_list = getattr(_library, "muon_ascend950_clip_list", None)
-if _clip_list is not None:
-    _clip_list.argtypes = [ctypes.py_object, ctypes.c_void_p, ctypes.py_object, ctypes.c_double, ctypes.c_int]
-    _library.muon_ascend950_clip_message.restype = ctypes.c_char_p
+_clip_list = _list_entry(_library)
 _CLIP_ERRORS = {1: ValueError, 2: TypeError, 3: NotImplementedError, 4: RuntimeError}
 _LONG_LIST = 32
 _PLAIN = {torch.Tensor}

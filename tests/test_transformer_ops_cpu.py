@@ -231,6 +231,33 @@ def test_clip_is_checked():
             pkg.clip_gradients([_cuda(3, dtype=I64)], 1.0)
 
 
+def test_lists_are_read_only_where_tensors_are_as_expected():
+    """A library that does not find the tensor in torch's objects, or cannot tell,
+    is not given lists: calls go through the operator."""
+    reads = transformer._library.muon_ascend950_clip_reads
+    for t in (torch.zeros(3), torch.zeros(2, 2)[0], torch.nn.Parameter(torch.zeros(1))):
+        assert reads(t) == t._cdata
+    assert transformer._clip_list is not None and reads(object()) == 0  # too small to hold a tensor
+
+    class Library:
+        muon_ascend950_clip_list = muon_ascend950_clip_message = transformer._clip_list
+
+        def __init__(self, reads=None):
+            if reads is not None:
+                self.muon_ascend950_clip_reads = reads
+
+    class Entry:
+        def __init__(self, answer):
+            self.answer = answer
+
+        def __call__(self, t):
+            return self.answer(t)
+
+    for library in (object(), Library(), Library(Entry(lambda t: 0)), Library(Entry(lambda t: t._cdata + 8))):
+        assert transformer._list_entry(library) is None
+    assert transformer._list_entry(Library(Entry(lambda t: t._cdata))) is transformer._clip_list
+
+
 def test_forward_mode_is_refused():
     from torch.autograd import forward_ad
 
