@@ -468,6 +468,8 @@ std::tuple<Tensor, Tensor> RotaryAutograd(const Tensor& q, const OptTensor& key,
   };
   const Tensor& k = Given(key);
   NoTangents({&q, &k, &frequencies}, "rotary");
+  TORCH_CHECK_NOT_IMPLEMENTED(!Recorded({&frequencies}),
+                              "rotary: frequencies have no gradient (pass them detached, or without recording)");
   if (!Recorded({&q, &k})) return call();
   auto node = MakeNode<RotaryBackward>(q, k);
   auto result = call();

@@ -223,7 +223,8 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor], positions: torch.Te
     64 bits, products in fp32, and each output is rounded once.
 
     Returns the two turned tensors, contiguous (None without ``key``).
-    Differentiable in ``query`` and ``key``.
+    Differentiable in ``query`` and ``key``; frequencies that require a gradient
+    are refused (NotImplementedError).
     """
     try:
         turned, turned_key = _rotary(query, key, positions, frequencies, interleaved, scale)

@@ -271,6 +271,19 @@ def test_forward_mode_is_refused():
                 call(forward_ad.make_dual(q.clone(), torch.ones_like(q)))
 
 
+def test_rotary_refuses_frequencies_that_want_a_gradient():
+    with _fake():
+        q, at = _cuda(4, 2, 64, dtype=F32), _cuda(4, dtype=I64)
+        f = torch.empty(32, dtype=F64, device="cuda", requires_grad=True)
+        for leaf in (q, q.clone().requires_grad_(True)):
+            for key in (None, leaf):
+                with pytest.raises(NotImplementedError):
+                    pkg.rotary(leaf, key, at, f)
+                assert pkg.rotary(leaf, key, at, f.detach())[0].requires_grad == leaf.requires_grad
+        with torch.no_grad():
+            pkg.rotary(q, None, at, f)
+
+
 def test_fake_backward_kernels():
     with _fake():
         ops = torch.ops.muon_ascend950
