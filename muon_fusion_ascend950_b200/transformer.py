@@ -198,7 +198,7 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ca
     """
     try:
         if scale is None:
-            scale = query.shape[-1] ** -0.5
+            scale = max(1, query.shape[-1]) ** -0.5
         if window is not None and window < 1:
             raise ValueError(f"window must be positive, got {window}")
         return _attention(query, key, value, offsets, lengths, causal, window or 0, scale, False)[0]

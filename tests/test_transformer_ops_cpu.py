@@ -194,6 +194,11 @@ def test_attention_is_checked(kw, error):
                 attention(**kw)
 
 
+def test_attention_refuses_heads_without_elements():
+    with _fake(), pytest.raises(ValueError):
+        attention(q=(2, 6, 4, 0), k=(2, 6, 2, 0))
+
+
 @pytest.mark.parametrize("q,k,at,f,kw,error", [
     ((2, 6, 4, 64), (2, 6, 1, 64), (2, 6), 32, {}, None), ((2, 6, 4, 64), None, (6,), 16, dict(interleaved=True), None),
     ((6, 4, 64), None, (6,), 0, {}, None), ((4, 64), (2, 64), (), 1, {}, None), ((2, 3, 6, 1, 7), None, (2, 3, 6), 3, {}, None),
