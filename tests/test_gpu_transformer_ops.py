@@ -984,3 +984,18 @@ def test_debug_sync_waits_for_every_call(pkg, monkeypatch):
             torch.cuda._sleep(100_000_000)
             call()
             assert torch.cuda.current_stream().query() == sync
+
+
+def test_a_lower_wait_limit_reaches_every_kernel(pkg):
+    """The limit read back is the largest of the kernels' copies: one that was
+    left behind shows when the limit is lowered."""
+    from muon_fusion_ascend950_b200.capi import capi
+
+    api = capi()
+    before = api.train_wait_limit_ns()
+    previous = api.set_wait_limit_ns(before // 2)
+    try:
+        assert previous == before and api.train_wait_limit_ns() == before // 2
+    finally:
+        api.set_wait_limit_ns(previous)
+    assert api.train_wait_limit_ns() == before
