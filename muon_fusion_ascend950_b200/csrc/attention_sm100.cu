@@ -851,15 +851,14 @@ __device__ __forceinline__ float warp_top(float v) {
 // that share a key head, and the largest |v| of each tile of keys, over the rows
 // that count: what others hold reaches nothing.  A block a tile, a row a thread.
 __global__ void __launch_bounds__(kTile)
-    tops_kernel(const __grid_constant__ Problem p, float2* query_top, float* key_top, uint32_t query_items, int query_tiles,
-                int key_tiles) {
+    tops_kernel(const __grid_constant__ Problem p, float2* query_top, float* key_top, int query_tiles, int key_tiles) {
   __shared__ float2 of_warp[kTile / 32];
   begin_kernel();
-  const bool queries = blockIdx.x < query_items;
+  const bool queries = blockIdx.y == 0;
   const int rows = queries ? p.length : p.keys, tiles = queries ? query_tiles : key_tiles;
+  if (blockIdx.x >= static_cast<uint32_t>(tiles) * p.kv_heads) return;
   int kv_head;
-  const Tile t = find_tile(p, static_cast<int>(blockIdx.x - (queries ? 0 : query_items)), rows, p.kv_heads, kTileShift, tiles,
-                           false, &kv_head);
+  const Tile t = find_tile(p, blockIdx.x, rows, p.kv_heads, kTileShift, tiles, false, &kv_head);
   if (!t.found) return;
   const int row = t.first + threadIdx.x;
   const int64_t at = static_cast<int64_t>(t.batch) * rows + t.row0 + row;
@@ -1724,11 +1723,9 @@ int backward(const muon_train_attention_args& a, const muon_train_attention_grad
   if (rc != MUON_POLAR_OK) return rc;
   if constexpr (!kBf16<T>) {
     const int64_t query_tiles = tiles_of(a, a.length, kTile), key_tiles = tiles_of(a, a.keys, kTile);
-    const uint32_t query_items = static_cast<uint32_t>(query_tiles * a.kv_heads),
-                   key_items = static_cast<uint32_t>(key_tiles * a.kv_heads);
     p.section = static_cast<int>(a.batch * a.kv_heads);  // all
-    rc = launch(tops_kernel, dim3(query_items + key_items), kTile, 0, 1, true, stream, p,
-                reinterpret_cast<float2*>(workspace + w.query_top), workspace + w.key_top, query_items,
+    rc = launch(tops_kernel, dim3(static_cast<unsigned>((query_tiles > key_tiles ? query_tiles : key_tiles) * a.kv_heads), 2),
+                kTile, 0, 1, true, stream, p, reinterpret_cast<float2*>(workspace + w.query_top), workspace + w.key_top,
                 static_cast<int>(query_tiles), static_cast<int>(key_tiles));
     if (rc != MUON_POLAR_OK) return rc;
   }
