@@ -29,13 +29,16 @@
 // below fp16's range, and ds by a factor for each query (dq) or key (dk), of what
 // its own row can reach (ds_exponent).
 //
-// What bounds it (heads of 128, bf16): power for long sequences (2 x 8192 both
-// ways, 16 heads: forward 1000 us, 1100 TFLOP/s; backward 3320, 1160 TFLOP/s of
-// its seven products, at 1.57 GHz), the latency of scores, probabilities and
-// product one after another for shorter ones (4096 causal, 37 heads: 167 and
-// 529 us, 950 and 750 TFLOP/s of the products needed).  With heads of 64 the
-// exponentials and the issue slots come first (2 x 8192, 16 heads: 750 and 2240
-// us, 733 and 614 TFLOP/s).
+// What bounds it (heads of 128, bf16): the latency of scores, probabilities and
+// product one after another, which two tiles in flight cover in part (the tensor
+// pipe is busy in 53 to 67% of the cycles), and in the backward pass two more
+// products than needed.  Long sequences also draw 1000 W, which brings the clock
+// to 1.57-1.7 GHz (2 x 8192 both ways, 16 heads: forward 1000 us, 1100 TFLOP/s;
+// backward 3320, 1160 TFLOP/s of its seven products; plain products sustain 1382
+// at that power); shorter ones do not (4096 causal, 37 heads: 167 and 529 us, 950
+// and 750 TFLOP/s of the products needed).  With heads of 64 the exponentials and
+// the issue slots come first (2 x 8192, 16 heads: 750 and 2240 us, 733 and 614
+// TFLOP/s).
 #include <cuda.h>
 
 #include <type_traits>
@@ -204,9 +207,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 // The items of a block, a tile of a head each.  The grid has a block for each
 // item; one that runs takes over those that have not begun, in the order of
 // their indices, which goes from the items with the most tiles to those with
-// the fewest.  The warp that loads asks, every warp takes the answer for itself.  (Dealt out in fixed turns, two
-// padded batch entries of 8192 and some 5000 tokens took 804 us forward, 699
-// with a block an item, whose start and end stand alone.)
+// the fewest.  The warp that loads asks, every warp takes the answer for itself.
+// (Dealt out in fixed turns, two padded batch entries of 8192 and some 5000
+// tokens took 804 us forward, 699 with a block an item, whose start and end
+// stand alone.)
 constexpr int kAnswers = 4;
 struct Items {
   __align__(16) uint4 answer[kAnswers];
@@ -441,9 +445,10 @@ struct Forward {
 // same rows where an even number of heads shares a key head, else neighbours of
 // one head, of which one has more keys under a causal mask, and a short sequence
 // may have one only (16 heads over 4, 1024 packed sequences of 64 tokens: 667 us
-// with neighbours, 441 with two heads; 8 x 4096 causal of 128: 585 and 562).  Keys and values pass through a
-// ring of tiles, keys j, values j, keys j + 1 and so on.  Loads and products go
-// on to the next item while the results of the last are written.
+// with neighbours, 441 with two heads; 8 x 4096 causal of 128: 585 and 562).
+// Keys and values pass through a ring of tiles, keys j, values j, keys j + 1 and
+// so on.  Loads and products go on to the next item while the results of the last
+// are written.
 struct Pair {
   int head, heads_on, rows_on;  // of the first tile; from it to the second
   Tile t;
@@ -935,11 +940,11 @@ struct Keys {
   }
 };
 
-// Scores stand the other way round, a key a thread:
-// p^T and ds^T are left operands as they are.  The warps 0-3 take queries 0 to
-// 63 of each tile, 4-7 the others.  While the scores of the next tile are
-// computed ds is worked on, while dp is computed the next p.  4096 both ways, 37 heads of
-// 128: 492 us alone, with the tensor pipe busy in 67% of the cycles.
+// Scores stand the other way round, a key a thread: p^T and ds^T are left
+// operands as they are.  The warps 0-3 take queries 0 to 63 of each tile, 4-7 the
+// others.  While the scores of the next tile are computed ds is worked on, while
+// dp is computed the next p.  4096 both ways, 37 heads of 128: 492 us alone, with
+// the tensor pipe busy in 67% of the cycles.
 template <typename T, int kCols>
 __global__ void __launch_bounds__(kThreads, 1)
     key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1254,11 +1259,11 @@ struct Queries {
   }
 };
 
-// Two tiles of scores in tensor memory, one of
-// dp: the products of the next keys run while ds is worked on, which takes the
-// place of its scores.  Half of the warps may be done with the next ds before
-// the product with the present one has been issued, so those barriers are two.  4096
-// both ways, 37 heads of 128: 447 us alone, tensor pipe 53%.
+// Two tiles of scores in tensor memory, one of dp: the products of the next keys
+// run while ds is worked on, which takes the place of its scores.  Half of the
+// warps may be done with the next ds before the product with the present one has
+// been issued, so those barriers are two.  4096 both ways, 37 heads of 128: 447 us
+// alone, tensor pipe 53%.
 template <typename T, int kCols>
 __global__ void __launch_bounds__(kThreads, 1)
     query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

@@ -9,7 +9,6 @@
 // Bound by memory: the vocabulary is read once (and the gradient written
 // once); the lists are a thousandth of it.
 #include <algorithm>
-#include <algorithm>
 #include <cfloat>
 
 #include "sm100_ptx.cuh"

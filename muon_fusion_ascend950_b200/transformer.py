@@ -193,8 +193,10 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ca
 
     Returns the output with the query's shape.  Products are summed, and the
     softmax is taken, in fp32; probabilities are rounded to the inputs' type
-    before they multiply the values.  Differentiable in the three tensors; all
-    sums run in a fixed order.
+    before they multiply the values, and so are the gradients of the scores
+    before they multiply queries and keys.  Differentiable in the three tensors;
+    all sums run in a fixed order.  The backward pass computes all three gradients,
+    also where one of them is wanted.
     """
     try:
         if scale is None:
@@ -220,7 +222,8 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor], positions: torch.Te
     elements ``i`` and ``i + pairs`` of a head (``2 i`` and ``2 i + 1`` when
     ``interleaved``), is turned by ``position * frequencies[i]`` and multiplied
     by ``scale``; elements from ``2 * pairs`` on are copied.  Angles are taken in
-    64 bits, products in fp32, and each output is rounded once.
+    64 bits, their cosines and sines, the scaling and the products in fp32, and
+    each output is rounded once.
 
     Returns the two turned tensors, contiguous (None without ``key``).
     Differentiable in ``query`` and ``key``; frequencies that require a gradient
@@ -249,7 +252,10 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, stretch: str = "none"
       slowest pair turns ``factor`` times slower and the fastest stays;
     * ``"ramp"``: pairs that turn ``fast_turns`` times or more within
       ``trained_length`` stay, those with ``slow_turns`` or fewer are divided by
-      ``factor``, between them linearly; ``scale`` is ``0.1 log(factor) + 1``.
+      ``factor``; between them the share that stays grows linearly with the
+      pair's number of turns.  (Models trained with a ramp that is linear in the
+      pair's index need frequencies of their own.)  ``scale`` is ``0.1
+      log(factor) + 1``.
     """
     if dim < 2 or dim % 2:
         raise ValueError(f"dim must be even and positive, got {dim}")
