@@ -516,6 +516,41 @@ def test_fp16_gradients_of_sequences_and_heads_of_different_sizes(pkg, causal):
     check_fp16_gradients(pkg, *(t.flatten(0, 1) for t in (q, k, v, go)), parts, causal, offsets=offsets)
 
 
+@pytest.mark.parametrize("kv_heads", [1, 2])
+def test_fp16_gradients_of_more_sequences_than_a_warp_looks_at(pkg, kv_heads):
+    """Each token's results are those of its sequence among few others, which
+    are larger or smaller; offsets that descend leave no tensor."""
+    rng = random.Random(6)
+    ends = [7]
+    while len(ends) < 401:
+        ends.append(ends[-1] + rng.choice([0, 1, rng.randint(100, 300)]))
+    total = ends[-1] + 200
+    q, k, v, go = attention_inputs(1, total, total, 4, kv_heads, 64, F16, seed=36)
+    for a, b in zip(ends, ends[1:]):
+        v[0, a:b] *= rng.choice([1e-2, 1.0, 1e3])
+        go[0, a:b] *= rng.choice([1e-2, 1.0, 10.0])
+
+    def step(first, last):
+        rows = slice(ends[first], ends[last])
+        leaves = [t[0, rows].detach().requires_grad_(True) for t in (q, k, v)]
+        out = pkg.attention(*leaves, causal=True, window=200,
+                            offsets=torch.tensor(ends[first:last + 1], device="cuda") - ends[first])
+        return [out.detach(), *torch.autograd.grad(out, leaves, go[0, rows])]
+
+    leaves = [t[0].detach().requires_grad_(True) for t in (q, k, v)]
+    out = pkg.attention(*leaves, causal=True, window=200, offsets=torch.tensor(ends, device="cuda"))
+    got = [out.detach(), *torch.autograd.grad(out, leaves, go[0])]
+    for t in got:
+        assert not t[:7].any() and not t[ends[-1]:].any()
+    for first in range(0, 400, 10):
+        for a, b in zip(got, step(first, first + 10)):
+            assert torch.equal(a[ends[first]:ends[first + 10]], b)
+    for bad in ([300, 0], [50, 20, 290, 100], [-100, -50], [total, total + 100], [0, 1 << 30, 3]):
+        out = pkg.attention(*leaves, causal=True, offsets=torch.tensor(bad, device="cuda"))
+        torch.autograd.grad(out, leaves, go[0])
+    torch.cuda.synchronize()
+
+
 def test_fp16_gradients_beside_single_large_rows(pkg):
     """One token of a sequence with large values, another with a large gradient."""
     q, k, v, go = attention_inputs(2, 1200, 1200, 4, 2, 128, F16, seed=33)
